@@ -103,6 +103,20 @@ SIGNATURES = {
     "cllm_hip_attention_dev": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _P, _P]),
     "cllm_hip_attention_rope_dev": (_I, [_P, _P, _P, _I, _I, _I, _I, ctypes.c_float, _P, _P]),
     "cllm_hip_attention_plan": (ctypes.c_char_p, [_I, _I, _I, _I, _I]),
+    "cllm_hip_kv4_page_bytes": (_SZ, [_I, _I, _I]),
+    "cllm_hip_kv4_work_ints": (_SZ, [_I, _I, _I]),
+    "cllm_hip_kv4_extend_dev": (_I, [_P, _P, _P, _I, _P, _P]),
+    "cllm_hip_kv4_fork_dev": (_I, [_P, _P, _P, _I, _P]),
+    "cllm_hip_kv4_truncate_dev": (_I, [_P, _P, _P, _I, _P]),
+    "cllm_hip_kv4_compact_dev": (_I, [_P, _P, _P]),
+    "cllm_hip_kv4_copy_pages_dev": (_I, [_P, _P, _P, _I, _P]),
+    "cllm_hip_kv4_store_dev": (_I, [_P, _I, _P, _P, _P, _I, ctypes.c_float, _P, _P, _I, _I, _P]),
+    "cllm_hip_kv4_load_dev": (_I, [_P, _I, _P, _P, _I, _I, _P, _P, _P]),
+    "cllm_hip_kv4_attention_ws_bytes": (_SZ, [_P, _I, _I, _I, _I, _I]),
+    "cllm_hip_kv4_attention_dev": (_I, [_P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _SZ, _P]),
+    "cllm_hip_kv4_attention_plan": (ctypes.c_char_p, [_P, _I, _I, _I, _I, _I]),
+    "cllm_hip_logprobs_ws_bytes": (_SZ, [_I, _I, _I]),
+    "cllm_hip_logprobs_dev": (_I, [_P, _I64, _I, _I, _P, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
 }
 
 
@@ -653,3 +667,285 @@ def dequantize_rows_dev(w, t: int, in_dim: int, ids, out=None):
     _check(load_library().cllm_hip_dequantize_rows_dev(_tp(w), int(t), int(in_dim), _tp(ids),
                                                        int(n), _tp(out), _stream()))
     return out
+
+
+# ---- the paged KV cache in 4 bits -----------------------------------------------------------
+
+class _Kv4CacheStruct(ctypes.Structure):
+    """cllm_hip_kv4_cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("pages", "table", "lens", "refs", "work")] + [
+        (n, ctypes.c_int) for n in ("n_layers", "n_pages", "page_size", "n_head_kv", "head_dim",
+                                    "max_seqs", "max_pages")]
+
+
+def kv4_page_bytes(page_size: int, n_head_kv: int, head_dim: int) -> int:
+    """Bytes of a page of one layer (0 for a shape that is not supported)."""
+    return int(load_library().cllm_hip_kv4_page_bytes(int(page_size), int(n_head_kv), int(head_dim)))
+
+
+def _tensor(who: str, name: str, t, dtype, like, numel=None, optional=False):
+    """t's address, after a check of what the kernels take from it: dtype, contiguous, on the
+    device of `like`, of numel elements (when given)."""
+    if t is None:
+        if optional:
+            return None
+        raise RuntimeError(f"{who}: {name} is None")
+    if t.dtype != dtype:
+        raise RuntimeError(f"{who}: {name} must be {dtype}, not {t.dtype}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{who}: {name} must be contiguous")
+    if t.device != like.device:
+        raise RuntimeError(f"{who}: {name} is on {t.device}, not on {like.device}")
+    if numel is not None and t.numel() != numel:
+        raise RuntimeError(f"{who}: {name} has {t.numel()} elements, not {numel}")
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def _on_current(who: str, t):
+    import torch
+    if not t.is_cuda:
+        raise RuntimeError(f"{who}: needs CUDA tensors, not {t.device}")
+    if t.device.index != torch.cuda.current_device():
+        raise RuntimeError(f"{who}: tensors are on {t.device}, the current device is "
+                           f"cuda:{torch.cuda.current_device()}")
+
+
+class Kv4Cache:
+    """A paged KV cache in 4 bits (cllm_hip_kv4_cache, include/cllm_hip.h): pages (uint8,
+    n_layers x n_pages x page bytes), table (int32, max_seqs x max_pages page ids, -1: none), lens
+    (int32, max_seqs) and refs (int32, n_pages). Kv4Cache(...) makes an empty one on the device,
+    from_tensors wraps a caller's. The kv4_*_dev functions work on it, on torch's current stream."""
+
+    def __init__(self, n_layers: int, n_pages: int, max_seqs: int, max_pages: int, *,
+                 page_size: int = 64, n_head_kv: int, head_dim: int, device="cuda"):
+        import torch
+        nbytes = kv4_page_bytes(page_size, n_head_kv, head_dim)
+        if nbytes == 0 or min(n_layers, n_pages, max_seqs, max_pages) <= 0:
+            raise RuntimeError("Kv4Cache: page_size must be a power of two from 32 to 1024, head_dim "
+                               "64, 128 or 256, and every count positive")
+        i32 = dict(dtype=torch.int32, device=device)
+        self._set(torch.empty((n_layers, n_pages, nbytes), dtype=torch.uint8, device=device),
+                  torch.full((max_seqs, max_pages), -1, **i32), torch.zeros(max_seqs, **i32),
+                  torch.zeros(n_pages, **i32), page_size, n_head_kv, head_dim)
+
+    @classmethod
+    def from_tensors(cls, pages, table, lens, refs, *, page_size: int, n_head_kv: int, head_dim: int):
+        self = cls.__new__(cls)
+        self._set(pages, table, lens, refs, page_size, n_head_kv, head_dim)
+        return self
+
+    def _set(self, pages, table, lens, refs, page_size, n_head_kv, head_dim):
+        import torch
+        nbytes = kv4_page_bytes(page_size, n_head_kv, head_dim)
+        if pages.dim() != 3 or pages.shape[2] != nbytes or nbytes == 0:
+            raise RuntimeError(f"Kv4Cache: pages must be n_layers x n_pages x {nbytes} bytes")
+        if table.dim() != 2:
+            raise RuntimeError("Kv4Cache: table must be max_seqs x max_pages")
+        work = load_library().cllm_hip_kv4_work_ints(pages.shape[1], table.shape[0], table.shape[1])
+        self.pages, self.table, self.lens, self.refs = pages, table, lens, refs
+        self.work = torch.empty(int(work), dtype=torch.int32, device=pages.device)
+        who = "Kv4Cache"
+        self.struct = _Kv4CacheStruct(
+            _tensor(who, "pages", pages, torch.uint8, pages),
+            _tensor(who, "table", table, torch.int32, pages),
+            _tensor(who, "lens", lens, torch.int32, pages, table.shape[0]),
+            _tensor(who, "refs", refs, torch.int32, pages, pages.shape[1]),
+            ctypes.c_void_p(self.work.data_ptr()), pages.shape[0], pages.shape[1], int(page_size),
+            int(n_head_kv), int(head_dim), table.shape[0], table.shape[1])
+
+    @property
+    def _ref(self):
+        return ctypes.byref(self.struct)
+
+
+def _kv4_batch(who, cache, q_start, slots, rows):
+    """(slots, q_start, n_seqs) of a batch, checked."""
+    import torch
+    _on_current(who, cache.pages)
+    qs = _tensor(who, "q_start", q_start, torch.int32, cache.pages)
+    n_seqs = q_start.numel() - 1
+    if n_seqs < 0:
+        raise RuntimeError(f"{who}: q_start has n_seqs + 1 elements")
+    if slots is None and n_seqs > cache.table.shape[0]:
+        raise RuntimeError(f"{who}: {n_seqs} sequences, {cache.table.shape[0]} slots")
+    return _tensor(who, "slots", slots, torch.int32, cache.pages, n_seqs, optional=True), qs, n_seqs
+
+
+def kv4_extend_dev(cache: Kv4Cache, slots, counts, status=None):
+    """Adds counts[i] tokens to slot slots[i] (int32 CUDA tensors; slots None: slot i) with the pages
+    they need, copies of shared partly filled pages included. Returns status (int32, one element, on
+    the device): 0, the number of pages missing, or -1 for bad entries; unless it is 0 nothing has
+    changed."""
+    import torch
+    who = "kv4_extend"
+    _on_current(who, cache.pages)
+    c = _tensor(who, "counts", counts, torch.int32, cache.pages)
+    n = counts.numel()
+    if slots is None and n > cache.table.shape[0]:
+        raise RuntimeError(f"{who}: {n} counts, {cache.table.shape[0]} slots")
+    s = _tensor(who, "slots", slots, torch.int32, cache.pages, n, optional=True)
+    if status is None:
+        status = torch.empty(1, dtype=torch.int32, device=cache.pages.device)
+    _check(load_library().cllm_hip_kv4_extend_dev(
+        cache._ref, s, c, n, _tensor(who, "status", status, torch.int32, cache.pages, 1), _stream()))
+    return status
+
+
+def kv4_fork_dev(cache: Kv4Cache, src, dst) -> None:
+    """Slot dst[i] becomes a copy of slot src[i] (int32 CUDA tensors), all at once; the pages are
+    shared."""
+    import torch
+    who = "kv4_fork"
+    _on_current(who, cache.pages)
+    s = _tensor(who, "src", src, torch.int32, cache.pages)
+    d = _tensor(who, "dst", dst, torch.int32, cache.pages, src.numel())
+    _check(load_library().cllm_hip_kv4_fork_dev(cache._ref, s, d, src.numel(), _stream()))
+
+
+def kv4_truncate_dev(cache: Kv4Cache, slots, new_lens=None) -> None:
+    """Cuts slot slots[i] to new_lens[i] tokens (None: to 0, freeing the sequences) and releases the
+    pages past them."""
+    import torch
+    who = "kv4_truncate"
+    _on_current(who, cache.pages)
+    s = _tensor(who, "slots", slots, torch.int32, cache.pages)
+    n = _tensor(who, "new_lens", new_lens, torch.int32, cache.pages, slots.numel(), optional=True)
+    _check(load_library().cllm_hip_kv4_truncate_dev(cache._ref, s, n, slots.numel(), _stream()))
+
+
+def kv4_compact_dev(cache: Kv4Cache, n_live=None):
+    """Moves the pages in use to the front of the pool; returns their number (int32, one element, on
+    the device)."""
+    import torch
+    who = "kv4_compact"
+    _on_current(who, cache.pages)
+    if n_live is None:
+        n_live = torch.empty(1, dtype=torch.int32, device=cache.pages.device)
+    _check(load_library().cllm_hip_kv4_compact_dev(
+        cache._ref, _tensor(who, "n_live", n_live, torch.int32, cache.pages, 1), _stream()))
+    return n_live
+
+
+def kv4_copy_pages_dev(cache: Kv4Cache, src, dst) -> None:
+    """Copies page src[i] to page dst[i] (int32 CUDA tensors) in every layer."""
+    import torch
+    who = "kv4_copy_pages"
+    _on_current(who, cache.pages)
+    s = _tensor(who, "src", src, torch.int32, cache.pages)
+    d = _tensor(who, "dst", dst, torch.int32, cache.pages, src.numel())
+    _check(load_library().cllm_hip_kv4_copy_pages_dev(cache._ref, s, d, src.numel(), _stream()))
+
+
+def kv4_store_dev(cache: Kv4Cache, layer: int, k, v, q_start, slots=None, q=None, n_head: int = 0,
+                  theta_base: float = 0.0) -> None:
+    """Stores the rows k and v (float32, n_rows x n_head_kv x head_dim) as the last tokens of the
+    batch's sequences: sequence i is slot slots[i] (None: slot i) and has rows q_start[i] ..
+    q_start[i + 1]. theta_base > 0: the keys, and the query rows q in place, get the NEOX rotation of
+    rope_neox2_dev at their positions first."""
+    import torch
+    who = "kv4_store"
+    s, qs, n_seqs = _kv4_batch(who, cache, q_start, slots, k)
+    width = cache.struct.n_head_kv * cache.struct.head_dim
+    kp = _tensor(who, "k", k, torch.float32, cache.pages)
+    if k.numel() % width:
+        raise RuntimeError(f"{who}: k has {k.numel()} elements, rows have {width}")
+    n_rows = k.numel() // width
+    vp = _tensor(who, "v", v, torch.float32, cache.pages, k.numel())
+    qp = _tensor(who, "q", q, torch.float32, cache.pages, n_rows * int(n_head) * cache.struct.head_dim,
+                 optional=True)
+    _check(load_library().cllm_hip_kv4_store_dev(cache._ref, int(layer), kp, vp, qp, int(n_head),
+                                                 float(theta_base), s, qs, n_seqs, n_rows, _stream()))
+
+
+def kv4_load_dev(cache: Kv4Cache, layer: int, q_start, n_rows: int, slots=None, k=None, v=None):
+    """The rows' keys and values as float32 (n_rows x n_head_kv * head_dim), the batch as
+    kv4_store_dev's (rows of no sequence are left as they are)."""
+    import torch
+    who = "kv4_load"
+    s, qs, n_seqs = _kv4_batch(who, cache, q_start, slots, None)
+    width = cache.struct.n_head_kv * cache.struct.head_dim
+    out = []
+    for name, t in (("k", k), ("v", v)):
+        if t is None:
+            t = torch.empty((int(n_rows), width), dtype=torch.float32, device=cache.pages.device)
+        _tensor(who, name, t, torch.float32, cache.pages, int(n_rows) * width)
+        out.append(t)
+    _check(load_library().cllm_hip_kv4_load_dev(cache._ref, int(layer), s, qs, n_seqs, int(n_rows),
+                                                _tp(out[0]), _tp(out[1]), _stream()))
+    return tuple(out)
+
+
+def kv4_attention_dev(cache: Kv4Cache, layer: int, q, q_start, *, n_head: int, max_rows: int,
+                      max_len: int, slots=None, out=None):
+    """Grouped-query attention of the rows q (float32, n_rows x n_head x head_dim) over the cache,
+    the batch as kv4_store_dev's: row t of a sequence with r rows sees positions [0, len - r + t].
+    max_rows and max_len bound a sequence's rows and tokens. Returns out (n_rows x n_head *
+    head_dim); a row that sees nothing is 0, one of no sequence is left as it is."""
+    import torch
+    who = "kv4_attention"
+    s, qs, n_seqs = _kv4_batch(who, cache, q_start, slots, q)
+    width = int(n_head) * cache.struct.head_dim
+    qp = _tensor(who, "q", q, torch.float32, cache.pages)
+    if width <= 0 or q.numel() % width:
+        raise RuntimeError(f"{who}: q has {q.numel()} elements, rows have {width}")
+    n_rows = q.numel() // width
+    if out is None:
+        out = torch.empty((n_rows, width), dtype=torch.float32, device=q.device)
+    op = _tensor(who, "out", out, torch.float32, cache.pages, n_rows * width)
+    lib = load_library()
+    args = (n_seqs, n_rows, int(max_rows), int(max_len), int(n_head))
+    nbytes = int(lib.cllm_hip_kv4_attention_ws_bytes(cache._ref, *args))
+    # scratch from torch's allocator: a captured call's belongs to its graph
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _check(lib.cllm_hip_kv4_attention_dev(cache._ref, int(layer), qp, s, qs, *args, op, _tp(ws), nbytes,
+                                          _stream()))
+    return out
+
+
+def kv4_attention_plan(cache: Kv4Cache, n_seqs: int, n_rows: int, max_rows: int, max_len: int,
+                       n_head: int) -> str:
+    """The kernel and launch plan of kv4_attention_dev for this shape."""
+    return load_library().cllm_hip_kv4_attention_plan(cache._ref, int(n_seqs), int(n_rows), int(max_rows),
+                                                      int(max_len), int(n_head)).decode()
+
+
+# ---- log probabilities ------------------------------------------------------------------------
+
+@dataclass
+class LogProbs:
+    """What logprobs_dev returns: CUDA tensors (None: not asked for)."""
+    logprobs: object      # float32 [n_rows], of the given tokens
+    ranks: object         # int32 [n_rows], tokens ahead of them
+    entropy: object       # float32 [n_rows]
+    lse: object           # float32 [n_rows]
+    top_ids: object       # int32 [n_rows, top_k]
+    top_logprobs: object  # float32 [n_rows, top_k]
+
+
+def logprobs_dev(logits, tokens=None, top_k: int = 0) -> LogProbs:
+    """Log probabilities of the rows of logits (float32 (n_rows, vocab), any row stride, unit stride
+    along a row): of the given tokens (int32 (n_rows,)) with their ranks, the entropy and
+    log-sum-exp, and the top_k (at most 64) largest with their ids, equal logits by ids."""
+    import torch
+    who = "logprobs"
+    if logits.dim() != 2 or logits.dtype != torch.float32:
+        raise RuntimeError(f"{who}: logits must be float32 n_rows x vocab")
+    _on_current(who, logits)
+    m, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise RuntimeError(f"{who}: the logits of a row must lie side by side")
+    stride = logits.stride(0) if m > 1 else vocab
+    tp = _tensor(who, "tokens", tokens, torch.int32, logits, m, optional=True)
+    new = lambda dt, *shape: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
+    r = LogProbs(new(torch.float32, m) if tokens is not None else None,
+                 new(torch.int32, m) if tokens is not None else None,
+                 new(torch.float32, m), new(torch.float32, m),
+                 new(torch.int32, m, int(top_k)), new(torch.float32, m, int(top_k)))
+    lib = load_library()
+    nbytes = int(lib.cllm_hip_logprobs_ws_bytes(m, vocab, int(top_k)))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
+    _check(lib.cllm_hip_logprobs_dev(_tp(logits), int(stride), m, vocab, tp, int(top_k), _tp(r.logprobs),
+                                     _tp(r.ranks), _tp(r.entropy), _tp(r.lse),
+                                     _tp(r.top_ids) if top_k else None,
+                                     _tp(r.top_logprobs) if top_k else None, _tp(ws), nbytes, _stream()))
+    return r

@@ -31,6 +31,7 @@
 #include "../../include/cllm_hip.h"
 #include "ggml_blocks.h"
 #include "gguf_file.h"
+#include "kv4.h"
 #include "launch.h"
 
 using namespace cllm_hip;
@@ -1683,6 +1684,262 @@ int cllm_hip_attention_rope_dev(const float* q, float* k_cache, const float* v_c
     if (!(theta_base > 0.0f)) return set_err(CLLM_HIP_E_ARG, "attention: theta_base must be positive");
     return attention_impl(q, k_cache, v_cache, 1, pos0, n_head, n_head_kv, head_dim, out, stream,
                           theta_base);
+}
+
+// ---- the paged KV cache in 4 bits, and log probabilities ----------------------------------
+
+static bool aligned4(const void* p) { return ((uintptr_t)p & 3u) == 0; }
+
+size_t cllm_hip_kv4_page_bytes(int page_size, int n_head_kv, int head_dim) {
+    if (page_size < 32 || page_size > 1024 || (page_size & (page_size - 1)) || n_head_kv <= 0 ||
+        n_head_kv > 1024 || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        return 0;
+    return (size_t)n_head_kv * (size_t)(page_size / 32) * 36 * (size_t)head_dim;
+}
+
+size_t cllm_hip_kv4_work_ints(int n_pages, int max_seqs, int max_pages) {
+    if (n_pages <= 0 || max_seqs <= 0 || max_pages <= 0) return 0;
+    return (size_t)kv4_work_ints(n_pages, max_seqs, max_pages);
+}
+
+// The checked form of a cache. work: the call needs the cache's work array.
+static int kv4_view(const char* who, const cllm_hip_kv4_cache* c, bool work, Kv4View* v) {
+    if (!c) return set_err(CLLM_HIP_E_ARG, "%s: null cache", who);
+    const size_t pb = cllm_hip_kv4_page_bytes(c->page_size, c->n_head_kv, c->head_dim);
+    if (pb == 0)
+        return set_err(CLLM_HIP_E_ARG,
+                       "%s: page_size must be a power of two from 32 to 1024, head_dim 64, 128 or 256, "
+                       "n_head_kv 1 to 1024", who);
+    if (c->n_layers <= 0 || c->n_pages <= 0 || c->n_pages > (1 << 28) || c->max_seqs <= 0 || c->max_pages <= 0 ||
+        (int64_t)c->max_pages * c->page_size > INT32_MAX / 2)
+        return set_err(CLLM_HIP_E_ARG, "%s: bad cache shape", who);
+    if (!c->pages || !c->table || !c->lens || !c->refs || (work && !c->work))
+        return set_err(CLLM_HIP_E_ARG, "%s: null pointer in the cache", who);
+    if (!aligned16(c->pages) || !aligned4(c->table) || !aligned4(c->lens) || !aligned4(c->refs) || !aligned4(c->work))
+        return set_err(CLLM_HIP_E_ARG, "%s: misaligned device pointer in the cache", who);
+    v->pages = (uint8_t*)c->pages;
+    v->table = c->table;
+    v->lens = c->lens;
+    v->refs = c->refs;
+    v->work = c->work;
+    v->n_layers = c->n_layers;
+    v->n_pages = c->n_pages;
+    v->n_kv = c->n_head_kv;
+    v->hd = c->head_dim;
+    v->max_seqs = c->max_seqs;
+    v->max_pages = c->max_pages;
+    v->page_shift = __builtin_ctz((unsigned)c->page_size);
+    v->page_bytes = (int64_t)pb;
+    return CLLM_HIP_OK;
+}
+
+// The batch arguments that store, load and attention share.
+static int kv4_batch(const char* who, const Kv4View& v, int layer, const int32_t* slots, const int32_t* q_start,
+                     int n_seqs, int n_rows) {
+    if (layer < 0 || layer >= v.n_layers) return set_err(CLLM_HIP_E_ARG, "%s: no layer %d", who, layer);
+    if (n_seqs < 0 || n_rows < 0 || n_seqs > 65536 || n_rows > (1 << 26))
+        return set_err(CLLM_HIP_E_ARG, "%s: bad batch shape", who);
+    if (n_seqs > 0 && n_rows > 0) {
+        if (!q_start) return set_err(CLLM_HIP_E_ARG, "%s: null pointer", who);
+        if (!aligned4(slots) || !aligned4(q_start)) return set_err(CLLM_HIP_E_ARG, "%s: misaligned device pointer", who);
+    }
+    return CLLM_HIP_OK;
+}
+
+int cllm_hip_kv4_store_dev(const cllm_hip_kv4_cache* cache, int layer, const float* k, const float* v, float* q,
+                           int n_head, float theta_base, const int32_t* slots, const int32_t* q_start, int n_seqs,
+                           int n_rows, void* stream) {
+    Kv4View c;
+    int rc = kv4_view("kv4_store", cache, false, &c);
+    if (rc || (rc = kv4_batch("kv4_store", c, layer, slots, q_start, n_seqs, n_rows))) return rc;
+    if (!(theta_base >= 0.0f) || theta_base > 3.0e38f)
+        return set_err(CLLM_HIP_E_ARG, "kv4_store: theta_base must be 0 (no rotation) or positive");
+    if (q && (theta_base == 0.0f || n_head <= 0 || n_head > 65536))
+        return set_err(CLLM_HIP_E_ARG, "kv4_store: q is given to be rotated: n_head and theta_base must be positive");
+    if (n_seqs == 0 || n_rows == 0) return CLLM_HIP_OK;
+    if (!k || !v) return set_err(CLLM_HIP_E_ARG, "kv4_store: null pointer");
+    if (!aligned16(k) || !aligned16(v) || !aligned16(q))
+        return set_err(CLLM_HIP_E_ARG, "kv4_store: misaligned device pointer");
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_kv4_store(c, layer, k, v, q, n_head, theta_base, slots, q_start, n_seqs, n_rows,
+                             (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+int cllm_hip_kv4_load_dev(const cllm_hip_kv4_cache* cache, int layer, const int32_t* slots, const int32_t* q_start,
+                          int n_seqs, int n_rows, float* k, float* v, void* stream) {
+    Kv4View c;
+    int rc = kv4_view("kv4_load", cache, false, &c);
+    if (rc || (rc = kv4_batch("kv4_load", c, layer, slots, q_start, n_seqs, n_rows))) return rc;
+    if (n_seqs == 0 || n_rows == 0) return CLLM_HIP_OK;
+    if (!k || !v) return set_err(CLLM_HIP_E_ARG, "kv4_load: null pointer");
+    if (!aligned16(k) || !aligned16(v)) return set_err(CLLM_HIP_E_ARG, "kv4_load: misaligned device pointer");
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_kv4_load(c, layer, slots, q_start, n_seqs, n_rows, k, v, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+static int kv4_attention_args(const char* who, const cllm_hip_kv4_cache* cache, int n_seqs, int n_rows, int max_rows,
+                              int max_len, int n_head, Kv4View* c, Kv4AttnPlan* p) {
+    int rc = kv4_view(who, cache, false, c);
+    if (rc) return rc;
+    if (n_seqs < 0 || n_rows < 0 || max_rows < 0 || max_len < 0 || n_seqs > 65536 || n_rows > (1 << 26))
+        return set_err(CLLM_HIP_E_ARG, "%s: bad batch shape", who);
+    if (n_head <= 0 || n_head % c->n_kv != 0 || n_head > 65536)
+        return set_err(CLLM_HIP_E_ARG, "%s: n_head must be a multiple of n_head_kv", who);
+    if (n_seqs == 0 || n_rows == 0 || max_rows == 0) {
+        *p = Kv4AttnPlan{0, 0, 1, 1};
+        return CLLM_HIP_OK;
+    }
+    max_rows = std::min(max_rows, n_rows);
+    max_len = std::min(max_len, c->max_pages << c->page_shift);
+    *p = kv4_attention_plan(*c, n_seqs, max_rows, max_len, n_head);
+    if (!kv4_attention_fits(*p, *c, n_seqs)) return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
+    return CLLM_HIP_OK;
+}
+
+size_t cllm_hip_kv4_attention_ws_bytes(const cllm_hip_kv4_cache* cache, int n_seqs, int n_rows, int max_rows,
+                                       int max_len, int n_head) {
+    Kv4View c;
+    Kv4AttnPlan p;
+    if (kv4_attention_args("kv4_attention", cache, n_seqs, n_rows, max_rows, max_len, n_head, &c, &p)) return 0;
+    return kv4_attention_ws_bytes(p, n_rows, n_head, c.hd);
+}
+
+const char* cllm_hip_kv4_attention_plan(const cllm_hip_kv4_cache* cache, int n_seqs, int n_rows, int max_rows,
+                                        int max_len, int n_head) {
+    static thread_local char buf[96];
+    Kv4View c;
+    Kv4AttnPlan p;
+    if (kv4_attention_args("kv4_attention", cache, n_seqs, n_rows, max_rows, max_len, n_head, &c, &p) ||
+        p.col_tiles == 0)
+        return "none";
+    snprintf(buf, sizeof buf, "%s<%d> columns=%d chunk=%d splits=%d", "k_kv4_attention", c.hd, p.col_tiles,
+             p.chunk_tiles * 32, p.splits);
+    return buf;
+}
+
+int cllm_hip_kv4_attention_dev(const cllm_hip_kv4_cache* cache, int layer, const float* q, const int32_t* slots,
+                               const int32_t* q_start, int n_seqs, int n_rows, int max_rows, int max_len, int n_head,
+                               float* out, void* ws, size_t ws_bytes, void* stream) {
+    Kv4View c;
+    Kv4AttnPlan p;
+    int rc = kv4_attention_args("kv4_attention", cache, n_seqs, n_rows, max_rows, max_len, n_head, &c, &p);
+    if (rc || (rc = kv4_batch("kv4_attention", c, layer, slots, q_start, n_seqs, n_rows))) return rc;
+    if (p.col_tiles == 0) return CLLM_HIP_OK;
+    if (!q || !out) return set_err(CLLM_HIP_E_ARG, "kv4_attention: null pointer");
+    if (!aligned16(q) || !aligned16(out) || !aligned16(ws))
+        return set_err(CLLM_HIP_E_ARG, "kv4_attention: misaligned device pointer");
+    const size_t need = kv4_attention_ws_bytes(p, n_rows, n_head, c.hd);
+    if (need > 0 && (!ws || ws_bytes < need))
+        return set_err(CLLM_HIP_E_ARG, "kv4_attention: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, need);
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_kv4_attention(c, p, layer, q, slots, q_start, n_seqs, n_rows, std::min(max_rows, n_rows), n_head, out,
+                                 ws, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+// The list arguments of the page calls: n entries, at most max_n.
+static int kv4_list(const char* who, const void* a, const void* b, int n, int max_n) {
+    if (n < 0 || n > max_n) return set_err(CLLM_HIP_E_ARG, "%s: %d entries, at most %d", who, n, max_n);
+    if (n > 0 && (!a || !aligned4(a) || !aligned4(b)))
+        return set_err(CLLM_HIP_E_ARG, "%s: null or misaligned device pointer", who);
+    return CLLM_HIP_OK;
+}
+
+int cllm_hip_kv4_extend_dev(const cllm_hip_kv4_cache* cache, const int32_t* slots, const int32_t* counts, int n,
+                            int32_t* status, void* stream) {
+    Kv4View c;
+    int rc = kv4_view("kv4_extend", cache, true, &c);
+    if (rc || (rc = kv4_list("kv4_extend", counts, slots, n, 1024))) return rc;
+    if (!status || !aligned4(status)) return set_err(CLLM_HIP_E_ARG, "kv4_extend: null or misaligned status pointer");
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_kv4_extend(c, slots, counts, n, status, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+int cllm_hip_kv4_fork_dev(const cllm_hip_kv4_cache* cache, const int32_t* src, const int32_t* dst, int n,
+                          void* stream) {
+    Kv4View c;
+    int rc = kv4_view("kv4_fork", cache, true, &c);
+    if (rc || (rc = kv4_list("kv4_fork", src, dst, n, std::min(1024, c.max_seqs)))) return rc;
+    if (n == 0) return CLLM_HIP_OK;
+    if (!dst) return set_err(CLLM_HIP_E_ARG, "kv4_fork: null pointer");
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_kv4_fork(c, src, dst, n, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+int cllm_hip_kv4_truncate_dev(const cllm_hip_kv4_cache* cache, const int32_t* slots, const int32_t* new_lens, int n,
+                              void* stream) {
+    Kv4View c;
+    int rc = kv4_view("kv4_truncate", cache, false, &c);
+    if (rc || (rc = kv4_list("kv4_truncate", slots, new_lens, n, 65536))) return rc;
+    if (n == 0) return CLLM_HIP_OK;
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_kv4_truncate(c, slots, new_lens, n, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+int cllm_hip_kv4_compact_dev(const cllm_hip_kv4_cache* cache, int32_t* n_live, void* stream) {
+    Kv4View c;
+    int rc = kv4_view("kv4_compact", cache, true, &c);
+    if (rc) return rc;
+    if (!n_live || !aligned4(n_live)) return set_err(CLLM_HIP_E_ARG, "kv4_compact: null or misaligned n_live pointer");
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_kv4_compact(c, n_live, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+int cllm_hip_kv4_copy_pages_dev(const cllm_hip_kv4_cache* cache, const int32_t* src, const int32_t* dst, int n,
+                                void* stream) {
+    Kv4View c;
+    int rc = kv4_view("kv4_copy_pages", cache, false, &c);
+    if (rc || (rc = kv4_list("kv4_copy_pages", src, dst, n, 1 << 28))) return rc;
+    if (n == 0) return CLLM_HIP_OK;
+    if (!dst) return set_err(CLLM_HIP_E_ARG, "kv4_copy_pages: null pointer");
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_kv4_copy_pages(c, src, dst, n, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+size_t cllm_hip_logprobs_ws_bytes(int n_rows, int vocab, int top_k) {
+    if (n_rows <= 0 || vocab <= 0 || top_k < 0 || top_k > kMaxTopK) return 0;
+    return logprobs_ws_bytes(n_rows, vocab, top_k);
+}
+
+int cllm_hip_logprobs_dev(const float* logits, int64_t row_stride, int n_rows, int vocab, const int32_t* tokens,
+                          int top_k, float* logprobs, int32_t* ranks, float* entropy, float* lse, int32_t* top_ids,
+                          float* top_logprobs, void* ws, size_t ws_bytes, void* stream) {
+    if (n_rows < 0 || vocab <= 0 || vocab > (1 << 30) || row_stride < vocab)
+        return set_err(CLLM_HIP_E_ARG, "logprobs: bad shape");
+    if (top_k < 0 || top_k > kMaxTopK || top_k > vocab)
+        return set_err(CLLM_HIP_E_ARG, "logprobs: top_k must be 0 to %d and at most vocab", kMaxTopK);
+    if (!tokens && (logprobs || ranks)) return set_err(CLLM_HIP_E_ARG, "logprobs: logprobs and ranks need tokens");
+    if (n_rows == 0) return CLLM_HIP_OK;
+    if (!logits) return set_err(CLLM_HIP_E_ARG, "logprobs: null pointer");
+    if (!aligned4(logits) || !aligned4(tokens) || !aligned4(logprobs) || !aligned4(ranks) || !aligned4(entropy) ||
+        !aligned4(lse) || !aligned4(top_ids) || !aligned4(top_logprobs) || !aligned16(ws))
+        return set_err(CLLM_HIP_E_ARG, "logprobs: misaligned device pointer");
+    if ((double)n_rows * ((vocab + 8191) / 8192) > 2147483647.0)
+        return set_err(CLLM_HIP_E_ARG, "logprobs: batch too large for one launch");
+    const size_t need = logprobs_ws_bytes(n_rows, vocab, top_k);
+    if (!ws || ws_bytes < need)
+        return set_err(CLLM_HIP_E_ARG, "logprobs: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, need);
+    DeviceState* st;
+    int rc = acquire(&st);
+    if (rc) return rc;
+    HIP_TRY(launch_logprobs(logits, row_stride, n_rows, vocab, tokens, top_k, logprobs, ranks, entropy, lse, top_ids,
+                            top_logprobs, ws, (hipStream_t)stream));
+    return CLLM_HIP_OK;
 }
 
 // ---- GGUF files (gguf.cpp:122-275 of the reference) ---------------------------------------

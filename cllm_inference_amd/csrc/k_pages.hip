@@ -1,0 +1,366 @@
+// k_pages.hip -- the page work of the paged KV cache: extending sequences (with copies of shared,
+// partly filled pages), forking, truncating and freeing them, moving the pages in use to the front
+// of the pool, and copying pages. All bookkeeping is on the device: nothing waits for the host.
+//
+// Every decision follows from the arrays alone (free pages are taken lowest id first, entries in
+// the order given), so a call's result does not depend on timing; the atomics on reference counts
+// are integer additions, which commute.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "device_utils.h"
+#include "kv4.h"
+
+namespace cllm_hip {
+namespace {
+
+constexpr int kThreads = 1024;   // of the one-workgroup bookkeeping kernels
+constexpr int kMaxEntries = 1024;
+
+// Sum of v over the threads before this one; total receives the workgroup's. All threads call it.
+__device__ __forceinline__ int block_scan(int v, int& total) {
+    __shared__ int sums[kThreads / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int incl = v;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int y = __shfl_up(incl, d, 64);
+        if (lane >= d) incl += y;
+    }
+    __syncthreads();  // the sums of the call before have been read
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+        if (w < wave) before += sums[w];
+        total += sums[w];
+    }
+    return before + incl - v;
+}
+
+__device__ __forceinline__ int pages_of(int64_t len, int shift) {
+    return (int)((len + ((int64_t)1 << shift) - 1) >> shift);
+}
+
+// Extends entry i (thread i) by counts[i] tokens. work: [0] copies, then (source, destination)
+// pairs, then the list of taken pages at 1 + 2 * kMaxEntries.
+__global__ __launch_bounds__(kThreads) void k_kv4_extend(Kv4View c, const int32_t* __restrict__ slots,
+                                                         const int32_t* __restrict__ counts, int n,
+                                                         int32_t* __restrict__ status) {
+    __shared__ int s_slot[kMaxEntries], s_page[kMaxEntries];
+    __shared__ int s_bad, s_copies;
+    const int tid = threadIdx.x;
+    if (tid == 0) s_bad = s_copies = 0;
+    int slot = -1, count = 0, len = 0, old_pages = 0, page = -1;
+    int64_t grow = 0;
+    bool bad = false;
+    if (tid < n) {
+        slot = slots ? slots[tid] : tid;
+        count = counts[tid];
+        bad = (unsigned)slot >= (unsigned)c.max_seqs || count < 0;
+        if (!bad) {
+            len = c.lens[slot];
+            const int64_t cap = (int64_t)c.max_pages << c.page_shift;
+            bad = len < 0 || len > cap || len + (int64_t)count > cap;
+        }
+        if (!bad) {
+            old_pages = pages_of(len, c.page_shift);
+            grow = pages_of(len + (int64_t)count, c.page_shift) - old_pages;
+            if (count > 0 && (len & ((1 << c.page_shift) - 1))) {
+                page = c.table[(int64_t)slot * c.max_pages + old_pages - 1];
+                bad = (unsigned)page >= (unsigned)c.n_pages;
+                if (bad) page = -1;
+            }
+        }
+        s_slot[tid] = slot;
+        s_page[tid] = page;
+    }
+    __syncthreads();
+    // entries before this one that hold the same page, which have left it by this one's turn
+    bool copy = false;
+    if (tid < n) {
+        int same = 0;
+        for (int j = 0; j < tid; ++j) {
+            bad |= s_slot[j] == slot;
+            same += page >= 0 && s_page[j] == page;
+        }
+        copy = page >= 0 && !bad && c.refs[page] - same > 1;
+        if (bad) s_bad = 1;
+    }
+    const int need = bad ? 0 : (int)grow + (copy ? 1 : 0);
+    int total;
+    const int first = block_scan(need, total);
+    if (s_bad || total == 0) {
+        if (tid == 0) {
+            *status = s_bad ? -1 : 0;
+            c.work[0] = 0;
+        }
+        if (!s_bad && tid < n && count > 0) c.lens[slot] = len + count;
+        return;
+    }
+    // the first `total` free pages
+    int32_t* taken = c.work + 1 + 2 * kMaxEntries;
+    int found = 0;
+    for (int base = 0; base < c.n_pages && found < total; base += 4 * kThreads) {
+        const int p0 = base + 4 * tid;
+        int free[4], k = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            free[i] = p0 + i < c.n_pages && c.refs[p0 + i] == 0;
+            k += free[i];
+        }
+        int here;
+        int at = found + block_scan(k, here);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (free[i]) {
+                if (at < total) taken[at] = p0 + i;
+                ++at;
+            }
+        }
+        found += here;
+    }
+    if (found < total) {  // nothing has been changed
+        if (tid == 0) {
+            *status = total - found;
+            c.work[0] = 0;
+        }
+        return;
+    }
+    __threadfence_block();
+    __syncthreads();
+    if (tid < n && count > 0) {
+        int32_t* row = c.table + (int64_t)slot * c.max_pages;
+        int at = first;
+        if (copy) {
+            const int dst = taken[at++];
+            const int i = atomicAdd(&s_copies, 1);
+            c.work[1 + 2 * i] = page;
+            c.work[2 + 2 * i] = dst;
+            row[old_pages - 1] = dst;
+            c.refs[dst] = 1;
+            atomicSub(&c.refs[page], 1);
+        }
+        for (int j = 0; j < (int)grow; ++j, ++at) {
+            const int dst = taken[at];
+            row[old_pages + j] = dst;
+            c.refs[dst] = 1;
+        }
+        c.lens[slot] = len + count;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        c.work[0] = s_copies;
+        *status = 0;
+    }
+}
+
+// Copies pages of every layer: pairs src[i * step] -> dst[i * step], i < n (or *n_dev). 16 KB a
+// step of a workgroup; a grid that fills the chip walks them, so a call without copies ends at once.
+// What bounds it: the HBM copy rate.
+constexpr int kCopyChunk = 16384;
+__device__ __forceinline__ void copy_pages(const Kv4View& c, const int32_t* src, const int32_t* dst, int step,
+                                           int n, int64_t first, int64_t stride) {
+    const int64_t chunks = (c.page_bytes + kCopyChunk - 1) / kCopyChunk;
+    const int64_t total = (int64_t)n * c.n_layers * chunks;
+    for (int64_t u = first; u < total; u += stride) {
+        const int64_t chunk = u % chunks, lp = u / chunks;
+        const int i = (int)(lp / c.n_layers), layer = (int)(lp % c.n_layers);
+        const int s = src[(int64_t)i * step], d = dst[(int64_t)i * step];
+        if ((unsigned)s >= (unsigned)c.n_pages || (unsigned)d >= (unsigned)c.n_pages || s == d) continue;
+        const int64_t from = ((int64_t)layer * c.n_pages + s) * c.page_bytes + chunk * kCopyChunk;
+        const int64_t to = ((int64_t)layer * c.n_pages + d) * c.page_bytes + chunk * kCopyChunk;
+        const int bytes = (int)min((int64_t)kCopyChunk, c.page_bytes - chunk * kCopyChunk);
+        u32x4 x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = (j * 256 + (int)threadIdx.x) * 16;
+            if (at < bytes) x[j] = ld_u32x4_nt(c.pages + from + at);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int at = (j * 256 + (int)threadIdx.x) * 16;
+            if (at < bytes) *(u32x4*)(c.pages + to + at) = x[j];
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void k_kv4_copy(Kv4View c, const int32_t* src, const int32_t* dst, int step,
+                                                  int n, const int32_t* n_dev) {
+    copy_pages(c, src, dst, step, n_dev ? *n_dev : n, blockIdx.x, gridDim.x);
+}
+
+// Whether an earlier entry names the same slot: the earlier one stands.
+__device__ __forceinline__ bool named_before(const int32_t* slots, int i) {
+    int found = 0;
+    for (int j = threadIdx.x; j < i; j += blockDim.x) found |= slots[j] == slots[i];
+    return __syncthreads_or(found);
+}
+
+// Fork, first launch (a workgroup per entry): the source's pages and length are written to work and
+// counted once more. Every source is read before any destination is written, so the entries act at
+// once (a beam search's permutation).
+__global__ __launch_bounds__(256) void k_kv4_fork_read(Kv4View c, const int32_t* __restrict__ src,
+                                                       const int32_t* __restrict__ dst) {
+    const int i = blockIdx.x, s = src[i], d = dst[i];
+    if ((unsigned)s >= (unsigned)c.max_seqs || (unsigned)d >= (unsigned)c.max_seqs || named_before(dst, i)) return;
+    int32_t* to = c.work + (int64_t)i * (c.max_pages + 1);
+    const int32_t* row = c.table + (int64_t)s * c.max_pages;
+    for (int p = threadIdx.x; p < c.max_pages; p += 256) {
+        const int page = row[p];
+        to[1 + p] = page;
+        if ((unsigned)page < (unsigned)c.n_pages) atomicAdd(&c.refs[page], 1);
+    }
+    if (threadIdx.x == 0) to[0] = c.lens[s];
+}
+
+// Second launch: the destination leaves its pages and takes those of the source.
+__global__ __launch_bounds__(256) void k_kv4_fork_write(Kv4View c, const int32_t* __restrict__ src,
+                                                        const int32_t* __restrict__ dst) {
+    const int i = blockIdx.x, s = src[i], d = dst[i];
+    if ((unsigned)s >= (unsigned)c.max_seqs || (unsigned)d >= (unsigned)c.max_seqs || named_before(dst, i)) return;
+    const int32_t* from = c.work + (int64_t)i * (c.max_pages + 1);
+    int32_t* row = c.table + (int64_t)d * c.max_pages;
+    for (int p = threadIdx.x; p < c.max_pages; p += 256) {
+        const int page = row[p];
+        if ((unsigned)page < (unsigned)c.n_pages) atomicSub(&c.refs[page], 1);
+        row[p] = from[1 + p];
+    }
+    if (threadIdx.x == 0) c.lens[d] = from[0];
+}
+
+__global__ __launch_bounds__(256) void k_kv4_truncate(Kv4View c, const int32_t* __restrict__ slots,
+                                                      const int32_t* __restrict__ new_lens) {
+    const int i = blockIdx.x, slot = slots[i];
+    if ((unsigned)slot >= (unsigned)c.max_seqs || named_before(slots, i)) return;
+    const int len = min(max(c.lens[slot], 0), max(new_lens ? new_lens[i] : 0, 0));
+    int32_t* row = c.table + (int64_t)slot * c.max_pages;
+    for (int p = pages_of(len, c.page_shift) + threadIdx.x; p < c.max_pages; p += 256) {
+        const int page = row[p];
+        if ((unsigned)page < (unsigned)c.n_pages) atomicSub(&c.refs[page], 1);
+        row[p] = -1;
+    }
+    __syncthreads();  // the length has been read by all
+    if (threadIdx.x == 0) c.lens[slot] = len;
+}
+
+// Compaction, first launch: n = pages in use; the pages in use at ids from n on, ascending, go to
+// the free ids below n, ascending. work: [0] moves, (source, destination) pairs, then the new id of
+// each page from n on at 1 + 2 n_pages + id.
+__global__ __launch_bounds__(kThreads) void k_kv4_compact_plan(Kv4View c, int32_t* __restrict__ n_live) {
+    const int tid = threadIdx.x;
+    int mine = 0, n;
+    for (int p = tid; p < c.n_pages; p += kThreads) mine += c.refs[p] > 0;
+    (void)block_scan(mine, n);
+    int holes = 0, moves = 0;
+    for (int base = 0; base < c.n_pages; base += 4 * kThreads) {
+        const int p0 = base + 4 * tid;
+        bool live[4];
+        int k = 0;  // holes below n in the low half, moved pages in the high half
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = p0 + i;
+            live[i] = p < c.n_pages && c.refs[p] > 0;
+            if (p < n && !live[i]) k += 1;
+            if (p >= n && live[i]) k += 1 << 16;
+        }
+        int here;
+        const int before = block_scan(k, here);
+        int hole = holes + (before & 0xFFFF), move = moves + (before >> 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = p0 + i;
+            if (p < n && !live[i]) c.work[2 + 2 * hole++] = p;
+            if (p >= n && live[i]) c.work[1 + 2 * move++] = p;
+            if (p >= n && p < c.n_pages && !live[i]) c.work[1 + 2 * (int64_t)c.n_pages + p] = p;
+        }
+        holes += here & 0xFFFF;
+        moves += here >> 16;
+    }
+    __threadfence_block();
+    __syncthreads();
+    for (int i = tid; i < moves; i += kThreads) {
+        const int s = c.work[1 + 2 * i], d = c.work[2 + 2 * i];
+        c.work[1 + 2 * (int64_t)c.n_pages + s] = d;
+        c.refs[d] = c.refs[s];
+        c.refs[s] = 0;
+    }
+    if (tid == 0) {
+        c.work[0] = moves;
+        *n_live = n;
+    }
+}
+
+// Second launch: the tables' ids (the first `remap` workgroups) and the pages themselves. A moved
+// page's place is at n or above and its new one below, so no copy reads what another writes.
+__global__ __launch_bounds__(256) void k_kv4_compact_move(Kv4View c, const int32_t* __restrict__ n_live, int remap) {
+    if ((int)blockIdx.x >= remap) {
+        copy_pages(c, c.work + 1, c.work + 2, 2, c.work[0], (int)blockIdx.x - remap, (int)gridDim.x - remap);
+        return;
+    }
+    const int n = *n_live;
+    const int64_t entries = (int64_t)c.max_seqs * c.max_pages;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < entries; i += (int64_t)remap * 256) {
+        const int page = c.table[i];
+        if (page >= n && page < c.n_pages) c.table[i] = c.work[1 + 2 * (int64_t)c.n_pages + page];
+    }
+}
+
+int copy_grid(const Kv4View& c, int64_t n) {
+    const int64_t units = n * c.n_layers * ((c.page_bytes + kCopyChunk - 1) / kCopyChunk);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(units, 2048));
+}
+
+}  // namespace
+
+int64_t kv4_work_ints(int n_pages, int max_seqs, int max_pages) {
+    const int64_t extend = 1 + 2 * (int64_t)kMaxEntries + n_pages, compact = 1 + 3 * (int64_t)n_pages;
+    const int64_t fork = (int64_t)std::min(max_seqs, kMaxEntries) * ((int64_t)max_pages + 1);
+    return std::max(fork, std::max(extend, compact));
+}
+
+hipError_t launch_kv4_extend(const Kv4View& c, const int32_t* slots, const int32_t* counts, int n,
+                             int32_t* status, hipStream_t stream) {
+    hipLaunchKernelGGL(k_kv4_extend, dim3(1), dim3(kThreads), 0, stream, c, slots, counts, n, status);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(k_kv4_copy, dim3((unsigned)copy_grid(c, n)), dim3(256), 0, stream, c, c.work + 1, c.work + 2, 2,
+                       0, c.work);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv4_fork(const Kv4View& c, const int32_t* src, const int32_t* dst, int n, hipStream_t stream) {
+    hipLaunchKernelGGL(k_kv4_fork_read, dim3((unsigned)n), dim3(256), 0, stream, c, src, dst);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(k_kv4_fork_write, dim3((unsigned)n), dim3(256), 0, stream, c, src, dst);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv4_truncate(const Kv4View& c, const int32_t* slots, const int32_t* new_lens, int n,
+                               hipStream_t stream) {
+    hipLaunchKernelGGL(k_kv4_truncate, dim3((unsigned)n), dim3(256), 0, stream, c, slots, new_lens);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv4_compact(const Kv4View& c, int32_t* n_live, hipStream_t stream) {
+    hipLaunchKernelGGL(k_kv4_compact_plan, dim3(1), dim3(kThreads), 0, stream, c, n_live);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t entries = (int64_t)c.max_seqs * c.max_pages;
+    const int remap = (int)std::min<int64_t>(256, (entries + 255) / 256);
+    hipLaunchKernelGGL(k_kv4_compact_move, dim3((unsigned)(remap + copy_grid(c, c.n_pages))), dim3(256), 0, stream, c,
+                       n_live, remap);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv4_copy_pages(const Kv4View& c, const int32_t* src, const int32_t* dst, int n, hipStream_t stream) {
+    hipLaunchKernelGGL(k_kv4_copy, dim3((unsigned)copy_grid(c, n)), dim3(256), 0, stream, c, src, dst, 1, n,
+                       (const int32_t*)nullptr);
+    return hipGetLastError();
+}
+
+}  // namespace cllm_hip

@@ -317,6 +317,136 @@ int cllm_hip_attention_rope_dev(const float* q, float* k_cache, const float* v_c
                                 int n_head, int n_head_kv, int head_dim, float theta_base,
                                 float* out, void* stream);
 
+/* ---- the paged KV cache in 4 bits (stream-ordered) --------------------------------------
+ * The cache of a server of many sequences: pages of page_size positions that sequences share,
+ * keys and values in 4 bits (0.5625 bytes per element; the fp32 cache of cllm_hip_attention_dev
+ * takes 4). No reference counterpart: the reference keeps one sequence in fp32
+ * (src/core/engine.cpp:486-495).
+ *
+ * An element is d * (c - 8), c a 4-bit code, d the scale of a block of 32 elements along a
+ * head: an fp16 number of 8 significant bits. Storing a block of fp32 values with maximum mx and
+ * minimum mn takes a = max(mx, -mn) / 8 rounded to bfloat16, at most 8160, then rounded to fp16;
+ * d = a where -mn >= mx, else -a; c = 8 + x / d rounded to the nearest integer (ties to even),
+ * held to 0 .. 15; c = 8 where d is 0. A position whose key or value row of a head holds an
+ * infinity or a NaN gives NaN to every query of the head's group that sees it (it reads back as
+ * NaN keys and zero values).
+ *
+ * The cache is the caller's memory: pages ([n_layers][n_pages][cllm_hip_kv4_page_bytes] bytes,
+ * 16-byte aligned; they need no initialisation), and three int32 arrays that the calls below read
+ * and keep: table ([max_seqs][max_pages] page ids, -1: none), lens ([max_seqs] tokens held) and
+ * refs ([n_pages], how many table entries name the page; 0: free). An empty cache has every table
+ * entry -1 and the rest 0. work is scratch of cllm_hip_kv4_work_ints ints for extend, fork and
+ * compact. A slot (row of table) is a sequence; its pages are those its tokens need. The calls
+ * on one cache are ordered by their stream; on several streams the caller orders them. The calls
+ * allocate nothing and read nothing back, so all of them can be captured into graphs.
+ *
+ * Page ids outside [0, n_pages) in a table are no page: attention does not see their positions,
+ * store drops their rows, load gives 0. Slots outside [0, max_seqs) are empty sequences. */
+typedef struct {
+    void* pages;
+    int32_t* table;
+    int32_t* lens;
+    int32_t* refs;
+    int32_t* work;
+    int n_layers, n_pages;
+    int page_size;  /* positions of a page: a power of two, 32 to 1024 */
+    int n_head_kv;
+    int head_dim;   /* 64, 128 or 256 */
+    int max_seqs, max_pages;
+} cllm_hip_kv4_cache;
+
+/* Bytes of a page of one layer (0 for a shape that is not supported), ints of work. */
+size_t cllm_hip_kv4_page_bytes(int page_size, int n_head_kv, int head_dim);
+size_t cllm_hip_kv4_work_ints(int n_pages, int max_seqs, int max_pages);
+
+/* Adds counts[i] tokens to slot slots[i] (null: slot i), i < n <= 1024, with the pages they need:
+ * free ones, lowest id first, in the order of the entries. A partly filled last page that other
+ * slots hold too is replaced by a copy (all layers; copy on write): of the entries that share one,
+ * in order, each takes a copy (before its other pages) as long as another holder is left.
+ * *status (device): 0; the number of pages missing; or -1 for a slot out of range or named twice,
+ * a negative count, or more than max_pages pages. Unless it is 0, nothing has changed. */
+int cllm_hip_kv4_extend_dev(const cllm_hip_kv4_cache* cache, const int32_t* slots,
+                            const int32_t* counts, int n, int32_t* status, void* stream);
+
+/* Slot dst[i] becomes a copy of slot src[i], i < n <= min(max_seqs, 1024): the pages are shared
+ * and counted, not copied, and what dst[i] held before is released. All sources are read before any
+ * destination changes (a beam search's permutation; src[i] == dst[i] changes nothing). An entry
+ * with a slot out of range, or whose destination an earlier entry names, is ignored. */
+int cllm_hip_kv4_fork_dev(const cllm_hip_kv4_cache* cache, const int32_t* src, const int32_t* dst,
+                          int n, void* stream);
+
+/* Cuts slot slots[i] to min(lens, new_lens[i]) tokens and releases the pages past them; new_lens
+ * null, or 0, frees the sequence. Slots out of range, or named by an earlier entry, are ignored. */
+int cllm_hip_kv4_truncate_dev(const cllm_hip_kv4_cache* cache, const int32_t* slots,
+                              const int32_t* new_lens, int n, void* stream);
+
+/* Moves the pages in use to the ids below their number *n_live (device): those from n_live on, in
+ * ascending order, to the free ids below it, in ascending order. Tables and refs follow. */
+int cllm_hip_kv4_compact_dev(const cllm_hip_kv4_cache* cache, int32_t* n_live, void* stream);
+
+/* Copies page src[i] to page dst[i], i < n, in every layer; pairs with an id that is no page are
+ * ignored. No page may be the destination of two pairs, or of one and the source of another. */
+int cllm_hip_kv4_copy_pages_dev(const cllm_hip_kv4_cache* cache, const int32_t* src,
+                                const int32_t* dst, int n, void* stream);
+
+/* The batch of the three calls below: n_seqs sequences; sequence i is slot slots[i] (null: slot i)
+ * and has rows [q_start[i], q_start[i + 1]) of the n_rows rows, which are its last tokens: of a
+ * sequence with r rows and lens tokens, row t stands at position lens - r + t (extend first, then
+ * store). slots and q_start (n_seqs + 1 ints, ascending, within n_rows) are device arrays. Rows of
+ * no sequence are neither read nor written.
+ *
+ * Stores the fp32 rows k and v (n_rows x n_head_kv x head_dim) in layer `layer`. theta_base > 0:
+ * the keys turn by the NEOX rotation of cllm_hip_rope_neox2_dev at their positions first, and so do
+ * the query rows q (n_rows x n_head x head_dim, in place) if q is not null; theta_base = 0: none. A
+ * slot may appear once. Rows at negative positions are dropped (their q stays as it is). */
+int cllm_hip_kv4_store_dev(const cllm_hip_kv4_cache* cache, int layer, const float* k,
+                           const float* v, float* q, int n_head, float theta_base,
+                           const int32_t* slots, const int32_t* q_start, int n_seqs, int n_rows,
+                           void* stream);
+
+/* Reads the rows' keys and values back as fp32 (0 at negative positions). */
+int cllm_hip_kv4_load_dev(const cllm_hip_kv4_cache* cache, int layer, const int32_t* slots,
+                          const int32_t* q_start, int n_seqs, int n_rows, float* k, float* v,
+                          void* stream);
+
+/* Grouped-query attention (attention, src/core/engine.cpp:114-146) of the rows q (n_rows x n_head
+ * x head_dim) over the cache: row t of a sequence with r rows sees positions [0, lens - r + t];
+ * a row that sees none gives 0. n_head is any multiple of n_head_kv. max_rows and max_len bound the
+ * rows and the tokens of a sequence: rows past max_rows are not computed; a max_len that is too
+ * small costs time only, and one near the longest sequence is fastest. ws: 16-byte aligned device
+ * scratch of cllm_hip_kv4_attention_ws_bytes bytes for the same arguments (0: may be null), free
+ * again when the call has run. */
+size_t cllm_hip_kv4_attention_ws_bytes(const cllm_hip_kv4_cache* cache, int n_seqs, int n_rows,
+                                       int max_rows, int max_len, int n_head);
+int cllm_hip_kv4_attention_dev(const cllm_hip_kv4_cache* cache, int layer, const float* q,
+                               const int32_t* slots, const int32_t* q_start, int n_seqs,
+                               int n_rows, int max_rows, int max_len, int n_head, float* out,
+                               void* ws, size_t ws_bytes, void* stream);
+
+/* The kernel and launch plan of that call ("none" for an unsupported shape); for tests and
+ * benchmarks. */
+const char* cllm_hip_kv4_attention_plan(const cllm_hip_kv4_cache* cache, int n_seqs, int n_rows,
+                                        int max_rows, int max_len, int n_head);
+
+/* ---- log probabilities (stream-ordered) -------------------------------------------------
+ * Of n_rows rows of fp32 logits (row i at logits + i * row_stride, vocab of them), in natural
+ * logarithms, each output null if not wanted:
+ *   lse[i]       log sum_j exp(x_j)
+ *   logprobs[i]  x_t - lse of the given token t = tokens[i]; -inf for a t outside the vocabulary
+ *   ranks[i]     how many tokens stand ahead of t: larger logits, and equal ones with lower ids;
+ *                -1 for a t outside the vocabulary
+ *   entropy[i]   -sum_j p_j log p_j, p = exp(x - lse)
+ *   top_ids, top_logprobs [n_rows][top_k]: the top_k (at most 64) largest, equal ones by ids
+ * A logit of -inf has probability 0; a row of nothing else has lse and logprobs -inf and entropy 0.
+ * A row with a NaN or +inf has NaN (its order counts NaN below -inf). ws: 16-byte aligned device
+ * scratch of cllm_hip_logprobs_ws_bytes bytes, free again when the call has run. No reference
+ * counterpart. */
+size_t cllm_hip_logprobs_ws_bytes(int n_rows, int vocab, int top_k);
+int cllm_hip_logprobs_dev(const float* logits, int64_t row_stride, int n_rows, int vocab,
+                          const int32_t* tokens, int top_k, float* logprobs, int32_t* ranks,
+                          float* entropy, float* lse, int32_t* top_ids, float* top_logprobs,
+                          void* ws, size_t ws_bytes, void* stream);
+
 /* ---- GGUF files ------------------------------------------------------------------------ */
 
 /* A GGUF file mapped read-only, parsed like GgufLoader::load (src/core/gguf.cpp:122-275):
