@@ -1790,13 +1790,13 @@ static int kv4_attention_args(const char* who, const cllm_hip_kv4_cache* cache, 
     if (n_head <= 0 || n_head % c->n_kv != 0 || n_head > 65536)
         return set_err(CLLM_HIP_E_ARG, "%s: n_head must be a multiple of n_head_kv", who);
     if (n_seqs == 0 || n_rows == 0 || max_rows == 0) {
-        *p = Kv4AttnPlan{0, 0, 1, 1};
+        *p = Kv4AttnPlan{2, 16, 0, 0};
         return CLLM_HIP_OK;
     }
     max_rows = std::min(max_rows, n_rows);
     max_len = std::min(max_len, c->max_pages << c->page_shift);
     *p = kv4_attention_plan(*c, n_seqs, max_rows, max_len, n_head);
-    if (!kv4_attention_fits(*p, *c, n_seqs)) return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
+    if (p->units > INT32_MAX) return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
     return CLLM_HIP_OK;
 }
 
@@ -1805,7 +1805,7 @@ size_t cllm_hip_kv4_attention_ws_bytes(const cllm_hip_kv4_cache* cache, int n_se
     Kv4View c;
     Kv4AttnPlan p;
     if (kv4_attention_args("kv4_attention", cache, n_seqs, n_rows, max_rows, max_len, n_head, &c, &p)) return 0;
-    return kv4_attention_ws_bytes(p, n_rows, n_head, c.hd);
+    return p.units == 0 ? 0 : kv4_attention_ws_bytes(p, c.hd);
 }
 
 const char* cllm_hip_kv4_attention_plan(const cllm_hip_kv4_cache* cache, int n_seqs, int n_rows, int max_rows,
@@ -1814,10 +1814,11 @@ const char* cllm_hip_kv4_attention_plan(const cllm_hip_kv4_cache* cache, int n_s
     Kv4View c;
     Kv4AttnPlan p;
     if (kv4_attention_args("kv4_attention", cache, n_seqs, n_rows, max_rows, max_len, n_head, &c, &p) ||
-        p.col_tiles == 0)
+        p.units == 0)
         return "none";
-    snprintf(buf, sizeof buf, "%s<%d> columns=%d chunk=%d splits=%d", "k_kv4_attention", c.hd, p.col_tiles,
-             p.chunk_tiles * 32, p.splits);
+    static const char* const modes[] = {"stream", "aligned", "whole"};
+    snprintf(buf, sizeof buf, "k_kv4_attention<%d> %s units=%lld workgroups=%lld", c.hd, modes[p.mode],
+             (long long)p.units, (long long)p.grid);
     return buf;
 }
 
@@ -1828,11 +1829,11 @@ int cllm_hip_kv4_attention_dev(const cllm_hip_kv4_cache* cache, int layer, const
     Kv4AttnPlan p;
     int rc = kv4_attention_args("kv4_attention", cache, n_seqs, n_rows, max_rows, max_len, n_head, &c, &p);
     if (rc || (rc = kv4_batch("kv4_attention", c, layer, slots, q_start, n_seqs, n_rows))) return rc;
-    if (p.col_tiles == 0) return CLLM_HIP_OK;
+    if (p.units == 0) return CLLM_HIP_OK;
     if (!q || !out) return set_err(CLLM_HIP_E_ARG, "kv4_attention: null pointer");
     if (!aligned16(q) || !aligned16(out) || !aligned16(ws))
         return set_err(CLLM_HIP_E_ARG, "kv4_attention: misaligned device pointer");
-    const size_t need = kv4_attention_ws_bytes(p, n_rows, n_head, c.hd);
+    const size_t need = kv4_attention_ws_bytes(p, c.hd);
     if (need > 0 && (!ws || ws_bytes < need))
         return set_err(CLLM_HIP_E_ARG, "kv4_attention: workspace of %zu bytes, %zu needed", ws ? ws_bytes : (size_t)0, need);
     DeviceState* st;

@@ -30,17 +30,27 @@ __device__ __forceinline__ f32x4 mfma(const h8& a, const h8& b, const f32x4& c) 
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Eight codes of a dword as exact fp16 d * (c - 8): pairs 1024 + c, minus 1032, times d. d[r]
-// scales codes 2 r and 2 r + 1. Every step is exact (kv4.h).
-__device__ __forceinline__ h8 dequant8(uint32_t w, const h2 (&d)[4]) {
-    const h2 off = {(_Float16)-1032.0f, (_Float16)-1032.0f};
-    h2 p[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const uint32_t m = ((w >> (4 * r)) & 0x000F000Fu) | 0x64006400u;
-        p[r] = (__builtin_bit_cast(h2, m) + off) * d[r];
+// Eight codes of a dword as exact fp16 d * (c - 8): the pair in bits 0-3 of the halves becomes
+// 1024 + c, that in bits 4-7 64 + c (no shift), less 1032 or 72, times d. d[r] scales codes 2 r and
+// 2 r + 1. Every step is exact (kv4.h). 13 VALU operations; an instruction reads one scalar
+// register or literal, so the or's constants lie in vector registers (Magic): v_and_or_b32.
+struct Magic {
+    uint32_t m1024, m64;
+    float minus1;  // (as a literal the compiler takes the product away, and v_fma_mix with it)
+    __device__ __forceinline__ Magic() {
+        asm("v_mov_b32 %0, 0x64006400" : "=v"(m1024));
+        asm("v_mov_b32 %0, 0x54005400" : "=v"(m64));
+        asm("v_mov_b32 %0, -1.0" : "=v"(minus1));
     }
-    return h8{p[0].x, p[0].y, p[1].x, p[1].y, p[2].x, p[2].y, p[3].x, p[3].y};
+};
+__device__ __forceinline__ h8 dequant8(uint32_t w, const h2 (&d)[4], const Magic& mg) {
+    const h2 off0 = {(_Float16)-1032.0f, (_Float16)-1032.0f}, off1 = {(_Float16)-72.0f, (_Float16)-72.0f};
+    const uint32_t w8 = w >> 8;
+    const h2 a = (__builtin_bit_cast(h2, (w & 0x000F000Fu) | mg.m1024) + off0) * d[0];
+    const h2 b = (__builtin_bit_cast(h2, (w & 0x00F000F0u) | mg.m64) + off1) * d[1];
+    const h2 e = (__builtin_bit_cast(h2, (w8 & 0x000F000Fu) | mg.m1024) + off0) * d[2];
+    const h2 f = (__builtin_bit_cast(h2, (w8 & 0x00F000F0u) | mg.m64) + off1) * d[3];
+    return h8{a.x, a.y, b.x, b.y, e.x, e.y, f.x, f.y};
 }
 
 __device__ __forceinline__ h2 pkrtz(float a, float b) {
@@ -48,92 +58,111 @@ __device__ __forceinline__ h2 pkrtz(float a, float b) {
 }
 
 // Eight fp32 values as fp16 hi + lo. hi is rounded towards zero, so the remainder is exact.
-__device__ __forceinline__ void split8(const float (&x)[8], h8& hi, h8& lo) {
+__device__ __forceinline__ void split8(const float (&x)[8], h8& hi, h8& lo, const Magic& mg) {
     h2 a[4], b[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
         a[r] = pkrtz(x[2 * r], x[2 * r + 1]);
-        b[r] = pkrtz(x[2 * r] - (float)a[r].x, x[2 * r + 1] - (float)a[r].y);
+        b[r] = pkrtz(__builtin_fmaf((float)a[r].x, mg.minus1, x[2 * r]), __builtin_fmaf((float)a[r].y, mg.minus1, x[2 * r + 1]));
     }
     hi = h8{a[0].x, a[0].y, a[1].x, a[1].y, a[2].x, a[2].y, a[3].x, a[3].y};
     lo = h8{b[0].x, b[0].y, b[1].x, b[1].y, b[2].x, b[2].y, b[3].x, b[3].y};
 }
 
+// Over the four 16-lane rows of the wave (lanes of one column), in every lane.
 __device__ __forceinline__ float max_over_g(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    v = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
 }
 __device__ __forceinline__ float sum_over_g(float v) {
     v += __shfl_xor(v, 16, 64);
     return v + __shfl_xor(v, 32, 64);
 }
 
-// What lane 16 g + n holds of a tile.
-template <int HD>
-struct TileRegs {
-    static constexpr int KW = HD / 32;            // key dwords of either half
-    static constexpr int NT = HD / 16, NB = HD / 32;
-    uint32_t k[2][KW];
-    uint32_t ks[HD == 256 ? 2 : 1];               // the lane's blocks: scales of both halves
-    uint32_t v[NT];
-    u32x4 vs[NB];
+// s_waitcnt vmcnt(N), and lgkmcnt(0) (gfx9 encoding, the other counters at max); no memory access
+// moves across either.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | 0x0F70);
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);
+    asm volatile("" ::: "memory");
+}
 
-    __device__ __forceinline__ void load_k(const uint8_t* tile, int lane) {
-        constexpr int W = KW < 4 ? KW : 4, C = KW / W;
+// A tile loaded straight into LDS (36 * HD bytes at `slot`) by one wave: 16 bytes a lane, the rest
+// 4 bytes a lane. The loads are the wave's own business: the compiler, which would wait for all of
+// them before any LDS read, does not see them, and wait_loads orders the reads.
+template <int HD>
+struct TileLoads {
+    static constexpr int BYTES = 36 * HD, WIDE = BYTES / 1024, NARROW = (BYTES - 1024 * WIDE) / 256;
+    static constexpr int COUNT = WIDE + NARROW;
+    static_assert(WIDE * 1024 + NARROW * 256 == BYTES, "a tile is whole loads");
+    static __device__ __forceinline__ void issue(const uint8_t* tile, const uint8_t* slot, int lane) {
+        const uint32_t m0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)slot;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int i = 0; i < WIDE; ++i)
+            asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+                         : : "v"(tile + 1024 * i + 16 * lane), "s"(m0 + 1024 * i) : "memory", "m0");
 #pragma unroll
-            for (int c = 0; c < C; ++c) {
-                const uint8_t* p = tile + ((t * C + c) * 64 + lane) * (4 * W);
-                if constexpr (W == 4) {
-                    const u32x4 x = *(const u32x4*)p;
-                    k[t][4 * c] = x.x; k[t][4 * c + 1] = x.y; k[t][4 * c + 2] = x.z; k[t][4 * c + 3] = x.w;
-                } else {
-                    const u32x2 x = *(const u32x2*)p;
-                    k[t][0] = x.x; k[t][1] = x.y;
+        for (int i = 0; i < NARROW; ++i)
+            asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
+                         : : "v"(tile + 1024 * WIDE + 256 * i + 4 * lane), "s"(m0 + 1024 * WIDE + 256 * i)
+                         : "memory", "m0");
+    }
+};
+
+// What lane 16 g + n reads of a tile in LDS: key fragments (rows are positions 16 t + n) and value
+// fragments (rows are elements 16 dt + n), as exact fp16.
+template <int HD>
+struct TileView {
+    static constexpr int KW = HD / 32, W = KW < 4 ? KW : 4, C = KW / W;
+    const uint8_t* p;
+    int lane;
+
+    // Key fragments c W .. c W + W - 1: the lane's elements there lie in one block.
+    __device__ __forceinline__ void keys(int t, int c, h8 (&k)[W], const Magic& mg) const {
+        const int g = lane >> 4, n = lane & 15;
+        const uint32_t b = ((const uint32_t*)(p + 32 * HD))[(HD == 64 ? g >> 1 : HD == 128 ? g : 2 * g + c) * 16 + n];
+        const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, b, t ? 0x03020302u : 0x01000100u));
+        const h2 d4[4] = {d, d, d, d};
+        const uint8_t* w = p + ((t * C + c) * 64 + lane) * (4 * W);
+        if constexpr (W == 4) {
+            const u32x4 x = *(const u32x4*)w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = dequant8(x[j], d4, mg);
+        } else {
+            const u32x2 x = *(const u32x2*)w;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) k[j] = dequant8(x[j], d4, mg);
+        }
+    }
+    // Value fragments 4 c .. 4 c + 3. EDGE: positions from `limit` on (counted from the tile's start)
+    // have bytes that no store has written, whose scales may be NaN.
+    template <bool EDGE>
+    __device__ __forceinline__ void values(int c, h8 (&v)[4], int limit, const Magic& mg) const {
+        const u32x4 x = *(const u32x4*)(p + 16 * HD + (c * 64 + lane) * 16);
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            u32x4 s = *(const u32x4*)(p + 34 * HD + ((2 * c + b) * 4 + (lane >> 4)) * 16);
+            if constexpr (EDGE) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int at = 16 * (r >> 1) + 4 * (lane >> 4) + 2 * (r & 1);
+                    s[r] &= (at < limit ? 0x0000FFFFu : 0u) | (at + 1 < limit ? 0xFFFF0000u : 0u);
                 }
             }
-        const uint32_t* s = (const uint32_t*)(tile + 32 * HD);
-        const int g = lane >> 4, n = lane & 15;
-        if constexpr (HD == 64) ks[0] = s[(g >> 1) * 16 + n];
-        if constexpr (HD == 128) ks[0] = s[g * 16 + n];
-        if constexpr (HD == 256) {
-            ks[0] = s[(2 * g) * 16 + n];
-            ks[1] = s[(2 * g + 1) * 16 + n];
+            const h2 d4[4] = {__builtin_bit_cast(h2, (uint32_t)s.x), __builtin_bit_cast(h2, (uint32_t)s.y),
+                              __builtin_bit_cast(h2, (uint32_t)s.z), __builtin_bit_cast(h2, (uint32_t)s.w)};
+            v[2 * b] = dequant8(x[2 * b], d4, mg);
+            v[2 * b + 1] = dequant8(x[2 * b + 1], d4, mg);
         }
-    }
-    __device__ __forceinline__ void load_v(const uint8_t* tile, int lane) {
-#pragma unroll
-        for (int c = 0; c < NT / 4; ++c) {
-            const u32x4 x = *(const u32x4*)(tile + 16 * HD + (c * 64 + lane) * 16);
-            v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = x.z; v[4 * c + 3] = x.w;
-        }
-#pragma unroll
-        for (int b = 0; b < NB; ++b) vs[b] = *(const u32x4*)(tile + 34 * HD + (b * 4 + (lane >> 4)) * 16);
-    }
-    // Value scales of positions past `limit` (counted from the tile's start): bytes that no store
-    // has written, which may be NaN.
-    __device__ __forceinline__ void mask_v(int g, int limit) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int p = 16 * (r >> 1) + 4 * g + 2 * (r & 1);
-            const uint32_t m = (p < limit ? 0x0000FFFFu : 0u) | (p + 1 < limit ? 0xFFFF0000u : 0u);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) vs[b][r] &= m;
-        }
-    }
-    __device__ __forceinline__ h8 key(int t, int j) const {
-        const uint32_t s = HD == 256 && j >= KW / 2 ? ks[HD == 256 ? 1 : 0] : ks[0];
-        const uint32_t d = __builtin_amdgcn_perm(s, s, t ? 0x03020302u : 0x01000100u);
-        const h2 dd = __builtin_bit_cast(h2, d);
-        const h2 d4[4] = {dd, dd, dd, dd};
-        return dequant8(k[t][j], d4);
-    }
-    __device__ __forceinline__ h8 value(int dt) const {
-        const u32x4 s = vs[dt / 2];
-        const h2 d4[4] = {__builtin_bit_cast(h2, (uint32_t)s.x), __builtin_bit_cast(h2, (uint32_t)s.y),
-                          __builtin_bit_cast(h2, (uint32_t)s.z), __builtin_bit_cast(h2, (uint32_t)s.w)};
-        return dequant8(v[dt], d4);
     }
 };
 
@@ -147,7 +176,7 @@ struct Queries {
 
     // q row scaled by a power of two so that its largest element lies in [2^14, 2^15): hi and lo
     // then keep 22 significant bits of every element that counts.
-    __device__ __forceinline__ void load(const float* row, bool valid, int g) {
+    __device__ __forceinline__ void load(const float* row, bool valid, int g, const Magic& mg) {
         float x[KW][8];
         float m = 0.0f;
 #pragma unroll
@@ -176,249 +205,401 @@ struct Queries {
         for (int j = 0; j < KW; ++j) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[j][i] = ldexpf(x[j][i], sh);
-            split8(x[j], hi[j], lo[j]);
+            split8(x[j], hi[j], lo[j], mg);
         }
     }
 };
 
-// The place of one workgroup's work.
-struct Place {
+// ---------------------------------------------------------------------------- the work's split
+//
+// A unit is a column tile of a KV head of a sequence: n tiles of positions (one at least, so that
+// rows that see nothing are written too). Only the device knows the lengths, so the workgroups find
+// their shares themselves, from sums over the sequences that each wave forms 64 at a time:
+//   few units (up to kAlignedUnits): unit u has ceil(n_u / Q) splits of equal size, one workgroup
+//   each, Q chosen so that all of them fit the grid; a workgroup has one unit, and the smallest
+//   batches (n_u <= kMinShare) need no join;
+//   many units: the units' tiles lie end to end and workgroup w takes tiles [w Q, (w + 1) Q), so
+//   the work is even whatever the lengths are, for a few restarts where a share crosses units.
+// A unit split over workgroups leaves partial results in slots (aligned: the workgroup; else unit +
+// workgroup, which grows along the staircase of pairs), and a second launch joins them.
+constexpr int kGrid = 512;          // two workgroups on each of 256 CUs
+constexpr int kAlignedUnits = 256;
+constexpr int kMinShare = 8;        // tiles
+
+struct SeqWork {
     Kv4Seq s;
-    int h, c0;          // KV head, first column
-    int n_cols;         // columns of the sequence and head: rows * G
-    int kv_end;         // positions the tile's last row sees
-    int vis_min;        // positions its first row sees
+    int rows;           // computed: rows past max_rows have no column tile
+    int units, tiles;   // units of the sequence, tiles of each
 };
-__device__ __forceinline__ Place place_of(const Kv4View& c, const int32_t* slots, const int32_t* q_start,
-                                          int seq, int h, int ct, int cols, int G, int n_rows, int max_rows) {
-    Place p;
-    p.s = kv4_seq(c, slots, q_start, seq, n_rows);
-    p.h = h;
-    p.c0 = ct * cols;
-    const int rows = min(p.s.rows, max_rows);  // rows past max_rows have no column tile
-    p.n_cols = rows * G;
-    const int t1 = min(rows - 1, (p.c0 + cols - 1) / G), t0 = p.c0 / G;
-    p.kv_end = max(0, p.s.len - p.s.rows + t1 + 1);
-    p.vis_min = p.s.len - p.s.rows + t0 + 1;
-    return p;
+struct AttnArgs {
+    const int32_t* slots;
+    const int32_t* q_start;
+    int n_seqs, n_rows, max_rows, n_head, G, cols;
+};
+__device__ __forceinline__ SeqWork seq_work(const Kv4View& c, const AttnArgs& a, int i) {
+    SeqWork w;
+    if (i >= a.n_seqs) {
+        w.s = Kv4Seq{0, 0, 0, 0};
+        w.rows = w.units = w.tiles = 0;
+        return w;
+    }
+    w.s = kv4_seq(c, a.slots, a.q_start, i, a.n_rows);
+    w.rows = min(w.s.rows, a.max_rows);
+    w.units = c.n_kv * ((w.rows * a.G + a.cols - 1) / a.cols);
+    w.tiles = max(1, (w.s.len - w.s.rows + w.rows + kTile - 1) / kTile);
+    return w;
+}
+__device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {  // inclusive
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t y = __shfl_up((long long)v, d, 64);
+        if (lane >= d) v += y;
+    }
+    return v;
 }
 
-// Tile tl of the place's sequence and head, null if it has no page.
-__device__ __forceinline__ const uint8_t* tile_of(const Kv4View& c, int layer, const Place& p, int tl) {
-    const int sub = c.page_shift - 5;
-    const int page = c.table[(int64_t)p.s.slot * c.max_pages + (tl >> sub)];
-    if ((unsigned)page >= (unsigned)c.n_pages) return nullptr;
-    return c.pages + ((int64_t)layer * c.n_pages + page) * c.page_bytes +
-           (((int64_t)p.h << sub) + (tl & ((1 << sub) - 1))) * (36 * c.hd);
+// How the batch is shared out: items are workgroups (aligned) or tiles.
+enum { kStream, kAligned, kWhole };  // kWhole: aligned, every unit one workgroup's (no join follows)
+struct Shares {
+    bool aligned;
+    int64_t q;      // tiles of a share
+    int64_t items;
+    __device__ __forceinline__ int64_t of(const SeqWork& w) const {
+        return (int64_t)w.units * (aligned ? (w.tiles + q - 1) / q : (int64_t)w.tiles);
+    }
+};
+__device__ __forceinline__ Shares shares_of(const Kv4View& c, const AttnArgs& a, int mode, int grid, int lane) {
+    int64_t units = 0, tiles = 0;
+    for (int i0 = 0; i0 < a.n_seqs; i0 += 64) {
+        const SeqWork w = seq_work(c, a, i0 + lane);
+        units += w.units;
+        tiles += (int64_t)w.units * w.tiles;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        units += __shfl_xor((long long)units, d, 64);
+        tiles += __shfl_xor((long long)tiles, d, 64);
+    }
+    Shares sh;
+    sh.aligned = mode != kStream;
+    sh.items = tiles;
+    // sum of ceil(n / Q) <= tiles / Q + units: within the grid (of 2 units at least)
+    const int64_t wgs = sh.aligned ? max((int64_t)1, grid - units) : grid;
+    sh.q = mode == kWhole ? INT32_MAX : max((int64_t)kMinShare, (tiles + wgs - 1) / wgs);
+    return sh;
 }
 
-// Partial results of split z for (row, head): unnormalised outputs part[((row * n_head + head) *
-// splits + z) * HD], and the running maximum (log2 units) and sum in ml.
+// The sequence that item (or unit, by_units) f falls to, f's place among the sequence's own, and what
+// the sequences before it have.
+struct Found {
+    SeqWork w;
+    int64_t rest, items_before, units_before;
+    bool ok;
+};
+__device__ __forceinline__ Found find_item(const Kv4View& c, const AttnArgs& a, const Shares& sh, int64_t f,
+                                           bool by_units, int lane) {
+    int64_t items = 0, units = 0;
+    Found r;
+    r.ok = false;
+    for (int i0 = 0; i0 < a.n_seqs; i0 += 64) {
+        const SeqWork w = seq_work(c, a, i0 + lane);
+        const int64_t mine = sh.of(w), incl = wave_scan(mine, lane), uincl = wave_scan((int64_t)w.units, lane);
+        const uint64_t past = __ballot((by_units ? units + uincl : items + incl) > f);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            r.w.s.slot = __builtin_amdgcn_readlane(w.s.slot, at);
+            r.w.s.r0 = __builtin_amdgcn_readlane(w.s.r0, at);
+            r.w.s.rows = __builtin_amdgcn_readlane(w.s.rows, at);
+            r.w.s.len = __builtin_amdgcn_readlane(w.s.len, at);
+            r.w.rows = __builtin_amdgcn_readlane(w.rows, at);
+            r.w.units = __builtin_amdgcn_readlane(w.units, at);
+            r.w.tiles = __builtin_amdgcn_readlane(w.tiles, at);
+            r.items_before = items + __shfl((long long)(incl - mine), at, 64);
+            r.units_before = units + __shfl((long long)(uincl - w.units), at, 64);
+            r.rest = f - (by_units ? r.units_before : r.items_before);
+            r.ok = true;
+            return r;
+        }
+        items += __shfl((long long)incl, 63, 64);
+        units += __shfl((long long)uincl, 63, 64);
+    }
+    return r;
+}
+
+// Partial results of slot i and column n: unnormalised outputs o[(i * cols + n) * HD], the running
+// maximum (log2 units) and sum ml[(i * cols + n) * 2].
 struct Parts {
     float* o;
     float* ml;
-    int splits;
 };
 
-// grid: splits x column tiles x KV heads x sequences, one workgroup of four waves each. The waves
-// walk the split's tiles alone (tile w, w + 4, ...), each with its own running maximum, and meet
-// once at the end. A wave loads the keys of its next tile when the scores have been formed and the
-// values when they have been used, so about 4.6 KB (HD 128) are in flight per wave.
+// One workgroup of four waves per share. The waves walk a unit's tiles alone (tile w, w + 4, ...),
+// each with its own running maximum, tiles coming through a ring of STAGES slots in LDS that the
+// wave fills itself, and meet once at the unit's end.
+//
+// What bounds it: VALU work, about 310 operations per tile and wave for dequantization (208) and the
+// softmax of 16 columns, beside the read of the cache.
 template <int HD>
-__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void k_kv4_attention(Kv4View c, int layer, const float* __restrict__ q,
-                                                          const int32_t* __restrict__ slots,
-                                                          const int32_t* __restrict__ q_start, int n_seqs,
-                                                          int n_rows, int max_rows, int n_head, int col_tiles,
-                                                          int chunk_tiles, Parts parts, float* __restrict__ out) {
-    constexpr int NT = HD / 16, KW = HD / 32;
-    const int G = n_head / c.n_kv;
-    int b = blockIdx.x;
-    const int sp = b % parts.splits;
-    b /= parts.splits;
-    const int ct = b % col_tiles;
-    b /= col_tiles;
-    const int h = b % c.n_kv;
-    const Place pl = place_of(c, slots, q_start, b / c.n_kv, h, ct, 16, G, n_rows, max_rows);
-    if (pl.c0 >= pl.n_cols) return;
-    const int tiles = (pl.kv_end + kTile - 1) / kTile;
-    const int n_splits = min(parts.splits, max(1, (tiles + chunk_tiles - 1) / chunk_tiles));
-    if (sp >= n_splits) return;
-    const int t_begin = sp * chunk_tiles, t_end = sp == n_splits - 1 ? tiles : t_begin + chunk_tiles;
+struct AttnLds {
+    static constexpr int STAGES = HD == 64 ? 4 : HD == 128 ? 4 : 2;
+    static constexpr int RING = STAGES * 36 * HD;
+    union {
+        uint8_t ring[4][RING];
+        f32x4 o[4][16][HD / 4 + 1];
+    };
+    float m[4][16], l[4][16];
+};
 
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, const float* __restrict__ q,
+                                                          AttnArgs a, int mode, Parts parts,
+                                                          float* __restrict__ out) {
+    constexpr int NT = HD / 16, W = TileView<HD>::W, STAGES = AttnLds<HD>::STAGES, NL = TileLoads<HD>::COUNT;
+    extern __shared__ __align__(16) uint8_t lds_bytes[];
+    AttnLds<HD>& lds = *(AttnLds<HD>*)lds_bytes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
-    const int col = pl.c0 + n;
-    const bool valid = col < pl.n_cols;
-    const int row = col / G, head = h * G + (col - row * G);
-    const int64_t qrow = (int64_t)(pl.s.r0 + row) * n_head + head;
-    const int vis = valid ? pl.s.len - pl.s.rows + row + 1 : 0;
-
-    Queries<HD> qs;
-    qs.load(q + qrow * HD, valid, g);
-
-    f32x4 acc[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = kNegInf, l = 0.0f;
-
-    TileRegs<HD> r;
-    int tl = t_begin + wave;
-    const uint8_t* tile = nullptr;
-    if (tl < t_end) {
-        tile = tile_of(c, layer, pl, tl);
-        if (tile) {
-            r.load_k(tile, lane);
-            r.load_v(tile, lane);
-        }
+    const Magic mg;
+    const Shares sh = shares_of(c, a, mode, gridDim.x, lane);
+    int64_t f = blockIdx.x, f_end = f + 1;  // items of this workgroup
+    if (!sh.aligned) {
+        f = blockIdx.x * sh.q;
+        f_end = min(f + sh.q, sh.items);
     }
-    while (tl < t_end) {
-        const int next = tl + 4;
-        const uint8_t* tile_next = next < t_end ? tile_of(c, layer, pl, next) : nullptr;
-        if (tile) {
-            f32x4 s[2];
+    const int sub = c.page_shift - 5;
+    const uint8_t* const layer_pages = c.pages + (int64_t)layer * c.n_pages * c.page_bytes;
+
+    while (f < f_end) {
+        const Found u = find_item(c, a, sh, f, false, lane);
+        if (!u.ok) return;
+        const SeqWork w = u.w;
+        // unit of the sequence, its tiles [t_begin, t_end) of this workgroup, whether it is split
+        int unit, t_begin, t_end;
+        bool split;
+        if (sh.aligned) {
+            const int n_split = (int)((w.tiles + sh.q - 1) / sh.q);
+            unit = (int)(u.rest / n_split);
+            const int z = (int)(u.rest - (int64_t)unit * n_split);
+            t_begin = (int)((int64_t)w.tiles * z / n_split);
+            t_end = (int)((int64_t)w.tiles * (z + 1) / n_split);
+            split = n_split > 1;
+            f = f_end;
+        } else {
+            unit = (int)(u.rest / w.tiles);
+            t_begin = (int)(u.rest - (int64_t)unit * w.tiles);
+            t_end = (int)min((int64_t)w.tiles, t_begin + (f_end - f));
+            split = t_begin > 0 || t_end < w.tiles;
+            f += t_end - t_begin;
+        }
+        unit = __builtin_amdgcn_readfirstlane(unit);
+        t_begin = __builtin_amdgcn_readfirstlane(t_begin);
+        t_end = __builtin_amdgcn_readfirstlane(t_end);
+        const int h = unit % c.n_kv, c0 = unit / c.n_kv * 16, n_cols = w.rows * a.G;
+        const int col = c0 + n;
+        const bool valid = col < n_cols;
+        const int row = col / a.G, head = h * a.G + (col - row * a.G);
+        const int vis = valid ? w.s.len - w.s.rows + row + 1 : 0;       // positions the column sees
+        const int vis_min = w.s.len - w.s.rows + c0 / a.G + 1;          // and the tile's first row
+        // the column tile's last row sees no tile from here on
+        const int last_row = min(w.rows - 1, (c0 + 15) / a.G);
+        t_end = min(t_end, max(t_begin, (max(0, w.s.len - w.s.rows + last_row + 1) + kTile - 1) / kTile));
+
+        // The wave's tiles first, first + 4, ...: a lane holds the page id of every 64th. A tile
+        // without a page loads the first bytes of page 0 instead, and all of it is masked: holes
+        // keeps a bit for each tile in the ring, the one in turn lowest.
+        const int first = t_begin + wave;
+        const int count = first < t_end ? (t_end - first + 3) / 4 : 0;
+        const int32_t* table = c.table + (int64_t)w.s.slot * c.max_pages;
+        int ids = -1;
+        uint32_t holes = 0;
+        const auto issue = [&](int i, int ahead) {
+            if ((i & 63) == 0) {
+                const int tl = first + 4 * (i + lane);
+                ids = tl < t_end ? table[tl >> sub] : -1;
+            }
+            const int tl = first + 4 * i, page = __builtin_amdgcn_readlane(ids, i & 63);
+            const bool none = (unsigned)page >= (unsigned)c.n_pages;
+            const uint8_t* p = layer_pages;
+            if (!none) p += page * c.page_bytes + (((int64_t)h << sub) + (tl & ((1 << sub) - 1))) * (36 * HD);
+            holes |= (none ? 1u : 0u) << ahead;
+            TileLoads<HD>::issue(p, lds.ring[wave] + (i % STAGES) * (36 * HD), lane);
+        };
+        for (int i = 0; i < min(count, STAGES - 1); ++i) issue(i, i);
+
+        Queries<HD> qs;
+        qs.load(q + ((int64_t)(w.s.r0 + row) * a.n_head + head) * HD, valid, g, mg);
+        f32x4 acc[NT];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                s[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = kNegInf, l = 0.0f;
+
+        // EDGE: the tile ends past what some column sees, or past the sequence, or has no page
+        const auto step = [&]<bool EDGE>(const TileView<HD>& tv, int p0, int len) {
+            f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-                for (int j = 0; j < KW; ++j) {
-                    const h8 k = r.key(t, j);
-                    s[t] = mfma(k, qs.hi[j], s[t]);
-                    s[t] = mfma(k, qs.lo[j], s[t]);
+            for (int kc = 0; kc < TileView<HD>::C; ++kc) {
+                h8 k[2][W];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) tv.keys(t, kc, k[t], mg);
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) s[t] = mfma(k[t][j], qs.hi[kc * W + j], s[t]);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) s[t] = mfma(k[t][j], qs.lo[kc * W + j], s[t]);
                 }
             }
-            if (tile_next) r.load_k(tile_next, lane);
-            const int p0 = tl * kTile;
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3] * qs.sc;
-            if (p0 + kTile > pl.vis_min) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (p0 + 16 * (e >> 2) + 4 * g + (e & 3) >= vis) x[e] = kNegInf;
-                if (p0 + kTile > pl.s.len) r.mask_v(g, pl.s.len - p0);
+            for (int e = 0; e < 8; ++e) {
+                x[e] = s[e >> 2][e & 3];
+                if (EDGE && p0 + 16 * (e >> 2) + 4 * g + (e & 3) >= min(vis, len)) x[e] = kNegInf;
             }
             float mx = x[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
-            mx = max_over_g(mx);
+            mx = max_over_g(mx) * qs.sc;
             if (__any(mx > m)) {
                 const float m_new = fmaxf(m, mx);
-                const float a = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+                const float r = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
                 m = m_new;
-                l *= a;
+                l *= r;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) acc[i] *= a;
+                for (int i = 0; i < NT; ++i) acc[i] *= r;
             }
-            // weights times 2^15: as fp16 pairs they keep 22 bits down to 2^-29 of the largest
-            const float mm = (m == kNegInf ? 0.0f : m) - 15.0f;
+            // weights times 2^15: as fp16 pairs they keep 20 bits down to 2^-19 of the largest
+            const float mm = 15.0f - (m == kNegInf ? 0.0f : m);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(x[e] - mm);
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], qs.sc, mm));
                 l += x[e];
             }
             h8 hi, lo;
-            split8(x, hi, lo);
+            split8(x, hi, lo, mg);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const h8 v = r.value(i);
-                acc[i] = mfma(v, hi, acc[i]);
-                acc[i] = mfma(v, lo, acc[i]);
+            for (int cc = 0; cc < NT / 4; ++cc) {
+                h8 v[4];
+                tv.template values<EDGE>(cc, v, len - p0, mg);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    acc[4 * cc + i] = mfma(v[i], hi, acc[4 * cc + i]);
+                    acc[4 * cc + i] = mfma(v[i], lo, acc[4 * cc + i]);
+                }
             }
-            if (tile_next) r.load_v(tile_next, lane);
-        } else if (tile_next) {
-            r.load_k(tile_next, lane);
-            r.load_v(tile_next, lane);
+        };
+        for (int i = 0; i < count; ++i) {
+            if (i + STAGES - 1 < count) {
+                wait_lds();  // the reads of the slot's last tile have returned
+                issue(i + STAGES - 1, STAGES - 1);
+                wait_loads<(STAGES - 1) * NL>();
+            } else {
+                wait_loads<0>();
+            }
+            const bool hole = holes & 1u;
+            holes >>= 1;
+            const int p0 = (first + 4 * i) * kTile;
+            const TileView<HD> tv = {lds.ring[wave] + (i % STAGES) * (36 * HD), lane};
+            if (hole || p0 + kTile > vis_min || p0 + kTile > w.s.len)
+                step.template operator()<true>(tv, p0, hole ? 0 : w.s.len);
+            else
+                step.template operator()<false>(tv, p0, w.s.len);
         }
-        tile = tile_next;
-        tl = next;
-    }
-    l = sum_over_g(l);
+        l = sum_over_g(l);
 
-    // the four waves' results meet: wave w's outputs of column n, elements 16 i + 4 g .. + 3
-    __shared__ float sm[4][16], sl[4][16];
-    __shared__ f32x4 so[4][16][HD / 4 + 1];
-    if (g == 0) {
-        sm[wave][n] = m;
-        sl[wave][n] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) so[wave][n][4 * i + g] = acc[i];
-    __syncthreads();
-    for (int i = threadIdx.x; i < 16 * (HD / 4); i += 256) {
-        const int cn = i / (HD / 4), d4 = i % (HD / 4);
-        const int cc = pl.c0 + cn;
-        if (cc >= pl.n_cols) continue;
-        float mm = sm[0][cn];
-#pragma unroll
-        for (int w = 1; w < 4; ++w) mm = fmaxf(mm, sm[w][cn]);
-        float ls = 0.0f;
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (mm != kNegInf) {
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float a = __builtin_amdgcn_exp2f(sm[w][cn] - mm);
-                ls += sl[w][cn] * a;
-                o += so[w][cn][d4] * a;
-            }
-        } else {
-            // nothing seen, or only NaN scores (their sums are NaN, an empty row's 0)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) ls += sl[w][cn];
+        // the four waves' results meet (in the ring's place): outputs of column n, elements 16 i + 4 g
+        // .. + 3 of each wave
+        if (g == 0) {
+            lds.m[wave][n] = m;
+            lds.l[wave][n] = l;
         }
-        const int rr = cc / G, hh = h * G + (cc - rr * G);
-        const int64_t idx = (int64_t)(pl.s.r0 + rr) * n_head + hh;
-        if (n_splits == 1) {
-            const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
-            *(f32x4*)(out + idx * HD + 4 * d4) = mm == kNegInf ? f32x4{ls, ls, ls, ls} : o * inv;
-        } else {
-            *(f32x4*)(parts.o + (idx * parts.splits + sp) * HD + 4 * d4) = o;
-            if (d4 == 0) {
-                parts.ml[(idx * parts.splits + sp) * 2] = mm;
-                parts.ml[(idx * parts.splits + sp) * 2 + 1] = ls;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NT; ++i) lds.o[wave][n][4 * i + g] = acc[i];
+        __syncthreads();
+        const int64_t slot = sh.aligned ? (int64_t)blockIdx.x : u.units_before + unit + blockIdx.x;
+        for (int i = threadIdx.x; i < 16 * (HD / 4); i += 256) {
+            const int cn = i / (HD / 4), d4 = i % (HD / 4);
+            const int cc = c0 + cn;
+            if (cc >= n_cols) break;
+            float mm = lds.m[0][cn];
+#pragma unroll
+            for (int v = 1; v < 4; ++v) mm = fmaxf(mm, lds.m[v][cn]);
+            float ls = 0.0f;
+            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (mm != kNegInf) {
+#pragma unroll
+                for (int v = 0; v < 4; ++v) {
+                    const float r = __builtin_amdgcn_exp2f(lds.m[v][cn] - mm);
+                    ls += lds.l[v][cn] * r;
+                    o += lds.o[v][cn][d4] * r;
+                }
+            } else {
+                // nothing seen, or only NaN scores (their sums are NaN, an empty row's 0)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) ls += lds.l[v][cn];
+            }
+            if (!split) {
+                const int rr = cc / a.G, hh = h * a.G + (cc - rr * a.G);
+                const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+                *(f32x4*)(out + ((int64_t)(w.s.r0 + rr) * a.n_head + hh) * HD + 4 * d4) =
+                    mm == kNegInf ? f32x4{ls, ls, ls, ls} : o * inv;
+            } else {
+                *(f32x4*)(parts.o + (slot * 16 + cn) * HD + 4 * d4) = o;
+                if (d4 == 0) {
+                    parts.ml[(slot * 16 + cn) * 2] = mm;
+                    parts.ml[(slot * 16 + cn) * 2 + 1] = ls;
+                }
             }
         }
+        __syncthreads();  // the LDS is free for the next unit's tiles
     }
 }
 
-// The splits of every (row, head) joined: grid column tiles x KV heads x sequences.
+// The splits of a unit joined: a workgroup per unit, as many as there may be.
 template <int HD>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, const int32_t* __restrict__ slots,
-                                                  const int32_t* __restrict__ q_start, int n_rows, int max_rows,
-                                                  int n_head, int cols, int col_tiles, int chunk_tiles, Parts parts,
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, AttnArgs a, int mode, int grid, Parts parts,
                                                   float* __restrict__ out) {
-    const int G = n_head / c.n_kv;
-    int b = blockIdx.x;
-    const int ct = b % col_tiles;
-    b /= col_tiles;
-    const int h = b % c.n_kv;
-    const Place pl = place_of(c, slots, q_start, b / c.n_kv, h, ct, cols, G, n_rows, max_rows);
-    if (pl.c0 >= pl.n_cols) return;
-    const int tiles = (pl.kv_end + kTile - 1) / kTile;
-    const int n_splits = min(parts.splits, max(1, (tiles + chunk_tiles - 1) / chunk_tiles));
-    if (n_splits == 1) return;
-    for (int i = threadIdx.x; i < cols * (HD / 4); i += 256) {
-        const int cc = pl.c0 + i / (HD / 4), d4 = i % (HD / 4);
-        if (cc >= pl.n_cols) break;
-        const int rr = cc / G, hh = h * G + (cc - rr * G);
-        const int64_t idx = (int64_t)(pl.s.r0 + rr) * n_head + hh;
-        const float* ml = parts.ml + idx * parts.splits * 2;
-        const float* po = parts.o + idx * parts.splits * HD + 4 * d4;
+    const int lane = threadIdx.x & 63;
+    const Shares sh = shares_of(c, a, mode, grid, lane);
+    const Found u = find_item(c, a, sh, blockIdx.x, true, lane);
+    if (!u.ok) return;
+    const SeqWork w = u.w;
+    const int unit = __builtin_amdgcn_readfirstlane((int)u.rest);
+    int64_t slot;
+    int n_split;
+    if (sh.aligned) {
+        n_split = (int)((w.tiles + sh.q - 1) / sh.q);
+        slot = u.items_before + (int64_t)unit * n_split;
+    } else {
+        const int64_t f0 = u.items_before + (int64_t)unit * w.tiles;
+        const int64_t first = f0 / sh.q;
+        n_split = (int)((f0 + w.tiles - 1) / sh.q - first + 1);
+        slot = u.units_before + unit + first;
+    }
+    if (n_split == 1) return;
+    const int h = unit % c.n_kv, c0 = unit / c.n_kv * a.cols, n_cols = w.rows * a.G;
+    for (int i = threadIdx.x; i < a.cols * (HD / 4); i += 256) {
+        const int cn = i / (HD / 4), cc = c0 + cn, d4 = i % (HD / 4);
+        if (cc >= n_cols) break;
+        const float* ml = parts.ml + (slot * a.cols + cn) * 2;
+        const float* po = parts.o + (slot * a.cols + cn) * HD + 4 * d4;
         float mm = kNegInf;
-        for (int z = 0; z < n_splits; ++z) mm = fmaxf(mm, ml[2 * z]);
+        for (int z = 0; z < n_split; ++z) mm = fmaxf(mm, ml[(int64_t)z * a.cols * 2]);
         float ls = 0.0f;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
         if (mm != kNegInf) {
-            for (int z = 0; z < n_splits; ++z) {
-                const float a = __builtin_amdgcn_exp2f(ml[2 * z] - mm);
-                ls += ml[2 * z + 1] * a;
-                o += *(const f32x4*)(po + (int64_t)z * HD) * a;
+            for (int z = 0; z < n_split; ++z) {
+                const float r = __builtin_amdgcn_exp2f(ml[(int64_t)z * a.cols * 2] - mm);
+                ls += ml[(int64_t)z * a.cols * 2 + 1] * r;
+                o += *(const f32x4*)(po + (int64_t)z * a.cols * HD) * r;
             }
             o *= ls == 0.0f ? 0.0f : 1.0f / ls;
         } else {
-            for (int z = 0; z < n_splits; ++z) ls += ml[2 * z + 1];
+            for (int z = 0; z < n_split; ++z) ls += ml[(int64_t)z * a.cols * 2 + 1];
             o = f32x4{ls, ls, ls, ls};
         }
-        *(f32x4*)(out + idx * HD + 4 * d4) = o;
+        const int rr = cc / a.G, hh = h * a.G + (cc - rr * a.G);
+        *(f32x4*)(out + ((int64_t)(w.s.r0 + rr) * a.n_head + hh) * HD + 4 * d4) = o;
     }
 }
 
@@ -730,42 +911,39 @@ hipError_t launch_kv4_load(const Kv4View& c, int layer, const int32_t* slots, co
 
 Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int max_len, int n_head) {
     Kv4AttnPlan p;
-    const int64_t cols = (int64_t)max_rows * (n_head / c.n_kv);
-    p.kind = 0;
-    p.col_tiles = (int)std::min<int64_t>((cols + 15) / 16, 1 << 30);
-    // splits for two workgroups on each of 256 CUs, of four tiles (one per wave) at least
-    const int tiles = std::max(1, (max_len + kTile - 1) / kTile);
-    const int64_t groups = (int64_t)n_seqs * c.n_kv * p.col_tiles;
-    const int want = (int)std::min<int64_t>(std::max<int64_t>(1, 1024 / std::max<int64_t>(1, groups)), tiles);
-    p.chunk_tiles = std::max(4, ((tiles + want - 1) / want + 3) / 4 * 4);
-    p.chunk_tiles = std::min(p.chunk_tiles, 64);
-    p.splits = (tiles + p.chunk_tiles - 1) / p.chunk_tiles;
+    p.cols = 16;
+    const int64_t tiles = std::max(1, (max_len + kTile - 1) / kTile);
+    p.units = (int64_t)n_seqs * c.n_kv * (((int64_t)max_rows * (n_head / c.n_kv) + p.cols - 1) / p.cols);
+    p.mode = p.units > kAlignedUnits ? kStream : tiles <= kMinShare ? kWhole : kAligned;
+    p.grid = p.mode == kStream ? kGrid
+             : p.mode == kWhole ? p.units
+                                : std::min<int64_t>(kGrid, p.units * (1 + (tiles + kMinShare - 1) / kMinShare));
     return p;
 }
 
-size_t kv4_attention_ws_bytes(const Kv4AttnPlan& p, int n_rows, int n_head, int hd) {
-    return p.splits == 1 ? 0 : (size_t)n_rows * n_head * p.splits * (hd + 2) * sizeof(float);
-}
-
-bool kv4_attention_fits(const Kv4AttnPlan& p, const Kv4View& c, int n_seqs) {
-    return (double)p.splits * p.col_tiles * c.n_kv * n_seqs < 2147483647.0;
+size_t kv4_attention_ws_bytes(const Kv4AttnPlan& p, int hd) {
+    return p.mode == kWhole ? 0 : (size_t)(p.units + p.grid) * p.cols * (hd + 2) * sizeof(float);
 }
 
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int layer, const float* q,
                                 const int32_t* slots, const int32_t* q_start, int n_seqs, int n_rows,
                                 int max_rows, int n_head, float* out, void* ws, hipStream_t stream) {
+    const AttnArgs a = {slots, q_start, n_seqs, n_rows, max_rows, n_head, n_head / c.n_kv, p.cols};
     Parts parts;
-    parts.splits = p.splits;
     parts.o = (float*)ws;
-    parts.ml = parts.o + (size_t)n_rows * n_head * p.splits * c.hd;
-    const unsigned groups = (unsigned)(p.col_tiles * c.n_kv * n_seqs);
-    KV4_HD(c.hd, hipLaunchKernelGGL((k_kv4_attention<HD>), dim3(groups * (unsigned)p.splits), dim3(256), 0, stream, c,
-                                    layer, q, slots, q_start, n_seqs, n_rows, max_rows, n_head, p.col_tiles,
-                                    p.chunk_tiles, parts, out));
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.splits == 1) return e;
-    KV4_HD(c.hd, hipLaunchKernelGGL((k_kv4_join<HD>), dim3(groups), dim3(256), 0, stream, c, slots, q_start, n_rows,
-                                    max_rows, n_head, 16, p.col_tiles, p.chunk_tiles, parts, out));
+    parts.ml = parts.o + (size_t)(p.units + p.grid) * p.cols * c.hd;
+    hipError_t e = hipSuccess;
+    KV4_HD(c.hd, {
+        static LdsLimit limit;
+        e = limit.raise((const void*)k_kv4_attention<HD>, sizeof(AttnLds<HD>));
+        if (e != hipSuccess) return e;
+        hipLaunchKernelGGL((k_kv4_attention<HD>), dim3((unsigned)p.grid), dim3(256), sizeof(AttnLds<HD>), stream, c,
+                           layer, q, a, p.mode, parts, out);
+    });
+    e = hipGetLastError();
+    if (e != hipSuccess || p.mode == kWhole) return e;
+    KV4_HD(c.hd, hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)p.units), dim3(256), 0, stream, c, a, p.mode,
+                                    (int)p.grid, parts, out));
     return hipGetLastError();
 }
 

@@ -62,15 +62,13 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4View& c, const int32_t* slots
 
 // Attention (k_kv4.hip). ws: kv4_attention_ws_bytes bytes.
 struct Kv4AttnPlan {
-    int kind;         // 0: one column tile per workgroup, 1: the many-row kernel
-    int col_tiles;    // column tiles (kind 0: of 16, kind 1: of the workgroup's columns) per KV head
-    int chunk_tiles;  // 32-position tiles of a sequence split
-    int splits;       // sequence splits at most
+    int mode;       // how the work is split over workgroups (k_kv4.hip)
+    int cols;       // (row, head) pairs of a workgroup
+    int64_t units;  // column tiles of the KV heads of the sequences, at most
+    int64_t grid;   // workgroups
 };
 Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int max_len, int n_head);
-size_t kv4_attention_ws_bytes(const Kv4AttnPlan& p, int n_rows, int n_head, int hd);
-// false when the launch would pass the grid's limits
-bool kv4_attention_fits(const Kv4AttnPlan& p, const Kv4View& c, int n_seqs);
+size_t kv4_attention_ws_bytes(const Kv4AttnPlan& p, int hd);
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int layer, const float* q,
                                 const int32_t* slots, const int32_t* q_start, int n_seqs, int n_rows,
                                 int max_rows, int n_head, float* out, void* ws, hipStream_t stream);
