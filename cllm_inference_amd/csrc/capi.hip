@@ -1817,7 +1817,7 @@ const char* cllm_hip_kv4_attention_plan(const cllm_hip_kv4_cache* cache, int n_s
         p.units == 0)
         return "none";
     static const char* const modes[] = {"stream", "aligned", "whole"};
-    snprintf(buf, sizeof buf, "k_kv4_attention<%d> %s units=%lld workgroups=%lld", c.hd, modes[p.mode],
+    snprintf(buf, sizeof buf, "k_kv4_attention<%d,%d> %s units=%lld workgroups=%lld", c.hd, 16 / p.cols, modes[p.mode],
              (long long)p.units, (long long)p.grid);
     return buf;
 }

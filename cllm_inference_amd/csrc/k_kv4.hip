@@ -36,11 +36,12 @@ __device__ __forceinline__ f32x4 mfma(const h8& a, const h8& b, const f32x4& c) 
 // register or literal, so the or's constants lie in vector registers (Magic): v_and_or_b32.
 struct Magic {
     uint32_t m1024, m64;
-    float minus1;  // (as a literal the compiler takes the product away, and v_fma_mix with it)
+    float minus1, zero;  // (as literals they would take v_fma_mix, which reads fp16, out of the products)
     __device__ __forceinline__ Magic() {
         asm("v_mov_b32 %0, 0x64006400" : "=v"(m1024));
         asm("v_mov_b32 %0, 0x54005400" : "=v"(m64));
         asm("v_mov_b32 %0, -1.0" : "=v"(minus1));
+        asm("v_mov_b32 %0, 0" : "=v"(zero));
     }
 };
 __device__ __forceinline__ h8 dequant8(uint32_t w, const h2 (&d)[4], const Magic& mg) {
@@ -52,6 +53,16 @@ __device__ __forceinline__ h8 dequant8(uint32_t w, const h2 (&d)[4], const Magic
     const h2 f = (__builtin_bit_cast(h2, (w8 & 0x00F000F0u) | mg.m64) + off1) * d[3];
     return h8{a.x, a.y, b.x, b.y, e.x, e.y, f.x, f.y};
 }
+
+// Codes of a dword as they are: pairs c * 2^-24 (fp16 subnormals, exact) for r = 0 and 2, 16 c * 2^-24
+// for r = 1 and 3. 5 VALU operations; the other operand of the product has the 16th of codes 2 r and
+// 2 r + 1 of the odd r (odd_pair).
+__device__ __forceinline__ h8 codes8(uint32_t w) {
+    const uint32_t w8 = w >> 8;
+    const uint32_t x[4] = {w & 0x000F000Fu, w & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u};
+    return __builtin_bit_cast(h8, *(const u32x4*)x);
+}
+__device__ __forceinline__ constexpr bool odd_pair(int e) { return (e >> 1) & 1; }
 
 __device__ __forceinline__ h2 pkrtz(float a, float b) {
     return __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
@@ -123,7 +134,7 @@ struct TileLoads {
 template <int HD>
 struct TileView {
     static constexpr int KW = HD / 32, W = KW < 4 ? KW : 4, C = KW / W;
-    const uint8_t* p;
+    uint8_t* p;
     int lane;
 
     // Key fragments c W .. c W + W - 1: the lane's elements there lie in one block.
@@ -143,21 +154,40 @@ struct TileView {
             for (int j = 0; j < 2; ++j) k[j] = dequant8(x[j], d4, mg);
         }
     }
-    // Value fragments 4 c .. 4 c + 3. EDGE: positions from `limit` on (counted from the tile's start)
-    // have bytes that no store has written, whose scales may be NaN.
-    template <bool EDGE>
-    __device__ __forceinline__ void values(int c, h8 (&v)[4], int limit, const Magic& mg) const {
+    // Their codes (codes8).
+    __device__ __forceinline__ void key_codes(int t, int c, h8 (&k)[W]) const {
+        const uint8_t* w = p + ((t * C + c) * 64 + lane) * (4 * W);
+        if constexpr (W == 4) {
+            const u32x4 x = *(const u32x4*)w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) k[j] = codes8(x[j]);
+        } else {
+            const u32x2 x = *(const u32x2*)w;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) k[j] = codes8(x[j]);
+        }
+    }
+    __device__ __forceinline__ void value_codes(int c, h8 (&v)[4]) const {
+        const u32x4 x = *(const u32x4*)(p + 16 * HD + (c * 64 + lane) * 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = codes8(x[j]);
+    }
+    // The value scales of positions from `limit` of the tile on become 0 in LDS: bytes that no store has
+    // written may be NaN.
+    __device__ __forceinline__ void mask_scales(int limit) const {
+        uint16_t* s = (uint16_t*)(p + 34 * HD);
+#pragma unroll
+        for (int i = 0; i < HD; i += 64) {
+            const int e = lane & 7, g = lane >> 3 & 3;
+            if (16 * (e >> 2) + 4 * g + (e & 3) >= limit) s[i + lane] = 0;
+        }
+    }
+    // Value fragments 4 c .. 4 c + 3.
+    __device__ __forceinline__ void values(int c, h8 (&v)[4], const Magic& mg) const {
         const u32x4 x = *(const u32x4*)(p + 16 * HD + (c * 64 + lane) * 16);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-            u32x4 s = *(const u32x4*)(p + 34 * HD + ((2 * c + b) * 4 + (lane >> 4)) * 16);
-            if constexpr (EDGE) {
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int at = 16 * (r >> 1) + 4 * (lane >> 4) + 2 * (r & 1);
-                    s[r] &= (at < limit ? 0x0000FFFFu : 0u) | (at + 1 < limit ? 0xFFFF0000u : 0u);
-                }
-            }
+            const u32x4 s = *(const u32x4*)(p + 34 * HD + ((2 * c + b) * 4 + (lane >> 4)) * 16);
             const h2 d4[4] = {__builtin_bit_cast(h2, (uint32_t)s.x), __builtin_bit_cast(h2, (uint32_t)s.y),
                               __builtin_bit_cast(h2, (uint32_t)s.z), __builtin_bit_cast(h2, (uint32_t)s.w)};
             v[2 * b] = dequant8(x[2 * b], d4, mg);
@@ -166,17 +196,20 @@ struct TileView {
     }
 };
 
-// The 16 columns of a column tile: (row, head) pairs c = row * G + head in group of one KV head,
-// column n of the tile in lanes 16 g + n.
-template <int HD>
+// The 16 columns of the products' second operand. A unit has 16 / SPREAD (row, head) pairs c = row * G
+// + head in group. SPREAD 1: column n is pair n. SPREAD NB = HD / 32: column n is pair n / NB for block
+// n % NB only, its query elements of other blocks 0: the products with plain codes then come out as
+// one sum per block, to be scaled there.
+template <int HD, int SPREAD>
 struct Queries {
     static constexpr int KW = HD / 32;
     h8 hi[KW], lo[KW];
-    float sc;  // score in log2 units = product * sc
+    float sc;    // score in log2 units = product * sc
+    float init;  // SPREAD > 1: -8 times the column's sum of elements, in the product's units
 
     // q row scaled by a power of two so that its largest element lies in [2^14, 2^15): hi and lo
     // then keep 22 significant bits of every element that counts.
-    __device__ __forceinline__ void load(const float* row, bool valid, int g, const Magic& mg) {
+    __device__ __forceinline__ void load(const float* row, bool valid, int g, int n, const Magic& mg) {
         float x[KW][8];
         float m = 0.0f;
 #pragma unroll
@@ -199,16 +232,46 @@ struct Queries {
         m = max_over_g(m);
         int sh = 0;
         if (m > 0.0f && m < __builtin_huge_valf())
-            sh = min(max(15 - __builtin_amdgcn_frexp_expf(m), -120), 120);
+            sh = min(max(15 - __builtin_amdgcn_frexp_expf(m), -120), 100);
         sc = ldexpf(kLog2e / sqrtf((float)HD), -sh);
+        float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[j][i] = ldexpf(x[j][i], sh);
+            for (int i = 0; i < 8; ++i) {
+                x[j][i] = ldexpf(x[j][i], sh);
+                if constexpr (SPREAD > 1) {
+                    if ((g * (HD / 4) + 8 * j) / 32 != n % SPREAD) x[j][i] = 0.0f;
+                    if (odd_pair(i)) x[j][i] *= 0.0625f;
+                }
+            }
             split8(x[j], hi[j], lo[j], mg);
+            if constexpr (SPREAD > 1) {  // (of the parts, so that a code of 8 weighs nothing)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    sum += ((float)hi[j][i] + (float)lo[j][i]) * (odd_pair(i) ? 16.0f : 1.0f);
+            }
+        }
+        if constexpr (SPREAD > 1) {
+            sc = ldexpf(sc, 24);
+            init = sum_over_g(sum) * (-8.0f * 0x1p-24f);
         }
     }
 };
+
+// Sum over the SPREAD columns of a pair (neighbouring lanes), in each of them. (Every lane has a source,
+// so the move needs no old value and folds into the addition.)
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+template <int SPREAD>
+__device__ __forceinline__ float sum_over_blocks(float v) {
+    if constexpr (SPREAD >= 2) v = add_dpp<DPP_QUAD_SWAP1>(v);
+    if constexpr (SPREAD >= 4) v = add_dpp<DPP_QUAD_SWAP2>(v);
+    if constexpr (SPREAD >= 8) v = add_dpp<DPP_ROW_HALF_MIRROR>(v);
+    return v;
+}
 
 // ---------------------------------------------------------------------------- the work's split
 //
@@ -249,6 +312,13 @@ __device__ __forceinline__ SeqWork seq_work(const Kv4View& c, const AttnArgs& a,
     w.tiles = max(1, (w.s.len - w.s.rows + w.rows + kTile - 1) / kTile);
     return w;
 }
+// The value of lane 0 (or of lane `at`), in scalar registers.
+__device__ __forceinline__ int64_t scalar(int64_t v) {
+    return ((int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+__device__ __forceinline__ int64_t scalar(int64_t v, int at) {
+    return ((int64_t)__builtin_amdgcn_readlane((int)(v >> 32), at) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)v, at);
+}
 __device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {  // inclusive
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -280,6 +350,8 @@ __device__ __forceinline__ Shares shares_of(const Kv4View& c, const AttnArgs& a,
         units += __shfl_xor((long long)units, d, 64);
         tiles += __shfl_xor((long long)tiles, d, 64);
     }
+    units = scalar(units);
+    tiles = scalar(tiles);
     Shares sh;
     sh.aligned = mode != kStream;
     sh.items = tiles;
@@ -314,14 +386,14 @@ __device__ __forceinline__ Found find_item(const Kv4View& c, const AttnArgs& a, 
             r.w.rows = __builtin_amdgcn_readlane(w.rows, at);
             r.w.units = __builtin_amdgcn_readlane(w.units, at);
             r.w.tiles = __builtin_amdgcn_readlane(w.tiles, at);
-            r.items_before = items + __shfl((long long)(incl - mine), at, 64);
-            r.units_before = units + __shfl((long long)(uincl - w.units), at, 64);
+            r.items_before = items + scalar(incl - mine, at);
+            r.units_before = units + scalar(uincl - w.units, at);
             r.rest = f - (by_units ? r.units_before : r.items_before);
             r.ok = true;
             return r;
         }
-        items += __shfl((long long)incl, 63, 64);
-        units += __shfl((long long)uincl, 63, 64);
+        items += scalar(incl, 63);
+        units += scalar(uincl, 63);
     }
     return r;
 }
@@ -350,11 +422,11 @@ struct AttnLds {
     float m[4][16], l[4][16];
 };
 
-template <int HD>
+template <int HD, int SPREAD>
 __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, const float* __restrict__ q,
                                                           AttnArgs a, int mode, Parts parts,
                                                           float* __restrict__ out) {
-    constexpr int NT = HD / 16, W = TileView<HD>::W, STAGES = AttnLds<HD>::STAGES, NL = TileLoads<HD>::COUNT;
+    constexpr int NT = HD / 16, W = TileView<HD>::W, COLS = 16 / SPREAD, STAGES = AttnLds<HD>::STAGES, NL = TileLoads<HD>::COUNT;
     extern __shared__ __align__(16) uint8_t lds_bytes[];
     AttnLds<HD>& lds = *(AttnLds<HD>*)lds_bytes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -394,14 +466,14 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
         unit = __builtin_amdgcn_readfirstlane(unit);
         t_begin = __builtin_amdgcn_readfirstlane(t_begin);
         t_end = __builtin_amdgcn_readfirstlane(t_end);
-        const int h = unit % c.n_kv, c0 = unit / c.n_kv * 16, n_cols = w.rows * a.G;
-        const int col = c0 + n;
+        const int h = unit % c.n_kv, c0 = unit / c.n_kv * COLS, n_cols = w.rows * a.G;
+        const int col = c0 + n / SPREAD;
         const bool valid = col < n_cols;
         const int row = col / a.G, head = h * a.G + (col - row * a.G);
         const int vis = valid ? w.s.len - w.s.rows + row + 1 : 0;       // positions the column sees
         const int vis_min = w.s.len - w.s.rows + c0 / a.G + 1;          // and the tile's first row
         // the column tile's last row sees no tile from here on
-        const int last_row = min(w.rows - 1, (c0 + 15) / a.G);
+        const int last_row = min(w.rows - 1, (c0 + COLS - 1) / a.G);
         t_end = min(t_end, max(t_begin, (max(0, w.s.len - w.s.rows + last_row + 1) + kTile - 1) / kTile));
 
         // The wave's tiles first, first + 4, ...: a lane holds the page id of every 64th. A tile
@@ -426,21 +498,36 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
         };
         for (int i = 0; i < min(count, STAGES - 1); ++i) issue(i, i);
 
-        Queries<HD> qs;
-        qs.load(q + ((int64_t)(w.s.r0 + row) * a.n_head + head) * HD, valid, g, mg);
+        Queries<HD, SPREAD> qs;
+        qs.load(q + ((int64_t)(w.s.r0 + row) * a.n_head + head) * HD, valid, g, n, mg);
         f32x4 acc[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = kNegInf, l = 0.0f;
+        // SPREAD > 1: the products with codes of 8 (every row the same), odd pairs' sum of weights, the
+        // bound of the value scales
+        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
+        float l_odd = 0.0f, bound = 0.0f;
+        int bound_ex = 0;
 
-        // EDGE: the tile ends past what some column sees, or past the sequence, or has no page
-        const auto step = [&]<bool EDGE>(const TileView<HD>& tv, int p0, int len) {
-            f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+        // edge: the tile ends past what some column sees, or past the sequence, or has no page (len 0)
+        const auto step = [&](const TileView<HD>& tv, int p0, int len, bool edge) {
+            if (edge) tv.mask_scales(len - p0);
+            f32x4 s[2];
+            u32x4 vs;  // SPREAD > 1: the value scales of the lane's block and positions
+            if constexpr (SPREAD > 1) {
+                s[0] = s[1] = f32x4{qs.init, qs.init, qs.init, qs.init};
+                vs = *(const u32x4*)(tv.p + 34 * HD + ((n % SPREAD) * 4 + g) * 16);
+            } else {
+                s[0] = s[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
 #pragma unroll
             for (int kc = 0; kc < TileView<HD>::C; ++kc) {
                 h8 k[2][W];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) tv.keys(t, kc, k[t], mg);
+                for (int t = 0; t < 2; ++t) {
+                    if constexpr (SPREAD > 1) tv.key_codes(t, kc, k[t]); else tv.keys(t, kc, k[t], mg);
+                }
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
 #pragma unroll
@@ -449,42 +536,91 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
                     for (int t = 0; t < 2; ++t) s[t] = mfma(k[t][j], qs.lo[kc * W + j], s[t]);
                 }
             }
+            if constexpr (SPREAD > 1) {  // the blocks' sums scaled (positions 4 g .. + 3 of both halves) and joined
+                const u32x4 ks = *(const u32x4*)(tv.p + 32 * HD + ((n % SPREAD) * 16 + 4 * g) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const h2 d = __builtin_bit_cast(h2, (uint32_t)ks[i]);
+                    s[0][i] = sum_over_blocks<SPREAD>(__builtin_fmaf(s[0][i], (float)d.x, mg.zero));
+                    s[1][i] = sum_over_blocks<SPREAD>(__builtin_fmaf(s[1][i], (float)d.y, mg.zero));
+                }
+            }
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = s[e >> 2][e & 3];
-                if (EDGE && p0 + 16 * (e >> 2) + 4 * g + (e & 3) >= min(vis, len)) x[e] = kNegInf;
+            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3];
+            if (edge) {
+                const int end = min(vis, len) - p0 - 4 * g;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = 16 * (e >> 2) + (e & 3) >= end ? kNegInf : x[e];
             }
             float mx = x[0];
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
             mx = max_over_g(mx) * qs.sc;
-            if (__any(mx > m)) {
+            bool grow = mx > m;
+            uint32_t d_max = 0;
+            if constexpr (SPREAD > 1) {  // the lane's largest |scale|, as fp16 bits
+                typedef uint16_t us2 __attribute__((ext_vector_type(2)));
+                us2 t = __builtin_bit_cast(us2, vs[0] & 0x7FFF7FFFu);
+#pragma unroll
+                for (int i = 1; i < 4; ++i)
+                    t = __builtin_elementwise_max(t, __builtin_bit_cast(us2, vs[i] & 0x7FFF7FFFu));
+                d_max = max((uint32_t)t.x, (uint32_t)t.y);
+                grow |= f16_to_f32(d_max) > bound;
+            }
+            if (__any(grow)) {
                 const float m_new = fmaxf(m, mx);
-                const float r = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+                float r = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
                 m = m_new;
+                if constexpr (SPREAD > 1) {
+                    // the weights times 2^(15 - bound_ex) times a scale below 2^bound_ex stay within
+                    // 2^15; a factor of two in hand, so that few tiles raise the bound
+                    const float all = max_over_g(f16_to_f32(d_max));
+                    if (all > bound) {
+                        const int ex = __builtin_amdgcn_frexp_expf(all) + 1;
+                        r = bound == 0.0f ? r : ldexpf(r, bound_ex - ex);
+                        bound_ex = ex;
+                        bound = ldexpf(1.0f, ex);
+                    }
+                    l_odd *= r;
+                    z *= r;
+                }
                 l *= r;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) acc[i] *= r;
             }
             // weights times 2^15: as fp16 pairs they keep 20 bits down to 2^-19 of the largest
-            const float mm = 15.0f - (m == kNegInf ? 0.0f : m);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], qs.sc, mm));
-                l += x[e];
-            }
+            const float mm = 15.0f - (m == kNegInf ? 0.0f : m) - (float)bound_ex;
             h8 hi, lo;
+            if constexpr (SPREAD > 1) {
+                const float mo = mm - 4.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const h2 d = __builtin_bit_cast(h2, (uint32_t)vs[e >> 1]);
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], qs.sc, odd_pair(e) ? mo : mm));
+                    (odd_pair(e) ? l_odd : l) += x[e];
+                    x[e] = __builtin_fmaf(x[e], (float)(e & 1 ? d.y : d.x), mg.zero);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], qs.sc, mm));
+                    l += x[e];
+                }
+            }
             split8(x, hi, lo, mg);
+            if constexpr (SPREAD > 1) {
+                z = mfma(codes8(0x88888888u), hi, z);
+                z = mfma(codes8(0x88888888u), lo, z);
+            }
 #pragma unroll
             for (int cc = 0; cc < NT / 4; ++cc) {
                 h8 v[4];
-                tv.template values<EDGE>(cc, v, len - p0, mg);
+                if constexpr (SPREAD > 1) tv.value_codes(cc, v); else tv.values(cc, v, mg);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    acc[4 * cc + i] = mfma(v[i], hi, acc[4 * cc + i]);
-                    acc[4 * cc + i] = mfma(v[i], lo, acc[4 * cc + i]);
-                }
+                for (int i = 0; i < 4; ++i) acc[4 * cc + i] = mfma(v[i], hi, acc[4 * cc + i]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[4 * cc + i] = mfma(v[i], lo, acc[4 * cc + i]);
             }
         };
         for (int i = 0; i < count; ++i) {
@@ -499,25 +635,32 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
             holes >>= 1;
             const int p0 = (first + 4 * i) * kTile;
             const TileView<HD> tv = {lds.ring[wave] + (i % STAGES) * (36 * HD), lane};
-            if (hole || p0 + kTile > vis_min || p0 + kTile > w.s.len)
-                step.template operator()<true>(tv, p0, hole ? 0 : w.s.len);
-            else
-                step.template operator()<false>(tv, p0, w.s.len);
+            step(tv, p0, hole ? 0 : w.s.len, hole || p0 + kTile > vis_min || p0 + kTile > w.s.len);
+        }
+        if constexpr (SPREAD > 1) {
+            // sums over codes become sums over values: less the codes of 8, 2^24 for their units, and
+            // the scales' bound taken out
+            l = ldexpf(l + 16.0f * l_odd, bound_ex);
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = ldexpf(acc[i][j] - z[j], 24 + bound_ex);
         }
         l = sum_over_g(l);
 
         // the four waves' results meet (in the ring's place): outputs of column n, elements 16 i + 4 g
         // .. + 3 of each wave
-        if (g == 0) {
-            lds.m[wave][n] = m;
-            lds.l[wave][n] = l;
+        if (g == 0 && n % SPREAD == 0) {
+            lds.m[wave][n / SPREAD] = m;
+            lds.l[wave][n / SPREAD] = l;
         }
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NT; ++i) lds.o[wave][n][4 * i + g] = acc[i];
+        for (int i = 0; i < NT; ++i)
+            if (SPREAD == 1 || i / 2 == n % SPREAD) lds.o[wave][n / SPREAD][4 * i + g] = acc[i];
         __syncthreads();
         const int64_t slot = sh.aligned ? (int64_t)blockIdx.x : u.units_before + unit + blockIdx.x;
-        for (int i = threadIdx.x; i < 16 * (HD / 4); i += 256) {
+        for (int i = threadIdx.x; i < COLS * (HD / 4); i += 256) {
             const int cn = i / (HD / 4), d4 = i % (HD / 4);
             const int cc = c0 + cn;
             if (cc >= n_cols) break;
@@ -544,10 +687,10 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
                 *(f32x4*)(out + ((int64_t)(w.s.r0 + rr) * a.n_head + hh) * HD + 4 * d4) =
                     mm == kNegInf ? f32x4{ls, ls, ls, ls} : o * inv;
             } else {
-                *(f32x4*)(parts.o + (slot * 16 + cn) * HD + 4 * d4) = o;
+                *(f32x4*)(parts.o + (slot * COLS + cn) * HD + 4 * d4) = o;
                 if (d4 == 0) {
-                    parts.ml[(slot * 16 + cn) * 2] = mm;
-                    parts.ml[(slot * 16 + cn) * 2 + 1] = ls;
+                    parts.ml[(slot * COLS + cn) * 2] = mm;
+                    parts.ml[(slot * COLS + cn) * 2 + 1] = ls;
                 }
             }
         }
@@ -883,11 +1026,11 @@ int segments_at_most(int n_seqs, int n_rows) {
 
 // ------------------------------------------------------------------------------- launchers
 
-#define KV4_HD(hd, CALL)                   \
-    switch (hd) {                          \
-        case 64: { constexpr int HD = 64; CALL; } break;   \
-        case 128: { constexpr int HD = 128; CALL; } break; \
-        default: { constexpr int HD = 256; CALL; } break;  \
+#define KV4_HD(hd, ...)                                           \
+    switch (hd) {                                                 \
+        case 64: { constexpr int HD = 64; __VA_ARGS__; } break;   \
+        case 128: { constexpr int HD = 128; __VA_ARGS__; } break; \
+        default: { constexpr int HD = 256; __VA_ARGS__; } break;  \
     }
 
 hipError_t launch_kv4_store(const Kv4View& c, int layer, const float* k, const float* v, float* q,
@@ -911,7 +1054,9 @@ hipError_t launch_kv4_load(const Kv4View& c, int layer, const int32_t* slots, co
 
 Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int max_len, int n_head) {
     Kv4AttnPlan p;
-    p.cols = 16;
+    // the columns carry the blocks where all (row, head) pairs of a KV head fit beside each other
+    const int nb = c.hd / 32;
+    p.cols = (int64_t)max_rows * (n_head / c.n_kv) * nb <= 16 ? 16 / nb : 16;
     const int64_t tiles = std::max(1, (max_len + kTile - 1) / kTile);
     p.units = (int64_t)n_seqs * c.n_kv * (((int64_t)max_rows * (n_head / c.n_kv) + p.cols - 1) / p.cols);
     p.mode = p.units > kAlignedUnits ? kStream : tiles <= kMinShare ? kWhole : kAligned;
@@ -925,6 +1070,17 @@ size_t kv4_attention_ws_bytes(const Kv4AttnPlan& p, int hd) {
     return p.mode == kWhole ? 0 : (size_t)(p.units + p.grid) * p.cols * (hd + 2) * sizeof(float);
 }
 
+template <int HD, int SPREAD>
+static hipError_t launch_attention(const Kv4View& c, const Kv4AttnPlan& p, int layer, const float* q, const AttnArgs& a,
+                                   const Parts& parts, float* out, hipStream_t stream) {
+    static LdsLimit limit;
+    const hipError_t e = limit.raise((const void*)k_kv4_attention<HD, SPREAD>, sizeof(AttnLds<HD>));
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_kv4_attention<HD, SPREAD>), dim3((unsigned)p.grid), dim3(256), sizeof(AttnLds<HD>), stream, c,
+                       layer, q, a, p.mode, parts, out);
+    return hipGetLastError();
+}
+
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int layer, const float* q,
                                 const int32_t* slots, const int32_t* q_start, int n_seqs, int n_rows,
                                 int max_rows, int n_head, float* out, void* ws, hipStream_t stream) {
@@ -934,13 +1090,9 @@ hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int laye
     parts.ml = parts.o + (size_t)(p.units + p.grid) * p.cols * c.hd;
     hipError_t e = hipSuccess;
     KV4_HD(c.hd, {
-        static LdsLimit limit;
-        e = limit.raise((const void*)k_kv4_attention<HD>, sizeof(AttnLds<HD>));
-        if (e != hipSuccess) return e;
-        hipLaunchKernelGGL((k_kv4_attention<HD>), dim3((unsigned)p.grid), dim3(256), sizeof(AttnLds<HD>), stream, c,
-                           layer, q, a, p.mode, parts, out);
+        e = p.cols == 16 ? launch_attention<HD, 1>(c, p, layer, q, a, parts, out, stream)
+                         : launch_attention<HD, HD / 32>(c, p, layer, q, a, parts, out, stream);
     });
-    e = hipGetLastError();
     if (e != hipSuccess || p.mode == kWhole) return e;
     KV4_HD(c.hd, hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)p.units), dim3(256), 0, stream, c, a, p.mode,
                                     (int)p.grid, parts, out));

@@ -184,10 +184,17 @@ class Cache:
         return np.where(ok[:, None, None], kv[0], 0.0), np.where(ok[:, None, None], kv[1], 0.0), ok
 
 
+def block_max(x):
+    """Of every element, the largest size in its block of 32: 8 d, as a block's extreme has code 0."""
+    b = np.abs(x).reshape(*x.shape[:-1], x.shape[-1] // 32, 32).max(-1, keepdims=True)
+    return np.broadcast_to(b, (*b.shape[:-1], 32)).reshape(x.shape)
+
+
 def attention(q, k, v, ok, first):
     """q [r, n_head, hd] over k, v [n, n_kv, hd] in 64 bits; row t sees positions <= first + t that
-    are ok. Returns the outputs, and per output the bounds the tolerance is made of: the largest
-    sum |q_i k_i| / sqrt(hd) of the row's positions, sum p |v| and sum |v|."""
+    are ok. Returns the outputs, and per output the bounds the tolerance is made of, with K and V
+    the block maxima (8 d) of k and v: the largest sum |q_i| K_i / sqrt(hd) of the row's positions,
+    sum p V and sum V."""
     r, n_head, hd = q.shape
     n, n_kv = k.shape[:2]
     g = n_head // n_kv
@@ -195,7 +202,8 @@ def attention(q, k, v, ok, first):
     out, size, mass, total = (np.zeros((r, n_kv, g, hd)) for _ in range(4))
     for h in range(n_kv):
         s = np.einsum("rgd,nd->rgn", q[:, h], k[:, h]) / np.sqrt(hd)
-        a = np.einsum("rgd,nd->rgn", np.abs(q[:, h]), np.abs(k[:, h])) / np.sqrt(hd)
+        a = np.einsum("rgd,nd->rgn", np.abs(q[:, h]), block_max(k[:, h])) / np.sqrt(hd)
+        size_v = block_max(v[:, h])
         for t in range(r):
             seen = ok & (np.arange(n) <= first + t)
             if not seen.any():
@@ -204,14 +212,18 @@ def attention(q, k, v, ok, first):
             p = np.exp(x - x.max(-1, keepdims=True))
             p /= p.sum(-1, keepdims=True)
             out[t, h] = p @ v[seen, h]
-            mass[t, h] = p @ np.abs(v[seen, h])
-            total[t, h] = np.abs(v[seen, h]).sum(0)
+            mass[t, h] = p @ size_v[seen]
+            total[t, h] = size_v[seen].sum(0)
             size[t, h] = a[t][:, seen].max(-1, keepdims=True)
     return [x.reshape(r, n_head, hd) for x in (out, size, mass, total)]
 
 
 def attention_bound(hd, n, size, mass, total):
-    """How far the kernel may be from the exact output. A query element as two fp16 parts is off by
+    """How far the kernel may be from the exact output. The products may run over plain codes c = 0 ..
+    15, d times the sum of weight times c less the sum of weight times 8: terms of up to 2 * 8 d and 8 d
+    whose sums are rounded, so rounding is relative to the block's 8 d and not to |d (c - 8)| (an element
+    of value 0 still adds 8 d twice); size, mass and total are made of 8 d, and the accumulations below
+    count three times (16 + 8 = 3 * 8). A query element as two fp16 parts is off by
     at most 2^-20 of itself, the fp32 accumulation of hd products by (hd + 8) 2^-24 of their
     magnitudes, the scaling to log2 units, the subtraction of the maximum and the exponential by
     2^-21 of the score's size and 2^-22; so a weight is off by at most d below, relatively, and the
@@ -220,5 +232,5 @@ def attention_bound(hd, n, size, mass, total):
     as the weights' sum is at least the largest (an output whose values lie under small weights only
     keeps an absolute accuracy). The running sums of a wave add one rounding per step:
     n / 16 of the denominator, n / 128 of the outputs, and the joins some 64."""
-    d = size * (2.0 ** -20 + (hd + 8) * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -21
-    return mass * (2.2 * d + 2.0 ** -20 + (n / 16 + n / 128 + 64) * 2.0 ** -24) + 2.0 ** -39 * total
+    d = size * (2.0 ** -20 + 3 * (hd + 8) * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -21
+    return mass * (2.2 * d + 2.0 ** -20 + (n / 16 + 3 * n / 128 + 3 * 64) * 2.0 ** -24) + 2.0 ** -39 * total
