@@ -107,25 +107,27 @@ __device__ __forceinline__ void wait_lds() {
     asm volatile("" ::: "memory");
 }
 
-// A tile loaded straight into LDS (36 * HD bytes at `slot`) by one wave: 16 bytes a lane, the rest
-// 4 bytes a lane. The loads are the wave's own business: the compiler, which would wait for all of
-// them before any LDS read, does not see them, and wait_loads orders the reads.
+// A tile loaded straight into LDS (36 * HD bytes at `slot`) by one wave, 16 bytes a lane, the last load
+// by part of the lanes. The loads are the wave's own business: the compiler, which would wait for all
+// of them before any LDS read, does not see them, and wait_loads orders the reads. ONCE: bytes that no
+// other workgroup reads (nontemporal: 64 sequences of 4096-8192 positions 108.6 -> 104.0 us).
+template <bool ONCE>
+__device__ __forceinline__ void load_to_lds(const uint8_t* from, uint32_t m0) {
+    if constexpr (ONCE)
+        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(from), "s"(m0) : "memory", "m0");
+    else
+        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(m0) : "memory", "m0");
+}
 template <int HD>
 struct TileLoads {
-    static constexpr int BYTES = 36 * HD, WIDE = BYTES / 1024, NARROW = (BYTES - 1024 * WIDE) / 256;
-    static constexpr int COUNT = WIDE + NARROW;
-    static_assert(WIDE * 1024 + NARROW * 256 == BYTES, "a tile is whole loads");
+    static constexpr int BYTES = 36 * HD, WHOLE = BYTES / 1024, REST = (BYTES - 1024 * WHOLE) / 16;
+    static constexpr int COUNT = WHOLE + (REST > 0);
+    template <bool ONCE>
     static __device__ __forceinline__ void issue(const uint8_t* tile, const uint8_t* slot, int lane) {
         const uint32_t m0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)slot;
 #pragma unroll
-        for (int i = 0; i < WIDE; ++i)
-            asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
-                         : : "v"(tile + 1024 * i + 16 * lane), "s"(m0 + 1024 * i) : "memory", "m0");
-#pragma unroll
-        for (int i = 0; i < NARROW; ++i)
-            asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
-                         : : "v"(tile + 1024 * WIDE + 256 * i + 4 * lane), "s"(m0 + 1024 * WIDE + 256 * i)
-                         : "memory", "m0");
+        for (int i = 0; i < WHOLE; ++i) load_to_lds<ONCE>(tile + 1024 * i + 16 * lane, m0 + 1024 * i);
+        if (REST > 0 && lane < REST) load_to_lds<ONCE>(tile + 1024 * WHOLE + 16 * lane, m0 + 1024 * WHOLE);
     }
 };
 
@@ -276,17 +278,17 @@ __device__ __forceinline__ float sum_over_blocks(float v) {
 // ---------------------------------------------------------------------------- the work's split
 //
 // A unit is a column tile of a KV head of a sequence: n tiles of positions (one at least, so that
-// rows that see nothing are written too). Only the device knows the lengths, so the workgroups find
-// their shares themselves, from sums over the sequences that each wave forms 64 at a time:
-//   few units (up to kAlignedUnits): unit u has ceil(n_u / Q) splits of equal size, one workgroup
-//   each, Q chosen so that all of them fit the grid; a workgroup has one unit, and the smallest
-//   batches (n_u <= kMinShare) need no join;
-//   many units: the units' tiles lie end to end and workgroup w takes tiles [w Q, (w + 1) Q), so
-//   the work is even whatever the lengths are, for a few restarts where a share crosses units.
-// A unit split over workgroups leaves partial results in slots (aligned: the workgroup; else unit +
-// workgroup, which grows along the staircase of pairs), and a second launch joins them.
-constexpr int kGrid = 512;          // two workgroups on each of 256 CUs
-constexpr int kAlignedUnits = 256;
+// rows that see nothing are written too). Only the device knows the lengths:
+//   direct, up to kDirectUnits units: `splits` workgroups per unit; a unit of n tiles uses
+//   min(splits, ceil(n / kMinShare)) of them, evenly, and the rest end at once. A workgroup finds its
+//   place from its index alone; with one split there is nothing to join.
+//   stream, more units: the units' tiles lie end to end and workgroup w takes tiles [w Q, (w + 1) Q),
+//   found from sums over the sequences that each wave forms 64 at a time: the work is even whatever
+//   the lengths are, for a few restarts where a share crosses units.
+// Partial results lie in slots (direct: unit * splits + split; stream: unit + workgroup, which grows
+// along the staircase of pairs), and a second launch joins them.
+constexpr int kGrid = 512;          // stream: two workgroups on each of 256 CUs
+constexpr int kDirectUnits = 256;
 constexpr int kMinShare = 8;        // tiles
 
 struct SeqWork {
@@ -328,55 +330,41 @@ __device__ __forceinline__ int64_t wave_scan(int64_t v, int lane) {  // inclusiv
     return v;
 }
 
-// How the batch is shared out: items are workgroups (aligned) or tiles.
-enum { kStream, kAligned, kWhole };  // kWhole: aligned, every unit one workgroup's (no join follows)
-struct Shares {
-    bool aligned;
-    int64_t q;      // tiles of a share
-    int64_t items;
-    __device__ __forceinline__ int64_t of(const SeqWork& w) const {
-        return (int64_t)w.units * (aligned ? (w.tiles + q - 1) / q : (int64_t)w.tiles);
-    }
-};
-__device__ __forceinline__ Shares shares_of(const Kv4View& c, const AttnArgs& a, int mode, int grid, int lane) {
-    int64_t units = 0, tiles = 0;
+// Stream: the tiles of a share, and the place of tile f: its sequence, unit and tile there.
+__device__ __forceinline__ int64_t share_of(const Kv4View& c, const AttnArgs& a, int grid, int64_t& total,
+                                            int64_t& n_units, int lane) {
+    int64_t tiles = 0, units = 0;
     for (int i0 = 0; i0 < a.n_seqs; i0 += 64) {
         const SeqWork w = seq_work(c, a, i0 + lane);
-        units += w.units;
         tiles += (int64_t)w.units * w.tiles;
+        units += w.units;
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        units += __shfl_xor((long long)units, d, 64);
         tiles += __shfl_xor((long long)tiles, d, 64);
+        units += __shfl_xor((long long)units, d, 64);
     }
-    units = scalar(units);
-    tiles = scalar(tiles);
-    Shares sh;
-    sh.aligned = mode != kStream;
-    sh.items = tiles;
-    // sum of ceil(n / Q) <= tiles / Q + units: within the grid (of 2 units at least)
-    const int64_t wgs = sh.aligned ? max((int64_t)1, grid - units) : grid;
-    sh.q = mode == kWhole ? INT32_MAX : max((int64_t)kMinShare, (tiles + wgs - 1) / wgs);
-    return sh;
+    n_units = scalar(units);
+    total = scalar(tiles);
+    const int64_t q = total < INT32_MAX / 2 ? (int64_t)(((uint32_t)total + (uint32_t)grid - 1) / (uint32_t)grid)
+                                            : (total + grid - 1) / grid;
+    return max((int64_t)kMinShare, q);
 }
-
-// The sequence that item (or unit, by_units) f falls to, f's place among the sequence's own, and what
-// the sequences before it have.
 struct Found {
     SeqWork w;
-    int64_t rest, items_before, units_before;
+    int unit, tile;           // of the sequence, of the unit
+    int64_t units_before;     // of the sequences before
     bool ok;
 };
-__device__ __forceinline__ Found find_item(const Kv4View& c, const AttnArgs& a, const Shares& sh, int64_t f,
-                                           bool by_units, int lane) {
+__device__ __forceinline__ Found find_tile(const Kv4View& c, const AttnArgs& a, int64_t f, int lane) {
     int64_t items = 0, units = 0;
     Found r;
     r.ok = false;
     for (int i0 = 0; i0 < a.n_seqs; i0 += 64) {
         const SeqWork w = seq_work(c, a, i0 + lane);
-        const int64_t mine = sh.of(w), incl = wave_scan(mine, lane), uincl = wave_scan((int64_t)w.units, lane);
-        const uint64_t past = __ballot((by_units ? units + uincl : items + incl) > f);
+        const int64_t mine = (int64_t)w.units * w.tiles;
+        const int64_t incl = wave_scan(mine, lane), uincl = wave_scan((int64_t)w.units, lane);
+        const uint64_t past = __ballot(items + incl > f);
         if (past) {
             const int at = __builtin_ctzll(past);
             r.w.s.slot = __builtin_amdgcn_readlane(w.s.slot, at);
@@ -386,9 +374,11 @@ __device__ __forceinline__ Found find_item(const Kv4View& c, const AttnArgs& a, 
             r.w.rows = __builtin_amdgcn_readlane(w.rows, at);
             r.w.units = __builtin_amdgcn_readlane(w.units, at);
             r.w.tiles = __builtin_amdgcn_readlane(w.tiles, at);
-            r.items_before = items + scalar(incl - mine, at);
             r.units_before = units + scalar(uincl - w.units, at);
-            r.rest = f - (by_units ? r.units_before : r.items_before);
+            const int64_t rest = f - items - scalar(incl - mine, at);
+            r.unit = __builtin_amdgcn_readfirstlane(
+                rest <= INT32_MAX ? (int)((uint32_t)rest / (uint32_t)r.w.tiles) : (int)(rest / r.w.tiles));
+            r.tile = __builtin_amdgcn_readfirstlane((int)(rest - (int64_t)r.unit * r.w.tiles));
             r.ok = true;
             return r;
         }
@@ -400,9 +390,16 @@ __device__ __forceinline__ Found find_item(const Kv4View& c, const AttnArgs& a, 
 
 // Partial results of slot i and column n: unnormalised outputs o[(i * cols + n) * HD], the running
 // maximum (log2 units) and sum ml[(i * cols + n) * 2].
+// map (stream): what the join needs of every unit, and their number.
+struct UnitMap {
+    int64_t slot;
+    int n_split, r0, rows, unit;
+};
 struct Parts {
     float* o;
     float* ml;
+    UnitMap* map;
+    int64_t* n_units;
 };
 
 // One workgroup of four waves per share. The waves walk a unit's tiles alone (tile w, w + 4, ...),
@@ -424,7 +421,7 @@ struct AttnLds {
 
 template <int HD, int SPREAD>
 __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, const float* __restrict__ q,
-                                                          AttnArgs a, int mode, Parts parts,
+                                                          AttnArgs a, int splits, Parts parts,
                                                           float* __restrict__ out) {
     constexpr int NT = HD / 16, W = TileView<HD>::W, COLS = 16 / SPREAD, STAGES = AttnLds<HD>::STAGES, NL = TileLoads<HD>::COUNT;
     extern __shared__ __align__(16) uint8_t lds_bytes[];
@@ -432,40 +429,52 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g = lane >> 4, n = lane & 15;
     const Magic mg;
-    const Shares sh = shares_of(c, a, mode, gridDim.x, lane);
-    int64_t f = blockIdx.x, f_end = f + 1;  // items of this workgroup
-    if (!sh.aligned) {
-        f = blockIdx.x * sh.q;
-        f_end = min(f + sh.q, sh.items);
-    }
     const int sub = c.page_shift - 5;
     const uint8_t* const layer_pages = c.pages + (int64_t)layer * c.n_pages * c.page_bytes;
+    int64_t f = 0, f_end = 1, share = 0;  // direct: one unit; stream: tiles
+    if (splits == 0) {
+        int64_t n_units;
+        share = share_of(c, a, gridDim.x, f_end, n_units, lane);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *parts.n_units = n_units;
+        f = blockIdx.x * share;
+        f_end = min(f + share, f_end);
+    }
 
     while (f < f_end) {
-        const Found u = find_item(c, a, sh, f, false, lane);
-        if (!u.ok) return;
-        const SeqWork w = u.w;
-        // unit of the sequence, its tiles [t_begin, t_end) of this workgroup, whether it is split
+        // the unit (of its sequence), its tiles [t_begin, t_end) of this workgroup, whether it is split
+        SeqWork w;
         int unit, t_begin, t_end;
+        int64_t slot;
         bool split;
-        if (sh.aligned) {
-            const int n_split = (int)((w.tiles + sh.q - 1) / sh.q);
-            unit = (int)(u.rest / n_split);
-            const int z = (int)(u.rest - (int64_t)unit * n_split);
+        if (splits > 0) {
+            f = f_end;
+            const int u = (int)blockIdx.x / splits, z = (int)blockIdx.x - u * splits;
+            const int per_seq = c.n_kv * ((a.max_rows * a.G + COLS - 1) / COLS);
+            const int seq = u / per_seq;
+            unit = u - seq * per_seq;
+            w = seq_work(c, a, seq);
+            const int n_split = min(splits, (w.tiles + kMinShare - 1) / kMinShare);
+            if (unit >= w.units || z >= n_split) return;
             t_begin = (int)((int64_t)w.tiles * z / n_split);
             t_end = (int)((int64_t)w.tiles * (z + 1) / n_split);
             split = n_split > 1;
-            f = f_end;
+            slot = blockIdx.x;
         } else {
-            unit = (int)(u.rest / w.tiles);
-            t_begin = (int)(u.rest - (int64_t)unit * w.tiles);
+            const Found u = find_tile(c, a, f, lane);
+            if (!u.ok) return;
+            w = u.w;
+            unit = u.unit;
+            t_begin = u.tile;
             t_end = (int)min((int64_t)w.tiles, t_begin + (f_end - f));
             split = t_begin > 0 || t_end < w.tiles;
+            slot = u.units_before + unit + blockIdx.x;
+            if (t_begin == 0 && threadIdx.x == 0) {
+                const int64_t last = (f + w.tiles - 1) / share;
+                parts.map[u.units_before + unit] =
+                    UnitMap{slot, (int)(last - blockIdx.x) + 1, w.s.r0, w.rows, unit};
+            }
             f += t_end - t_begin;
         }
-        unit = __builtin_amdgcn_readfirstlane(unit);
-        t_begin = __builtin_amdgcn_readfirstlane(t_begin);
-        t_end = __builtin_amdgcn_readfirstlane(t_end);
         const int h = unit % c.n_kv, c0 = unit / c.n_kv * COLS, n_cols = w.rows * a.G;
         const int col = c0 + n / SPREAD;
         const bool valid = col < n_cols;
@@ -494,7 +503,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
             const uint8_t* p = layer_pages;
             if (!none) p += page * c.page_bytes + (((int64_t)h << sub) + (tl & ((1 << sub) - 1))) * (36 * HD);
             holes |= (none ? 1u : 0u) << ahead;
-            TileLoads<HD>::issue(p, lds.ring[wave] + (i % STAGES) * (36 * HD), lane);
+            TileLoads<HD>::template issue<(SPREAD > 1)>(p, lds.ring[wave] + (i % STAGES) * (36 * HD), lane);
         };
         for (int i = 0; i < min(count, STAGES - 1); ++i) issue(i, i);
 
@@ -659,7 +668,6 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
         for (int i = 0; i < NT; ++i)
             if (SPREAD == 1 || i / 2 == n % SPREAD) lds.o[wave][n / SPREAD][4 * i + g] = acc[i];
         __syncthreads();
-        const int64_t slot = sh.aligned ? (int64_t)blockIdx.x : u.units_before + unit + blockIdx.x;
         for (int i = threadIdx.x; i < COLS * (HD / 4); i += 256) {
             const int cn = i / (HD / 4), d4 = i % (HD / 4);
             const int cc = c0 + cn;
@@ -698,52 +706,81 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
     }
 }
 
-// The splits of a unit joined: a workgroup per unit, as many as there may be.
+// The splits of a column joined by a group of HD / 4 lanes, four elements each: those z = first, first +
+// step, ... below n. A split that saw nothing has a maximum of -inf and adds exp2(-inf) = 0; one whose
+// scores were all NaN has a NaN sum, which no factor takes away.
+struct Joined {
+    float m, l;
+    f32x4 o;
+    __device__ __forceinline__ void add(float m_add, float l_add, const f32x4& o_add, float base) {
+        const float r = __builtin_amdgcn_exp2f(m_add - base);
+        l += l_add != l_add ? l_add : l_add * r;
+        o += o_add * r;
+    }
+    // (a NaN sum with nothing else seen: the outputs are it)
+    __device__ __forceinline__ f32x4 result() const {
+        return l != l ? f32x4{l, l, l, l} : o * (l == 0.0f ? 0.0f : 1.0f / l);
+    }
+};
 template <int HD>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, AttnArgs a, int mode, int grid, Parts parts,
+__device__ __forceinline__ Joined join_splits(const Parts& parts, int64_t slot, int cols, int cn, int d4, int first,
+                                              int step, int n) {
+    const float* ml = parts.ml + (slot * cols + cn) * 2;
+    const float* po = parts.o + (slot * cols + cn) * HD + 4 * d4;
+    Joined j = {kNegInf, 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+    for (int z = first; z < n; z += step) j.m = fmaxf(j.m, ml[(int64_t)z * cols * 2]);
+    const float base = j.m == kNegInf ? 0.0f : j.m;
+#pragma unroll 4
+    for (int z = first; z < n; z += step) {
+        const int64_t at = (int64_t)z * cols;
+        j.add(ml[at * 2], ml[at * 2 + 1], *(const f32x4*)(po + at * HD), base);
+    }
+    return j;
+}
+
+// Direct: a workgroup per column of every unit there may be; its groups take every GROUPS-th split, so
+// the loads of a long list are in flight together, and meet in LDS. Stream, where few units have more
+// than two splits: a workgroup per unit, a group per column.
+template <int HD>
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, AttnArgs a, int splits, Parts parts,
                                                   float* __restrict__ out) {
-    const int lane = threadIdx.x & 63;
-    const Shares sh = shares_of(c, a, mode, grid, lane);
-    const Found u = find_item(c, a, sh, blockIdx.x, true, lane);
-    if (!u.ok) return;
-    const SeqWork w = u.w;
-    const int unit = __builtin_amdgcn_readfirstlane((int)u.rest);
-    int64_t slot;
-    int n_split;
-    if (sh.aligned) {
-        n_split = (int)((w.tiles + sh.q - 1) / sh.q);
-        slot = u.items_before + (int64_t)unit * n_split;
-    } else {
-        const int64_t f0 = u.items_before + (int64_t)unit * w.tiles;
-        const int64_t first = f0 / sh.q;
-        n_split = (int)((f0 + w.tiles - 1) / sh.q - first + 1);
-        slot = u.units_before + unit + first;
+    constexpr int LANES = HD / 4, GROUPS = 256 / LANES;
+    __shared__ f32x4 so[GROUPS][LANES];
+    __shared__ float sm[GROUPS], sl[GROUPS];
+    const int d4 = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+    const auto store = [&](int unit, int r0, int rows, int cn, const f32x4& o) {
+        const int cc = unit / c.n_kv * a.cols + cn, rr = cc / a.G;
+        const int hh = unit % c.n_kv * a.G + (cc - rr * a.G);
+        if (rr < rows) *(f32x4*)(out + ((int64_t)(r0 + rr) * a.n_head + hh) * HD + 4 * d4) = o;
+    };
+    if (splits == 0) {
+        if (blockIdx.x >= *parts.n_units) return;
+        const UnitMap u = parts.map[blockIdx.x];
+        if (u.n_split == 1) return;
+        for (int cn = grp; cn < a.cols && u.unit / c.n_kv * a.cols + cn < u.rows * a.G; cn += GROUPS)
+            store(u.unit, u.r0, u.rows, cn, join_splits<HD>(parts, u.slot, a.cols, cn, d4, 0, 1, u.n_split).result());
+        return;
     }
-    if (n_split == 1) return;
-    const int h = unit % c.n_kv, c0 = unit / c.n_kv * a.cols, n_cols = w.rows * a.G;
-    for (int i = threadIdx.x; i < a.cols * (HD / 4); i += 256) {
-        const int cn = i / (HD / 4), cc = c0 + cn, d4 = i % (HD / 4);
-        if (cc >= n_cols) break;
-        const float* ml = parts.ml + (slot * a.cols + cn) * 2;
-        const float* po = parts.o + (slot * a.cols + cn) * HD + 4 * d4;
-        float mm = kNegInf;
-        for (int z = 0; z < n_split; ++z) mm = fmaxf(mm, ml[(int64_t)z * a.cols * 2]);
-        float ls = 0.0f;
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (mm != kNegInf) {
-            for (int z = 0; z < n_split; ++z) {
-                const float r = __builtin_amdgcn_exp2f(ml[(int64_t)z * a.cols * 2] - mm);
-                ls += ml[(int64_t)z * a.cols * 2 + 1] * r;
-                o += *(const f32x4*)(po + (int64_t)z * a.cols * HD) * r;
-            }
-            o *= ls == 0.0f ? 0.0f : 1.0f / ls;
-        } else {
-            for (int z = 0; z < n_split; ++z) ls += ml[(int64_t)z * a.cols * 2 + 1];
-            o = f32x4{ls, ls, ls, ls};
-        }
-        const int rr = cc / a.G, hh = h * a.G + (cc - rr * a.G);
-        *(f32x4*)(out + ((int64_t)(w.s.r0 + rr) * a.n_head + hh) * HD + 4 * d4) = o;
+    const int uu = (int)blockIdx.x / a.cols, cn = (int)blockIdx.x - uu * a.cols;
+    const int per_seq = c.n_kv * ((a.max_rows * a.G + a.cols - 1) / a.cols), seq = uu / per_seq;
+    const SeqWork w = seq_work(c, a, seq);
+    const int unit = uu - seq * per_seq, n_split = min(splits, (w.tiles + kMinShare - 1) / kMinShare);
+    if (unit >= w.units || n_split == 1 || unit / c.n_kv * a.cols + cn >= w.rows * a.G) return;
+    const Joined mine = join_splits<HD>(parts, (int64_t)uu * splits, a.cols, cn, d4, grp, GROUPS, n_split);
+    so[grp][d4] = mine.o;
+    if (d4 == 0) {
+        sm[grp] = mine.m;
+        sl[grp] = mine.l;
     }
+    __syncthreads();
+    if (grp > 0) return;
+    Joined all = {sm[0], 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+    for (int i = 1; i < GROUPS; ++i) all.m = fmaxf(all.m, sm[i]);
+    const float base = all.m == kNegInf ? 0.0f : all.m;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) all.add(sm[i], sl[i], so[i][d4], base);
+    store(unit, w.s.r0, w.rows, cn, all.result());
 }
 
 // ------------------------------------------------------------------------ store and load
@@ -1059,15 +1096,20 @@ Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int m
     p.cols = (int64_t)max_rows * (n_head / c.n_kv) * nb <= 16 ? 16 / nb : 16;
     const int64_t tiles = std::max(1, (max_len + kTile - 1) / kTile);
     p.units = (int64_t)n_seqs * c.n_kv * (((int64_t)max_rows * (n_head / c.n_kv) + p.cols - 1) / p.cols);
-    p.mode = p.units > kAlignedUnits ? kStream : tiles <= kMinShare ? kWhole : kAligned;
-    p.grid = p.mode == kStream ? kGrid
-             : p.mode == kWhole ? p.units
-                                : std::min<int64_t>(kGrid, p.units * (1 + (tiles + kMinShare - 1) / kMinShare));
+    p.splits = 0;
+    if (p.units > 0 && p.units <= kDirectUnits)
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + kMinShare - 1) / kMinShare, kGrid / p.units));
+    p.grid = p.splits > 0 ? p.units * p.splits : kGrid;
     return p;
 }
 
+static size_t kv4_attention_slots(const Kv4AttnPlan& p) {
+    return (size_t)(p.splits > 0 ? p.grid : p.units + p.grid);
+}
 size_t kv4_attention_ws_bytes(const Kv4AttnPlan& p, int hd) {
-    return p.mode == kWhole ? 0 : (size_t)(p.units + p.grid) * p.cols * (hd + 2) * sizeof(float);
+    if (p.splits == 1) return 0;
+    const size_t part = kv4_attention_slots(p) * p.cols * (hd + 2) * sizeof(float);
+    return p.splits > 0 ? part : part + p.units * sizeof(UnitMap) + sizeof(int64_t);
 }
 
 template <int HD, int SPREAD>
@@ -1077,7 +1119,7 @@ static hipError_t launch_attention(const Kv4View& c, const Kv4AttnPlan& p, int l
     const hipError_t e = limit.raise((const void*)k_kv4_attention<HD, SPREAD>, sizeof(AttnLds<HD>));
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((k_kv4_attention<HD, SPREAD>), dim3((unsigned)p.grid), dim3(256), sizeof(AttnLds<HD>), stream, c,
-                       layer, q, a, p.mode, parts, out);
+                       layer, q, a, p.splits, parts, out);
     return hipGetLastError();
 }
 
@@ -1087,15 +1129,17 @@ hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int laye
     const AttnArgs a = {slots, q_start, n_seqs, n_rows, max_rows, n_head, n_head / c.n_kv, p.cols};
     Parts parts;
     parts.o = (float*)ws;
-    parts.ml = parts.o + (size_t)(p.units + p.grid) * p.cols * c.hd;
+    parts.ml = parts.o + kv4_attention_slots(p) * p.cols * c.hd;
+    parts.map = (UnitMap*)(parts.ml + kv4_attention_slots(p) * p.cols * 2);
+    parts.n_units = (int64_t*)(parts.map + p.units);
     hipError_t e = hipSuccess;
     KV4_HD(c.hd, {
         e = p.cols == 16 ? launch_attention<HD, 1>(c, p, layer, q, a, parts, out, stream)
                          : launch_attention<HD, HD / 32>(c, p, layer, q, a, parts, out, stream);
     });
-    if (e != hipSuccess || p.mode == kWhole) return e;
-    KV4_HD(c.hd, hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)p.units), dim3(256), 0, stream, c, a, p.mode,
-                                    (int)p.grid, parts, out));
+    if (e != hipSuccess || p.splits == 1) return e;
+    KV4_HD(c.hd, hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)(p.splits > 0 ? p.units * p.cols : p.units)), dim3(256), 0, stream, c, a, p.splits,
+                                    parts, out));
     return hipGetLastError();
 }
 
