@@ -1790,13 +1790,13 @@ static int kv4_attention_args(const char* who, const cllm_hip_kv4_cache* cache, 
     if (n_head <= 0 || n_head % c->n_kv != 0 || n_head > 65536)
         return set_err(CLLM_HIP_E_ARG, "%s: n_head must be a multiple of n_head_kv", who);
     if (n_seqs == 0 || n_rows == 0 || max_rows == 0) {
-        *p = Kv4AttnPlan{1, 16, 0, 0};
+        *p = Kv4AttnPlan{false, 1, 16, 0, 0};
         return CLLM_HIP_OK;
     }
     max_rows = std::min(max_rows, n_rows);
     max_len = std::min(max_len, c->max_pages << c->page_shift);
     *p = kv4_attention_plan(*c, n_seqs, max_rows, max_len, n_head);
-    if (p->units > INT32_MAX / 16) return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
+    if (p->units > INT32_MAX / 128 || p->grid > INT32_MAX) return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
     return CLLM_HIP_OK;
 }
 
@@ -1816,8 +1816,10 @@ const char* cllm_hip_kv4_attention_plan(const cllm_hip_kv4_cache* cache, int n_s
     if (kv4_attention_args("kv4_attention", cache, n_seqs, n_rows, max_rows, max_len, n_head, &c, &p) ||
         p.units == 0)
         return "none";
-    snprintf(buf, sizeof buf, "k_kv4_attention<%d,%d> units=%lld splits=%d workgroups=%lld", c.hd, 16 / p.cols,
-             (long long)p.units, p.splits, (long long)p.grid);
+    const int n = p.many_rows ? snprintf(buf, sizeof buf, "k_kv4_many_rows<%d>", c.hd)
+                              : snprintf(buf, sizeof buf, "k_kv4_attention<%d,%d>", c.hd, 16 / p.cols);
+    snprintf(buf + n, sizeof buf - n, " units=%lld splits=%d workgroups=%lld", (long long)p.units, p.splits,
+             (long long)p.grid);
     return buf;
 }
 

@@ -706,6 +706,271 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
     }
 }
 
+// ------------------------------------------------------------------------------- many rows
+//
+// A workgroup of four waves has COLS (row, head) pairs of a KV head, NC column tiles of 16 to a wave.
+// Tiles are dequantized once for all of them, into fp16 fragments in LDS (fragment, lane, 16 bytes: no
+// bank is hit twice), TPI tiles at a time in two buffers: the codes of the tiles after the next are
+// loaded while the next ones' fragments are written and the present ones' are multiplied, with one
+// barrier a turn. Every wave has its own columns, so nothing else is shared.
+//
+// What bounds it: the MFMAs, four per 16 x 16 x 32 block of scores (two parts of the queries, two of the
+// weights).
+template <int HD>
+struct ManyRows {
+    static constexpr int NC = HD == 64 ? 4 : HD == 128 ? 2 : 1, COLS = 4 * NC * 16;
+    static constexpr int FRAGS = HD / 8;               // of a tile: HD / 16 of keys, then HD / 16 of values
+    static constexpr int TPI = HD == 256 ? 1 : 2;
+    static constexpr int LDS = 2 * TPI * FRAGS * 1024;
+};
+
+// A wave's part of a tile on its way to LDS: fragments wave, wave + 4, ... of keys and values.
+template <int HD>
+struct Staged {
+    static constexpr int KW = HD / 32, W = KW < 4 ? KW : 4, C = KW / W, PER = HD / 64;
+    uint32_t k[PER], v[PER], ks[C];
+    u32x4 vs[PER];
+    int limit;  // positions of the tile with values (0: no page)
+
+    // wave 0 .. 3; null: no page
+    __device__ __forceinline__ void load(const uint8_t* tile, int limit_, int wave, int lane) {
+        limit = tile ? limit_ : 0;
+        if (!tile) return;
+        const int g = lane >> 4, n = lane & 15;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int f = wave + 4 * i, t = f / KW, j = f % KW;
+            k[i] = *(const uint32_t*)(tile + ((t * C + j / W) * 64 + lane) * (4 * W) + (j % W) * 4);
+            v[i] = *(const uint32_t*)(tile + 16 * HD + ((f / 4) * 64 + lane) * 16 + (f % 4) * 4);
+            vs[i] = *(const u32x4*)(tile + 34 * HD + ((f / 2) * 4 + g) * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            ks[i] = ((const uint32_t*)(tile + 32 * HD))[(HD == 64 ? g >> 1 : HD == 128 ? g : 2 * g + i) * 16 + n];
+    }
+    __device__ __forceinline__ void store(uint8_t* frags, int wave, int lane, const Magic& mg) {
+        const int g = lane >> 4;
+        if (limit < kTile) {  // bytes that no store has written: their scales may be NaN
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int at = 16 * (r >> 1) + 4 * g + 2 * (r & 1);
+                const uint32_t m = (at < limit ? 0x0000FFFFu : 0u) | (at + 1 < limit ? 0xFFFF0000u : 0u);
+#pragma unroll
+                for (int i = 0; i < PER; ++i) vs[i][r] &= m;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int f = wave + 4 * i, t = f / KW;
+            const uint32_t b = ks[C == 2 ? i & 1 : 0];
+            const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, b, t ? 0x03020302u : 0x01000100u));
+            const h2 dk[4] = {d, d, d, d};
+            *(h8*)(frags + f * 1024 + lane * 16) = dequant8(k[i], dk, mg);
+            const h2 dv[4] = {__builtin_bit_cast(h2, (uint32_t)vs[i].x), __builtin_bit_cast(h2, (uint32_t)vs[i].y),
+                              __builtin_bit_cast(h2, (uint32_t)vs[i].z), __builtin_bit_cast(h2, (uint32_t)vs[i].w)};
+            *(h8*)(frags + (HD / 16 + f) * 1024 + lane * 16) = dequant8(v[i], dv, mg);
+        }
+    }
+};
+
+// grid units * splits. Heavy units come first (a sequence's last rows see the most), and the second
+// workgroup of each CU (of 256) gets the light ones in ascending order.
+template <int HD>
+__global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, const float* __restrict__ q,
+                                                          AttnArgs a, int splits, Parts parts,
+                                                          float* __restrict__ out) {
+    using S = ManyRows<HD>;
+    constexpr int NT = HD / 16, KW = HD / 32, NC = S::NC, TPI = S::TPI;
+    extern __shared__ __align__(16) uint8_t lds_bytes[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const Magic mg;
+
+    const int cts = (a.max_rows * a.G + S::COLS - 1) / S::COLS;
+    int b = blockIdx.x;
+    const int total = gridDim.x;
+    if (b >= 256 && b < min(512, total)) b = 256 + (min(512, total) - 1 - b);
+    const int h = b % c.n_kv;
+    b /= c.n_kv;
+    const int z = b % splits;
+    b /= splits;
+    const int seq = b % a.n_seqs, from_last = b / a.n_seqs;
+    const SeqWork w = seq_work(c, a, seq);
+    const int n_cols = w.rows * a.G, my_cts = (n_cols + S::COLS - 1) / S::COLS;
+    if (from_last >= my_cts) return;
+    const int ct = my_cts - 1 - from_last, c0 = ct * S::COLS;
+    const int p0_seq = w.s.len - w.s.rows;  // position of row 0
+    const int last_row = min(w.rows - 1, (c0 + S::COLS - 1) / a.G);
+    // the unit's own tiles, shared evenly; the join counts with w.tiles >= these
+    const int tiles = max(1, (max(0, p0_seq + last_row + 1) + kTile - 1) / kTile);
+    const int n_split = min(splits, (w.tiles + kMinShare - 1) / kMinShare);
+    if (z >= n_split) return;
+    const int t_begin = (int)((int64_t)tiles * z / n_split), t_end = (int)((int64_t)tiles * (z + 1) / n_split);
+
+    // this wave's columns
+    Queries<HD, 1> qs[NC];
+    int vis[NC];
+    int wave_vis = 0, wave_min = INT32_MAX;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int col = c0 + (wave * NC + i) * 16 + n;
+        const bool valid = col < n_cols;
+        const int row = col / a.G, head = h * a.G + (col - row * a.G);
+        vis[i] = valid ? max(0, p0_seq + row + 1) : 0;
+        qs[i].load(q + ((int64_t)(w.s.r0 + (valid ? row : 0)) * a.n_head + head) * HD, valid, g, n, mg);
+        const int first = c0 + (wave * NC + i) * 16;
+        if (first < n_cols) {
+            wave_vis = max(wave_vis, max(0, p0_seq + min(w.rows - 1, (first + 15) / a.G) + 1));
+            wave_min = min(wave_min, max(0, p0_seq + first / a.G + 1));
+        }
+    }
+    f32x4 acc[NC][NT];
+    float m[NC], l[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        m[i] = kNegInf;
+        l[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    const int sub = c.page_shift - 5;
+    const int32_t* table = c.table + (int64_t)w.s.slot * c.max_pages;
+    const uint8_t* const layer_pages = c.pages + (int64_t)layer * c.n_pages * c.page_bytes;
+    Staged<HD> st[TPI];
+    uint32_t holes = 0;  // bit per tile of the staged turn
+    const auto load = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < TPI; ++i) {
+            const int tl = t0 + i;
+            const uint8_t* p = nullptr;
+            if (tl < t_end) {
+                const int page = table[tl >> sub];
+                if ((unsigned)page < (unsigned)c.n_pages)
+                    p = layer_pages + page * c.page_bytes + (((int64_t)h << sub) + (tl & ((1 << sub) - 1))) * (36 * HD);
+            }
+            holes = (holes & ~(1u << i)) | ((p == nullptr ? 1u : 0u) << i);
+            st[i].load(p, min(kTile, w.s.len - tl * kTile), wave, lane);
+        }
+    };
+    const auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < TPI; ++i) st[i].store(lds_bytes + (buf * TPI + i) * S::FRAGS * 1024, wave, lane, mg);
+    };
+
+    const auto step = [&](const uint8_t* frags, int p0, bool hole) {
+        f32x4 s[NC][2];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) s[i][0] = s[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const h8 k = *(const h8*)(frags + (t * KW + j) * 1024 + lane * 16);
+#pragma unroll
+                for (int i = 0; i < NC; ++i) s[i][t] = mfma(k, qs[i].hi[j], s[i][t]);
+#pragma unroll
+                for (int i = 0; i < NC; ++i) s[i][t] = mfma(k, qs[i].lo[j], s[i][t]);
+            }
+        }
+        if (hole || p0 + kTile > wave_min) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int end = hole ? -1 : vis[i] - p0 - 4 * g;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    s[i][e >> 2][e & 3] = 16 * (e >> 2) + (e & 3) >= end ? kNegInf : s[i][e >> 2][e & 3];
+            }
+        }
+        float mx[NC];
+        bool grow = false;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            mx[i] = s[i][0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) mx[i] = fmaxf(mx[i], s[i][e >> 2][e & 3]);
+            mx[i] = max_over_g(mx[i]) * qs[i].sc;
+            grow |= mx[i] > m[i];
+        }
+        if (__any(grow)) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const float m_new = fmaxf(m[i], mx[i]);
+                const float r = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m[i] - m_new);
+                m[i] = m_new;
+                l[i] *= r;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] *= r;
+            }
+        }
+        h8 hi[NC], lo[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const float mm = 15.0f - (m[i] == kNegInf ? 0.0f : m[i]);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e >> 2][e & 3], qs[i].sc, mm));
+                l[i] += x[e];
+            }
+            split8(x, hi[i], lo[i], mg);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const h8 v = *(const h8*)(frags + (NT + j) * 1024 + lane * 16);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) acc[i][j] = mfma(v, hi[i], acc[i][j]);
+#pragma unroll
+            for (int i = 0; i < NC; ++i) acc[i][j] = mfma(v, lo[i], acc[i][j]);
+        }
+    };
+
+    load(t_begin);
+    uint32_t holes_now = holes;
+    put(0);
+    load(t_begin + TPI);
+    __syncthreads();
+    int buf = 0;
+    for (int t0 = t_begin; t0 < t_end; t0 += TPI, buf ^= 1) {
+        const uint32_t holes_next = holes;
+        if (t0 + TPI < t_end) {
+            put(buf ^ 1);
+            load(t0 + 2 * TPI);
+        }
+#pragma unroll
+        for (int i = 0; i < TPI; ++i) {
+            const int p0 = (t0 + i) * kTile;
+            if (t0 + i < t_end && p0 < wave_vis)
+                step(lds_bytes + (buf * TPI + i) * S::FRAGS * 1024, p0, (holes_now >> i) & 1);
+        }
+        holes_now = holes_next;
+        __syncthreads();
+    }
+
+    const int64_t slot = ((int64_t)(seq * cts + ct) * c.n_kv + h) * splits + z;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int cn = (wave * NC + i) * 16 + n, col = c0 + cn;
+        const float ls = sum_over_g(l[i]);
+        if (col >= n_cols) continue;
+        if (n_split == 1) {
+            const int row = col / a.G, head = h * a.G + (col - row * a.G);
+            float* o = out + ((int64_t)(w.s.r0 + row) * a.n_head + head) * HD + 4 * g;
+            const float inv = ls == 0.0f ? 0.0f : 1.0f / ls;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) *(f32x4*)(o + 16 * j) = ls != ls ? f32x4{ls, ls, ls, ls} : acc[i][j] * inv;
+        } else {
+            float* o = parts.o + (slot * S::COLS + cn) * HD + 4 * g;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) *(f32x4*)(o + 16 * j) = acc[i][j];
+            if (g == 0) {
+                parts.ml[(slot * S::COLS + cn) * 2] = m[i];
+                parts.ml[(slot * S::COLS + cn) * 2 + 1] = ls;
+            }
+        }
+    }
+}
+
 // The splits of a column joined by a group of HD / 4 lanes, four elements each: those z = first, first +
 // step, ... below n. A split that saw nothing has a maximum of -inf and adds exp2(-inf) = 0; one whose
 // scores were all NaN has a NaN sum, which no factor takes away.
@@ -738,9 +1003,10 @@ __device__ __forceinline__ Joined join_splits(const Parts& parts, int64_t slot, 
     return j;
 }
 
-// Direct: a workgroup per column of every unit there may be; its groups take every GROUPS-th split, so
-// the loads of a long list are in flight together, and meet in LDS. Stream, where few units have more
-// than two splits: a workgroup per unit, a group per column.
+// Up to kFewSplits splits (many rows, or streamed shares): a workgroup has a unit's GROUPS columns, one
+// each. More: a workgroup per column, whose groups take every GROUPS-th split, so the loads of a long
+// list are in flight together, and meet in LDS.
+constexpr int kFewSplits = 4;
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, AttnArgs a, int splits, Parts parts,
                                                   float* __restrict__ out) {
@@ -753,16 +1019,30 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, AttnArgs a, int spl
         const int hh = unit % c.n_kv * a.G + (cc - rr * a.G);
         if (rr < rows) *(f32x4*)(out + ((int64_t)(r0 + rr) * a.n_head + hh) * HD + 4 * d4) = o;
     };
-    if (splits == 0) {
-        if (blockIdx.x >= *parts.n_units) return;
-        const UnitMap u = parts.map[blockIdx.x];
-        if (u.n_split == 1) return;
-        for (int cn = grp; cn < a.cols && u.unit / c.n_kv * a.cols + cn < u.rows * a.G; cn += GROUPS)
-            store(u.unit, u.r0, u.rows, cn, join_splits<HD>(parts, u.slot, a.cols, cn, d4, 0, 1, u.n_split).result());
+    const int per_seq = c.n_kv * ((a.max_rows * a.G + a.cols - 1) / a.cols);
+    if (splits <= kFewSplits) {
+        const int per_unit = (a.cols + GROUPS - 1) / GROUPS, uu = (int)blockIdx.x / per_unit;
+        const int cn = ((int)blockIdx.x - uu * per_unit) * GROUPS + grp;
+        UnitMap u;
+        if (splits == 0) {
+            if (uu >= *parts.n_units) return;
+            u = parts.map[uu];
+        } else {
+            const int seq = uu / per_seq;
+            const SeqWork w = seq_work(c, a, seq);
+            u.unit = uu - seq * per_seq;
+            if (u.unit >= w.units) return;
+            u.n_split = min(splits, (w.tiles + kMinShare - 1) / kMinShare);
+            u.slot = (int64_t)uu * splits;
+            u.r0 = w.s.r0;
+            u.rows = w.rows;
+        }
+        if (u.n_split == 1 || cn >= a.cols || u.unit / c.n_kv * a.cols + cn >= u.rows * a.G) return;
+        store(u.unit, u.r0, u.rows, cn, join_splits<HD>(parts, u.slot, a.cols, cn, d4, 0, 1, u.n_split).result());
         return;
     }
     const int uu = (int)blockIdx.x / a.cols, cn = (int)blockIdx.x - uu * a.cols;
-    const int per_seq = c.n_kv * ((a.max_rows * a.G + a.cols - 1) / a.cols), seq = uu / per_seq;
+    const int seq = uu / per_seq;
     const SeqWork w = seq_work(c, a, seq);
     const int unit = uu - seq * per_seq, n_split = min(splits, (w.tiles + kMinShare - 1) / kMinShare);
     if (unit >= w.units || n_split == 1 || unit / c.n_kv * a.cols + cn >= w.rows * a.G) return;
@@ -1089,16 +1369,28 @@ hipError_t launch_kv4_load(const Kv4View& c, int layer, const int32_t* slots, co
     return hipGetLastError();
 }
 
+// Columns of a KV head up to which the one-tile kernel runs: it reads the cache once per 16 of them.
+constexpr int kFewCols = 64;
+
 Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int max_len, int n_head) {
     Kv4AttnPlan p;
+    const int64_t cols = (int64_t)max_rows * (n_head / c.n_kv);
+    const int64_t tiles = std::max(1, (max_len + kTile - 1) / kTile), shares = (tiles + kMinShare - 1) / kMinShare;
+    p.many_rows = cols > kFewCols;
+    if (p.many_rows) {
+        KV4_HD(c.hd, p.cols = ManyRows<HD>::COLS);
+        p.units = (int64_t)n_seqs * c.n_kv * ((cols + p.cols - 1) / p.cols);
+        p.splits = (int)std::max<int64_t>(1, std::min(shares, p.units > 0 ? kGrid / p.units : 1));
+        p.grid = p.units * p.splits;
+        return p;
+    }
     // the columns carry the blocks where all (row, head) pairs of a KV head fit beside each other
     const int nb = c.hd / 32;
-    p.cols = (int64_t)max_rows * (n_head / c.n_kv) * nb <= 16 ? 16 / nb : 16;
-    const int64_t tiles = std::max(1, (max_len + kTile - 1) / kTile);
-    p.units = (int64_t)n_seqs * c.n_kv * (((int64_t)max_rows * (n_head / c.n_kv) + p.cols - 1) / p.cols);
+    p.cols = cols * nb <= 16 ? 16 / nb : 16;
+    p.units = (int64_t)n_seqs * c.n_kv * ((cols + p.cols - 1) / p.cols);
     p.splits = 0;
     if (p.units > 0 && p.units <= kDirectUnits)
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((tiles + kMinShare - 1) / kMinShare, kGrid / p.units));
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(shares, kGrid / p.units));
     p.grid = p.splits > 0 ? p.units * p.splits : kGrid;
     return p;
 }
@@ -1123,6 +1415,17 @@ static hipError_t launch_attention(const Kv4View& c, const Kv4AttnPlan& p, int l
     return hipGetLastError();
 }
 
+template <int HD>
+static hipError_t launch_many_rows(const Kv4View& c, const Kv4AttnPlan& p, int layer, const float* q, const AttnArgs& a,
+                                   const Parts& parts, float* out, hipStream_t stream) {
+    static LdsLimit limit;
+    const hipError_t e = limit.raise((const void*)k_kv4_many_rows<HD>, ManyRows<HD>::LDS);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((k_kv4_many_rows<HD>), dim3((unsigned)p.grid), dim3(256), ManyRows<HD>::LDS, stream, c, layer, q,
+                       a, p.splits, parts, out);
+    return hipGetLastError();
+}
+
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int layer, const float* q,
                                 const int32_t* slots, const int32_t* q_start, int n_seqs, int n_rows,
                                 int max_rows, int n_head, float* out, void* ws, hipStream_t stream) {
@@ -1134,12 +1437,16 @@ hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int laye
     parts.n_units = (int64_t*)(parts.map + p.units);
     hipError_t e = hipSuccess;
     KV4_HD(c.hd, {
-        e = p.cols == 16 ? launch_attention<HD, 1>(c, p, layer, q, a, parts, out, stream)
-                         : launch_attention<HD, HD / 32>(c, p, layer, q, a, parts, out, stream);
+        e = p.many_rows ? launch_many_rows<HD>(c, p, layer, q, a, parts, out, stream)
+            : p.cols == 16 ? launch_attention<HD, 1>(c, p, layer, q, a, parts, out, stream)
+                           : launch_attention<HD, HD / 32>(c, p, layer, q, a, parts, out, stream);
     });
     if (e != hipSuccess || p.splits == 1) return e;
-    KV4_HD(c.hd, hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)(p.splits > 0 ? p.units * p.cols : p.units)), dim3(256), 0, stream, c, a, p.splits,
-                                    parts, out));
+    KV4_HD(c.hd, {
+        constexpr int GROUPS = 256 / (HD / 4);
+        const int64_t blocks = p.units * (p.splits <= kFewSplits ? (p.cols + GROUPS - 1) / GROUPS : p.cols);
+        hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)blocks), dim3(256), 0, stream, c, a, p.splits, parts, out);
+    });
     return hipGetLastError();
 }
 

@@ -62,6 +62,7 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4View& c, const int32_t* slots
 
 // Attention (k_kv4.hip). ws: kv4_attention_ws_bytes bytes.
 struct Kv4AttnPlan {
+    bool many_rows; // the kernel for many rows
     int splits;     // workgroups per unit, 0: shares across units (k_kv4.hip)
     int cols;       // (row, head) pairs of a workgroup
     int64_t units;  // column tiles of the KV heads of the sequences, at most
