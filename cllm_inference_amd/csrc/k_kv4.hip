@@ -25,6 +25,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNegInf = -__builtin_huge_valf();
 constexpr int kTile = 32;  // positions of a tile
+// Weights are exp2(score - m + kTop), m the running maximum when the accumulators were last rescaled:
+// they are not until a score passes m by kSlack (with scores of unit spread, a tile in three raised the
+// maximum of some column). Weights stay within 2^15, and the fp16 parts of one that is the largest so far
+// reach down to 2^-24, 2^-35 of it.
+constexpr float kTop = 11.0f, kSlack = 4.0f;
 
 __device__ __forceinline__ f32x4 mfma(const h8& a, const h8& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -287,7 +292,8 @@ __device__ __forceinline__ float sum_over_blocks(float v) {
 //   the lengths are, for a few restarts where a share crosses units.
 // Partial results lie in slots (direct: unit * splits + split; stream: unit + workgroup, which grows
 // along the staircase of pairs), and a second launch joins them.
-constexpr int kGrid = 512;          // stream: two workgroups on each of 256 CUs
+constexpr int kCus = 256;
+constexpr int kGrid = 2 * kCus;     // workgroups of the one-tile kernel that run at once
 constexpr int kDirectUnits = 256;
 constexpr int kMinShare = 8;        // tiles
 
@@ -566,7 +572,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
             mx = max_over_g(mx) * qs.sc;
-            bool grow = mx > m;
+            bool grow = mx > m + kSlack;
             uint32_t d_max = 0;
             if constexpr (SPREAD > 1) {  // the lane's largest |scale|, as fp16 bits
                 typedef uint16_t us2 __attribute__((ext_vector_type(2)));
@@ -582,8 +588,8 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
                 float r = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
                 m = m_new;
                 if constexpr (SPREAD > 1) {
-                    // the weights times 2^(15 - bound_ex) times a scale below 2^bound_ex stay within
-                    // 2^15; a factor of two in hand, so that few tiles raise the bound
+                    // the weights times a scale below 2^bound_ex times 2^-bound_ex stay within 2^15; a
+                    // factor of two in hand, so that few tiles raise the bound
                     const float all = max_over_g(f16_to_f32(d_max));
                     if (all > bound) {
                         const int ex = __builtin_amdgcn_frexp_expf(all) + 1;
@@ -598,8 +604,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
 #pragma unroll
                 for (int i = 0; i < NT; ++i) acc[i] *= r;
             }
-            // weights times 2^15: as fp16 pairs they keep 20 bits down to 2^-19 of the largest
-            const float mm = 15.0f - (m == kNegInf ? 0.0f : m) - (float)bound_ex;
+            const float mm = kTop - (m == kNegInf ? 0.0f : m) - (float)bound_ex;
             h8 hi, lo;
             if constexpr (SPREAD > 1) {
                 const float mo = mm - 4.0f;
@@ -708,47 +713,50 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
 
 // ------------------------------------------------------------------------------- many rows
 //
-// A workgroup of four waves has COLS (row, head) pairs of a KV head, NC column tiles of 16 to a wave.
-// Tiles are dequantized once for all of them, into fp16 fragments in LDS (fragment, lane, 16 bytes: no
-// bank is hit twice), TPI tiles at a time in two buffers: the codes of the tiles after the next are
-// loaded while the next ones' fragments are written and the present ones' are multiplied, with one
-// barrier a turn. Every wave has its own columns, so nothing else is shared.
+// A workgroup of eight waves has COLS (row, head) pairs of a KV head, NC column tiles of 16 to a wave.
+// Waves 0-3 take the first half of a turn's TURN tiles, waves 4-7, with the same columns, the second
+// half; the two meet at the end. Tiles are dequantized once for all waves, into fp16 fragments in LDS
+// (fragment, lane, 16 bytes: no bank is hit twice), a turn at a time in two buffers: the codes of the
+// turn after the next are loaded while the next one's fragments are written and the present ones are
+// multiplied, with one barrier a turn.
 //
-// What bounds it: the MFMAs, four per 16 x 16 x 32 block of scores (two parts of the queries, two of the
-// weights).
+// What bounds it: VALU beside MFMA work. 32 positions x 32 columns of HD 128 take 64 MFMAs of 16 cycles
+// (two parts of the queries, two of the weights) and about 190 VALU operations, 75 of them the wave's
+// share of the dequantization.
 template <int HD>
 struct ManyRows {
     static constexpr int NC = HD == 64 ? 4 : HD == 128 ? 2 : 1, COLS = 4 * NC * 16;
-    static constexpr int FRAGS = HD / 8;               // of a tile: HD / 16 of keys, then HD / 16 of values
-    static constexpr int TPI = HD == 256 ? 1 : 2;
-    static constexpr int LDS = 2 * TPI * FRAGS * 1024;
+    static constexpr int FRAGS = HD / 8;  // of a tile: HD / 16 of keys, then HD / 16 of values
+    static constexpr int TURN = HD == 256 ? 2 : 4;
+    static constexpr int RING = 2 * TURN * FRAGS * 1024;
+    // the second half's results: accumulators, then maxima and sums
+    static constexpr int MEET = 4 * NC * (HD / 16) * 1024, LDS = RING > MEET + 4 * NC * 512 ? RING : MEET + 4 * NC * 512;
+    // HD 64 has four fragments of either kind: waves 0-3 stage a turn's even tiles, waves 4-7 the odd ones
+    static constexpr int SKIP = HD == 64 ? 2 : 1, STAGED = TURN / SKIP;
 };
 
-// A wave's part of a tile on its way to LDS: fragments wave, wave + 4, ... of keys and values.
+// A wave's part of a tile on its way to LDS: key and value fragments f0, f0 + 8.
 template <int HD>
 struct Staged {
-    static constexpr int KW = HD / 32, W = KW < 4 ? KW : 4, C = KW / W, PER = HD / 64;
-    uint32_t k[PER], v[PER], ks[C];
+    static constexpr int KW = HD / 32, W = KW < 4 ? KW : 4, C = KW / W, PER = HD == 256 ? 2 : 1;
+    uint32_t k[PER], v[PER], ks;
     u32x4 vs[PER];
     int limit;  // positions of the tile with values (0: no page)
 
-    // wave 0 .. 3; null: no page
-    __device__ __forceinline__ void load(const uint8_t* tile, int limit_, int wave, int lane) {
+    __device__ __forceinline__ void load(const uint8_t* tile, int limit_, int f0, int lane) {
         limit = tile ? limit_ : 0;
         if (!tile) return;
         const int g = lane >> 4, n = lane & 15;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int f = wave + 4 * i, t = f / KW, j = f % KW;
+            const int f = f0 + 8 * i, t = f / KW, j = f % KW;
             k[i] = *(const uint32_t*)(tile + ((t * C + j / W) * 64 + lane) * (4 * W) + (j % W) * 4);
             v[i] = *(const uint32_t*)(tile + 16 * HD + ((f / 4) * 64 + lane) * 16 + (f % 4) * 4);
             vs[i] = *(const u32x4*)(tile + 34 * HD + ((f / 2) * 4 + g) * 16);
         }
-#pragma unroll
-        for (int i = 0; i < C; ++i)
-            ks[i] = ((const uint32_t*)(tile + 32 * HD))[(HD == 64 ? g >> 1 : HD == 128 ? g : 2 * g + i) * 16 + n];
+        ks = ((const uint32_t*)(tile + 32 * HD))[(HD == 64 ? g >> 1 : HD == 128 ? g : 2 * g + f0 / 4) * 16 + n];
     }
-    __device__ __forceinline__ void store(uint8_t* frags, int wave, int lane, const Magic& mg) {
+    __device__ __forceinline__ void store(uint8_t* frags, int f0, int lane, const Magic& mg) {
         const int g = lane >> 4;
         if (limit < kTile) {  // bytes that no store has written: their scales may be NaN
 #pragma unroll
@@ -761,9 +769,8 @@ struct Staged {
         }
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int f = wave + 4 * i, t = f / KW;
-            const uint32_t b = ks[C == 2 ? i & 1 : 0];
-            const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(b, b, t ? 0x03020302u : 0x01000100u));
+            const int f = f0 + 8 * i;
+            const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(ks, ks, f / KW ? 0x03020302u : 0x01000100u));
             const h2 dk[4] = {d, d, d, d};
             *(h8*)(frags + f * 1024 + lane * 16) = dequant8(k[i], dk, mg);
             const h2 dv[4] = {__builtin_bit_cast(h2, (uint32_t)vs[i].x), __builtin_bit_cast(h2, (uint32_t)vs[i].y),
@@ -773,35 +780,45 @@ struct Staged {
     }
 };
 
-// grid units * splits. Heavy units come first (a sequence's last rows see the most), and the second
-// workgroup of each CU (of 256) gets the light ones in ascending order.
+// grid units * splits, the heaviest first, so that the last ones to start are short: the sequences by
+// their tiles (up to 64 of them), the last rows of a sequence before the first, and all KV heads of a
+// column tile side by side.
 template <int HD>
-__global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, const float* __restrict__ q,
+__global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, const float* __restrict__ q,
                                                           AttnArgs a, int splits, Parts parts,
                                                           float* __restrict__ out) {
     using S = ManyRows<HD>;
-    constexpr int NT = HD / 16, KW = HD / 32, NC = S::NC, TPI = S::TPI;
+    constexpr int NT = HD / 16, KW = HD / 32, NC = S::NC, TURN = S::TURN;
     extern __shared__ __align__(16) uint8_t lds_bytes[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int half = wave >> 2, cw = wave & 3;
     const int g = lane >> 4, n = lane & 15;
     const Magic mg;
 
     const int cts = (a.max_rows * a.G + S::COLS - 1) / S::COLS;
     int b = blockIdx.x;
-    const int total = gridDim.x;
-    if (b >= 256 && b < min(512, total)) b = 256 + (min(512, total) - 1 - b);
     const int h = b % c.n_kv;
     b /= c.n_kv;
     const int z = b % splits;
     b /= splits;
-    const int seq = b % a.n_seqs, from_last = b / a.n_seqs;
+    const int from_last = b % cts;
+    int seq = b / cts;
+    if (a.n_seqs <= 64) {
+        const int mine = lane < a.n_seqs ? seq_work(c, a, lane).tiles : -1;
+        int rank = 0;
+        for (int j = 0; j < a.n_seqs; ++j) {
+            const int t = __builtin_amdgcn_readlane(mine, j);
+            rank += t > mine || (t == mine && j < lane);
+        }
+        seq = __builtin_ctzll(__ballot(rank == seq && lane < a.n_seqs));
+    }
     const SeqWork w = seq_work(c, a, seq);
     const int n_cols = w.rows * a.G, my_cts = (n_cols + S::COLS - 1) / S::COLS;
     if (from_last >= my_cts) return;
     const int ct = my_cts - 1 - from_last, c0 = ct * S::COLS;
     const int p0_seq = w.s.len - w.s.rows;  // position of row 0
     const int last_row = min(w.rows - 1, (c0 + S::COLS - 1) / a.G);
-    // the unit's own tiles, shared evenly; the join counts with w.tiles >= these
+    // the unit's own tiles in as many splits as the join counts (by the sequence's)
     const int tiles = max(1, (max(0, p0_seq + last_row + 1) + kTile - 1) / kTile);
     const int n_split = min(splits, (w.tiles + kMinShare - 1) / kMinShare);
     if (z >= n_split) return;
@@ -813,12 +830,11 @@ __global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, 
     int wave_vis = 0, wave_min = INT32_MAX;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int col = c0 + (wave * NC + i) * 16 + n;
+        const int first = c0 + (cw * NC + i) * 16, col = first + n;
         const bool valid = col < n_cols;
-        const int row = col / a.G, head = h * a.G + (col - row * a.G);
+        const int row = valid ? col / a.G : 0, head = h * a.G + (valid ? col - row * a.G : 0);
         vis[i] = valid ? max(0, p0_seq + row + 1) : 0;
-        qs[i].load(q + ((int64_t)(w.s.r0 + (valid ? row : 0)) * a.n_head + head) * HD, valid, g, n, mg);
-        const int first = c0 + (wave * NC + i) * 16;
+        qs[i].load(q + ((int64_t)(w.s.r0 + row) * a.n_head + head) * HD, valid, g, n, mg);
         if (first < n_cols) {
             wave_vis = max(wave_vis, max(0, p0_seq + min(w.rows - 1, (first + 15) / a.G) + 1));
             wave_min = min(wave_min, max(0, p0_seq + first / a.G + 1));
@@ -837,11 +853,13 @@ __global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, 
     const int sub = c.page_shift - 5;
     const int32_t* table = c.table + (int64_t)w.s.slot * c.max_pages;
     const uint8_t* const layer_pages = c.pages + (int64_t)layer * c.n_pages * c.page_bytes;
-    Staged<HD> st[TPI];
-    uint32_t holes = 0;  // bit per tile of the staged turn
+    const int f0 = HD == 64 ? cw : wave;
+    Staged<HD> st[S::STAGED];
+    uint32_t holes = 0;  // a bit per tile of the turn
     const auto load = [&](int t0) {
+        holes = 0;
 #pragma unroll
-        for (int i = 0; i < TPI; ++i) {
+        for (int i = 0; i < TURN; ++i) {
             const int tl = t0 + i;
             const uint8_t* p = nullptr;
             if (tl < t_end) {
@@ -849,13 +867,19 @@ __global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, 
                 if ((unsigned)page < (unsigned)c.n_pages)
                     p = layer_pages + page * c.page_bytes + (((int64_t)h << sub) + (tl & ((1 << sub) - 1))) * (36 * HD);
             }
-            holes = (holes & ~(1u << i)) | ((p == nullptr ? 1u : 0u) << i);
-            st[i].load(p, min(kTile, w.s.len - tl * kTile), wave, lane);
+            holes |= (p == nullptr ? 1u : 0u) << i;
+            if (S::SKIP == 1)
+                st[i].load(p, min(kTile, w.s.len - tl * kTile), f0, lane);
+            else if (i % 2 == half)
+                st[i / 2].load(p, min(kTile, w.s.len - tl * kTile), f0, lane);
         }
     };
     const auto put = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < TPI; ++i) st[i].store(lds_bytes + (buf * TPI + i) * S::FRAGS * 1024, wave, lane, mg);
+        for (int i = 0; i < S::STAGED; ++i) {
+            const int tile = S::SKIP == 1 ? i : 2 * i + half;
+            st[i].store(lds_bytes + (buf * TURN + tile) * S::FRAGS * 1024, f0, lane, mg);
+        }
     };
 
     const auto step = [&](const uint8_t* frags, int p0, bool hole) {
@@ -890,7 +914,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, 
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx[i] = fmaxf(mx[i], s[i][e >> 2][e & 3]);
             mx[i] = max_over_g(mx[i]) * qs[i].sc;
-            grow |= mx[i] > m[i];
+            grow |= mx[i] > m[i] + kSlack;
         }
         if (__any(grow)) {
 #pragma unroll
@@ -906,7 +930,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, 
         h8 hi[NC], lo[NC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const float mm = 15.0f - (m[i] == kNegInf ? 0.0f : m[i]);
+            const float mm = kTop - (m[i] == kNegInf ? 0.0f : m[i]);
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -928,30 +952,49 @@ __global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, 
     load(t_begin);
     uint32_t holes_now = holes;
     put(0);
-    load(t_begin + TPI);
+    load(t_begin + TURN);
     __syncthreads();
     int buf = 0;
-    for (int t0 = t_begin; t0 < t_end; t0 += TPI, buf ^= 1) {
+    for (int t0 = t_begin; t0 < t_end; t0 += TURN, buf ^= 1) {
         const uint32_t holes_next = holes;
-        if (t0 + TPI < t_end) {
+        if (t0 + TURN < t_end) {
             put(buf ^ 1);
-            load(t0 + 2 * TPI);
+            load(t0 + 2 * TURN);
         }
 #pragma unroll
-        for (int i = 0; i < TPI; ++i) {
-            const int p0 = (t0 + i) * kTile;
-            if (t0 + i < t_end && p0 < wave_vis)
-                step(lds_bytes + (buf * TPI + i) * S::FRAGS * 1024, p0, (holes_now >> i) & 1);
+        for (int i = 0; i < TURN / 2; ++i) {
+            const int tl = t0 + half * (TURN / 2) + i, p0 = tl * kTile;
+            if (tl < t_end && p0 < wave_vis)
+                step(lds_bytes + (buf * TURN + half * (TURN / 2) + i) * S::FRAGS * 1024, p0,
+                     (holes_now >> (half * (TURN / 2) + i)) & 1);
         }
         holes_now = holes_next;
         __syncthreads();
     }
 
+    // the halves meet: waves 4-7 hand over what waves 0-3 hold in the same lanes and registers
+    f32x4* const meet = (f32x4*)lds_bytes;
+    float2* const meet_ml = (float2*)(lds_bytes + S::MEET);
+    if (half == 1) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) meet[((cw * NC + i) * NT + j) * 64 + lane] = acc[i][j];
+            meet_ml[(cw * NC + i) * 64 + lane] = float2{m[i], l[i]};
+        }
+    }
+    __syncthreads();
+    if (half == 1) return;
     const int64_t slot = ((int64_t)(seq * cts + ct) * c.n_kv + h) * splits + z;
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
-        const int cn = (wave * NC + i) * 16 + n, col = c0 + cn;
-        const float ls = sum_over_g(l[i]);
+        const float2 other = meet_ml[(cw * NC + i) * 64 + lane];
+        const float m_all = fmaxf(m[i], other.x), base = m_all == kNegInf ? 0.0f : m_all;
+        const float r0 = __builtin_amdgcn_exp2f(m[i] - base), r1 = __builtin_amdgcn_exp2f(other.x - base);
+        const float ls = sum_over_g((l[i] != l[i] ? l[i] : l[i] * r0) + (other.y != other.y ? other.y : other.y * r1));
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = acc[i][j] * r0 + meet[((cw * NC + i) * NT + j) * 64 + lane] * r1;
+        const int cn = (cw * NC + i) * 16 + n, col = c0 + cn;
         if (col >= n_cols) continue;
         if (n_split == 1) {
             const int row = col / a.G, head = h * a.G + (col - row * a.G);
@@ -964,7 +1007,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_many_rows(Kv4View c, int layer, 
 #pragma unroll
             for (int j = 0; j < NT; ++j) *(f32x4*)(o + 16 * j) = acc[i][j];
             if (g == 0) {
-                parts.ml[(slot * S::COLS + cn) * 2] = m[i];
+                parts.ml[(slot * S::COLS + cn) * 2] = m_all;
                 parts.ml[(slot * S::COLS + cn) * 2 + 1] = ls;
             }
         }
@@ -1380,7 +1423,7 @@ Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int m
     if (p.many_rows) {
         KV4_HD(c.hd, p.cols = ManyRows<HD>::COLS);
         p.units = (int64_t)n_seqs * c.n_kv * ((cols + p.cols - 1) / p.cols);
-        p.splits = (int)std::max<int64_t>(1, std::min(shares, p.units > 0 ? kGrid / p.units : 1));
+        p.splits = (int)std::max<int64_t>(1, std::min(shares, p.units > 0 ? kCus / p.units : 1));
         p.grid = p.units * p.splits;
         return p;
     }
@@ -1421,7 +1464,7 @@ static hipError_t launch_many_rows(const Kv4View& c, const Kv4AttnPlan& p, int l
     static LdsLimit limit;
     const hipError_t e = limit.raise((const void*)k_kv4_many_rows<HD>, ManyRows<HD>::LDS);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_kv4_many_rows<HD>), dim3((unsigned)p.grid), dim3(256), ManyRows<HD>::LDS, stream, c, layer, q,
+    hipLaunchKernelGGL((k_kv4_many_rows<HD>), dim3((unsigned)p.grid), dim3(512), ManyRows<HD>::LDS, stream, c, layer, q,
                        a, p.splits, parts, out);
     return hipGetLastError();
 }

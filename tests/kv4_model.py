@@ -227,10 +227,10 @@ def attention_bound(hd, n, size, mass, total):
     at most 2^-20 of itself, the fp32 accumulation of hd products by (hd + 8) 2^-24 of their
     magnitudes, the scaling to log2 units, the subtraction of the maximum and the exponential by
     2^-21 of the score's size and 2^-22; so a weight is off by at most d below, relatively, and the
-    quotient of two sums of weights by 2 d. A weight as two fp16 parts, the largest at 2^15, adds 2^-20
-    of itself, or 2^-24 below fp16's normal numbers, 2^-39 of the largest: that times sum |v| in all,
+    quotient of two sums of weights by 2 d. A weight as two fp16 parts, the largest between 2^11 and 2^15,
+    adds 2^-20 of itself, or 2^-24 below fp16's normal numbers, 2^-35 of the largest: that times sum |v| in all,
     as the weights' sum is at least the largest (an output whose values lie under small weights only
     keeps an absolute accuracy). The running sums of a wave add one rounding per step:
     n / 16 of the denominator, n / 128 of the outputs, and the joins some 64."""
     d = size * (2.0 ** -20 + 3 * (hd + 8) * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -21
-    return mass * (2.2 * d + 2.0 ** -20 + (n / 16 + 3 * n / 128 + 3 * 64) * 2.0 ** -24) + 2.0 ** -39 * total
+    return mass * (2.2 * d + 2.0 ** -20 + (n / 16 + 3 * n / 128 + 3 * 64) * 2.0 ** -24) + 2.0 ** -35 * total
