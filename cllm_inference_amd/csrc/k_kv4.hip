@@ -731,51 +731,69 @@ struct ManyRows {
     static constexpr int RING = 2 * TURN * FRAGS * 1024;
     // the second half's results: accumulators, then maxima and sums
     static constexpr int MEET = 4 * NC * (HD / 16) * 1024, LDS = RING > MEET + 4 * NC * 512 ? RING : MEET + 4 * NC * 512;
-    // HD 64 has four fragments of either kind: waves 0-3 stage a turn's even tiles, waves 4-7 the odd ones
-    static constexpr int SKIP = HD == 64 ? 2 : 1, STAGED = TURN / SKIP;
+    // a tile is staged in KINDS pieces of four fragments, HD / 64 of keys and HD / 64 of values
+    static constexpr int KINDS = HD / 32, STAGED = TURN * KINDS / 8;
 };
 
-// A wave's part of a tile on its way to LDS: key and value fragments f0, f0 + 8.
+// A wave's piece of a tile on its way to LDS: 16 bytes of codes a lane, four fragments. Key pieces are
+// chunks (t, c) of the tile's key codes (HD 64: both halves t), value pieces chunks c of its value codes.
 template <int HD>
 struct Staged {
-    static constexpr int KW = HD / 32, W = KW < 4 ? KW : 4, C = KW / W, PER = HD == 256 ? 2 : 1;
-    uint32_t k[PER], v[PER], ks;
-    u32x4 vs[PER];
+    static constexpr int KW = HD / 32, KEYS = HD / 64;
+    u32x4 x, s0, s1;
     int limit;  // positions of the tile with values (0: no page)
 
-    __device__ __forceinline__ void load(const uint8_t* tile, int limit_, int f0, int lane) {
+    __device__ __forceinline__ void load(const uint8_t* tile, int limit_, int kind, int lane) {
         limit = tile ? limit_ : 0;
         if (!tile) return;
         const int g = lane >> 4, n = lane & 15;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int f = f0 + 8 * i, t = f / KW, j = f % KW;
-            k[i] = *(const uint32_t*)(tile + ((t * C + j / W) * 64 + lane) * (4 * W) + (j % W) * 4);
-            v[i] = *(const uint32_t*)(tile + 16 * HD + ((f / 4) * 64 + lane) * 16 + (f % 4) * 4);
-            vs[i] = *(const u32x4*)(tile + 34 * HD + ((f / 2) * 4 + g) * 16);
-        }
-        ks = ((const uint32_t*)(tile + 32 * HD))[(HD == 64 ? g >> 1 : HD == 128 ? g : 2 * g + f0 / 4) * 16 + n];
-    }
-    __device__ __forceinline__ void store(uint8_t* frags, int f0, int lane, const Magic& mg) {
-        const int g = lane >> 4;
-        if (limit < kTile) {  // bytes that no store has written: their scales may be NaN
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int at = 16 * (r >> 1) + 4 * g + 2 * (r & 1);
-                const uint32_t m = (at < limit ? 0x0000FFFFu : 0u) | (at + 1 < limit ? 0xFFFF0000u : 0u);
-#pragma unroll
-                for (int i = 0; i < PER; ++i) vs[i][r] &= m;
+        if (kind < KEYS) {
+            if constexpr (HD == 64) {
+                const u32x2 a = *(const u32x2*)(tile + lane * 8), b = *(const u32x2*)(tile + 512 + lane * 8);
+                x = u32x4{a.x, a.y, b.x, b.y};
+                s0.x = ((const uint32_t*)(tile + 32 * HD))[(g >> 1) * 16 + n];
+            } else {
+                x = *(const u32x4*)(tile + (kind * 64 + lane) * 16);
+                s0.x = ((const uint32_t*)(tile + 32 * HD))[(HD == 128 ? g : 2 * g + (kind & 1)) * 16 + n];
             }
+        } else {
+            const int c = kind - KEYS;
+            x = *(const u32x4*)(tile + 16 * HD + (c * 64 + lane) * 16);
+            s0 = *(const u32x4*)(tile + 34 * HD + ((2 * c) * 4 + g) * 16);
+            s1 = *(const u32x4*)(tile + 34 * HD + ((2 * c + 1) * 4 + g) * 16);
         }
+    }
+    __device__ __forceinline__ void store(uint8_t* frags, int kind, int lane, const Magic& mg) {
+        if (kind < KEYS) {
+            const auto put = [&](uint32_t w, int t, int j) {
+                const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(s0.x, s0.x, t ? 0x03020302u : 0x01000100u));
+                const h2 d4[4] = {d, d, d, d};
+                *(h8*)(frags + (t * KW + j) * 1024 + lane * 16) = dequant8(w, d4, mg);
+            };
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int f = f0 + 8 * i;
-            const h2 d = __builtin_bit_cast(h2, __builtin_amdgcn_perm(ks, ks, f / KW ? 0x03020302u : 0x01000100u));
-            const h2 dk[4] = {d, d, d, d};
-            *(h8*)(frags + f * 1024 + lane * 16) = dequant8(k[i], dk, mg);
-            const h2 dv[4] = {__builtin_bit_cast(h2, (uint32_t)vs[i].x), __builtin_bit_cast(h2, (uint32_t)vs[i].y),
-                              __builtin_bit_cast(h2, (uint32_t)vs[i].z), __builtin_bit_cast(h2, (uint32_t)vs[i].w)};
-            *(h8*)(frags + (HD / 16 + f) * 1024 + lane * 16) = dequant8(v[i], dv, mg);
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (HD == 64) put(x[i], i >> 1, i & 1);
+                if constexpr (HD == 128) put(x[i], kind, i);
+                if constexpr (HD == 256) put(x[i], kind >> 1, (kind & 1) * 4 + i);
+            }
+        } else {
+            if (limit < kTile) {  // bytes that no store has written: their scales may be NaN
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int at = 16 * (r >> 1) + 4 * (lane >> 4) + 2 * (r & 1);
+                    const uint32_t m = (at < limit ? 0x0000FFFFu : 0u) | (at + 1 < limit ? 0xFFFF0000u : 0u);
+                    s0[r] &= m;
+                    s1[r] &= m;
+                }
+            }
+            const int c = kind - KEYS;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const u32x4 s = i < 2 ? s0 : s1;
+                const h2 d4[4] = {__builtin_bit_cast(h2, (uint32_t)s.x), __builtin_bit_cast(h2, (uint32_t)s.y),
+                                  __builtin_bit_cast(h2, (uint32_t)s.z), __builtin_bit_cast(h2, (uint32_t)s.w)};
+                *(h8*)(frags + (HD / 16 + 4 * c + i) * 1024 + lane * 16) = dequant8(x[i], d4, mg);
+            }
         }
     }
 };
@@ -853,7 +871,8 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
     const int sub = c.page_shift - 5;
     const int32_t* table = c.table + (int64_t)w.s.slot * c.max_pages;
     const uint8_t* const layer_pages = c.pages + (int64_t)layer * c.n_pages * c.page_bytes;
-    const int f0 = HD == 64 ? cw : wave;
+    // the wave's pieces of a turn: the same kind of tiles wave / KINDS, + 8 / KINDS
+    const int kind = wave % S::KINDS, tile0 = wave / S::KINDS;
     Staged<HD> st[S::STAGED];
     uint32_t holes = 0;  // a bit per tile of the turn
     const auto load = [&](int t0) {
@@ -868,21 +887,18 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
                     p = layer_pages + page * c.page_bytes + (((int64_t)h << sub) + (tl & ((1 << sub) - 1))) * (36 * HD);
             }
             holes |= (p == nullptr ? 1u : 0u) << i;
-            if (S::SKIP == 1)
-                st[i].load(p, min(kTile, w.s.len - tl * kTile), f0, lane);
-            else if (i % 2 == half)
-                st[i / 2].load(p, min(kTile, w.s.len - tl * kTile), f0, lane);
+            if (i % (8 / S::KINDS) == tile0) st[i / (8 / S::KINDS)].load(p, min(kTile, w.s.len - tl * kTile), kind, lane);
         }
     };
     const auto put = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < S::STAGED; ++i) {
-            const int tile = S::SKIP == 1 ? i : 2 * i + half;
-            st[i].store(lds_bytes + (buf * TURN + tile) * S::FRAGS * 1024, f0, lane, mg);
-        }
+        for (int i = 0; i < S::STAGED; ++i)
+            st[i].store(lds_bytes + (buf * TURN + tile0 + i * (8 / S::KINDS)) * S::FRAGS * 1024, kind, lane, mg);
     };
 
     const auto step = [&](const uint8_t* frags, int p0, bool hole) {
+        // (the wave that forms scores goes first: its neighbour's softmax fills the gaps; 3% less time)
+        __builtin_amdgcn_s_setprio(1);
         f32x4 s[NC][2];
 #pragma unroll
         for (int i = 0; i < NC; ++i) s[i][0] = s[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -927,6 +943,7 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
                 for (int j = 0; j < NT; ++j) acc[i][j] *= r;
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         h8 hi[NC], lo[NC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
@@ -956,8 +973,10 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
     __syncthreads();
     int buf = 0;
     for (int t0 = t_begin; t0 < t_end; t0 += TURN, buf ^= 1) {
+        // of the two waves on a SIMD (w and w + 4) one writes its fragments before its steps and one
+        // after, so that the one's VALU work runs beside the other's MFMAs
         const uint32_t holes_next = holes;
-        if (t0 + TURN < t_end) {
+        if (half == 0 && t0 + TURN < t_end) {
             put(buf ^ 1);
             load(t0 + 2 * TURN);
         }
@@ -967,6 +986,10 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
             if (tl < t_end && p0 < wave_vis)
                 step(lds_bytes + (buf * TURN + half * (TURN / 2) + i) * S::FRAGS * 1024, p0,
                      (holes_now >> (half * (TURN / 2) + i)) & 1);
+        }
+        if (half == 1 && t0 + TURN < t_end) {
+            put(buf ^ 1);
+            load(t0 + 2 * TURN);
         }
         holes_now = holes_next;
         __syncthreads();
