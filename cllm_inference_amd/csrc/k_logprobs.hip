@@ -52,24 +52,32 @@ __device__ __forceinline__ uint64_t entry_of(uint32_t key, int id) {
     return ((uint64_t)key << 32) | (uint32_t)~id;
 }
 
+// Over the wave, in every lane (DPP inside rows of 16, row swaps between them).
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
-    return v;
+    v = fmaxf(v, dpp_f32<DPP_QUAD_SWAP1>(v));
+    v = fmaxf(v, dpp_f32<DPP_QUAD_SWAP2>(v));
+    v = fmaxf(v, dpp_f32<DPP_ROW_HALF_MIRROR>(v));
+    v = fmaxf(v, dpp_f32<DPP_ROW_MIRROR>(v));
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    v = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
 }
 
-// The wave's 64 values in descending order, lane i the i-th (bitonic).
-__device__ __forceinline__ float wave_sort(float v, int lane) {
-#pragma unroll
-    for (int k = 2; k <= 64; k <<= 1) {
-#pragma unroll
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            const float o = __shfl_xor(v, j, 64);
-            const bool keep_max = ((lane & j) == 0) == ((lane & k) == 0);
-            v = keep_max ? fmaxf(v, o) : fminf(v, o);
-        }
+// A value that at least q (1 .. 64) of the wave's values v (max the largest, none NaN) reach, close to
+// the q-th largest: bisection between the smallest above -inf and the largest, on ballots. -inf where
+// fewer are above it.
+__device__ __forceinline__ float wave_bound(float v, float max, int q) {
+    if (__popcll(__ballot(v > kNegInf)) < q) return kNegInf;
+    float lo = -wave_max(v > kNegInf ? -v : kNegInf), hi = max;
+    if (q == 1) return hi;
+    for (int i = 0; i < 12; ++i) {
+        const float mid = 0.5f * lo + 0.5f * hi;
+        const int c = __popcll(__ballot(v >= mid));
+        if (c >= q) lo = mid; else hi = mid;
+        if (c == q) break;
     }
-    return v;
+    return lo;
 }
 
 // Sum over the workgroup, in every thread; buf: a value per wave, free to write.
@@ -89,7 +97,7 @@ __device__ __forceinline__ int block_sum(int v, int* buf) {
 __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restrict__ logits, int64_t stride, int vocab,
                                                             const int32_t* __restrict__ tokens, int top_k, int parts,
                                                             Part* __restrict__ part, uint64_t* __restrict__ top) {
-    __shared__ float s_f[4][kWaves];
+    __shared__ float s_f[2][kWaves];
     __shared__ int s_i[2][kWaves];
     __shared__ int s_count;
     __shared__ uint64_t s_cand[kCand];
@@ -100,7 +108,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
     const int n = min(kPart, vocab - base);
     if (tid == 0) s_count = 0;
 
-    // -inf past the row's end: adds nothing to a sum, and candidates check the index
+    // -inf past the row's end: adds nothing to a sum, and is no candidate above a bound
     float x[kVecs][4];
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
@@ -118,60 +126,100 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
     const bool have = (unsigned)tok < (unsigned)vocab;
     const float xt = have ? x0[tok] : 0.0f;
 
-    float tmax = kNegInf;  // (NaN never wins)
+    float vmax[kVecs], tmax = kNegInf;  // (NaN never wins)
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) tmax = fmaxf(tmax, x[i][j]);
-    const float wmax = wave_max(tmax);
-    // a bound that at least top_k of the part's logits reach: each wave's (top_k / 4)-th largest
-    // thread maximum is reached by a quarter of them in every wave, its top_k-th by all of them
-    float b_all = kNegInf, b_own = kNegInf;
-    if (top_k > 0) {
-        const float sorted = wave_sort(tmax, lane);
-        b_all = __shfl(sorted, (top_k + kWaves - 1) / kWaves - 1, 64);
-        b_own = __shfl(sorted, top_k - 1, 64);
+    for (int i = 0; i < kVecs; ++i) {
+        vmax[i] = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
+        tmax = fmaxf(tmax, vmax[i]);
     }
-    if (lane == 0) {
-        s_f[0][wave] = wmax;
-        s_f[1][wave] = b_all;
-        s_f[2][wave] = b_own;
+    // a bound that at least top_k of the part's logits reach: a quarter of them in every wave
+    const float wmax = wave_max(tmax);
+    if (lane == 0) s_f[0][wave] = wmax;
+    if (top_k > 0) {
+        const float b = wave_bound(tmax, wmax, (top_k + kWaves - 1) / kWaves);
+        if (lane == 0) s_f[1][wave] = b;
     }
     __syncthreads();
-    float m = s_f[0][0], bound = s_f[1][0], own = s_f[2][0];
+    float m = s_f[0][0], bound = s_f[1][0];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) {
         m = fmaxf(m, s_f[0][w]);
         bound = fminf(bound, s_f[1][w]);
-        own = fmaxf(own, s_f[2][w]);
     }
-    bound = fmaxf(bound, own);
-    const float mu = m == kNegInf ? 0.0f : m;  // (no logit above -inf)
 
+    // candidates: the logits at the bound or above
+    if (top_k > 0 && bound > kNegInf) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+            if (vmax[i] >= bound) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (x[i][j] >= bound) {
+                        const int c = atomicAdd(&s_count, 1);
+                        if (c < kCand) s_cand[c] = entry_of(key_of(x[i][j]), base + (i * kThreads + tid) * 4 + j);
+                    }
+                }
+            }
+        }
+    }
+
+    // tokens ahead of the given one: those above it, and its equals with lower ids
+    int ahead = 0;
+    if (have && xt == xt) {
+        const int rel = tok - base;  // its place in the part, if it is there
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) ahead += __popcll(__ballot(x[i][j] > xt));
+        ahead = lane == 0 ? ahead : 0;
+        bool ties = false;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) ties |= vmax[i] >= xt;  // only then can one of the vector equal it
+        if (rel > 0 && __any(ties)) {
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = (i * kThreads + tid) * 4 + j;
+                    ahead += x[i][j] == xt && at < min(rel, n);
+                }
+        }
+    } else if (have) {  // a NaN: behind all numbers
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int at = (i * kThreads + tid) * 4 + j;
+                ahead += at < n && (x[i][j] == x[i][j] || base + at < tok);
+            }
+    }
+
+    // the sums, without the logits that equal the maximum: they are counted
+    int equal = 0;
+    const float mu = m == kNegInf ? 0.0f : m;  // (no logit above -inf)
+    float y[kVecs][4];
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[i][j] = x[i][j] - mu;
+    if (__any(tmax == mu)) {
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                equal += y[i][j] == 0.0f;
+                y[i][j] = y[i][j] == 0.0f ? kNegInf : y[i][j];
+            }
+    }
     float sum = 0.0f, ent = 0.0f;
-    int equal = 0, ahead = 0;
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            // (exp of -200 and less is 0; NaN passes both selects)
-            const float d = x[i][j] - mu;
-            const float e = __builtin_amdgcn_exp2f(d * kLog2e);
-            equal += d == 0.0f;
-            sum += d == 0.0f ? 0.0f : e;
-            ent -= (d < -200.0f ? 0.0f : d) * e;
-        }
-    }
-    if (have) {
-        const uint32_t kt = key_of(xt);
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int at = (i * kThreads + tid) * 4 + j;
-                const uint32_t k = key_of(x[i][j]);
-                ahead += at < n && (k > kt || (k == kt && base + at < tok));
-            }
+            const float e = __builtin_amdgcn_exp2f(y[i][j] * kLog2e);
+            sum += e;
+            // (exp of -200 and less is 0; a NaN stays in e)
+            ent = __builtin_fmaf(fmaxf(y[i][j], -200.0f), -e, ent);
         }
     }
     sum = wave_sum(sum);
@@ -187,21 +235,6 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
         s_f[1][wave] = ent;
         s_i[0][wave] = equal;
         s_i[1][wave] = ahead;
-    }
-
-    // candidates: the logits at the bound or above
-    if (top_k > 0) {
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int at = (i * kThreads + tid) * 4 + j;
-                if (x[i][j] >= bound && at < n) {
-                    const int c = atomicAdd(&s_count, 1);
-                    if (c < kCand) s_cand[c] = entry_of(key_of(x[i][j]), base + at);
-                }
-            }
-        }
     }
     __syncthreads();
     if (tid == 0) {
@@ -221,9 +254,33 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
     uint64_t* out = top + ((int64_t)row * parts + z) * top_k;
     int count = s_count;
     const int want = min(top_k, n);
-    if (count > kCand) {
-        // Many logits equal the bound (a mask's -inf, a coarse grid of values): of those only the
-        // first by index can be wanted. The index below which top_k of them lie, by bisection.
+    if (bound == kNegInf) {
+        // Few logits above -inf (a mask, a short part): all of those, and the first ids, of which no
+        // more than `above` are no -inf. (A NaN counts as too many.)
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) above += x[i][j] > kNegInf ? 1 : x[i][j] != x[i][j] ? kCand : 0;
+        above = block_sum(above, s_i[0]);
+        if (above <= kCand / 2 - kMaxTopK) {
+            const int first = min(n, want + above);
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = (i * kThreads + tid) * 4 + j;
+                    if (x[i][j] > kNegInf || at < first) {
+                        const int c = atomicAdd(&s_count, 1);
+                        s_cand[c] = entry_of(key_of(x[i][j]), base + at);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        count = s_count;
+    } else if (count > kCand) {
+        // Many logits equal the bound (a coarse grid of values): of those only the first by index can be wanted. The index below which top_k of them lie, by bisection.
         int lo = 0, hi = kPart, above = 0;
         for (int step = 0; step < 14; ++step) {
             const int mid = step == 0 ? 0 : (lo + hi) >> 1;  // (first: the logits above the bound)
@@ -303,7 +360,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
 }
 
 // One workgroup per row: the parts' sums, then the row's largest logits out of the parts' lists. An
-// entry's place is its place in its own list and, by bisection, the entries above it in the others.
+// entry's place is the number of entries above it: counted in LDS over a short list, else its place in
+// its own list and, by bisection, those of the others.
+constexpr int kCount = 512, kStage = 4096;  // entries counted, entries held in LDS
 __global__ __launch_bounds__(kThreads) void k_logprobs_join(const float* __restrict__ logits, int64_t stride, int vocab,
                                                             const int32_t* __restrict__ tokens, int top_k, int parts,
                                                             const Part* __restrict__ part,
@@ -312,15 +371,24 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(const float* __restr
                                                             float* __restrict__ entropy, float* __restrict__ lse,
                                                             int32_t* __restrict__ top_ids,
                                                             float* __restrict__ top_logprobs) {
-    __shared__ double s_log;
-    __shared__ float s_max;
+    __shared__ uint64_t s_top[kStage];
+    __shared__ float s_log, s_max;
+    __shared__ int s_none;
     const int row = blockIdx.x, tid = threadIdx.x;
     const Part* p = part + (int64_t)row * parts;
+    const uint64_t* t = top + (int64_t)row * parts * top_k;
+    const int64_t entries = (int64_t)parts * top_k;
+    const bool staged = entries <= kStage;
+    if (staged)
+        for (int i = tid; i < entries; i += kThreads) s_top[i] = t[i];
     if (tid < 64) {
+        const int tok = tokens ? tokens[row] : -1;
+        const bool have = (unsigned)tok < (unsigned)vocab;
+        const float xt = have && logprobs ? logits[(int64_t)row * stride + tok] : kNegInf;
         float m = kNegInf;
         for (int z = tid; z < parts; z += 64) m = fmaxf(m, p[z].max);
         m = wave_max(m);
-        double sum = 0.0, ent = 0.0;
+        float sum = 0.0f, ent = 0.0f;
         int equal = 0, ahead = 0;
         for (int z = tid; z < parts; z += 64) {
             const Part a = p[z];
@@ -332,58 +400,59 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(const float* __restr
             } else if (a.max == kNegInf) {
                 sum += a.sum;  // 0, or NaN
             } else {
-                const double d = (double)m - a.max, w = exp(-d), s = (double)a.sum + a.equal;
+                const float d = m - a.max, s = a.sum + (float)a.equal, w = __builtin_amdgcn_exp2f(-d * kLog2e);
                 sum += w * s;
                 ent += w * (a.ent + d * s);
             }
         }
+        sum = wave_sum(sum);
+        ent = wave_sum(ent);
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            sum += __shfl_xor(sum, d, 64);
-            ent += __shfl_xor(ent, d, 64);
             equal += __shfl_xor(equal, d, 64);
             ahead += __shfl_xor(ahead, d, 64);
         }
         if (tid == 0) {
-            const bool none = m == kNegInf;
-            // without a logit above -inf the sums are of exp(x) = 0, or NaN
-            const double rest = sum + (equal - 1), log_s = none ? sum : log1p(rest);
+            // without a logit above -inf the sum is 0, or NaN
+            const bool none = m == kNegInf && sum == 0.0f;
+            const float rest = sum + (float)(m == kNegInf ? 0 : equal - 1);
+            const float log_s = m == kNegInf ? sum : log1pf(rest);
             s_log = log_s;
             s_max = m;
-            if (entropy) entropy[row] = (float)(none ? sum : log_s + ent / (1.0 + rest));
-            if (lse) lse[row] = none && sum == 0.0 ? kNegInf : (float)(m + log_s);
-            const int tok = tokens ? tokens[row] : -1;
-            const bool have = (unsigned)tok < (unsigned)vocab;
-            if (logprobs) {
-                const float xt = have ? logits[(int64_t)row * stride + tok] : kNegInf;
-                const double lp = none ? (sum == 0.0 ? (double)kNegInf : sum) : ((double)xt - m) - log_s;
-                logprobs[row] = have ? (float)lp : kNegInf;
-            }
+            s_none = none;
+            if (entropy) entropy[row] = none ? 0.0f : log_s + ent / (1.0f + rest);
+            if (lse) lse[row] = none ? kNegInf : m + log_s;
+            if (logprobs) logprobs[row] = none || !have ? kNegInf : (xt - m) - log_s;
             if (ranks) ranks[row] = have ? ahead : -1;
         }
     }
     if (top_k == 0) return;
     __syncthreads();
-    const uint64_t* t = top + (int64_t)row * parts * top_k;
-    for (int i = tid; i < parts * top_k; i += kThreads) {
-        const int z = i / top_k;
-        const uint64_t e = t[i];
+    for (int64_t i = tid; i < entries; i += kThreads) {
+        const uint64_t e = staged ? s_top[i] : t[i];
         if (e == 0) continue;
-        int above = i - z * top_k;
-        for (int o = 0; o < parts && above < top_k; ++o) {
-            if (o == z) continue;
-            int lo = 0, hi = top_k;  // entries of list o above e
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (t[o * top_k + mid] > e) lo = mid + 1; else hi = mid;
+        int above = 0;
+        if (entries <= kCount) {
+#pragma unroll 8
+            for (int o = 0; o < entries; ++o) above += s_top[o] > e;
+        } else {
+            const int z = (int)(i / top_k);
+            above = (int)(i - (int64_t)z * top_k);
+            for (int o = 0; o < parts && above < top_k; ++o) {
+                if (o == z) continue;
+                int lo = 0, hi = top_k;  // entries of list o above e
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    const int64_t at = (int64_t)o * top_k + mid;
+                    if ((staged ? s_top[at] : t[at]) > e) lo = mid + 1; else hi = mid;
+                }
+                above += lo;
             }
-            above += lo;
         }
         if (above >= top_k) continue;
         const float x = value_of((uint32_t)(e >> 32));
-        const double lp = s_max == kNegInf ? (s_log == 0.0 ? (double)kNegInf : s_log) : ((double)x - s_max) - s_log;
         if (top_ids) top_ids[(int64_t)row * top_k + above] = (int32_t)~(uint32_t)e;
-        if (top_logprobs) top_logprobs[(int64_t)row * top_k + above] = (float)lp;
+        if (top_logprobs) top_logprobs[(int64_t)row * top_k + above] = s_none ? kNegInf : (x - s_max) - s_log;
     }
 }
 
