@@ -52,6 +52,14 @@ __device__ __forceinline__ uint64_t entry_of(uint32_t key, int id) {
     return ((uint64_t)key << 32) | (uint32_t)~id;
 }
 
+// The largest that is no NaN (v_max3_f32; fmaxf would quieten a signalling NaN of each operand first,
+// an operation per logit).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
 // Over the wave, in every lane (DPP inside rows of 16, row swaps between them).
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, dpp_f32<DPP_QUAD_SWAP1>(v));
@@ -129,7 +137,7 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
     float vmax[kVecs], tmax = kNegInf;  // (NaN never wins)
 #pragma unroll
     for (int i = 0; i < kVecs; ++i) {
-        vmax[i] = fmaxf(fmaxf(x[i][0], x[i][1]), fmaxf(x[i][2], x[i][3]));
+        vmax[i] = max3(x[i][0], x[i][1], max3(x[i][2], x[i][3], kNegInf));
         tmax = fmaxf(tmax, vmax[i]);
     }
     // a bound that at least top_k of the part's logits reach: a quarter of them in every wave
@@ -163,52 +171,53 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
         }
     }
 
-    // tokens ahead of the given one: those above it, and its equals with lower ids
+    // Tokens ahead of the given one: those above it, and its equals with lower ids, which are above the
+    // next number below it.
     int ahead = 0;
-    if (have && xt == xt) {
+    if (have && xt > kNegInf) {
         const int rel = tok - base;  // its place in the part, if it is there
+        const uint32_t u = __builtin_bit_cast(uint32_t, xt);
+        const float below = __builtin_bit_cast(float, xt > 0.0f ? u - 1 : xt < 0.0f ? u + 1 : 0x80000001u);
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i)
+        for (int i = 0; i < kVecs; ++i) {
+            const float than = (i * kThreads + tid) * 4 + 3 < rel ? below : xt;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) ahead += __popcll(__ballot(x[i][j] > xt));
+            for (int j = 0; j < 4; ++j) ahead += __popcll(__ballot(x[i][j] > than));
+        }
         ahead = lane == 0 ? ahead : 0;
-        bool ties = false;
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) ties |= vmax[i] >= xt;  // only then can one of the vector equal it
-        if (rel > 0 && __any(ties)) {
+        if (rel >= 0 && rel < n && (rel >> 8 & (kWaves - 1)) == wave) {  // the wave with the token's own vector
 #pragma unroll
             for (int i = 0; i < kVecs; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int at = (i * kThreads + tid) * 4 + j;
-                    ahead += x[i][j] == xt && at < min(rel, n);
+                    const int at = (i * kThreads + tid) * 4;
+                    ahead += at + 3 >= rel && at + j < rel && x[i][j] == xt;
                 }
         }
-    } else if (have) {  // a NaN: behind all numbers
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int at = (i * kThreads + tid) * 4 + j;
-                ahead += at < n && (x[i][j] == x[i][j] || base + at < tok);
-            }
+    } else if (have) {  // -inf, or a NaN: behind all numbers
+        const uint32_t kt = key_of(xt);
+#pragma unroll 1
+        for (int at = tid; at < n; at += kThreads) {
+            const uint32_t k = key_of(x0[base + at]);
+            ahead += k > kt || (k == kt && base + at < tok);
+        }
     }
 
     // the sums, without the logits that equal the maximum: they are counted
+    // (in x's own registers: what is left to do with the logits is rare, and reads them again)
     int equal = 0;
     const float mu = m == kNegInf ? 0.0f : m;  // (no logit above -inf)
-    float y[kVecs][4];
 #pragma unroll
     for (int i = 0; i < kVecs; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[i][j] = x[i][j] - mu;
+        for (int j = 0; j < 4; ++j) x[i][j] -= mu;
     if (__any(tmax == mu)) {
 #pragma unroll
         for (int i = 0; i < kVecs; ++i)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                equal += y[i][j] == 0.0f;
-                y[i][j] = y[i][j] == 0.0f ? kNegInf : y[i][j];
+                equal += x[i][j] == 0.0f;
+                x[i][j] = x[i][j] == 0.0f ? kNegInf : x[i][j];
             }
     }
     float sum = 0.0f, ent = 0.0f;
@@ -216,10 +225,10 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
     for (int i = 0; i < kVecs; ++i) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float e = __builtin_amdgcn_exp2f(y[i][j] * kLog2e);
+            const float e = __builtin_amdgcn_exp2f(x[i][j] * kLog2e);
             sum += e;
             // (exp of -200 and less is 0; a NaN stays in e)
-            ent = __builtin_fmaf(fmaxf(y[i][j], -200.0f), -e, ent);
+            ent = __builtin_fmaf(__builtin_amdgcn_fmed3f(x[i][j], -200.0f, 0.0f), -e, ent);
         }
     }
     sum = wave_sum(sum);
@@ -254,68 +263,45 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
     uint64_t* out = top + ((int64_t)row * parts + z) * top_k;
     int count = s_count;
     const int want = min(top_k, n);
+    // What follows up to the ranking is rare; it reads the logits again, one at a time, so that the
+    // kernel's registers are those of the work above (64 a thread instead of 109).
+    const auto each = [&](auto f) {
+#pragma unroll 1
+        for (int at = tid; at < n; at += kThreads) f(at, x0[base + at]);
+    };
     if (bound == kNegInf) {
         // Few logits above -inf (a mask, a short part): all of those, and the first ids, of which no
         // more than `above` are no -inf. (A NaN counts as too many.)
         int above = 0;
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) above += x[i][j] > kNegInf ? 1 : x[i][j] != x[i][j] ? kCand : 0;
+        each([&](int, float v) { above += v > kNegInf ? 1 : v != v ? kCand : 0; });
         above = block_sum(above, s_i[0]);
         if (above <= kCand / 2 - kMaxTopK) {
             const int first = min(n, want + above);
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = (i * kThreads + tid) * 4 + j;
-                    if (x[i][j] > kNegInf || at < first) {
-                        const int c = atomicAdd(&s_count, 1);
-                        s_cand[c] = entry_of(key_of(x[i][j]), base + at);
-                    }
-                }
-            }
+            each([&](int at, float v) {
+                if (v > kNegInf || at < first) s_cand[atomicAdd(&s_count, 1)] = entry_of(key_of(v), base + at);
+            });
         }
         __syncthreads();
         count = s_count;
     } else if (count > kCand) {
-        // Many logits equal the bound (a coarse grid of values): of those only the first by index can be wanted. The index below which top_k of them lie, by bisection.
-        int lo = 0, hi = kPart, above = 0;
-        for (int step = 0; step < 14; ++step) {
-            const int mid = step == 0 ? 0 : (lo + hi) >> 1;  // (first: the logits above the bound)
-            int k = 0;
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = (i * kThreads + tid) * 4 + j;
-                    k += at < n && (step == 0 ? x[i][j] > bound : x[i][j] == bound && at < mid);
-                }
-            k = block_sum(k, s_i[0]);
-            if (step == 0) {
-                above = k;
-                if (above > kCand - kMaxTopK) break;
-            } else if (k >= top_k) {
-                hi = mid;
-            } else {
-                lo = mid;
-            }
-        }
+        // Many logits equal the bound (a coarse grid of values): of those only the first by index can
+        // be wanted. The index below which top_k of them lie, by bisection.
+        int above = 0;
+        each([&](int, float v) { above += v > bound; });
+        above = block_sum(above, s_i[0]);
         if (above <= kCand - kMaxTopK) {
+            int lo = 0, hi = kPart;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                int k = 0;
+                each([&](int at, float v) { k += v == bound && at < mid; });
+                if (block_sum(k, s_i[0]) >= top_k) hi = mid; else lo = mid;
+            }
             if (tid == 0) s_count = 0;
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int at = (i * kThreads + tid) * 4 + j;
-                    if (at < n && (x[i][j] > bound || (x[i][j] == bound && at < hi))) {
-                        const int c = atomicAdd(&s_count, 1);
-                        if (c < kCand) s_cand[c] = entry_of(key_of(x[i][j]), base + at);
-                    }
-                }
-            }
+            each([&](int at, float v) {
+                if (v > bound || (v == bound && at < hi)) s_cand[atomicAdd(&s_count, 1)] = entry_of(key_of(v), base + at);
+            });
             __syncthreads();
             count = s_count;
         }
@@ -335,15 +321,10 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
     uint64_t last = ~0ull;
     for (int r = 0; r < top_k; ++r) {
         uint64_t best = 0;
-#pragma unroll
-        for (int i = 0; i < kVecs; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int at = (i * kThreads + tid) * 4 + j;
-                const uint64_t e = at < n ? entry_of(key_of(x[i][j]), base + at) : 0;
-                if (e < last && e > best) best = e;
-            }
-        }
+        each([&](int at, float v) {
+            const uint64_t e = entry_of(key_of(v), base + at);
+            if (e < last && e > best) best = e;
+        });
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint64_t o = __shfl_xor((unsigned long long)best, d, 64);
