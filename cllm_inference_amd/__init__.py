@@ -683,31 +683,32 @@ def kv4_page_bytes(page_size: int, n_head_kv: int, head_dim: int) -> int:
     return int(load_library().cllm_hip_kv4_page_bytes(int(page_size), int(n_head_kv), int(head_dim)))
 
 
-def _tensor(who: str, name: str, t, dtype, like, numel=None, optional=False):
-    """t's address, after a check of what the kernels take from it: dtype, contiguous, on the
-    device of `like`, of numel elements (when given)."""
+def _addr(who: str, name: str, t, dtype, device: int, numel: int = -1) -> int:
+    """t's address, after a check of what the kernels take from it: dtype, contiguous, on CUDA device
+    `device`, of numel elements (when given)."""
+    if (t is not None and t.dtype is dtype and t.is_contiguous() and t.get_device() == device
+            and (numel < 0 or t.numel() == numel)):
+        return t.data_ptr()
     if t is None:
-        if optional:
-            return None
         raise RuntimeError(f"{who}: {name} is None")
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise RuntimeError(f"{who}: {name} must be {dtype}, not {t.dtype}")
     if not t.is_contiguous():
         raise RuntimeError(f"{who}: {name} must be contiguous")
-    if t.device != like.device:
-        raise RuntimeError(f"{who}: {name} is on {t.device}, not on {like.device}")
-    if numel is not None and t.numel() != numel:
-        raise RuntimeError(f"{who}: {name} has {t.numel()} elements, not {numel}")
-    return ctypes.c_void_p(t.data_ptr())
+    if t.get_device() != device:
+        raise RuntimeError(f"{who}: {name} is on {t.device}, not on cuda:{device}")
+    raise RuntimeError(f"{who}: {name} has {t.numel()} elements, not {numel}")
 
 
-def _on_current(who: str, t):
+def _current(who: str, device: int):
+    """(torch, the address of torch's current stream on `device`), which must be the current one."""
     import torch
-    if not t.is_cuda:
-        raise RuntimeError(f"{who}: needs CUDA tensors, not {t.device}")
-    if t.device.index != torch.cuda.current_device():
-        raise RuntimeError(f"{who}: tensors are on {t.device}, the current device is "
+    if device != torch._C._cuda_getDevice():
+        if device < 0:
+            raise RuntimeError(f"{who}: needs CUDA tensors")
+        raise RuntimeError(f"{who}: tensors are on cuda:{device}, the current device is "
                            f"cuda:{torch.cuda.current_device()}")
+    return torch, torch._C._cuda_getCurrentRawStream(device)
 
 
 class Kv4Cache:
@@ -736,39 +737,49 @@ class Kv4Cache:
 
     def _set(self, pages, table, lens, refs, page_size, n_head_kv, head_dim):
         import torch
+        who = "Kv4Cache"
         nbytes = kv4_page_bytes(page_size, n_head_kv, head_dim)
         if pages.dim() != 3 or pages.shape[2] != nbytes or nbytes == 0:
-            raise RuntimeError(f"Kv4Cache: pages must be n_layers x n_pages x {nbytes} bytes")
+            raise RuntimeError(f"{who}: pages must be n_layers x n_pages x {nbytes} bytes")
         if table.dim() != 2:
-            raise RuntimeError("Kv4Cache: table must be max_seqs x max_pages")
+            raise RuntimeError(f"{who}: table must be max_seqs x max_pages")
+        if not pages.is_cuda:
+            raise RuntimeError(f"{who}: needs CUDA tensors, not {pages.device}")
+        self.device = dev = pages.get_device()
         work = load_library().cllm_hip_kv4_work_ints(pages.shape[1], table.shape[0], table.shape[1])
         self.pages, self.table, self.lens, self.refs = pages, table, lens, refs
         self.work = torch.empty(int(work), dtype=torch.int32, device=pages.device)
-        who = "Kv4Cache"
         self.struct = _Kv4CacheStruct(
-            _tensor(who, "pages", pages, torch.uint8, pages),
-            _tensor(who, "table", table, torch.int32, pages),
-            _tensor(who, "lens", lens, torch.int32, pages, table.shape[0]),
-            _tensor(who, "refs", refs, torch.int32, pages, pages.shape[1]),
-            ctypes.c_void_p(self.work.data_ptr()), pages.shape[0], pages.shape[1], int(page_size),
-            int(n_head_kv), int(head_dim), table.shape[0], table.shape[1])
+            _addr(who, "pages", pages, torch.uint8, dev), _addr(who, "table", table, torch.int32, dev),
+            _addr(who, "lens", lens, torch.int32, dev, table.shape[0]),
+            _addr(who, "refs", refs, torch.int32, dev, pages.shape[1]), self.work.data_ptr(),
+            pages.shape[0], pages.shape[1], int(page_size), int(n_head_kv), int(head_dim),
+            table.shape[0], table.shape[1])
+        self._ref = ctypes.addressof(self.struct)
+        self._shape = (int(n_head_kv), int(head_dim), table.shape[0])  # of what the calls check
+        self._ws = {}  # attention scratch bytes by batch shape
 
-    @property
-    def _ref(self):
-        return ctypes.byref(self.struct)
+    def attention_ws_bytes(self, *args) -> int:
+        """cllm_hip_kv4_attention_ws_bytes for (n_seqs, n_rows, max_rows, max_len, n_head)."""
+        n = self._ws.get(args)
+        if n is None:
+            if len(self._ws) >= 1024:
+                self._ws.clear()
+            n = self._ws[args] = int(load_library().cllm_hip_kv4_attention_ws_bytes(self._ref, *args))
+        return n
 
 
-def _kv4_batch(who, cache, q_start, slots, rows):
+def _kv4_batch(who, cache, i32, q_start, slots):
     """(slots, q_start, n_seqs) of a batch, checked."""
-    import torch
-    _on_current(who, cache.pages)
-    qs = _tensor(who, "q_start", q_start, torch.int32, cache.pages)
+    qs = _addr(who, "q_start", q_start, i32, cache.device)
     n_seqs = q_start.numel() - 1
     if n_seqs < 0:
         raise RuntimeError(f"{who}: q_start has n_seqs + 1 elements")
-    if slots is None and n_seqs > cache.table.shape[0]:
-        raise RuntimeError(f"{who}: {n_seqs} sequences, {cache.table.shape[0]} slots")
-    return _tensor(who, "slots", slots, torch.int32, cache.pages, n_seqs, optional=True), qs, n_seqs
+    if slots is not None:
+        return _addr(who, "slots", slots, i32, cache.device, n_seqs), qs, n_seqs
+    if n_seqs > cache._shape[2]:
+        raise RuntimeError(f"{who}: {n_seqs} sequences, {cache._shape[2]} slots")
+    return None, qs, n_seqs
 
 
 def kv4_extend_dev(cache: Kv4Cache, slots, counts, status=None):
@@ -776,64 +787,63 @@ def kv4_extend_dev(cache: Kv4Cache, slots, counts, status=None):
     they need, copies of shared partly filled pages included. Returns status (int32, one element, on
     the device): 0, the number of pages missing, or -1 for bad entries; unless it is 0 nothing has
     changed."""
-    import torch
-    who = "kv4_extend"
-    _on_current(who, cache.pages)
-    c = _tensor(who, "counts", counts, torch.int32, cache.pages)
+    who, dev = "kv4_extend", cache.device
+    torch, stream = _current(who, dev)
+    i32 = torch.int32
+    c = _addr(who, "counts", counts, i32, dev)
     n = counts.numel()
-    if slots is None and n > cache.table.shape[0]:
-        raise RuntimeError(f"{who}: {n} counts, {cache.table.shape[0]} slots")
-    s = _tensor(who, "slots", slots, torch.int32, cache.pages, n, optional=True)
+    s = None
+    if slots is not None:
+        s = _addr(who, "slots", slots, i32, dev, n)
+    elif n > cache._shape[2]:
+        raise RuntimeError(f"{who}: {n} counts, {cache._shape[2]} slots")
     if status is None:
-        status = torch.empty(1, dtype=torch.int32, device=cache.pages.device)
-    _check(load_library().cllm_hip_kv4_extend_dev(
-        cache._ref, s, c, n, _tensor(who, "status", status, torch.int32, cache.pages, 1), _stream()))
+        status = torch.empty(1, dtype=i32, device=cache.pages.device)
+    _check(load_library().cllm_hip_kv4_extend_dev(cache._ref, s, c, n, _addr(who, "status", status, i32, dev, 1),
+                                                  stream))
     return status
 
 
 def kv4_fork_dev(cache: Kv4Cache, src, dst) -> None:
     """Slot dst[i] becomes a copy of slot src[i] (int32 CUDA tensors), all at once; the pages are
     shared."""
-    import torch
-    who = "kv4_fork"
-    _on_current(who, cache.pages)
-    s = _tensor(who, "src", src, torch.int32, cache.pages)
-    d = _tensor(who, "dst", dst, torch.int32, cache.pages, src.numel())
-    _check(load_library().cllm_hip_kv4_fork_dev(cache._ref, s, d, src.numel(), _stream()))
+    who, dev = "kv4_fork", cache.device
+    torch, stream = _current(who, dev)
+    n = src.numel()
+    _check(load_library().cllm_hip_kv4_fork_dev(cache._ref, _addr(who, "src", src, torch.int32, dev),
+                                                _addr(who, "dst", dst, torch.int32, dev, n), n, stream))
 
 
 def kv4_truncate_dev(cache: Kv4Cache, slots, new_lens=None) -> None:
     """Cuts slot slots[i] to new_lens[i] tokens (None: to 0, freeing the sequences) and releases the
     pages past them."""
-    import torch
-    who = "kv4_truncate"
-    _on_current(who, cache.pages)
-    s = _tensor(who, "slots", slots, torch.int32, cache.pages)
-    n = _tensor(who, "new_lens", new_lens, torch.int32, cache.pages, slots.numel(), optional=True)
-    _check(load_library().cllm_hip_kv4_truncate_dev(cache._ref, s, n, slots.numel(), _stream()))
+    who, dev = "kv4_truncate", cache.device
+    torch, stream = _current(who, dev)
+    n = slots.numel()
+    new = None if new_lens is None else _addr(who, "new_lens", new_lens, torch.int32, dev, n)
+    _check(load_library().cllm_hip_kv4_truncate_dev(cache._ref, _addr(who, "slots", slots, torch.int32, dev), new,
+                                                    n, stream))
 
 
 def kv4_compact_dev(cache: Kv4Cache, n_live=None):
     """Moves the pages in use to the front of the pool; returns their number (int32, one element, on
     the device)."""
-    import torch
-    who = "kv4_compact"
-    _on_current(who, cache.pages)
+    who, dev = "kv4_compact", cache.device
+    torch, stream = _current(who, dev)
     if n_live is None:
         n_live = torch.empty(1, dtype=torch.int32, device=cache.pages.device)
-    _check(load_library().cllm_hip_kv4_compact_dev(
-        cache._ref, _tensor(who, "n_live", n_live, torch.int32, cache.pages, 1), _stream()))
+    _check(load_library().cllm_hip_kv4_compact_dev(cache._ref, _addr(who, "n_live", n_live, torch.int32, dev, 1),
+                                                   stream))
     return n_live
 
 
 def kv4_copy_pages_dev(cache: Kv4Cache, src, dst) -> None:
     """Copies page src[i] to page dst[i] (int32 CUDA tensors) in every layer."""
-    import torch
-    who = "kv4_copy_pages"
-    _on_current(who, cache.pages)
-    s = _tensor(who, "src", src, torch.int32, cache.pages)
-    d = _tensor(who, "dst", dst, torch.int32, cache.pages, src.numel())
-    _check(load_library().cllm_hip_kv4_copy_pages_dev(cache._ref, s, d, src.numel(), _stream()))
+    who, dev = "kv4_copy_pages", cache.device
+    torch, stream = _current(who, dev)
+    n = src.numel()
+    _check(load_library().cllm_hip_kv4_copy_pages_dev(cache._ref, _addr(who, "src", src, torch.int32, dev),
+                                                      _addr(who, "dst", dst, torch.int32, dev, n), n, stream))
 
 
 def kv4_store_dev(cache: Kv4Cache, layer: int, k, v, q_start, slots=None, q=None, n_head: int = 0,
@@ -842,37 +852,40 @@ def kv4_store_dev(cache: Kv4Cache, layer: int, k, v, q_start, slots=None, q=None
     batch's sequences: sequence i is slot slots[i] (None: slot i) and has rows q_start[i] ..
     q_start[i + 1]. theta_base > 0: the keys, and the query rows q in place, get the NEOX rotation of
     rope_neox2_dev at their positions first."""
-    import torch
-    who = "kv4_store"
-    s, qs, n_seqs = _kv4_batch(who, cache, q_start, slots, k)
-    width = cache.struct.n_head_kv * cache.struct.head_dim
-    kp = _tensor(who, "k", k, torch.float32, cache.pages)
-    if k.numel() % width:
-        raise RuntimeError(f"{who}: k has {k.numel()} elements, rows have {width}")
-    n_rows = k.numel() // width
-    vp = _tensor(who, "v", v, torch.float32, cache.pages, k.numel())
-    qp = _tensor(who, "q", q, torch.float32, cache.pages, n_rows * int(n_head) * cache.struct.head_dim,
-                 optional=True)
-    _check(load_library().cllm_hip_kv4_store_dev(cache._ref, int(layer), kp, vp, qp, int(n_head),
-                                                 float(theta_base), s, qs, n_seqs, n_rows, _stream()))
+    who, dev = "kv4_store", cache.device
+    torch, stream = _current(who, dev)
+    f32 = torch.float32
+    s, qs, n_seqs = _kv4_batch(who, cache, torch.int32, q_start, slots)
+    n_kv, hd, _ = cache._shape
+    kp = _addr(who, "k", k, f32, dev)
+    n = k.numel()
+    n_rows = n // (n_kv * hd)
+    if n_rows * n_kv * hd != n:
+        raise RuntimeError(f"{who}: k has {n} elements, rows have {n_kv * hd}")
+    vp = _addr(who, "v", v, f32, dev, n)
+    qp = None if q is None else _addr(who, "q", q, f32, dev, n_rows * int(n_head) * hd)
+    _check(load_library().cllm_hip_kv4_store_dev(cache._ref, layer, kp, vp, qp, n_head, theta_base, s, qs, n_seqs,
+                                                 n_rows, stream))
 
 
 def kv4_load_dev(cache: Kv4Cache, layer: int, q_start, n_rows: int, slots=None, k=None, v=None):
     """The rows' keys and values as float32 (n_rows x n_head_kv * head_dim), the batch as
     kv4_store_dev's (rows of no sequence are left as they are)."""
-    import torch
-    who = "kv4_load"
-    s, qs, n_seqs = _kv4_batch(who, cache, q_start, slots, None)
-    width = cache.struct.n_head_kv * cache.struct.head_dim
-    out = []
-    for name, t in (("k", k), ("v", v)):
-        if t is None:
-            t = torch.empty((int(n_rows), width), dtype=torch.float32, device=cache.pages.device)
-        _tensor(who, name, t, torch.float32, cache.pages, int(n_rows) * width)
-        out.append(t)
-    _check(load_library().cllm_hip_kv4_load_dev(cache._ref, int(layer), s, qs, n_seqs, int(n_rows),
-                                                _tp(out[0]), _tp(out[1]), _stream()))
-    return tuple(out)
+    who, dev = "kv4_load", cache.device
+    torch, stream = _current(who, dev)
+    f32 = torch.float32
+    s, qs, n_seqs = _kv4_batch(who, cache, torch.int32, q_start, slots)
+    n_rows = int(n_rows)
+    shape = (n_rows, cache._shape[0] * cache._shape[1])
+    if k is None:
+        k = torch.empty(shape, dtype=f32, device=cache.pages.device)
+    if v is None:
+        v = torch.empty(shape, dtype=f32, device=cache.pages.device)
+    n = shape[0] * shape[1]
+    _check(load_library().cllm_hip_kv4_load_dev(cache._ref, layer, s, qs, n_seqs, n_rows,
+                                                _addr(who, "k", k, f32, dev, n), _addr(who, "v", v, f32, dev, n),
+                                                stream))
+    return k, v
 
 
 def kv4_attention_dev(cache: Kv4Cache, layer: int, q, q_start, *, n_head: int, max_rows: int,
@@ -881,24 +894,25 @@ def kv4_attention_dev(cache: Kv4Cache, layer: int, q, q_start, *, n_head: int, m
     the batch as kv4_store_dev's: row t of a sequence with r rows sees positions [0, len - r + t].
     max_rows and max_len bound a sequence's rows and tokens. Returns out (n_rows x n_head *
     head_dim); a row that sees nothing is 0, one of no sequence is left as it is."""
-    import torch
-    who = "kv4_attention"
-    s, qs, n_seqs = _kv4_batch(who, cache, q_start, slots, q)
-    width = int(n_head) * cache.struct.head_dim
-    qp = _tensor(who, "q", q, torch.float32, cache.pages)
-    if width <= 0 or q.numel() % width:
-        raise RuntimeError(f"{who}: q has {q.numel()} elements, rows have {width}")
-    n_rows = q.numel() // width
+    who, dev = "kv4_attention", cache.device
+    torch, stream = _current(who, dev)
+    f32 = torch.float32
+    s, qs, n_seqs = _kv4_batch(who, cache, torch.int32, q_start, slots)
+    width = n_head * cache._shape[1]
+    qp = _addr(who, "q", q, f32, dev)
+    n = q.numel()
+    n_rows = n // width if width > 0 else 0
+    if width <= 0 or n_rows * width != n:
+        raise RuntimeError(f"{who}: q has {n} elements, rows have {width}")
     if out is None:
-        out = torch.empty((n_rows, width), dtype=torch.float32, device=q.device)
-    op = _tensor(who, "out", out, torch.float32, cache.pages, n_rows * width)
-    lib = load_library()
-    args = (n_seqs, n_rows, int(max_rows), int(max_len), int(n_head))
-    nbytes = int(lib.cllm_hip_kv4_attention_ws_bytes(cache._ref, *args))
+        out = torch.empty((n_rows, width), dtype=f32, device=q.device)
+    args = (n_seqs, n_rows, max_rows, max_len, n_head)
+    nbytes = cache.attention_ws_bytes(*args)
     # scratch from torch's allocator: a captured call's belongs to its graph
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _check(lib.cllm_hip_kv4_attention_dev(cache._ref, int(layer), qp, s, qs, *args, op, _tp(ws), nbytes,
-                                          _stream()))
+    _check(load_library().cllm_hip_kv4_attention_dev(
+        cache._ref, layer, qp, s, qs, n_seqs, n_rows, max_rows, max_len, n_head,
+        _addr(who, "out", out, f32, dev, n), ws.data_ptr() if nbytes else None, nbytes, stream))
     return out
 
 
@@ -926,26 +940,34 @@ def logprobs_dev(logits, tokens=None, top_k: int = 0) -> LogProbs:
     """Log probabilities of the rows of logits (float32 (n_rows, vocab), any row stride, unit stride
     along a row): of the given tokens (int32 (n_rows,)) with their ranks, the entropy and
     log-sum-exp, and the top_k (at most 64) largest with their ids, equal logits by ids."""
-    import torch
-    who = "logprobs"
-    if logits.dim() != 2 or logits.dtype != torch.float32:
+    who, dev = "logprobs", logits.get_device()
+    torch, stream = _current(who, dev)
+    f32, i32, device = torch.float32, torch.int32, logits.device
+    if logits.dim() != 2 or logits.dtype is not f32:
         raise RuntimeError(f"{who}: logits must be float32 n_rows x vocab")
-    _on_current(who, logits)
     m, vocab = logits.shape
-    if vocab > 1 and logits.stride(1) != 1:
+    stride, along = logits.stride()
+    if vocab > 1 and along != 1:
         raise RuntimeError(f"{who}: the logits of a row must lie side by side")
-    stride = logits.stride(0) if m > 1 else vocab
-    tp = _tensor(who, "tokens", tokens, torch.int32, logits, m, optional=True)
-    new = lambda dt, *shape: torch.empty(shape, dtype=dt, device=logits.device)  # noqa: E731
-    r = LogProbs(new(torch.float32, m) if tokens is not None else None,
-                 new(torch.int32, m) if tokens is not None else None,
-                 new(torch.float32, m), new(torch.float32, m),
-                 new(torch.int32, m, int(top_k)), new(torch.float32, m, int(top_k)))
+    if m <= 1:
+        stride = vocab
     lib = load_library()
-    nbytes = int(lib.cllm_hip_logprobs_ws_bytes(m, vocab, int(top_k)))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=logits.device) if nbytes else None
-    _check(lib.cllm_hip_logprobs_dev(_tp(logits), int(stride), m, vocab, tp, int(top_k), _tp(r.logprobs),
-                                     _tp(r.ranks), _tp(r.entropy), _tp(r.lse),
-                                     _tp(r.top_ids) if top_k else None,
-                                     _tp(r.top_logprobs) if top_k else None, _tp(ws), nbytes, _stream()))
+    nbytes = int(lib.cllm_hip_logprobs_ws_bytes(m, vocab, top_k))
+    tp = lp = ranks = tid = ttop = None
+    per_row = 3 if tokens is not None else 2
+    per = torch.empty((per_row, m), dtype=f32, device=device).unbind(0)
+    if tokens is not None:
+        tp = _addr(who, "tokens", tokens, i32, dev, m)
+        lp, ranks = per[2], torch.empty(m, dtype=i32, device=device)
+    top_ids = torch.empty((m, top_k), dtype=i32, device=device)
+    top_lp = torch.empty((m, top_k), dtype=f32, device=device)
+    if top_k:
+        tid, ttop = top_ids.data_ptr(), top_lp.data_ptr()
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    r = LogProbs(lp, ranks, per[0], per[1], top_ids, top_lp)
+    _check(lib.cllm_hip_logprobs_dev(logits.data_ptr(), stride, m, vocab, tp, top_k,
+                                     None if lp is None else lp.data_ptr(),
+                                     None if ranks is None else ranks.data_ptr(), per[0].data_ptr(),
+                                     per[1].data_ptr(), tid, ttop, None if ws is None else ws.data_ptr(), nbytes,
+                                     stream))
     return r
