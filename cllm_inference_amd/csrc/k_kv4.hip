@@ -1246,8 +1246,8 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
     const int h = blockIdx.y;
     const int sub = c.page_shift - 5;
     const int page = c.table[(int64_t)sg.s.slot * c.max_pages + (sg.tile >> sub)];
-    if ((unsigned)page >= (unsigned)c.n_pages) return;  // no page: the rows have no place
-    uint8_t* tile = c.pages + ((int64_t)layer * c.n_pages + page) * c.page_bytes +
+    const bool none = (unsigned)page >= (unsigned)c.n_pages;
+    uint8_t* tile = c.pages + ((int64_t)layer * c.n_pages + (none ? 0 : page)) * c.page_bytes +
                     (((int64_t)h << sub) + (sg.tile & ((1 << sub) - 1))) * (36 * HD);
     if (tid < kTile) bad[tid] = 0;
     __syncthreads();
@@ -1256,15 +1256,29 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
     const int p = tid >> 3, d0 = (tid & 7) * PER;
     const bool on = p >= sg.a && p < sg.b;
     const int64_t src = ((int64_t)(sg.row + p - sg.a) * c.n_kv + h) * HD;
+    // all that is read is on its way before the page id (and with it the tile) is known: both rows,
+    // and then the value dwords of which only some positions change
+    float both[2][PER];
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-        float x[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) x[i] = 0.0f;
+        for (int i = 0; i < PER; ++i) both[kv][i] = 0.0f;
+        if (on) {
+#pragma unroll
+            for (int i = 0; i < PER; i += 4) *(f32x4*)(both[kv] + i) = *(const f32x4*)((kv ? v : k) + src + d0 + i);
+        }
+    }
+    if (none) return;  // no page: the rows have no place
+    const bool whole = sg.a == 0 && sg.b == kTile;
+    uint32_t old[4 * HD / 256];
+#pragma unroll
+    for (int i = 0; i < 4 * HD / 256; ++i)
+        old[i] = whole ? 0u : ((const uint32_t*)(tile + 16 * HD))[i * 256 + tid];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        float (&x)[PER] = both[kv];
         if (on) {
             const float* base = (kv ? v : k) + src;
-#pragma unroll
-            for (int i = 0; i < PER; i += 4) *(f32x4*)(x + i) = *(const f32x4*)(base + d0 + i);
             if (kv == 0 && theta_base > 0.0f) {
                 const bool upper = d0 >= HALF;
                 const int j0 = upper ? d0 - HALF : d0;
@@ -1318,8 +1332,9 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
         ((uint32_t*)tile)[i] = bad[pos] ? 0x88888888u : x;
     }
     // value dwords
-    const bool whole = sg.a == 0 && sg.b == kTile;
-    for (int i = tid; i < 4 * HD; i += 256) {
+#pragma unroll
+    for (int turn = 0; turn < 4 * HD / 256; ++turn) {
+        const int i = turn * 256 + tid;
         const int w = i % 4, nn = i / 4 % 16, g = i / 64 % 4, cc = i / 256;
         const int dim = 16 * (4 * cc + w) + nn;
         uint32_t x = 0, mask = 0;
@@ -1332,8 +1347,7 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
             }
         }
         if (!mask) continue;
-        uint32_t* dst = (uint32_t*)(tile + 16 * HD) + i;
-        *dst = whole ? x : (*dst & ~mask) | x;
+        ((uint32_t*)(tile + 16 * HD))[i] = (old[turn] & ~mask) | x;
     }
     // scales
     for (int i = tid; i < 2 * kTile * NB; i += 256) {

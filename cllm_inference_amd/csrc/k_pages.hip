@@ -200,36 +200,66 @@ __device__ __forceinline__ bool named_before(const int32_t* slots, int i) {
     return __syncthreads_or(found);
 }
 
-// Fork, first launch (a workgroup per entry): the source's pages and length are written to work and
-// counted once more. Every source is read before any destination is written, so the entries act at
-// once (a beam search's permutation).
-__global__ __launch_bounds__(256) void k_kv4_fork_read(Kv4View c, const int32_t* __restrict__ src,
-                                                       const int32_t* __restrict__ dst) {
-    const int i = blockIdx.x, s = src[i], d = dst[i];
-    if ((unsigned)s >= (unsigned)c.max_seqs || (unsigned)d >= (unsigned)c.max_seqs || named_before(dst, i)) return;
+// Fork. Every source is read (its pages and length written to work, and counted once more) before any
+// destination is written, so the entries act at once (a beam search's permutation): in two launches with
+// a workgroup per entry, or, up to kForkOne table entries, in one workgroup with a barrier between.
+__device__ __forceinline__ void fork_read(const Kv4View& c, int i, int s, int first, int step) {
     int32_t* to = c.work + (int64_t)i * (c.max_pages + 1);
     const int32_t* row = c.table + (int64_t)s * c.max_pages;
-    for (int p = threadIdx.x; p < c.max_pages; p += 256) {
+    for (int p = first; p < c.max_pages; p += step) {
         const int page = row[p];
         to[1 + p] = page;
         if ((unsigned)page < (unsigned)c.n_pages) atomicAdd(&c.refs[page], 1);
     }
-    if (threadIdx.x == 0) to[0] = c.lens[s];
+    if (first == 0) to[0] = c.lens[s];
 }
-
-// Second launch: the destination leaves its pages and takes those of the source.
-__global__ __launch_bounds__(256) void k_kv4_fork_write(Kv4View c, const int32_t* __restrict__ src,
-                                                        const int32_t* __restrict__ dst) {
-    const int i = blockIdx.x, s = src[i], d = dst[i];
-    if ((unsigned)s >= (unsigned)c.max_seqs || (unsigned)d >= (unsigned)c.max_seqs || named_before(dst, i)) return;
+// The destination leaves its pages and takes those of the source.
+__device__ __forceinline__ void fork_write(const Kv4View& c, int i, int d, int first, int step) {
     const int32_t* from = c.work + (int64_t)i * (c.max_pages + 1);
     int32_t* row = c.table + (int64_t)d * c.max_pages;
-    for (int p = threadIdx.x; p < c.max_pages; p += 256) {
+    for (int p = first; p < c.max_pages; p += step) {
         const int page = row[p];
         if ((unsigned)page < (unsigned)c.n_pages) atomicSub(&c.refs[page], 1);
         row[p] = from[1 + p];
     }
-    if (threadIdx.x == 0) c.lens[d] = from[0];
+    if (first == 0) c.lens[d] = from[0];
+}
+__device__ __forceinline__ bool slots_ok(const Kv4View& c, int s, int d) {
+    return (unsigned)s < (unsigned)c.max_seqs && (unsigned)d < (unsigned)c.max_seqs;
+}
+
+__global__ __launch_bounds__(256) void k_kv4_fork(Kv4View c, const int32_t* __restrict__ src,
+                                                  const int32_t* __restrict__ dst, int write) {
+    const int i = blockIdx.x, s = src[i], d = dst[i];
+    if (!slots_ok(c, s, d) || named_before(dst, i)) return;
+    if (write) fork_write(c, i, d, threadIdx.x, 256); else fork_read(c, i, s, threadIdx.x, 256);
+}
+
+// A wave per entry, in turns; the entries that stand are found once.
+constexpr int kForkOne = 16384, kForkEntries = 128;
+__global__ __launch_bounds__(kThreads) void k_kv4_fork_one(Kv4View c, const int32_t* __restrict__ src,
+                                                           const int32_t* __restrict__ dst, int n) {
+    __shared__ int s_src[kForkEntries], s_dst[kForkEntries];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (tid < n) {
+        s_src[tid] = src[tid];
+        s_dst[tid] = dst[tid];
+    }
+    __syncthreads();
+    bool ok = false;
+    if (tid < n) {
+        ok = slots_ok(c, s_src[tid], s_dst[tid]);
+        for (int j = 0; j < tid; ++j) ok &= s_dst[j] != s_dst[tid];
+    }
+    __syncthreads();
+    if (tid < n && !ok) s_src[tid] = -1;
+    __syncthreads();
+    for (int i = wave; i < n; i += kThreads / 64)
+        if (s_src[i] >= 0) fork_read(c, i, s_src[i], lane, 64);
+    __threadfence_block();
+    __syncthreads();
+    for (int i = wave; i < n; i += kThreads / 64)
+        if (s_src[i] >= 0) fork_write(c, i, s_dst[i], lane, 64);
 }
 
 __global__ __launch_bounds__(256) void k_kv4_truncate(Kv4View c, const int32_t* __restrict__ slots,
@@ -333,10 +363,14 @@ hipError_t launch_kv4_extend(const Kv4View& c, const int32_t* slots, const int32
 }
 
 hipError_t launch_kv4_fork(const Kv4View& c, const int32_t* src, const int32_t* dst, int n, hipStream_t stream) {
-    hipLaunchKernelGGL(k_kv4_fork_read, dim3((unsigned)n), dim3(256), 0, stream, c, src, dst);
+    if (n <= kForkEntries && (int64_t)n * c.max_pages <= kForkOne) {
+        hipLaunchKernelGGL(k_kv4_fork_one, dim3(1), dim3(kThreads), 0, stream, c, src, dst, n);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(k_kv4_fork, dim3((unsigned)n), dim3(256), 0, stream, c, src, dst, 0);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_kv4_fork_write, dim3((unsigned)n), dim3(256), 0, stream, c, src, dst);
+    hipLaunchKernelGGL(k_kv4_fork, dim3((unsigned)n), dim3(256), 0, stream, c, src, dst, 1);
     return hipGetLastError();
 }
 
