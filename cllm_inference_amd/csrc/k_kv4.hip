@@ -1188,23 +1188,22 @@ __device__ __forceinline__ _Float16 scale_of(float mx, float mn) {
     return -mn >= mx ? d : (_Float16)-d;
 }
 
-// x / d to the nearest integer, ties to even, exactly: the quotient's rounding is checked against
-// the remainder, which an FMA gives without error (x and d * q agree to within d).
-__device__ __forceinline__ uint32_t code_of(float x, float d, float inv) {
+// x / d to the nearest integer, ties to even, exactly: the rounded product with 1 / d is checked against
+// the remainder, which an FMA gives without error (x and d * t agree to within d), and is at most one
+// off, or a tie. (x and d finite, d not 0.)
+__device__ __forceinline__ uint32_t code_of(float x, float d, float inv, float half) {
     float t = __builtin_rintf(x * inv);
-    if (fabsf(t) < 16.0f) {
-        const float rem = __builtin_fmaf(-t, d, x), half = 0.5f * fabsf(d);
-        const float up = (rem < 0.0f) == (d < 0.0f) ? 1.0f : -1.0f;  // the next integer on rem's side
+    const float rem = __builtin_fmaf(-t, d, x);
+    if (fabsf(rem) >= half && fabsf(t) < 16.0f) {  // (rare; past 16 the code is 0 or 15 anyway)
         const bool odd = __builtin_fmaf(-2.0f, __builtin_floorf(0.5f * t), t) != 0.0f;
-        if (fabsf(rem) > half || (fabsf(rem) == half && odd)) t += up;
+        if (fabsf(rem) > half || odd) t += (rem < 0.0f) == (d < 0.0f) ? 1.0f : -1.0f;
     }
-    t = fminf(fmaxf(t, -8.0f), 7.0f);
-    return (uint32_t)((int)t + 8);
+    return (uint32_t)((int)__builtin_amdgcn_fmed3f(t, -8.0f, 7.0f) + 8);
 }
 
 // grid (segments at most, KV heads [+ query head groups when q is rotated]). A workgroup reads the
-// segment's rows of its head once, quantizes them into LDS and writes the tile's dwords. A dword of
-// keys belongs to one position; a dword of values to eight, of which only the segment's change.
+// segment's rows of its head once and quantizes them, eight threads to a position; a dword of keys is
+// eight elements of one position, a dword of values one element of eight positions, which meet in LDS.
 // theta_base > 0: keys turn by the NEOX rotation of k_rope_neox at their positions first, and the
 // workgroups past the KV heads turn the query rows in place.
 template <int HD>
@@ -1214,9 +1213,7 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
                                                    const int32_t* __restrict__ q_start, int n_seqs, int n_rows) {
     constexpr int HALF = HD / 2, PER = HD / 8, NB = HD / 32;
     __shared__ float cs[kTile][HALF], sn[kTile][HALF], power[HALF];
-    __shared__ uint8_t codes[2][kTile][HD + 4];
-    __shared__ _Float16 scales[2][kTile][NB];
-    __shared__ int bad[kTile];
+    __shared__ uint8_t codes[kTile][HD + 4];  // of the values
     const Segment sg = find_segment(c, slots, q_start, n_seqs, n_rows, blockIdx.x);
     if (sg.tile < 0) return;
     const int tid = threadIdx.x;
@@ -1249,9 +1246,6 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
     const bool none = (unsigned)page >= (unsigned)c.n_pages;
     uint8_t* tile = c.pages + ((int64_t)layer * c.n_pages + (none ? 0 : page)) * c.page_bytes +
                     (((int64_t)h << sub) + (sg.tile & ((1 << sub) - 1))) * (36 * HD);
-    if (tid < kTile) bad[tid] = 0;
-    __syncthreads();
-
     // thread: position tid / 8, elements (tid % 8) * PER .. of both rows
     const int p = tid >> 3, d0 = (tid & 7) * PER;
     const bool on = p >= sg.a && p < sg.b;
@@ -1291,14 +1285,25 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
                 }
             }
         }
-        // a block's 32 elements lie in 32 / PER threads
-        float mx = x[0], mn = x[0];
-        bool finite = true;
+    }
+    // a row that is not finite: known to the position's eight threads
+    bool finite = true;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
+    for (int i = 0; i < PER; ++i)
+        finite &= fabsf(both[0][i]) < __builtin_huge_valf() && fabsf(both[1][i]) < __builtin_huge_valf();
+    int bad = finite ? 0 : 1;
+    bad |= dpp_i32<DPP_QUAD_SWAP1>(bad);
+    bad |= dpp_i32<DPP_QUAD_SWAP2>(bad);
+    bad |= dpp_i32<DPP_ROW_HALF_MIRROR>(bad);
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+        // a block's 32 elements lie in 32 / PER threads (the whole wave takes part)
+        float (&x)[PER] = both[kv];
+        float mx = x[0], mn = x[0];
+#pragma unroll
+        for (int i = 1; i < PER; ++i) {
             mx = fmaxf(mx, x[i]);
             mn = fminf(mn, x[i]);
-            finite &= fabsf(x[i]) < __builtin_huge_valf();
         }
         if constexpr (PER <= 16) {
             mx = fmaxf(mx, dpp_f32<DPP_QUAD_SWAP1>(mx));
@@ -1308,30 +1313,35 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
             mx = fmaxf(mx, dpp_f32<DPP_QUAD_SWAP2>(mx));
             mn = fminf(mn, dpp_f32<DPP_QUAD_SWAP2>(mn));
         }
-        if (on && !finite) bad[p] = 1;  // (every writer writes the same)
-        const _Float16 dh = scale_of(mx, mn);
-        const float d = (float)dh, inv = d == 0.0f ? 0.0f : 1.0f / d;
-        if (on) {
+        if (!on) continue;
+        _Float16 dh = scale_of(mx, mn);
+        const float d = (float)dh;
+        const bool plain = d != 0.0f && !bad;
+        const float inv = plain ? 1.0f / d : 0.0f, half = plain ? 0.5f * fabsf(d) : 1.0f;
+        // eight elements are a key dword of the tile, which belongs to the position alone
+        constexpr int W = NB < 4 ? NB : 4, C = NB / W;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) codes[kv][p][d0 + i] = (uint8_t)(d == 0.0f ? 8u : code_of(x[i], d, inv));
-            if (d0 % 32 == 0) scales[kv][p][d0 / 32] = dh;
+        for (int j = 0; j < PER; j += 8) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t code = plain ? code_of(x[j + i], d, inv, half) : 8u;
+                if (kv) codes[p][d0 + j + i] = (uint8_t)code;
+                w |= code << (4 * (i / 2 + 4 * (i % 2)));
+            }
+            const int g = (d0 + j) / (HD / 4), f = (d0 + j) % (HD / 4) / 8;
+            if (kv == 0) ((uint32_t*)tile)[(((p / 16 * C + f / W) * 4 + g) * 16 + p % 16) * W + f % W] = w;
+        }
+        if (d0 % 32 == 0) {
+            if (bad) dh = kv ? (_Float16)0.0f : (_Float16)__builtin_nanf("");
+            const int b = d0 / 32;
+            const int place = kv ? (b * 4 + p % 16 / 4) * 8 + p / 16 * 4 + p % 4 : (b * 16 + p % 16) * 2 + p / 16;
+            ((_Float16*)(tile + (kv ? 34 : 32) * HD))[place] = dh;
         }
     }
     __syncthreads();
 
-    // key dwords, in the tile's order
-    constexpr int W = NB < 4 ? NB : 4, C = NB / W;
-    for (int i = tid; i < 4 * HD; i += 256) {
-        const int w = i % W, nn = i / W % 16, g = i / W / 16 % 4, t = i / W / 64 / C, cc = i / W / 64 % C;
-        const int pos = 16 * t + nn;
-        if (pos < sg.a || pos >= sg.b) continue;
-        const uint8_t* e = &codes[0][pos][g * (HD / 4) + 8 * (cc * W + w)];
-        uint32_t x = 0;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x |= (uint32_t)e[j] << (4 * (j / 2 + 4 * (j % 2)));
-        ((uint32_t*)tile)[i] = bad[pos] ? 0x88888888u : x;
-    }
-    // value dwords
+    // value dwords, of which only the segment's positions change
 #pragma unroll
     for (int turn = 0; turn < 4 * HD / 256; ++turn) {
         const int i = turn * 256 + tid;
@@ -1342,21 +1352,12 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
         for (int j = 0; j < 8; ++j) {
             const int pos = 16 * (j / 4) + 4 * g + j % 4, sh = 4 * (j / 2 + 4 * (j % 2));
             if (pos >= sg.a && pos < sg.b) {
-                x |= (uint32_t)(bad[pos] ? 8 : codes[1][pos][dim]) << sh;
+                x |= (uint32_t)codes[pos][dim] << sh;
                 mask |= 15u << sh;
             }
         }
         if (!mask) continue;
         ((uint32_t*)(tile + 16 * HD))[i] = (old[turn] & ~mask) | x;
-    }
-    // scales
-    for (int i = tid; i < 2 * kTile * NB; i += 256) {
-        const int kv = i / (kTile * NB), b = i / kTile % NB, pos = i % kTile;
-        if (pos < sg.a || pos >= sg.b) continue;
-        _Float16 d = scales[kv][pos][b];
-        if (bad[pos]) d = kv ? (_Float16)0.0f : (_Float16)__builtin_nanf("");
-        const int place = kv ? (b * 4 + pos % 16 / 4) * 8 + pos / 16 * 4 + pos % 4 : (b * 16 + pos % 16) * 2 + pos / 16;
-        ((_Float16*)(tile + (kv ? 34 : 32) * HD))[place] = d;
     }
 }
 
