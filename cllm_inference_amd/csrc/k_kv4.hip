@@ -41,12 +41,11 @@ __device__ __forceinline__ f32x4 mfma(const h8& a, const h8& b, const f32x4& c) 
 // register or literal, so the or's constants lie in vector registers (Magic): v_and_or_b32.
 struct Magic {
     uint32_t m1024, m64;
-    float minus1, zero;  // (as literals they would take v_fma_mix, which reads fp16, out of the products)
+    float minus1;  // (as a literal it would take v_fma_mix, which reads fp16, out of the products)
     __device__ __forceinline__ Magic() {
         asm("v_mov_b32 %0, 0x64006400" : "=v"(m1024));
         asm("v_mov_b32 %0, 0x54005400" : "=v"(m64));
         asm("v_mov_b32 %0, -1.0" : "=v"(minus1));
-        asm("v_mov_b32 %0, 0" : "=v"(zero));
     }
 };
 __device__ __forceinline__ h8 dequant8(uint32_t w, const h2 (&d)[4], const Magic& mg) {
@@ -58,16 +57,6 @@ __device__ __forceinline__ h8 dequant8(uint32_t w, const h2 (&d)[4], const Magic
     const h2 f = (__builtin_bit_cast(h2, (w8 & 0x00F000F0u) | mg.m64) + off1) * d[3];
     return h8{a.x, a.y, b.x, b.y, e.x, e.y, f.x, f.y};
 }
-
-// Codes of a dword as they are: pairs c * 2^-24 (fp16 subnormals, exact) for r = 0 and 2, 16 c * 2^-24
-// for r = 1 and 3. 5 VALU operations; the other operand of the product has the 16th of codes 2 r and
-// 2 r + 1 of the odd r (odd_pair).
-__device__ __forceinline__ h8 codes8(uint32_t w) {
-    const uint32_t w8 = w >> 8;
-    const uint32_t x[4] = {w & 0x000F000Fu, w & 0x00F000F0u, w8 & 0x000F000Fu, w8 & 0x00F000F0u};
-    return __builtin_bit_cast(h8, *(const u32x4*)x);
-}
-__device__ __forceinline__ constexpr bool odd_pair(int e) { return (e >> 1) & 1; }
 
 __device__ __forceinline__ h2 pkrtz(float a, float b) {
     return __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(a, b));
@@ -83,6 +72,17 @@ __device__ __forceinline__ void split8(const float (&x)[8], h8& hi, h8& lo, cons
     }
     hi = h8{a[0].x, a[0].y, a[1].x, a[1].y, a[2].x, a[2].y, a[3].x, a[3].y};
     lo = h8{b[0].x, b[0].y, b[1].x, b[1].y, b[2].x, b[2].y, b[3].x, b[3].y};
+}
+
+// The high parts of eight values (low 0), or their low parts (low -1).
+__device__ __forceinline__ h8 part8(const float (&x)[8], float low) {
+    h2 b[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const h2 a = pkrtz(x[2 * r], x[2 * r + 1]);
+        b[r] = pkrtz(__builtin_fmaf((float)a.x, low, x[2 * r]), __builtin_fmaf((float)a.y, low, x[2 * r + 1]));
+    }
+    return h8{b[0].x, b[0].y, b[1].x, b[1].y, b[2].x, b[2].y, b[3].x, b[3].y};
 }
 
 // Over the four 16-lane rows of the wave (lanes of one column), in every lane.
@@ -161,24 +161,6 @@ struct TileView {
             for (int j = 0; j < 2; ++j) k[j] = dequant8(x[j], d4, mg);
         }
     }
-    // Their codes (codes8).
-    __device__ __forceinline__ void key_codes(int t, int c, h8 (&k)[W]) const {
-        const uint8_t* w = p + ((t * C + c) * 64 + lane) * (4 * W);
-        if constexpr (W == 4) {
-            const u32x4 x = *(const u32x4*)w;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) k[j] = codes8(x[j]);
-        } else {
-            const u32x2 x = *(const u32x2*)w;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) k[j] = codes8(x[j]);
-        }
-    }
-    __device__ __forceinline__ void value_codes(int c, h8 (&v)[4]) const {
-        const u32x4 x = *(const u32x4*)(p + 16 * HD + (c * 64 + lane) * 16);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = codes8(x[j]);
-    }
     // The value scales of positions from `limit` of the tile on become 0 in LDS: bytes that no store has
     // written may be NaN.
     __device__ __forceinline__ void mask_scales(int limit) const {
@@ -203,16 +185,14 @@ struct TileView {
     }
 };
 
-// The 16 columns of the products' second operand. A unit has 16 / SPREAD (row, head) pairs c = row * G
-// + head in group. SPREAD 1: column n is pair n. SPREAD NB = HD / 32: column n is pair n / NB for block
-// n % NB only, its query elements of other blocks 0: the products with plain codes then come out as
-// one sum per block, to be scaled there.
-template <int HD, int SPREAD>
+// The 16 columns of the products' second operand. PARTS 1: column n is (row, head) pair n of the unit's
+// 16, and there is a second operand for the low parts. PARTS 2: column n is the high (n even) or low part
+// of pair n / 2 of the unit's 8, and half the products do.
+template <int HD, int PARTS>
 struct Queries {
     static constexpr int KW = HD / 32;
-    h8 hi[KW], lo[KW];
-    float sc;    // score in log2 units = product * sc
-    float init;  // SPREAD > 1: -8 times the column's sum of elements, in the product's units
+    h8 hi[KW], lo[PARTS == 1 ? KW : 1];
+    float sc;  // score in log2 units = product * sc
 
     // q row scaled by a power of two so that its largest element lies in [2^14, 2^15): hi and lo
     // then keep 22 significant bits of every element that counts.
@@ -239,45 +219,22 @@ struct Queries {
         m = max_over_g(m);
         int sh = 0;
         if (m > 0.0f && m < __builtin_huge_valf())
-            sh = min(max(15 - __builtin_amdgcn_frexp_expf(m), -120), 100);
+            sh = min(max(15 - __builtin_amdgcn_frexp_expf(m), -120), 120);
         sc = ldexpf(kLog2e / sqrtf((float)HD), -sh);
-        float sum = 0.0f;
+        const float low = n & 1 ? mg.minus1 : 0.0f;
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[j][i] = ldexpf(x[j][i], sh);
-                if constexpr (SPREAD > 1) {
-                    if ((g * (HD / 4) + 8 * j) / 32 != n % SPREAD) x[j][i] = 0.0f;
-                    if (odd_pair(i)) x[j][i] *= 0.0625f;
-                }
-            }
-            split8(x[j], hi[j], lo[j], mg);
-            if constexpr (SPREAD > 1) {  // (of the parts, so that a code of 8 weighs nothing)
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    sum += ((float)hi[j][i] + (float)lo[j][i]) * (odd_pair(i) ? 16.0f : 1.0f);
-            }
-        }
-        if constexpr (SPREAD > 1) {
-            sc = ldexpf(sc, 24);
-            init = sum_over_g(sum) * (-8.0f * 0x1p-24f);
+            for (int i = 0; i < 8; ++i) x[j][i] = ldexpf(x[j][i], sh);
+            if constexpr (PARTS == 1) split8(x[j], hi[j], lo[j], mg); else hi[j] = part8(x[j], low);
         }
     }
 };
 
-// Sum over the SPREAD columns of a pair (neighbouring lanes), in each of them. (Every lane has a source,
-// so the move needs no old value and folds into the addition.)
-template <int CTRL>
-__device__ __forceinline__ float add_dpp(float v) {
-    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
-}
-template <int SPREAD>
-__device__ __forceinline__ float sum_over_blocks(float v) {
-    if constexpr (SPREAD >= 2) v = add_dpp<DPP_QUAD_SWAP1>(v);
-    if constexpr (SPREAD >= 4) v = add_dpp<DPP_QUAD_SWAP2>(v);
-    if constexpr (SPREAD >= 8) v = add_dpp<DPP_ROW_HALF_MIRROR>(v);
-    return v;
+// Sum over the two columns of a pair (neighbouring lanes), in both. (Every lane has a source, so the
+// move needs no old value and folds into the addition.)
+__device__ __forceinline__ float add_pair(float v) {
+    return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), DPP_QUAD_SWAP1, 0xF, 0xF, true));
 }
 
 // ---------------------------------------------------------------------------- the work's split
@@ -293,7 +250,7 @@ __device__ __forceinline__ float sum_over_blocks(float v) {
 // Partial results lie in slots (direct: unit * splits + split; stream: unit + workgroup, which grows
 // along the staircase of pairs), and a second launch joins them.
 constexpr int kCus = 256;
-constexpr int kGrid = 2 * kCus;     // workgroups of the one-tile kernel that run at once
+constexpr int kGrid = 2 * kCus;     // direct: workgroups at most, unless there are more units
 constexpr int kDirectUnits = 256;
 constexpr int kMinShare = 8;        // tiles
 
@@ -412,11 +369,13 @@ struct Parts {
 // each with its own running maximum, tiles coming through a ring of STAGES slots in LDS that the
 // wave fills itself, and meet once at the unit's end.
 //
-// What bounds it: VALU work, about 310 operations per tile and wave for dequantization (208) and the
-// softmax of 16 columns, beside the read of the cache.
+// What bounds it: the read of the cache, and beside it about 240 VALU operations per tile and wave for
+// dequantization (208 at HD 128) and the softmax of its 16 columns.
 template <int HD>
 struct AttnLds {
-    static constexpr int STAGES = HD == 64 ? 4 : HD == 128 ? 4 : 2;
+    // waves on a SIMD, which is workgroups on a CU, and slots a wave: within 512 registers and 160 KB
+    // (64 sequences of 4096-8192 positions, HD 128: 2 and 4 101 us, 3 and 2 94, 4 and 2 103)
+    static constexpr int WAVES = HD == 64 ? 4 : HD == 128 ? 3 : 2, STAGES = HD == 64 ? 4 : 2;
     static constexpr int RING = STAGES * 36 * HD;
     union {
         uint8_t ring[4][RING];
@@ -425,11 +384,11 @@ struct AttnLds {
     float m[4][16], l[4][16];
 };
 
-template <int HD, int SPREAD>
-__global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, const float* __restrict__ q,
-                                                          AttnArgs a, int splits, Parts parts,
+template <int HD, int PARTS>
+__global__ __launch_bounds__(256, AttnLds<HD>::WAVES) void k_kv4_attention(Kv4View c, int layer, const float* __restrict__ q,
+                                                          AttnArgs a, int splits, bool once, Parts parts,
                                                           float* __restrict__ out) {
-    constexpr int NT = HD / 16, W = TileView<HD>::W, COLS = 16 / SPREAD, STAGES = AttnLds<HD>::STAGES, NL = TileLoads<HD>::COUNT;
+    constexpr int NT = HD / 16, W = TileView<HD>::W, COLS = 16 / PARTS, STAGES = AttnLds<HD>::STAGES, NL = TileLoads<HD>::COUNT;
     extern __shared__ __align__(16) uint8_t lds_bytes[];
     AttnLds<HD>& lds = *(AttnLds<HD>*)lds_bytes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -482,7 +441,7 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
             f += t_end - t_begin;
         }
         const int h = unit % c.n_kv, c0 = unit / c.n_kv * COLS, n_cols = w.rows * a.G;
-        const int col = c0 + n / SPREAD;
+        const int col = c0 + n / PARTS;
         const bool valid = col < n_cols;
         const int row = col / a.G, head = h * a.G + (col - row * a.G);
         const int vis = valid ? w.s.len - w.s.rows + row + 1 : 0;       // positions the column sees
@@ -509,60 +468,42 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
             const uint8_t* p = layer_pages;
             if (!none) p += page * c.page_bytes + (((int64_t)h << sub) + (tl & ((1 << sub) - 1))) * (36 * HD);
             holes |= (none ? 1u : 0u) << ahead;
-            TileLoads<HD>::template issue<(SPREAD > 1)>(p, lds.ring[wave] + (i % STAGES) * (36 * HD), lane);
+            const uint8_t* slot_lds = lds.ring[wave] + (i % STAGES) * (36 * HD);
+            if (once) TileLoads<HD>::template issue<true>(p, slot_lds, lane);
+            else TileLoads<HD>::template issue<false>(p, slot_lds, lane);
         };
         for (int i = 0; i < min(count, STAGES - 1); ++i) issue(i, i);
 
-        Queries<HD, SPREAD> qs;
+        Queries<HD, PARTS> qs;
         qs.load(q + ((int64_t)(w.s.r0 + row) * a.n_head + head) * HD, valid, g, n, mg);
         f32x4 acc[NT];
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = kNegInf, l = 0.0f;
-        // SPREAD > 1: the products with codes of 8 (every row the same), odd pairs' sum of weights, the
-        // bound of the value scales
-        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f};
-        float l_odd = 0.0f, bound = 0.0f;
-        int bound_ex = 0;
+        const float low = n & 1 ? mg.minus1 : 0.0f;  // (PARTS 2)
 
         // edge: the tile ends past what some column sees, or past the sequence, or has no page (len 0)
         const auto step = [&](const TileView<HD>& tv, int p0, int len, bool edge) {
             if (edge) tv.mask_scales(len - p0);
-            f32x4 s[2];
-            u32x4 vs;  // SPREAD > 1: the value scales of the lane's block and positions
-            if constexpr (SPREAD > 1) {
-                s[0] = s[1] = f32x4{qs.init, qs.init, qs.init, qs.init};
-                vs = *(const u32x4*)(tv.p + 34 * HD + ((n % SPREAD) * 4 + g) * 16);
-            } else {
-                s[0] = s[1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
+            f32x4 s[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int kc = 0; kc < TileView<HD>::C; ++kc) {
                 h8 k[2][W];
 #pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    if constexpr (SPREAD > 1) tv.key_codes(t, kc, k[t]); else tv.keys(t, kc, k[t], mg);
-                }
+                for (int t = 0; t < 2; ++t) tv.keys(t, kc, k[t], mg);
 #pragma unroll
                 for (int j = 0; j < W; ++j) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t) s[t] = mfma(k[t][j], qs.hi[kc * W + j], s[t]);
+                    if constexpr (PARTS == 1) {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) s[t] = mfma(k[t][j], qs.lo[kc * W + j], s[t]);
-                }
-            }
-            if constexpr (SPREAD > 1) {  // the blocks' sums scaled (positions 4 g .. + 3 of both halves) and joined
-                const u32x4 ks = *(const u32x4*)(tv.p + 32 * HD + ((n % SPREAD) * 16 + 4 * g) * 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const h2 d = __builtin_bit_cast(h2, (uint32_t)ks[i]);
-                    s[0][i] = sum_over_blocks<SPREAD>(__builtin_fmaf(s[0][i], (float)d.x, mg.zero));
-                    s[1][i] = sum_over_blocks<SPREAD>(__builtin_fmaf(s[1][i], (float)d.y, mg.zero));
+                        for (int t = 0; t < 2; ++t) s[t] = mfma(k[t][j], qs.lo[kc * W + j], s[t]);
+                    }
                 }
             }
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = s[e >> 2][e & 3];
+            for (int e = 0; e < 8; ++e) x[e] = PARTS == 1 ? s[e >> 2][e & 3] : add_pair(s[e >> 2][e & 3]);
             if (edge) {
                 const int end = min(vis, len) - p0 - 4 * g;
 #pragma unroll
@@ -572,69 +513,32 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
             mx = max_over_g(mx) * qs.sc;
-            bool grow = mx > m + kSlack;
-            uint32_t d_max = 0;
-            if constexpr (SPREAD > 1) {  // the lane's largest |scale|, as fp16 bits
-                typedef uint16_t us2 __attribute__((ext_vector_type(2)));
-                us2 t = __builtin_bit_cast(us2, vs[0] & 0x7FFF7FFFu);
-#pragma unroll
-                for (int i = 1; i < 4; ++i)
-                    t = __builtin_elementwise_max(t, __builtin_bit_cast(us2, vs[i] & 0x7FFF7FFFu));
-                d_max = max((uint32_t)t.x, (uint32_t)t.y);
-                grow |= f16_to_f32(d_max) > bound;
-            }
-            if (__any(grow)) {
+            if (__any(mx > m + kSlack)) {
                 const float m_new = fmaxf(m, mx);
-                float r = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
+                const float r = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
                 m = m_new;
-                if constexpr (SPREAD > 1) {
-                    // the weights times a scale below 2^bound_ex times 2^-bound_ex stay within 2^15; a
-                    // factor of two in hand, so that few tiles raise the bound
-                    const float all = max_over_g(f16_to_f32(d_max));
-                    if (all > bound) {
-                        const int ex = __builtin_amdgcn_frexp_expf(all) + 1;
-                        r = bound == 0.0f ? r : ldexpf(r, bound_ex - ex);
-                        bound_ex = ex;
-                        bound = ldexpf(1.0f, ex);
-                    }
-                    l_odd *= r;
-                    z *= r;
-                }
                 l *= r;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) acc[i] *= r;
             }
-            const float mm = kTop - (m == kNegInf ? 0.0f : m) - (float)bound_ex;
+            const float mm = kTop - (m == kNegInf ? 0.0f : m);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], qs.sc, mm));
+                l += x[e];
+            }
             h8 hi, lo;
-            if constexpr (SPREAD > 1) {
-                const float mo = mm - 4.0f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const h2 d = __builtin_bit_cast(h2, (uint32_t)vs[e >> 1]);
-                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], qs.sc, odd_pair(e) ? mo : mm));
-                    (odd_pair(e) ? l_odd : l) += x[e];
-                    x[e] = __builtin_fmaf(x[e], (float)(e & 1 ? d.y : d.x), mg.zero);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], qs.sc, mm));
-                    l += x[e];
-                }
-            }
-            split8(x, hi, lo, mg);
-            if constexpr (SPREAD > 1) {
-                z = mfma(codes8(0x88888888u), hi, z);
-                z = mfma(codes8(0x88888888u), lo, z);
-            }
+            if constexpr (PARTS == 1) split8(x, hi, lo, mg); else hi = part8(x, low);
 #pragma unroll
             for (int cc = 0; cc < NT / 4; ++cc) {
                 h8 v[4];
-                if constexpr (SPREAD > 1) tv.value_codes(cc, v); else tv.values(cc, v, mg);
+                tv.values(cc, v, mg);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[4 * cc + i] = mfma(v[i], hi, acc[4 * cc + i]);
+                if constexpr (PARTS == 1) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[4 * cc + i] = mfma(v[i], lo, acc[4 * cc + i]);
+                    for (int i = 0; i < 4; ++i) acc[4 * cc + i] = mfma(v[i], lo, acc[4 * cc + i]);
+                }
             }
         };
         for (int i = 0; i < count; ++i) {
@@ -651,27 +555,24 @@ __global__ __launch_bounds__(256, 2) void k_kv4_attention(Kv4View c, int layer, 
             const TileView<HD> tv = {lds.ring[wave] + (i % STAGES) * (36 * HD), lane};
             step(tv, p0, hole ? 0 : w.s.len, hole || p0 + kTile > vis_min || p0 + kTile > w.s.len);
         }
-        if constexpr (SPREAD > 1) {
-            // sums over codes become sums over values: less the codes of 8, 2^24 for their units, and
-            // the scales' bound taken out
-            l = ldexpf(l + 16.0f * l_odd, bound_ex);
+        if constexpr (PARTS == 2) {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = ldexpf(acc[i][j] - z[j], 24 + bound_ex);
+                for (int j = 0; j < 4; ++j) acc[i][j] = add_pair(acc[i][j]);
         }
         l = sum_over_g(l);
 
         // the four waves' results meet (in the ring's place): outputs of column n, elements 16 i + 4 g
         // .. + 3 of each wave
-        if (g == 0 && n % SPREAD == 0) {
-            lds.m[wave][n / SPREAD] = m;
-            lds.l[wave][n / SPREAD] = l;
+        if (g == 0 && n % PARTS == 0) {
+            lds.m[wave][n / PARTS] = m;
+            lds.l[wave][n / PARTS] = l;
         }
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NT; ++i)
-            if (SPREAD == 1 || i / 2 == n % SPREAD) lds.o[wave][n / SPREAD][4 * i + g] = acc[i];
+            if (PARTS == 1 || i % 2 == n % 2) lds.o[wave][n / PARTS][4 * i + g] = acc[i];
         __syncthreads();
         for (int i = threadIdx.x; i < COLS * (HD / 4); i += 256) {
             const int cn = i / (HD / 4), d4 = i % (HD / 4);
@@ -1465,14 +1366,12 @@ Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int m
         p.grid = p.units * p.splits;
         return p;
     }
-    // the columns carry the blocks where all (row, head) pairs of a KV head fit beside each other
-    const int nb = c.hd / 32;
-    p.cols = cols * nb <= 16 ? 16 / nb : 16;
+    p.cols = cols <= 8 ? 8 : 16;
     p.units = (int64_t)n_seqs * c.n_kv * ((cols + p.cols - 1) / p.cols);
     p.splits = 0;
     if (p.units > 0 && p.units <= kDirectUnits)
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(shares, kGrid / p.units));
-    p.grid = p.splits > 0 ? p.units * p.splits : kGrid;
+    KV4_HD(c.hd, p.grid = p.splits > 0 ? p.units * p.splits : kCus * AttnLds<HD>::WAVES);
     return p;
 }
 
@@ -1485,14 +1384,14 @@ size_t kv4_attention_ws_bytes(const Kv4AttnPlan& p, int hd) {
     return p.splits > 0 ? part : part + p.units * sizeof(UnitMap) + sizeof(int64_t);
 }
 
-template <int HD, int SPREAD>
+template <int HD, int PARTS>
 static hipError_t launch_attention(const Kv4View& c, const Kv4AttnPlan& p, int layer, const float* q, const AttnArgs& a,
                                    const Parts& parts, float* out, hipStream_t stream) {
     static LdsLimit limit;
-    const hipError_t e = limit.raise((const void*)k_kv4_attention<HD, SPREAD>, sizeof(AttnLds<HD>));
+    const hipError_t e = limit.raise((const void*)k_kv4_attention<HD, PARTS>, sizeof(AttnLds<HD>));
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((k_kv4_attention<HD, SPREAD>), dim3((unsigned)p.grid), dim3(256), sizeof(AttnLds<HD>), stream, c,
-                       layer, q, a, p.splits, parts, out);
+    hipLaunchKernelGGL((k_kv4_attention<HD, PARTS>), dim3((unsigned)p.grid), dim3(256), sizeof(AttnLds<HD>), stream, c,
+                       layer, q, a, p.splits, a.max_rows * a.G <= p.cols, parts, out);
     return hipGetLastError();
 }
 
@@ -1520,7 +1419,7 @@ hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int laye
     KV4_HD(c.hd, {
         e = p.many_rows ? launch_many_rows<HD>(c, p, layer, q, a, parts, out, stream)
             : p.cols == 16 ? launch_attention<HD, 1>(c, p, layer, q, a, parts, out, stream)
-                           : launch_attention<HD, HD / 32>(c, p, layer, q, a, parts, out, stream);
+                           : launch_attention<HD, 2>(c, p, layer, q, a, parts, out, stream);
     });
     if (e != hipSuccess || p.splits == 1) return e;
     KV4_HD(c.hd, {

@@ -184,17 +184,10 @@ class Cache:
         return np.where(ok[:, None, None], kv[0], 0.0), np.where(ok[:, None, None], kv[1], 0.0), ok
 
 
-def block_max(x):
-    """Of every element, the largest size in its block of 32: 8 d, as a block's extreme has code 0."""
-    b = np.abs(x).reshape(*x.shape[:-1], x.shape[-1] // 32, 32).max(-1, keepdims=True)
-    return np.broadcast_to(b, (*b.shape[:-1], 32)).reshape(x.shape)
-
-
 def attention(q, k, v, ok, first):
     """q [r, n_head, hd] over k, v [n, n_kv, hd] in 64 bits; row t sees positions <= first + t that
-    are ok. Returns the outputs, and per output the bounds the tolerance is made of, with K and V
-    the block maxima (8 d) of k and v: the largest sum |q_i| K_i / sqrt(hd) of the row's positions,
-    sum p V and sum V."""
+    are ok. Returns the outputs, and per output the bounds the tolerance is made of: the largest
+    sum |q_i k_i| / sqrt(hd) of the row's positions, sum p |v| and sum |v|."""
     r, n_head, hd = q.shape
     n, n_kv = k.shape[:2]
     g = n_head // n_kv
@@ -202,8 +195,8 @@ def attention(q, k, v, ok, first):
     out, size, mass, total = (np.zeros((r, n_kv, g, hd)) for _ in range(4))
     for h in range(n_kv):
         s = np.einsum("rgd,nd->rgn", q[:, h], k[:, h]) / np.sqrt(hd)
-        a = np.einsum("rgd,nd->rgn", np.abs(q[:, h]), block_max(k[:, h])) / np.sqrt(hd)
-        size_v = block_max(v[:, h])
+        a = np.einsum("rgd,nd->rgn", np.abs(q[:, h]), np.abs(k[:, h])) / np.sqrt(hd)
+        size_v = np.abs(v[:, h])
         for t in range(r):
             seen = ok & (np.arange(n) <= first + t)
             if not seen.any():
@@ -219,18 +212,23 @@ def attention(q, k, v, ok, first):
 
 
 def attention_bound(hd, n, size, mass, total):
-    """How far the kernel may be from the exact output. The products may run over plain codes c = 0 ..
-    15, d times the sum of weight times c less the sum of weight times 8: terms of up to 2 * 8 d and 8 d
-    whose sums are rounded, so rounding is relative to the block's 8 d and not to |d (c - 8)| (an element
-    of value 0 still adds 8 d twice); size, mass and total are made of 8 d, and the accumulations below
-    count three times (16 + 8 = 3 * 8). A query element as two fp16 parts is off by
-    at most 2^-20 of itself, the fp32 accumulation of hd products by (hd + 8) 2^-24 of their
-    magnitudes, the scaling to log2 units, the subtraction of the maximum and the exponential by
-    2^-21 of the score's size and 2^-22; so a weight is off by at most d below, relatively, and the
+    """How far the kernel may be from the exact output. The keys and values enter exactly. A query
+    element as two fp16 parts is off by at most 2^-20 of itself, the fp32 accumulation of hd products by
+    (hd + 8) 2^-24 of their magnitudes, the scaling to log2 units, the subtraction of the maximum and the
+    exponential by 2^-21 of the score's size and 2^-22; so a weight is off by at most d below, relatively, and the
     quotient of two sums of weights by 2 d. A weight as two fp16 parts, the largest between 2^11 and 2^15,
     adds 2^-20 of itself, or 2^-24 below fp16's normal numbers, 2^-35 of the largest: that times sum |v| in all,
     as the weights' sum is at least the largest (an output whose values lie under small weights only
     keeps an absolute accuracy). The running sums of a wave add one rounding per step:
     n / 16 of the denominator, n / 128 of the outputs, and the joins some 64."""
-    d = size * (2.0 ** -20 + 3 * (hd + 8) * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -21
-    return mass * (2.2 * d + 2.0 ** -20 + (n / 16 + 3 * n / 128 + 3 * 64) * 2.0 ** -24) + 2.0 ** -35 * total
+    d = size * (2.0 ** -20 + (hd + 8) * 2.0 ** -24 + 2.0 ** -21) + 2.0 ** -21
+    return mass * (2.2 * d + 2.0 ** -20 + (n / 16 + n / 128 + 64) * 2.0 ** -24) + 2.0 ** -35 * total
+
+
+def attention_rms_bound():
+    """And how far in the root mean square over all outputs, relative to theirs: every error above is a
+    rounding, of either sign (the parts' truncations follow the signs of the elements they truncate), so
+    over hd products and many outputs the largest of them, 2^-20 of a score of unit spread and of a weight,
+    counts about once: 4 * 2^-20 covers both, the accumulations and the values' spread. (A loss of bits
+    common to all terms, as of subnormal operands that are not normalised, is 2^-16 here.)"""
+    return 2.0 ** -18

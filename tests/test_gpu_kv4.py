@@ -77,7 +77,7 @@ class Pair:
             assert np.array_equal(k[a:b], mk, equal_nan=True), s
             assert np.array_equal(v[a:b], mv, equal_nan=True), s
 
-    def attend(self, rng, layer, slots, rows, n_head, scale=1.0, max_rows=None, max_len=None):
+    def attend(self, rng, layer, slots, rows, n_head, scale=1.0, max_rows=None, max_len=None, rms=False):
         starts = np.concatenate([[0], np.cumsum(rows)])
         q = (rng.standard_normal((starts[-1], n_head, self.hd)) * scale).astype(np.float32)
         max_len = max(1, int(self.m.lens[slots].max())) if max_len is None else max_len
@@ -94,6 +94,10 @@ class Pair:
             bound = M.attention_bound(self.hd, n, *sizes)
             err = np.abs(out[a:b] - want)
             assert (err <= bound).all(), (s, float((err - bound).max()), float(err.max()))
+            if rms:
+                e = float(np.sqrt((err ** 2).mean() / (want ** 2).mean()))
+                print("rms", e, flush=True)
+                assert e <= M.attention_rms_bound()
         return out
 
 
@@ -252,7 +256,7 @@ def test_attention(gpu, hd, n_kv, group, page, lens, rows):
     slots = list(rng.permutation(len(lens)))
     assert p.extend(slots, lens) == 0
     p.store(rng, 1, slots, lens)
-    p.attend(rng, 1, slots, rows, n_kv * group, scale=1.5)
+    p.attend(rng, 1, slots, rows, n_kv * group, scale=1.5, rms=True)
 
 
 @pytest.mark.parametrize("hd,n,rows,max_len", [(128, 5000, 1, None), (64, 3000, 4, None), (128, 1111, 1, 8192),
@@ -263,6 +267,7 @@ def test_attention_over_splits(gpu, hd, n, rows, max_len):
     p = Pair(gpu, 1, 100, 2, 80 if max_len != 8192 else 128, 64, 2, hd)
     assert p.extend([0, 1], [n, 30]) == 0
     p.store(rng, 0, [0, 1], [n, 30])
+    p.attend(rng, 0, [0, 1], [rows, 1], 8, scale=1.0, max_len=max_len, rms=True)
     p.attend(rng, 0, [0, 1], [rows, 1], 8, scale=2.0, max_len=max_len)
 
 
