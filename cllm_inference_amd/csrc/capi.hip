@@ -1711,7 +1711,7 @@ static int kv4_view(const char* who, const cllm_hip_kv4_cache* c, bool work, Kv4
                        "%s: page_size must be a power of two from 32 to 1024, head_dim 64, 128 or 256, "
                        "n_head_kv 1 to 1024", who);
     if (c->n_layers <= 0 || c->n_pages <= 0 || c->n_pages > (1 << 28) || c->max_seqs <= 0 || c->max_pages <= 0 ||
-        (int64_t)c->max_pages * c->page_size > INT32_MAX / 2)
+        (int64_t)c->max_pages * c->page_size > INT32_MAX / 2 || (int64_t)c->max_seqs * c->max_pages > INT32_MAX)
         return set_err(CLLM_HIP_E_ARG, "%s: bad cache shape", who);
     if (!c->pages || !c->table || !c->lens || !c->refs || (work && !c->work))
         return set_err(CLLM_HIP_E_ARG, "%s: null pointer in the cache", who);

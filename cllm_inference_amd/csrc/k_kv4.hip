@@ -1272,8 +1272,8 @@ __global__ __launch_bounds__(256) void k_kv4_load(Kv4View c, int layer, const in
     constexpr int NB = HD / 32;
     if ((int)blockIdx.x >= segments) {
         const Kv4Seq s = kv4_seq(c, slots, q_start, (int)blockIdx.x - segments, n_rows);
-        for (int i = threadIdx.x; i < (s.rows - s.len) * HD; i += 256) {
-            const int64_t at = ((int64_t)(s.r0 + i / HD) * c.n_kv + blockIdx.y) * HD + i % HD;
+        for (int64_t i = threadIdx.x; i < (int64_t)(s.rows - s.len) * HD; i += 256) {
+            const int64_t at = ((s.r0 + i / HD) * c.n_kv + blockIdx.y) * HD + i % HD;
             k[at] = 0.0f;
             v[at] = 0.0f;
         }

@@ -516,3 +516,127 @@ def test_bindings_refuse(gpu):
         with pytest.raises(RuntimeError):
             call()
             print("not refused:", i)
+
+
+# ---- the largest, and several at once ---------------------------------------------------------------
+
+def test_many_sequences(gpu):
+    """More sequences than a wave has lanes, empty ones among them: shares that cross sequences, segments
+    found past the first 64, and many rows of many sequences."""
+    rng = np.random.default_rng(41)
+    n, page = 150, 32
+    lens = rng.integers(0, 90, n)
+    lens[[3, 70, 149]] = [400, 0, 333]
+    p = Pair(gpu, 1, int(sum(-(-x // page) for x in lens)) + 2, n, 16, page, 2, 64)
+    slots = rng.permutation(n).tolist()
+    assert p.extend(slots, lens.tolist()) == 0
+    p.store(rng, 0, slots, lens.tolist())
+    p.check_rows(0, list(range(n)))
+    held = [int(p.m.lens[s]) for s in slots]
+    p.attend(rng, 0, slots, [min(1, x) for x in held], 4)           # decode, units of one column tile
+    p.attend(rng, 0, slots, [min(5, x) for x in held], 4)           # drafts
+    p.attend(rng, 0, slots, held, 4)                                # every row of every sequence
+    plan = gpu.kv4_attention_plan(p.c, n, n, 1, 400, 4)
+    assert "splits=0" in plan, plan
+
+
+def test_rows_past_max_rows_stay(gpu):
+    import torch
+    rng = np.random.default_rng(43)
+    p = Pair(gpu, 1, 30, 1, 20, 32, 2, 64)
+    assert p.extend([0], [300]) == 0
+    p.store(rng, 0, [0], [300])
+    q = torch.randn(200, 256, device="cuda")
+    full = gpu.kv4_attention_dev(p.c, 0, q, _i32([0, 200]), n_head=4, max_rows=200, max_len=300)
+    for max_rows in (3, 150):
+        out = torch.full_like(q, 5.0)
+        gpu.kv4_attention_dev(p.c, 0, q, _i32([0, 200]), n_head=4, max_rows=max_rows, max_len=300, out=out)
+        assert (out[max_rows:] == 5).all()
+        assert torch.allclose(out[:max_rows], full[:max_rows], rtol=1e-4, atol=1e-5)
+
+
+def test_a_pool_past_4_gib(gpu):
+    """Page and layer offsets past 32 bits, in every call that moves or reads pages."""
+    import torch
+    rng = np.random.default_rng(47)
+    page, n_kv, hd, layers, n_pages = 1024, 8, 256, 2, 1200  # 2.36 MB a page: 5.7 GB
+    c = gpu.Kv4Cache(layers, n_pages, 2, 4, page_size=page, n_head_kv=n_kv, head_dim=hd)
+    assert c.pages.numel() > (1 << 32) + (1 << 30)
+    assert int(gpu.kv4_extend_dev(c, None, _i32([70, 1030]))) == 0
+    c.table[0, 0], c.table[1, 0], c.table[1, 1] = 1199, 1100, 1198
+    c.refs.zero_()
+    c.refs[[1199, 1100, 1198]] = 1
+    k = rng.standard_normal((100, n_kv, hd)).astype(np.float32)
+    v = rng.standard_normal((100, n_kv, hd)).astype(np.float32)
+    starts = _i32([0, 70, 100])
+    gpu.kv4_store_dev(c, 1, _dev(k), _dev(v), starts)
+    mk, mv = M.stored(k, v)
+    q = rng.standard_normal((70, 8, hd)).astype(np.float32)
+    want, *sizes = M.attention(q, mk[:70], mv[:70], np.ones(70, bool), 0)
+
+    def check():
+        gk, gv = gpu.kv4_load_dev(c, 1, starts, 100)
+        assert np.array_equal(gk.cpu().numpy().reshape(mk.shape), mk)
+        assert np.array_equal(gv.cpu().numpy().reshape(mv.shape), mv)
+        for rows in (70, 1):
+            out = gpu.kv4_attention_dev(c, 1, _dev(q[70 - rows:]), _i32([0, rows]), n_head=8, max_rows=rows, max_len=70)
+            err = np.abs(out.cpu().numpy().reshape(rows, 8, hd) - want[70 - rows:])
+            assert (err <= M.attention_bound(hd, 70, *sizes)[70 - rows:]).all()
+
+    check()
+    gpu.kv4_copy_pages_dev(c, _i32([1199]), _i32([1197]))
+    c.table[0, 0] = 1197
+    check()
+    c.refs[1197], c.refs[1199] = 1, 0
+    assert int(gpu.kv4_compact_dev(c)) == 3
+    assert sorted(c.table[c.table >= 0].tolist()) == [0, 1, 2]
+    check()
+    gpu.kv4_fork_dev(c, _i32([0]), _i32([1]))
+    assert int(gpu.kv4_extend_dev(c, _i32([1]), _i32([1]))) == 0  # a copy on write
+    torch.cuda.synchronize()
+
+
+def test_two_streams_and_two_graphs(gpu):
+    """Attention calls that run at once, eager and as graphs, have scratch of their own."""
+    import torch
+    rng = np.random.default_rng(53)
+    p = Pair(gpu, 1, 200, 3, 80, 64, 2, 128)
+    assert p.extend([0, 1, 2], [5000, 4000, 900]) == 0
+    p.store(rng, 0, [0, 1, 2], [5000, 4000, 900])
+    starts = _i32([0, 1, 2, 3])
+    qs = [torch.randn(3, 1024, device="cuda") for _ in range(2)]
+    run = lambda q, out=None: gpu.kv4_attention_dev(p.c, 0, q, starts, n_head=8, max_rows=1, max_len=5000, out=out)  # noqa: E731
+    want = [run(q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], []
+    for q, s in zip(qs, streams):
+        g, out = torch.cuda.CUDAGraph(), torch.empty_like(q)
+        with torch.cuda.graph(g, stream=s):
+            run(q, out)
+        graphs.append(g)
+        outs.append(out)
+    for turn in range(5):
+        got = [[], []]
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    if turn % 2:
+                        graphs[i].replay()
+                    else:
+                        got[i].append(run(qs[i]))
+        torch.cuda.synchronize()
+        for i in range(2):
+            for o in got[i] or [outs[i]]:
+                assert torch.equal(o, want[i]), (turn, i)
+        torch.randn(1 << 18, device="cuda")
+
+
+def test_host_tensors_are_refused(gpu):
+    import torch
+    z = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(RuntimeError, match="needs CUDA tensors"):
+        gpu.Kv4Cache.from_tensors(torch.zeros((1, 2, gpu.kv4_page_bytes(32, 1, 64)), dtype=torch.uint8), z(1, 1), z(1),
+                                  z(2), page_size=32, n_head_kv=1, head_dim=64)
+    with pytest.raises(RuntimeError, match="needs CUDA tensors"):
+        gpu.logprobs_dev(torch.zeros(2, 5))

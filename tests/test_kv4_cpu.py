@@ -43,6 +43,7 @@ def test_sizes():
     (dict(page_size=48), "page_size"), (dict(page_size=2048), "page_size"), (dict(head_dim=96), "head_dim"),
     (dict(n_head_kv=0), "n_head_kv"), (dict(n_layers=0), "shape"), (dict(n_pages=0), "shape"),
     (dict(max_seqs=0), "shape"), (dict(max_pages=-1), "shape"), (dict(max_pages=1 << 26), "shape"),
+    (dict(max_seqs=1 << 20, max_pages=1 << 12), "shape"),
     (dict(pages=0), "null"), (dict(table=0), "null"), (dict(lens=0), "null"), (dict(refs=0), "null"),
     (dict(work=0), "null"), (dict(pages=PTR + 8), "misaligned"), (dict(table=PTR + 2), "misaligned"),
     (dict(refs=PTR + 1), "misaligned"),
