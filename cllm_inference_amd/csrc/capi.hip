@@ -1796,7 +1796,7 @@ static int kv4_attention_args(const char* who, const cllm_hip_kv4_cache* cache, 
     max_rows = std::min(max_rows, n_rows);
     max_len = std::min(max_len, c->max_pages << c->page_shift);
     *p = kv4_attention_plan(*c, n_seqs, max_rows, max_len, n_head);
-    if (p->units > INT32_MAX / 128 || p->grid > INT32_MAX) return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
+    if (!kv4_attention_fits(*p, c->hd)) return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
     return CLLM_HIP_OK;
 }
 
@@ -1931,7 +1931,7 @@ int cllm_hip_logprobs_dev(const float* logits, int64_t row_stride, int n_rows, i
     if (!aligned4(logits) || !aligned4(tokens) || !aligned4(logprobs) || !aligned4(ranks) || !aligned4(entropy) ||
         !aligned4(lse) || !aligned4(top_ids) || !aligned4(top_logprobs) || !aligned16(ws))
         return set_err(CLLM_HIP_E_ARG, "logprobs: misaligned device pointer");
-    if ((double)n_rows * ((vocab + 8191) / 8192) > 2147483647.0)
+    if ((int64_t)n_rows * ((vocab + 8191) / 8192) > UINT32_MAX / 256)  // (a launch's threads are counted in 32 bits)
         return set_err(CLLM_HIP_E_ARG, "logprobs: batch too large for one launch");
     const size_t need = logprobs_ws_bytes(n_rows, vocab, top_k);
     if (!ws || ws_bytes < need)

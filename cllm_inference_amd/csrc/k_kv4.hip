@@ -743,6 +743,37 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
     if (z >= n_split) return;
     const int t_begin = (int)((int64_t)tiles * z / n_split), t_end = (int)((int64_t)tiles * (z + 1) / n_split);
 
+    const int sub = c.page_shift - 5;
+    const int32_t* table = c.table + (int64_t)w.s.slot * c.max_pages;
+    const uint8_t* const layer_pages = c.pages + (int64_t)layer * c.n_pages * c.page_bytes;
+    // the wave's pieces of a turn: the same kind of tiles wave / KINDS, + 8 / KINDS
+    const int kind = wave % S::KINDS, tile0 = wave / S::KINDS;
+    Staged<HD> st[S::STAGED];
+    uint32_t holes = 0;  // a bit per tile of the turn
+    int ids = -1;        // page ids of 64 tiles, one a lane
+    const auto load = [&](int t0) {
+        holes = 0;
+        const int at = (t0 - t_begin) & 63;
+        if (at == 0) ids = t0 + lane < t_end ? table[(t0 + lane) >> sub] : -1;
+#pragma unroll
+        for (int i = 0; i < TURN; ++i) {
+            const int tl = t0 + i, page = __builtin_amdgcn_readlane(ids, at + i);
+            const uint8_t* p = nullptr;
+            if ((unsigned)page < (unsigned)c.n_pages)
+                p = layer_pages + page * c.page_bytes + (((int64_t)h << sub) + (tl & ((1 << sub) - 1))) * (36 * HD);
+            holes |= (p == nullptr ? 1u : 0u) << i;
+            if (i % (8 / S::KINDS) == tile0) st[i / (8 / S::KINDS)].load(p, min(kTile, w.s.len - tl * kTile), kind, lane);
+        }
+    };
+    const auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < S::STAGED; ++i)
+            st[i].store(lds_bytes + (buf * TURN + tile0 + i * (8 / S::KINDS)) * S::FRAGS * 1024, kind, lane, mg);
+    };
+
+    load(t_begin);
+    uint32_t holes_now = holes;
+
     // this wave's columns
     Queries<HD, 1> qs[NC];
     int vis[NC];
@@ -768,34 +799,6 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-
-    const int sub = c.page_shift - 5;
-    const int32_t* table = c.table + (int64_t)w.s.slot * c.max_pages;
-    const uint8_t* const layer_pages = c.pages + (int64_t)layer * c.n_pages * c.page_bytes;
-    // the wave's pieces of a turn: the same kind of tiles wave / KINDS, + 8 / KINDS
-    const int kind = wave % S::KINDS, tile0 = wave / S::KINDS;
-    Staged<HD> st[S::STAGED];
-    uint32_t holes = 0;  // a bit per tile of the turn
-    const auto load = [&](int t0) {
-        holes = 0;
-#pragma unroll
-        for (int i = 0; i < TURN; ++i) {
-            const int tl = t0 + i;
-            const uint8_t* p = nullptr;
-            if (tl < t_end) {
-                const int page = table[tl >> sub];
-                if ((unsigned)page < (unsigned)c.n_pages)
-                    p = layer_pages + page * c.page_bytes + (((int64_t)h << sub) + (tl & ((1 << sub) - 1))) * (36 * HD);
-            }
-            holes |= (p == nullptr ? 1u : 0u) << i;
-            if (i % (8 / S::KINDS) == tile0) st[i / (8 / S::KINDS)].load(p, min(kTile, w.s.len - tl * kTile), kind, lane);
-        }
-    };
-    const auto put = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < S::STAGED; ++i)
-            st[i].store(lds_bytes + (buf * TURN + tile0 + i * (8 / S::KINDS)) * S::FRAGS * 1024, kind, lane, mg);
-    };
 
     const auto step = [&](const uint8_t* frags, int p0, bool hole) {
         // (the wave that forms scores goes first: its neighbour's softmax fills the gaps; 3% less time)
@@ -867,8 +870,6 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
         }
     };
 
-    load(t_begin);
-    uint32_t holes_now = holes;
     put(0);
     load(t_begin + TURN);
     __syncthreads();
@@ -1375,6 +1376,16 @@ Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int m
     return p;
 }
 
+// Workgroups of the join: per unit its columns in groups, or one a column (k_kv4_join).
+static int64_t join_grid(const Kv4AttnPlan& p, int hd) {
+    const int groups = 256 / (hd / 4);
+    return p.splits == 1 ? 0 : p.units * (p.splits <= kFewSplits ? (p.cols + groups - 1) / groups : p.cols);
+}
+// A launch's threads are counted in 32 bits.
+bool kv4_attention_fits(const Kv4AttnPlan& p, int hd) {
+    return p.units <= INT32_MAX && p.grid <= UINT32_MAX / (p.many_rows ? 512 : 256) && join_grid(p, hd) <= UINT32_MAX / 256;
+}
+
 static size_t kv4_attention_slots(const Kv4AttnPlan& p) {
     return (size_t)(p.splits > 0 ? p.grid : p.units + p.grid);
 }
@@ -1423,9 +1434,8 @@ hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int laye
     });
     if (e != hipSuccess || p.splits == 1) return e;
     KV4_HD(c.hd, {
-        constexpr int GROUPS = 256 / (HD / 4);
-        const int64_t blocks = p.units * (p.splits <= kFewSplits ? (p.cols + GROUPS - 1) / GROUPS : p.cols);
-        hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)blocks), dim3(256), 0, stream, c, a, p.splits, parts, out);
+        hipLaunchKernelGGL((k_kv4_join<HD>), dim3((unsigned)join_grid(p, HD)), dim3(256), 0, stream, c, a, p.splits, parts,
+                           out);
     });
     return hipGetLastError();
 }

@@ -69,6 +69,7 @@ struct Kv4AttnPlan {
     int64_t grid;   // workgroups
 };
 Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int max_len, int n_head);
+bool kv4_attention_fits(const Kv4AttnPlan& p, int hd);
 size_t kv4_attention_ws_bytes(const Kv4AttnPlan& p, int hd);
 hipError_t launch_kv4_attention(const Kv4View& c, const Kv4AttnPlan& p, int layer, const float* q,
                                 const int32_t* slots, const int32_t* q_start, int n_seqs, int n_rows,

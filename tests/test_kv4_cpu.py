@@ -113,6 +113,22 @@ def test_bad_arguments_are_refused():
     assert fork(r, None, None, 0, None) == 0
 
 
+def test_launches_past_32_bits_are_refused():
+    """The threads of a launch are counted in 32 bits."""
+    lib = C.load_library()
+    c = _cache(max_pages=4096, max_seqs=65536)
+    r = ctypes.byref(c)
+    for args in ((65536, 1 << 26, 1 << 26, 100, 65536), (65536, 1 << 26, 1024, 100, 64), (65536, 1 << 26, 8, 100000, 65536)):
+        assert lib.cllm_hip_kv4_attention_dev(r, 0, PTR, None, PTR, *args, PTR, PTR, 1 << 60, None) == 3, args
+        assert "too large" in _err()
+        assert lib.cllm_hip_kv4_attention_ws_bytes(r, *args) == 0
+        assert lib.cllm_hip_kv4_attention_plan(r, *args) == b"none"
+    assert lib.cllm_hip_kv4_attention_plan(r, 65536, 65536, 1, 100000, 16) != b"none"
+    f = lib.cllm_hip_logprobs_dev
+    assert f(PTR, 100, 1 << 24, 100, PTR, 0, PTR, PTR, PTR, PTR, None, None, PTR, 1 << 60, None) == 3
+    assert "too large" in _err()
+
+
 def test_logprobs_refusals():
     f = C.load_library().cllm_hip_logprobs_dev
     ok = dict(logits=PTR, stride=100, rows=2, vocab=100, tokens=PTR, k=5, lp=PTR, rk=PTR, en=PTR, ls=PTR, ti=PTR,
