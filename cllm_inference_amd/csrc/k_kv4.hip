@@ -241,18 +241,25 @@ __device__ __forceinline__ float add_pair(float v) {
 //
 // A unit is a column tile of a KV head of a sequence: n tiles of positions (one at least, so that
 // rows that see nothing are written too). Only the device knows the lengths:
-//   direct, up to kDirectUnits units: `splits` workgroups per unit; a unit of n tiles uses
-//   min(splits, ceil(n / kMinShare)) of them, evenly, and the rest end at once. A workgroup finds its
-//   place from its index alone; with one split there is nothing to join.
-//   stream, more units: the units' tiles lie end to end and workgroup w takes tiles [w Q, (w + 1) Q),
-//   found from sums over the sequences that each wave forms 64 at a time: the work is even whatever
-//   the lengths are, for a few restarts where a share crosses units.
+//   direct: `splits` workgroups per unit; a unit of n tiles uses min(splits, ceil(n / kMinShare)) of
+//   them, evenly, and the rest end at once. A workgroup finds its place from its index alone; with one
+//   split there is nothing to join.
+//   stream: the units' tiles lie end to end and workgroup w takes tiles [w Q, (w + 1) Q), found from
+//   sums over the sequences that each wave forms 64 at a time: the work is even whatever the lengths
+//   are, for a few restarts where a share crosses units and a join (8 to 20 us more than direct where
+//   contexts are short).
+// Direct up to kDirectUnits units or kDirectLen positions. One row, 8 KV heads of 128, us direct /
+// stream: 16 sequences of 1000-8000 31 / 34; 24 of 1000-8000 56 / 41, of 100-6000 37 / 49, of 6000
+// 46 / 40, of 4000 35 / 37; 64 of 1000-8000 90 / 77, of 4096-8192 102 / 95, of 6000 83 / 90, of 100-1000
+// 17 / 29, of 300 12 / 22; 256 of 100-2000 76 / 133.
 // Partial results lie in slots (direct: unit * splits + split; stream: unit + workgroup, which grows
 // along the staircase of pairs), and a second launch joins them.
 constexpr int kCus = 256;
 constexpr int kGrid = 2 * kCus;     // direct: workgroups at most, unless there are more units
-constexpr int kDirectUnits = 256;
-constexpr int kMinShare = 8;        // tiles
+constexpr int kDirectUnits = 128, kDirectLen = 6144;
+// Tiles of a share: one sequence of 600 positions (8 KV heads of 128) 4 9.6 us, 8 10.8, 16 11.4; of 8000
+// 15.3, 12.5, 13.7; 16 sequences of up to 2047 (2 KV heads of 64) 10.4, 10.0, 11.6.
+constexpr int kMinShare = 8;
 
 struct SeqWork {
     Kv4Seq s;
@@ -974,7 +981,7 @@ __device__ __forceinline__ Joined join_splits(const Parts& parts, int64_t slot, 
 // Up to kFewSplits splits (many rows, or streamed shares): a workgroup has a unit's GROUPS columns, one
 // each. More: a workgroup per column, whose groups take every GROUPS-th split, so the loads of a long
 // list are in flight together, and meet in LDS.
-constexpr int kFewSplits = 4;
+constexpr int kFewSplits = 4;  // 8 sequences of 96 columns (HD 64): 3 66.6 us, 4 49.2, 6 49.8
 template <int HD>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4View c, AttnArgs a, int splits, Parts parts,
                                                   float* __restrict__ out) {
@@ -1352,27 +1359,35 @@ hipError_t launch_kv4_load(const Kv4View& c, int layer, const int32_t* slots, co
     return hipGetLastError();
 }
 
-// Columns of a KV head up to which the one-tile kernel runs: it reads the cache once per 16 of them.
-constexpr int kFewCols = 64;
+// The kernel of one column tile reads the cache once per 16 columns and dequantizes it as often, which
+// the many columns of k_kv4_many_rows share; but those fill the chip with few of them. So the former
+// takes up to kFewCols columns, and on, where contexts are short, up to kFewColsShort (heads of 64: at any
+// length) and what it has workgroups at once for. us, one tile / many rows, 8 KV heads of 4 query heads each:
+//   1 sequence of 4000, 64 rows: heads of 64 16.3 / 27.8, 128 20.9 / 29.1, 256 31.6 / 36.8
+//   1 of 128, 128 rows: 6.0 / 15.0, 7.5 / 14.7, 10.9 / 16.1; 128 rows of 8000: 48 / 46, 69 / 58, 105 / 97
+//   8 of 2000-4000, 24 rows: 35 / 49, 47 / 48, 75 / 91; 8 of 2000-4000, 64 rows: 58 / 57, 88 / 78, 155 / 156
+//   16 of 8000, 17 rows: 68 / 153, 103 / 137, 198 / 363; 16 of 8000, 32 rows: 111 / 155, 169 / 142, 343 / 378
+//   4 of 12000, 32 rows: 64 / 78, 93 / 71, 165 / 137
+constexpr int kFewCols = 96, kFewColsShort = 128;
 
 Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int max_len, int n_head) {
     Kv4AttnPlan p;
     const int64_t cols = (int64_t)max_rows * (n_head / c.n_kv);
     const int64_t tiles = std::max(1, (max_len + kTile - 1) / kTile), shares = (tiles + kMinShare - 1) / kMinShare;
-    p.many_rows = cols > kFewCols;
+    p.cols = cols <= 8 ? 8 : 16;
+    p.units = (int64_t)n_seqs * c.n_kv * ((cols + p.cols - 1) / p.cols);
+    const bool short_ = max_len <= kDirectLen;
+    p.many_rows = cols > kFewCols && (cols > kFewColsShort || (c.hd > 64 && !short_)) && (p.units > kCus || !short_);
     if (p.many_rows) {
         KV4_HD(c.hd, p.cols = ManyRows<HD>::COLS);
         p.units = (int64_t)n_seqs * c.n_kv * ((cols + p.cols - 1) / p.cols);
-        p.splits = (int)std::max<int64_t>(1, std::min(shares, p.units > 0 ? kCus / p.units : 1));
+        p.splits = (int)std::max<int64_t>(1, std::min(shares, kCus / p.units));
         p.grid = p.units * p.splits;
         return p;
     }
-    p.cols = cols <= 8 ? 8 : 16;
-    p.units = (int64_t)n_seqs * c.n_kv * ((cols + p.cols - 1) / p.cols);
-    p.splits = 0;
-    if (p.units > 0 && p.units <= kDirectUnits)
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(shares, kGrid / p.units));
-    KV4_HD(c.hd, p.grid = p.splits > 0 ? p.units * p.splits : kCus * AttnLds<HD>::WAVES);
+    const bool direct = p.units <= kDirectUnits || short_;
+    p.splits = direct ? (int)std::max<int64_t>(1, std::min<int64_t>(shares, kGrid / p.units)) : 0;
+    KV4_HD(c.hd, p.grid = direct ? p.units * p.splits : kCus * AttnLds<HD>::WAVES);
     return p;
 }
 

@@ -271,6 +271,33 @@ def test_attention_over_splits(gpu, hd, n, rows, max_len):
     p.attend(rng, 0, [0, 1], [rows, 1], 8, scale=2.0, max_len=max_len)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("form,n_kv,group,seqs,rows,hint", [
+    ("k_kv4_attention splits=0", 8, 2, 20, 1, 8192),       # shares of equal work across units
+    ("k_kv4_attention splits=0", 4, 4, 9, 16, 8192),       # the same, four column tiles
+    ("k_kv4_attention splits=1", 8, 4, 70, 1, 200),        # a workgroup per unit
+    ("k_kv4_attention splits=2", 1, 8, 1, 100, 400),       # many column tiles of one sequence
+    ("k_kv4_many_rows", 2, 4, 3, 60, 8192),                # split
+    ("k_kv4_many_rows splits=1", 8, 4, 5, 44, 256),        # not split
+])
+def test_attention_in_every_form(gpu, hd, form, n_kv, group, seqs, rows, hint):
+    """Each kernel and split of the work, over ragged lengths with an empty sequence and rows that see
+    nothing (max_len is a hint: results do not depend on it)."""
+    rng = np.random.default_rng([hd, n_kv, group, seqs, rows])
+    p = Pair(gpu, 1, 5 * seqs + 8, seqs, 8192 // 64, 64, n_kv, hd)
+    slots = [int(x) for x in rng.permutation(seqs)]
+    lens = [int(x) for x in rng.integers(1, 1 + min(hint, 260), seqs)]
+    lens[0] = max(lens[0], rows)
+    if seqs > 1:
+        lens[1] = 0
+    assert p.extend(slots, lens) == 0
+    p.store(rng, 0, slots, lens)
+    r = [rows] + [int(x) for x in rng.integers(1, rows + 1, seqs - 1)]  # (more rows than positions, some)
+    plan = p.gpu.kv4_attention_plan(p.c, seqs, sum(r), rows, hint, n_kv * group)
+    assert all(word in plan.replace("<", " <") for word in form.split()), plan
+    p.attend(rng, 0, slots, r, n_kv * group, max_len=hint, rms=False)
+
+
 def test_attention_of_sharp_and_large_scores(gpu):
     """Queries whose scores spread over hundreds (one position has all the weight), tiny queries
     (nearly equal weights), and rows that differ by 2^60 in size beside one another."""
@@ -537,7 +564,34 @@ def test_many_sequences(gpu):
     p.attend(rng, 0, slots, [min(5, x) for x in held], 4)           # drafts
     p.attend(rng, 0, slots, held, 4)                                # every row of every sequence
     plan = gpu.kv4_attention_plan(p.c, n, n, 1, 400, 4)
-    assert "splits=0" in plan, plan
+    assert "splits=1" in plan, plan
+
+
+def test_many_sequences_in_shares(gpu):
+    """The same in shares of equal work (which contexts that may be long get), and rows past max_rows there
+    and in the kernel for many rows."""
+    import torch
+    rng = np.random.default_rng(42)
+    n, page = 150, 32
+    lens = rng.integers(0, 90, n)
+    lens[[3, 70, 149]] = [400, 0, 333]
+    p = Pair(gpu, 1, int(sum(-(-x // page) for x in lens)) + 2, n, 256, page, 2, 64)
+    slots = rng.permutation(n).tolist()
+    assert p.extend(slots, lens.tolist()) == 0
+    p.store(rng, 0, slots, lens.tolist())
+    held = [int(p.m.lens[s]) for s in slots]
+    assert "splits=0" in gpu.kv4_attention_plan(p.c, n, n, 1, 8192, 4)
+    p.attend(rng, 0, slots, [min(1, x) for x in held], 4, max_len=8192)
+    p.attend(rng, 0, slots, [min(5, x) for x in held], 4, max_len=8192)
+    q = torch.randn(400, 256, device="cuda")
+    full = gpu.kv4_attention_dev(p.c, 0, q, _i32([0, 400]), n_head=4, slots=_i32([slots[3]]), max_rows=400, max_len=8192)
+    for max_rows in (3, 150):
+        assert ("many" in gpu.kv4_attention_plan(p.c, 1, 400, max_rows, 8192, 4)) == (max_rows == 150)
+        out = torch.full_like(q, 5.0)
+        gpu.kv4_attention_dev(p.c, 0, q, _i32([0, 400]), n_head=4, slots=_i32([slots[3]]), max_rows=max_rows,
+                              max_len=8192, out=out)
+        assert (out[max_rows:] == 5).all()
+        assert torch.allclose(out[:max_rows], full[:max_rows], rtol=1e-4, atol=1e-5)
 
 
 def test_rows_past_max_rows_stay(gpu):
