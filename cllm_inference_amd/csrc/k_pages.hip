@@ -236,7 +236,8 @@ __global__ __launch_bounds__(256) void k_kv4_fork(Kv4View c, const int32_t* __re
 }
 
 // A wave per entry, in turns; the entries that stand are found once.
-constexpr int kForkOne = 16384, kForkEntries = 128;
+// (us, one launch / two: 8 beams of 40 pages 4.2 / 6.5, 16 of 64 4.6 / 6.2, 16 of 256 7.3 / 6.3, 128 of 128 27 / 7)
+constexpr int kForkOne = 2048, kForkEntries = 128;
 __global__ __launch_bounds__(kThreads) void k_kv4_fork_one(Kv4View c, const int32_t* __restrict__ src,
                                                            const int32_t* __restrict__ dst, int n) {
     __shared__ int s_src[kForkEntries], s_dst[kForkEntries];

@@ -71,6 +71,19 @@ def test_logprobs(gpu, rows, vocab, top_k, kind):
     _check(gpu, x, tok, top_k)
 
 
+def test_many_large_logits_in_every_part(gpu):
+    """Sixty-three of the 64 wanted could come from any stretch of the vocabulary but the last, whose
+    logits are low: no bound of the stretches' lists leaves few."""
+    rng = np.random.default_rng(8)
+    vocab, stretch = 151936, 8192
+    x = rng.standard_normal((3, vocab)).astype(np.float32)
+    for row in x:
+        for z in range(vocab // stretch):
+            row[z * stretch + rng.permutation(stretch)[:63]] = rng.uniform(50, 60, 63)
+    _check(gpu, x, x.argmax(1), 64)
+    _check(gpu, x, rng.integers(0, vocab, 3), 20)
+
+
 def test_equal_logits_stand_in_the_order_of_their_ids(gpu):
     """Rows of one value, and of two, over several parts; the lists keep the lowest ids."""
     x = np.zeros((4, 20000), np.float32)
