@@ -8,7 +8,7 @@
 // term of the entropy is positive.
 //
 // What bounds it: the read of the logits, and about 14 VALU operations beside each: 1021 rows of 32003 with
-// the top 20 29.4 us (4.5 TB/s) and 5 for the join; one row of 128256 6.8 and 4. A workgroup takes 8192 logits of one row (grid rows x
+// the top 20 29.4 us (4.5 TB/s) and 4 for the join; one row of 128256 6.9 and 4. A workgroup takes 8192 logits of one row (grid rows x
 // parts) and holds them in registers, 32 a thread, all loads in flight at once: its maximum first,
 // then its sums, the tokens ahead of the given one and its largest logits, without reading twice.
 // A second launch joins a row's parts.
