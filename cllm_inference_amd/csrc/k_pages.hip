@@ -45,17 +45,29 @@ __device__ __forceinline__ int pages_of(int64_t len, int shift) {
     return (int)((len + ((int64_t)1 << shift) - 1) >> shift);
 }
 
+// Puts a key >= 0 into a hash table in LDS (of -1 at first, twice as many places as keys); whether it
+// was there.
+constexpr int kHash = 2 * kMaxEntries;
+__device__ __forceinline__ bool hash_insert(int* table, int key) {
+    static_assert(kHash == 1 << 11, "the hash has 11 bits");
+    for (uint32_t h = (uint32_t)key * 2654435761u >> 21;; h = (h + 1) & (kHash - 1)) {
+        const int old = atomicCAS(&table[h], -1, key);
+        if (old == -1) return false;
+        if (old == key) return true;
+    }
+}
+
 // Extends entry i (thread i) by counts[i] tokens. One workgroup, as the entries depend on one another (who
-// shares a page, who takes which free one): bound by its chain of loads, 5.4 us for 8 entries.
-// work: [0] copies, then (source, destination)
-// pairs, then the list of taken pages at 1 + 2 * kMaxEntries.
+// shares a page, who takes which free one): bound by its chain of loads, 5.3 us with the copies' launch for 1
+// to 1024 entries. work: [0] copies, then (source, destination) pairs, then the list of taken pages at 1 + 2 * kMaxEntries.
 __global__ __launch_bounds__(kThreads) void k_kv4_extend(Kv4View c, const int32_t* __restrict__ slots,
                                                          const int32_t* __restrict__ counts, int n,
                                                          int32_t* __restrict__ status) {
-    __shared__ int s_slot[kMaxEntries], s_page[kMaxEntries];
-    __shared__ int s_bad, s_copies;
+    __shared__ int s_page[kMaxEntries], s_slots[kHash], s_pages[kHash];
+    __shared__ int s_bad, s_copies, s_twice;
     const int tid = threadIdx.x;
-    if (tid == 0) s_bad = s_copies = 0;
+    if (tid == 0) s_bad = s_copies = s_twice = 0;
+    for (int i = tid; i < kHash; i += kThreads) s_slots[i] = s_pages[i] = -1;
     int slot = -1, count = 0, len = 0, old_pages = 0, page = -1;
     int64_t grow = 0;
     bool bad = false;
@@ -77,30 +89,42 @@ __global__ __launch_bounds__(kThreads) void k_kv4_extend(Kv4View c, const int32_
                 if (bad) page = -1;
             }
         }
-        s_slot[tid] = slot;
         s_page[tid] = page;
     }
     __syncthreads();
-    // entries before this one that hold the same page, which have left it by this one's turn
+    if (tid < n) {
+        if (!bad) {
+            bad = hash_insert(s_slots, slot);
+            if (page >= 0 && hash_insert(s_pages, page)) s_twice = 1;
+        }
+        if (bad) s_bad = 1;
+    }
+    __syncthreads();
+    if (s_bad) {
+        if (tid == 0) {
+            *status = -1;
+            c.work[0] = 0;
+        }
+        return;
+    }
+    // entries before this one that hold the same page, which have left it by this one's turn (counted only
+    // if a page is named twice: a comparison with every entry before takes 45 us for 1024 entries)
     bool copy = false;
     if (tid < n) {
         int same = 0;
-        for (int j = 0; j < tid; ++j) {
-            bad |= s_slot[j] == slot;
-            same += page >= 0 && s_page[j] == page;
-        }
-        copy = page >= 0 && !bad && c.refs[page] - same > 1;
-        if (bad) s_bad = 1;
+        if (s_twice)
+            for (int j = 0; j < tid; ++j) same += s_page[j] == page;
+        copy = page >= 0 && c.refs[page] - same > 1;
     }
-    const int need = bad ? 0 : (int)grow + (copy ? 1 : 0);
+    const int need = tid < n ? (int)grow + (copy ? 1 : 0) : 0;
     int total;
     const int first = block_scan(need, total);
-    if (s_bad || total == 0) {
+    if (total == 0) {
         if (tid == 0) {
-            *status = s_bad ? -1 : 0;
+            *status = 0;
             c.work[0] = 0;
         }
-        if (!s_bad && tid < n && count > 0) c.lens[slot] = len + count;
+        if (tid < n && count > 0) c.lens[slot] = len + count;
         return;
     }
     // the first `total` free pages

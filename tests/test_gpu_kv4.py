@@ -594,6 +594,30 @@ def test_many_sequences_in_shares(gpu):
         assert torch.allclose(out[:max_rows], full[:max_rows], rtol=1e-4, atol=1e-5)
 
 
+def test_extending_a_thousand(gpu):
+    """1024 entries at once: pages that many of them hold, slots named twice far apart, too few pages."""
+    rng = np.random.default_rng(47)
+    n, page = 1024, 32
+    p = Pair(gpu, 1, 4 * n, n, 4, page, 1, 64)
+    roots = [int(x) for x in rng.permutation(n)[:40]]
+    assert p.extend(roots, [int(x) for x in rng.integers(1, 100, 40)]) == 0
+    p.fork([roots[int(x)] for x in rng.integers(0, 30, n)], list(range(n)))  # ten of the roots live no more
+    slots = [int(x) for x in rng.permutation(n)]
+    for first, second in ((0, n - 1), (511, 512), (1022, 1023)):
+        twice = list(slots)
+        twice[second] = twice[first]
+        assert p.extend(twice, [1] * n) == -1
+    assert p.extend(slots, [int(x) for x in rng.integers(0, 2, n)]) == 0     # some stay on shared pages
+    assert p.extend(slots[:700], [1] * 700) == 0
+    assert p.extend(slots, [1] * n) == 0                                     # none shared within
+    assert p.extend(slots, [4 * page] * n) == -1
+    assert p.extend(slots, [28 if x <= 100 else 0 for x in p.m.lens[slots]]) in (0, 1)
+    while p.extend(slots, [page if x <= 96 else 0 for x in p.m.lens[slots]]) == 0 and p.m.lens.min() <= 96:
+        pass
+    p.truncate(slots)
+    assert int(p.c.refs.abs().sum()) == 0
+
+
 def test_rows_past_max_rows_stay(gpu):
     import torch
     rng = np.random.default_rng(43)
