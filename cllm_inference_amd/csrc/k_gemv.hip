@@ -1011,10 +1011,11 @@ __device__ __forceinline__ void wait_vmcnt() {
 // One wave-load of 16 bytes per lane from g into LDS at lds + 16 * lane (global_load_lds).
 // Written as inline assembly so that the compiler does not track it: it would otherwise wait
 // for every load in flight before each LDS read of the kernel, since it cannot tell which LDS
-// bytes a load writes. The caller orders the reads with wait_vmcnt.
+// bytes a load writes. The caller orders the reads with wait_vmcnt. (A scalar write of M0 needs one
+// wait state before the load reads it, which the compiler cannot see here either: the s_nop.)
 __device__ __forceinline__ void dma16(const void* g, const uint8_t* lds) {
     const uint32_t m0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)lds;
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(g), "s"(m0) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(g), "s"(m0) : "memory", "m0");
 }
 
 template <uint32_t T, int MR, int S, int WV, bool NORM = false>

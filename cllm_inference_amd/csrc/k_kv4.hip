@@ -114,14 +114,16 @@ __device__ __forceinline__ void wait_lds() {
 
 // A tile loaded straight into LDS (36 * HD bytes at `slot`) by one wave, 16 bytes a lane, the last load
 // by part of the lanes. The loads are the wave's own business: the compiler, which would wait for all
-// of them before any LDS read, does not see them, and wait_loads orders the reads. ONCE: bytes that no
+// of them before any LDS read, does not see them, and wait_loads orders the reads. (Nor does it see that a
+// scalar write of M0 needs a wait state before the load: the s_nop.) ONCE: bytes that no
 // other workgroup reads (nontemporal: 64 sequences of 4096-8192 positions 108.6 -> 104.0 us).
 template <bool ONCE>
 __device__ __forceinline__ void load_to_lds(const uint8_t* from, uint32_t m0) {
     if constexpr (ONCE)
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(from), "s"(m0) : "memory", "m0");
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" : : "v"(from), "s"(m0) : "memory",
+                     "m0");
     else
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(m0) : "memory", "m0");
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(from), "s"(m0) : "memory", "m0");
 }
 template <int HD>
 struct TileLoads {
