@@ -402,7 +402,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_join(const float* __restr
             } else if (a.max == kNegInf) {
                 sum += a.sum;  // 0, or NaN
             } else {
-                const float d = m - a.max, s = a.sum + (float)a.equal, w = __builtin_amdgcn_exp2f(-d * kLog2e);
+                // (exp of -200 and less is 0, as in the part; a part of a mask's finite lowest values is farther,
+                // and that times its 8192 weights past fp32's range)
+                const float d = fminf(m - a.max, 200.0f), s = a.sum + (float)a.equal, w = __builtin_amdgcn_exp2f(-d * kLog2e);
                 sum += w * s;
                 ent += w * (a.ent + d * s);
             }

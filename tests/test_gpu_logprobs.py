@@ -155,3 +155,27 @@ def test_captured(gpu):
         for name in ("logprobs", "ranks", "entropy", "lse", "top_ids", "top_logprobs"):
             assert torch.equal(getattr(r, name), getattr(e, name)), (i, name)
         torch.randn(1 << 20, device="cuda")
+
+
+def test_masks_of_finite_values(gpu):
+    """Rows whose masked tokens hold the type's lowest value, or another far below the rest, over whole parts
+    of the vocabulary; and one token far above all others: finite, with the probabilities of -inf masks."""
+    rng = np.random.default_rng(12)
+    for vocab in (8193, 20000, 50257):
+        x = (rng.standard_normal((8, vocab)) * 3).astype(np.float32)
+        low = np.finfo(np.float32).min
+        x[0, 8192:] = low                       # the last part
+        x[1, :8192] = low                       # the first part
+        x[2, 100:] = -1e38
+        x[3] = low
+        x[3, [7, 8192]] = [1.0, 2.5]            # two tokens left
+        x[4, 8190:] = -np.inf                   # both kinds of masks
+        x[4, 8192:] = low
+        x[5, 8192] = 3e38                       # (differences past fp32's range from here)
+        x[6, 5:] = -1e30
+        x[7, :] = low                           # nothing but the mask: equal probabilities
+        tok = np.array([8192, 5, 3, 8192, 8192, 8192, 4, vocab - 1])
+        for top_k in (0, 5, 64):
+            got = _check(gpu, x, tok, top_k)
+            assert all(np.isfinite(got[n]).all() for n in ("entropy", "lse")), vocab
+            assert np.isfinite(got["logprobs"]).all()
