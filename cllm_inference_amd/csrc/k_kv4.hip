@@ -28,8 +28,14 @@ constexpr int kTile = 32;  // positions of a tile
 // Weights are exp2(score - m + kTop), m the running maximum when the accumulators were last rescaled:
 // they are not until a score passes m by kSlack (with scores of unit spread, a tile in three raised the
 // maximum of some column). Weights stay within 2^15, and the fp16 parts of one that is the largest so far
-// reach down to 2^-24, 2^-35 of it.
-constexpr float kTop = 11.0f, kSlack = 4.0f;
+// reach down to 2^-24, 2^-35 of it. The exponent is one FMA with kTop - m, whose rounding is common to a
+// column's weights. From |m| = 2^23 on that and m's own would pass the slack: there the difference with m
+// is formed first, of products rounded as m was, so that the largest weight stays within 2^15.
+constexpr float kTop = 11.0f, kSlack = 4.0f, kFar = 8388608.0f;
+__device__ __forceinline__ float far_from(float score, float sc, float m) {
+#pragma clang fp contract(off)
+    return score * sc - m;
+}
 
 __device__ __forceinline__ f32x4 mfma(const h8& a, const h8& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -494,6 +500,7 @@ __global__ __launch_bounds__(256, AttnLds<HD>::WAVES) void k_kv4_attention(Kv4Vi
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = kNegInf, l = 0.0f;
+        bool far = false;  // a column's maximum is kFar or more from 0 (of all lanes)
         const float low = n & 1 ? mg.minus1 : 0.0f;  // (PARTS 2)
 
         // edge: the tile ends past what some column sees, or past the sequence, or has no page (len 0)
@@ -527,18 +534,27 @@ __global__ __launch_bounds__(256, AttnLds<HD>::WAVES) void k_kv4_attention(Kv4Vi
 #pragma unroll
             for (int e = 1; e < 8; ++e) mx = fmaxf(mx, x[e]);
             mx = max_over_g(mx) * qs.sc;
-            if (__any(mx > m + kSlack)) {
+            float sc = qs.sc, mm = kTop - (m == kNegInf ? 0.0f : m);
+            if (__any(mx > m + kSlack) || far) {
                 const float m_new = fmaxf(m, mx);
                 const float r = m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - m_new);
                 m = m_new;
                 l *= r;
 #pragma unroll
                 for (int i = 0; i < NT; ++i) acc[i] *= r;
+                const float base = m == kNegInf ? 0.0f : m;
+                mm = kTop - base;
+                far = __any(fabsf(base) >= kFar);
+                if (__builtin_expect(far, 0)) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = far_from(x[e], sc, base);
+                    sc = 1.0f;
+                    mm = kTop;
+                }
             }
-            const float mm = kTop - (m == kNegInf ? 0.0f : m);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], qs.sc, mm));
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], sc, mm));
                 l += x[e];
             }
             h8 hi, lo;
@@ -808,6 +824,7 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
     }
     f32x4 acc[NC][NT];
     float m[NC], l[NC];
+    bool far = false;  // a column's maximum is kFar or more from 0 (of all lanes)
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
         m[i] = kNegInf;
@@ -852,7 +869,14 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
             mx[i] = max_over_g(mx[i]) * qs[i].sc;
             grow |= mx[i] > m[i] + kSlack;
         }
-        if (__any(grow)) {
+        float sc[NC], mm[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            sc[i] = qs[i].sc;
+            mm[i] = kTop - (m[i] == kNegInf ? 0.0f : m[i]);
+        }
+        if (__any(grow) || far) {
+            float most = 0.0f;
 #pragma unroll
             for (int i = 0; i < NC; ++i) {
                 const float m_new = fmaxf(m[i], mx[i]);
@@ -861,17 +885,30 @@ __global__ __launch_bounds__(512, 2) void k_kv4_many_rows(Kv4View c, int layer, 
                 l[i] *= r;
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[i][j] *= r;
+                const float base = m[i] == kNegInf ? 0.0f : m[i];
+                mm[i] = kTop - base;
+                most = fmaxf(most, fabsf(base));
+            }
+            far = __any(most >= kFar);
+            if (__builtin_expect(far, 0)) {
+#pragma unroll
+                for (int i = 0; i < NC; ++i) {
+                    const float base = m[i] == kNegInf ? 0.0f : m[i];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s[i][e >> 2][e & 3] = far_from(s[i][e >> 2][e & 3], sc[i], base);
+                    sc[i] = 1.0f;
+                    mm[i] = kTop;
+                }
             }
         }
         __builtin_amdgcn_s_setprio(0);
         h8 hi[NC], lo[NC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            const float mm = kTop - (m[i] == kNegInf ? 0.0f : m[i]);
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e >> 2][e & 3], qs[i].sc, mm));
+                x[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e >> 2][e & 3], sc[i], mm[i]));
                 l[i] += x[e];
             }
             split8(x, hi[i], lo[i], mg);

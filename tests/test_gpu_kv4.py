@@ -718,3 +718,37 @@ def test_host_tensors_are_refused(gpu):
                                   z(2), page_size=32, n_head_kv=1, head_dim=64)
     with pytest.raises(RuntimeError, match="needs CUDA tensors"):
         gpu.logprobs_dev(torch.zeros(2, 5))
+
+
+@pytest.mark.parametrize("hd,group,rows,n", [(64, 4, 1, 300), (128, 4, 1, 3000), (128, 4, 5, 700), (256, 2, 8, 400),
+                                             (128, 4, 130, 130), (64, 4, 150, 700)])
+@pytest.mark.parametrize("scale", [1e4, 1e8, 1e10, 1e12, 1e30])
+def test_attention_of_huge_scores(gpu, hd, group, rows, n, scale):
+    """Queries so large that one position has all the weight, scores of either sign: each output is that
+    position's value row, to the 2^-20 of a weight in two fp16 parts and three roundings."""
+    rng = np.random.default_rng([hd, group, rows, n])
+    p = Pair(gpu, 1, n // 64 + 2, 1, n // 64 + 2, 64, 1, hd)
+    assert p.extend([0], [n]) == 0
+    p.store(rng, 0, [0], [n])
+    k, v, _ = p.m.rows(0, 0, n)
+    # along a key the row sees (its score is the largest), or against one
+    along = rng.integers(0, n - rows + 1, (rows, group))
+    sign = np.where(rng.random((rows, group)) < 0.5, 1, -1)
+    sign[0] = -1
+    q = (k[along, 0] * (sign * scale)[..., None]).astype(np.float32)
+    print("huge", hd, group, rows, n, scale, gpu.kv4_attention_plan(p.c, 1, rows, rows, n, group), flush=True)
+    out = gpu.kv4_attention_dev(p.c, 0, _dev(q), _i32([0, rows]), n_head=group, max_rows=rows, max_len=n)
+    out = out.cpu().numpy().reshape(q.shape).astype(np.float64)
+    checked = 0
+    for t in range(rows):
+        x = q[t].astype(np.float64) @ k[:n - rows + t + 1, 0].T / np.sqrt(hd)
+        size = (np.abs(q[t].astype(np.float64)) @ np.abs(k[:n - rows + t + 1, 0].T)).max() / np.sqrt(hd)
+        for h in range(group):
+            best, *rest = np.argsort(-x[h])[:2]
+            # (scores are off by 2^-17 of their terms at most; closer ones may share the weight)
+            if rest and x[h, best] - x[h, rest[0]] < max(200.0, 2.0 ** -15 * size):
+                continue
+            want = v[best, 0]
+            assert (np.abs(out[t, h] - want) <= np.abs(want) * (2.0 ** -20 + 3 * 2.0 ** -24)).all(), (t, h)
+            checked += 1
+    assert checked >= rows * group // 2
