@@ -4,8 +4,9 @@
 // Attention of query row t of head h, over the keys k_j and values v_j the row sees:
 //   s_j = (q . k_j) / sqrt(HD),  y = sum_j exp(s_j) v_j / sum_j exp(s_j),
 // in one pass over the cache with the running maximum and sum of each (row, head). The keys and
-// values are exact fp16 numbers; the queries and the weights are fp32 and enter the fp16 MFMAs as
-// hi + lo pairs (22 significant bits), accumulated in fp32.
+// values are exact fp16 numbers (an MFMA keeps fewer bits of products with subnormal ones: kv4.h); the
+// queries and the weights are fp32 and enter the fp16 MFMAs as hi + lo pairs (22 significant bits),
+// accumulated in fp32.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
