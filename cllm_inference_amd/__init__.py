@@ -937,8 +937,8 @@ class LogProbs:
 
 
 def logprobs_dev(logits, tokens=None, top_k: int = 0) -> LogProbs:
-    """Log probabilities of the rows of logits (float32 (n_rows, vocab), any row stride, unit stride
-    along a row): of the given tokens (int32 (n_rows,)) with their ranks, the entropy and
+    """Log probabilities of the rows of logits (float32 (n_rows, vocab), unit stride along a row, a
+    row stride of vocab or more): of the given tokens (int32 (n_rows,)) with their ranks, the entropy and
     log-sum-exp, and the top_k (at most 64) largest with their ids, equal logits by ids."""
     who, dev = "logprobs", logits.get_device()
     torch, stream = _current(who, dev)

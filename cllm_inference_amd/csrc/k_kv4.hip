@@ -260,7 +260,8 @@ __device__ __forceinline__ float add_pair(float v) {
 // Direct up to kDirectUnits units or kDirectLen positions. One row, 8 KV heads of 128, us direct /
 // stream: 16 sequences of 1000-8000 31 / 34; 24 of 1000-8000 56 / 41, of 100-6000 37 / 49, of 6000
 // 46 / 40, of 4000 35 / 37; 64 of 1000-8000 90 / 77, of 4096-8192 102 / 95, of 6000 83 / 90, of 100-1000
-// 17 / 29, of 300 12 / 22; 256 of 100-2000 76 / 133.
+// 17 / 29, of 300 12 / 22; 256 of 100-2000 76 / 133. The host knows max_len only: 24 of 6000 get the slower
+// form, and short contexts under a max_len past kDirectLen (a captured call's bound) the stream's times.
 // Partial results lie in slots (direct: unit * splits + split; stream: unit + workgroup, which grows
 // along the staircase of pairs), and a second launch joins them.
 constexpr int kCus = 256;
@@ -389,9 +390,10 @@ struct Parts {
 //
 // What bounds it: the read of the cache, and beside it about 240 VALU operations per tile and wave for
 // dequantization (208 at HD 128) and the softmax of its 16 columns. 64 sequences of 4096-8192 positions,
-// 32 + 8 heads of 128 (485 MB): 95 us with the join, 5.1 TB/s (its loads alone 83, a one-launch read 69);
-// one sequence of 129: 7.2; 16 of up to 2047, 14 + 2 heads of 64: 10; 5 rows of 8 sequences of 700-5000,
-// 16 + 4 heads of 256: 29.
+// 32 + 8 heads of 128 (485 MB): 93 to 103 us with the join over several cards, 4.7 to 5.2 TB/s (its loads
+// alone 83, a one-launch read 69); one sequence of 129: 7.2; 16 of up to 2047, 14 + 2 heads of 64: 10 to 11;
+// 3 to 5 rows of 8 sequences of 800-4600, 16 + 4 heads of 256: 29, as its 20 columns are two units, each of which
+// dequantizes every tile.
 template <int HD>
 struct AttnLds {
     // waves on a SIMD, which is workgroups on a CU, and slots a wave: within 512 registers and 160 KB
@@ -652,11 +654,14 @@ __global__ __launch_bounds__(256, AttnLds<HD>::WAVES) void k_kv4_attention(Kv4Vi
 // turn after the next are loaded while the next one's fragments are written and the present ones are
 // multiplied, with one barrier a turn.
 //
-// What bounds it: VALU beside MFMA work. 32 positions x 32 columns of HD 128 take 64 MFMAs of 16 cycles
-// (two parts of the queries, two of the weights) and about 190 VALU operations, 75 of them the wave's
-// share of the dequantization. One prompt of 2048, 32 + 8 heads of 128: 91 us (34.4 GFLOP; 760 TFLOP/s of
-// both parts' products); 254-509 rows of 4 sequences of 2345-4744: 218 us (730 TFLOP/s). Heads of 64 and 256, four
-// sequences of 1500-6000: 135 and 416.
+// What bounds it: VALU and MFMA work that overlap little, and waiting. 32 positions x 32 columns of HD 128
+// take 64 MFMAs of 16 cycles (two parts of the queries, two of the weights) and about 190 VALU operations, 75
+// of them the wave's share of the dequantization. Counters, prompt / second turns below: a CU has work in 86 /
+// 72% of the time; of a SIMD's cycles then MFMA takes 33 / 39% and VALU 38 / 40%, LDS is busy 13 / 15% without
+// conflicts, and a wave waits for 36 / 33% (for the barrier of a turn and the loads). One prompt of 2048, 32 + 8
+// heads of 128: 91 us (34.4 GFLOP; 760 TFLOP/s of both parts' products); 288-499 rows of 4 sequences of
+// 2345-4744: 217 to 224 us (720). (At the clock of a long run; the first launches of a short one take 103 and
+// 246.) Heads of 64 and 256, four sequences of 1500-6000: 135 and 416.
 template <int HD>
 struct ManyRows {
     static constexpr int NC = HD == 64 ? 4 : HD == 128 ? 2 : 1, COLS = 4 * NC * 16;
@@ -1157,9 +1162,11 @@ __device__ __forceinline__ uint32_t code_of(float x, float d, float inv, float h
     return (uint32_t)((int)__builtin_amdgcn_fmed3f(t, -8.0f, 7.0f) + 8);
 }
 
-// What bounds it: the quantization's VALU work beside the rows' read; 12297 rows of 8 heads of 128
-// 21.8 us (100 MB of rows, 5.2 TB/s with the pages); 64 tokens 7.0: two dependent loads (length, page) before the
-// first store.
+// What bounds it: the quantization's VALU work beside the rows' read; 9534 rows of 8 heads of 128 21.5 us
+// (78 MB of rows, 4.1 TB/s with the pages); 64 tokens 7.0: two dependent loads (length, page) before the
+// first store. With the rotation its sines bind it, which every head's workgroup forms again: 12297 rows 25.6 us
+// without, 50 with rotated keys, 154 with 32 query heads too (whose read and write alone are 57 at the one-launch
+// read's rate); 64 tokens 7.1, 8.1, 8.3.
 // grid (segments at most, KV heads [+ query head groups when q is rotated]). A workgroup reads the
 // segment's rows of its head once and quantizes them, eight threads to a position; a dword of keys is
 // eight elements of one position, a dword of values one element of eight positions, which meet in LDS.
@@ -1321,7 +1328,7 @@ __global__ __launch_bounds__(256) void k_kv4_store(Kv4View c, int layer, const f
 }
 
 // The rows of the batch read back as fp32, d * (c - 8); rows without a place are 0. Bound by the writes:
-// 12297 rows of 8 heads of 128 21.1 us (5.4 TB/s), 64 tokens 5.1.
+// 9534 rows of 8 heads of 128 20.7 us (4.3 TB/s), 64 tokens 5.1.
 // grid (segments at most + sequences, KV heads): the workgroups past the segments write the rows of
 // sequences with more rows than positions that stand before the first position (0).
 template <int HD>
@@ -1419,6 +1426,8 @@ hipError_t launch_kv4_load(const Kv4View& c, int layer, const int32_t* slots, co
 //   8 of 2000-4000, 24 rows: 35 / 49, 47 / 48, 75 / 91; 8 of 2000-4000, 64 rows: 58 / 57, 88 / 78, 155 / 156
 //   16 of 8000, 17 rows: 68 / 153, 103 / 137, 198 / 363; 16 of 8000, 32 rows: 111 / 155, 169 / 142, 343 / 378
 //   4 of 12000, 32 rows: 64 / 78, 93 / 71, 165 / 137
+// (Between 97 and 128 columns of long contexts one rule serves 4 and 16 sequences: the latter, with heads of
+// 256, get the slower form, 378 instead of 343.)
 constexpr int kFewCols = 96, kFewColsShort = 128;
 
 Kv4AttnPlan kv4_attention_plan(const Kv4View& c, int n_seqs, int max_rows, int max_len, int n_head) {

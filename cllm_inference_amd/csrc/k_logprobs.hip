@@ -7,10 +7,12 @@
 // entropy keep their relative precision where one token has nearly all of the probability; every
 // term of the entropy is positive.
 //
-// What bounds it: the read of the logits, and about 14 VALU operations beside each: 1021 rows of 32003 with
-// the top 20 29.4 us (4.5 TB/s) and 4 for the join; one row of 128256 6.9 and 4. A workgroup takes 8192 logits of one row (grid rows x
-// parts) and holds them in registers, 32 a thread, all loads in flight at once: its maximum first,
-// then its sums, the tokens ahead of the given one and its largest logits, without reading twice.
+// What bounds it: VALU work, 22 operations a logit (79% of the cycles in which a CU has work), and the starts
+// and ends of two rounds of workgroups, each of which loads all that it reads before it works on it (a CU has
+// work in 70% of the launch): 1021 rows of 32003 29 us with the top 20 (4.5 TB/s), 23.6 without a list, 36 with the
+// top 64, and 4 to 6 for the join; one row of 128256 6.8 and 4. A workgroup takes 8192 logits of one row (grid
+// rows x parts) and holds them in registers, 32 a thread, all loads in flight at once: its maximum
+// first, then its sums, the tokens ahead of the given one and its largest logits, without reading twice.
 // A second launch joins a row's parts.
 #include <hip/hip_runtime.h>
 

@@ -58,8 +58,11 @@ __device__ __forceinline__ bool hash_insert(int* table, int key) {
 }
 
 // Extends entry i (thread i) by counts[i] tokens. One workgroup, as the entries depend on one another (who
-// shares a page, who takes which free one): bound by its chain of loads, 5.3 us with the copies' launch for 1
-// to 1024 entries. work: [0] copies, then (source, destination) pairs, then the list of taken pages at 1 + 2 * kMaxEntries.
+// shares a page, who takes which free one): bound by its chain of loads, 5.4 us for one entry and a new page
+// each, 6.7 for 1024; the copies' launch takes 1 to 2 us more without copies, 4.1 for the 7 of a beam step of 32
+// layers. Where entries share a last page the comparisons add to it: 16 that share one 6.2 us, 64 7.6, 256 13,
+// 1024 36. (Many pages at once are taken one after the other: 64 entries of 128 new pages 40 us, 1024 330.)
+// work: [0] copies, then (source, destination) pairs, then the list of taken pages at 1 + 2 * kMaxEntries.
 __global__ __launch_bounds__(kThreads) void k_kv4_extend(Kv4View c, const int32_t* __restrict__ slots,
                                                          const int32_t* __restrict__ counts, int n,
                                                          int32_t* __restrict__ status) {
@@ -107,8 +110,8 @@ __global__ __launch_bounds__(kThreads) void k_kv4_extend(Kv4View c, const int32_
         }
         return;
     }
-    // entries before this one that hold the same page, which have left it by this one's turn (counted only
-    // if a page is named twice: a comparison with every entry before takes 45 us for 1024 entries)
+    // entries before this one that hold the same page, which have left it by this one's turn (counted only if a
+    // page is named twice: a comparison with every entry before, 29 us for 1024 entries)
     bool copy = false;
     if (tid < n) {
         int same = 0;
@@ -187,7 +190,7 @@ __global__ __launch_bounds__(kThreads) void k_kv4_extend(Kv4View c, const int32_
 // Copies pages of every layer: pairs src[i * step] -> dst[i * step], i < n (or *n_dev). 16 KB a
 // step of a workgroup; a grid that fills the chip walks them, so a call without copies ends at once.
 // What bounds it: the HBM copy rate (151 MB out of a pool of 256 pages of 32 layers 47 us, 6.4 TB/s read
-// and written).
+// and written; 64 pages of 32 layers by copy_pages, the same bytes, 43 to 45).
 constexpr int kCopyChunk = 16384;
 __device__ __forceinline__ void copy_pages(const Kv4View& c, const int32_t* src, const int32_t* dst, int step,
                                            int n, int64_t first, int64_t stride) {
@@ -290,6 +293,7 @@ __global__ __launch_bounds__(kThreads) void k_kv4_fork_one(Kv4View c, const int3
         if (s_src[i] >= 0) fork_write(c, i, s_dst[i], lane, 64);
 }
 
+// One launch, a workgroup an entry: 64 entries of 128 pages freed 3.0 us, 1024 3.9.
 __global__ __launch_bounds__(256) void k_kv4_truncate(Kv4View c, const int32_t* __restrict__ slots,
                                                       const int32_t* __restrict__ new_lens) {
     const int i = blockIdx.x, slot = slots[i];

@@ -20,10 +20,11 @@
 // An element is d * (c - 8). The scale d has 8 significant bits, so the product (8 bits by a 3-bit
 // magnitude, or 8) is exact in fp16: dequantization adds no error to the quantization's. d is at
 // most 8160, so no element passes 65280. (Elements below 2^-14 are fp16 subnormals, exact too, but an
-// MFMA does not normalise them and keeps fewer bits of their products: outputs from values of 1e-5 are off by
-// 5e-7 in the root mean square, like any, from 1e-6 by 3e-6, from 3e-7 by 1e-5; keys of 1e-6 add 3e-7.) A position whose key or value row held an infinity or a
-// NaN has NaN as its key scales and 0 as its value scales: whatever sees it becomes NaN through its
-// score, and rows that do not see it stay clean (a NaN among the values would not: 0 * NaN is NaN).
+// MFMA does not normalise them and keeps fewer bits of their products: outputs from values of 1e-5 are
+// off by 5e-7 in the root mean square, like any, from 1e-6 by 3e-6, from 3e-7 by 1e-5; keys of 1e-6 add
+// 3e-7.) A position whose key or value row held an infinity or a NaN has NaN as its key scales and 0 as
+// its value scales: whatever sees it becomes NaN through its score, and rows that do not see it stay
+// clean (a NaN among the values would not: 0 * NaN is NaN).
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -363,8 +363,9 @@ size_t cllm_hip_kv4_work_ints(int n_pages, int max_seqs, int max_pages);
  * free ones, lowest id first, in the order of the entries. A partly filled last page that other
  * slots hold too is replaced by a copy (all layers; copy on write): of the entries that share one,
  * in order, each takes a copy (before its other pages) as long as another holder is left.
- * *status (device): 0; the number of pages missing; or -1 for a slot out of range or named twice,
- * a negative count, or more than max_pages pages. Unless it is 0, nothing has changed. */
+ * *status (device): 0; the number of pages missing; or -1 for a slot out of range or named twice, a
+ * negative count, more than max_pages pages, or a slot whose length is past its table or whose partly
+ * filled last page is no page. Unless it is 0, nothing has changed. */
 int cllm_hip_kv4_extend_dev(const cllm_hip_kv4_cache* cache, const int32_t* slots,
                             const int32_t* counts, int n, int32_t* status, void* stream);
 
@@ -412,8 +413,9 @@ int cllm_hip_kv4_load_dev(const cllm_hip_kv4_cache* cache, int layer, const int3
 /* Grouped-query attention (attention, src/core/engine.cpp:114-146) of the rows q (n_rows x n_head
  * x head_dim) over the cache: row t of a sequence with r rows sees positions [0, lens - r + t];
  * a row that sees none gives 0. n_head is any multiple of n_head_kv. max_rows and max_len bound the
- * rows and the tokens of a sequence: rows past max_rows are not computed; a max_len that is too
- * small costs time only, and one near the longest sequence is fastest. ws: 16-byte aligned device
+ * rows and the tokens of a sequence: rows past max_rows are not computed; max_len chooses how the work
+ * is split (and so the order of the sums): one that is too small or too large costs time only, and one near
+ * the longest sequence is fastest. ws: 16-byte aligned device
  * scratch of cllm_hip_kv4_attention_ws_bytes bytes for the same arguments (0: may be null), free
  * again when the call has run. */
 size_t cllm_hip_kv4_attention_ws_bytes(const cllm_hip_kv4_cache* cache, int n_seqs, int n_rows,
@@ -429,8 +431,8 @@ const char* cllm_hip_kv4_attention_plan(const cllm_hip_kv4_cache* cache, int n_s
                                         int max_rows, int max_len, int n_head);
 
 /* ---- log probabilities (stream-ordered) -------------------------------------------------
- * Of n_rows rows of fp32 logits (row i at logits + i * row_stride, vocab of them), in natural
- * logarithms, each output null if not wanted:
+ * Of n_rows rows of fp32 logits (row i at logits + i * row_stride, vocab of them; row_stride is vocab or
+ * more), in natural logarithms, each output null if not wanted:
  *   lse[i]       log sum_j exp(x_j)
  *   logprobs[i]  x_t - lse of the given token t = tokens[i]; -inf for a t outside the vocabulary
  *   ranks[i]     how many tokens stand ahead of t: larger logits, and equal ones with lower ids;
