@@ -267,7 +267,9 @@ __global__ __launch_bounds__(kThreads) void k_logprobs_part(const float* __restr
     int count = s_count;
     const int want = min(top_k, n);
     // What follows up to the ranking is rare; it reads the logits again, one at a time, so that the
-    // kernel's registers are those of the work above (64 a thread instead of 109).
+    // kernel's registers are those of the work above (64 a thread instead of 109). It is met by masks that leave one
+    // stretch of the ids: of 128256 logits -inf but for the first 600, top 20 121 us a call instead of 12, top
+    // 64 369 instead of 17; with the type's lowest value for -inf, 97 and 100.
     const auto each = [&](auto f) {
 #pragma unroll 1
         for (int at = tid; at < n; at += kThreads) f(at, x0[base + at]);
