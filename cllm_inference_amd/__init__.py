@@ -87,6 +87,17 @@ SIGNATURES = {
                                              _P]),
     "cllm_hip_rmsnorm_gemv_swiglu_dev": (_I, [_U, _I, _I, _P, _P, _P, _P, _P, _P, ctypes.c_float,
                                               _P, _P]),
+    "cllm_hip_group_rows_dev": (_I, [_P, _I, _I, _P, _P, _P]),
+    "cllm_hip_moe_route_dev": (_I, [_P, _I64, _P, _I, _I, _I, _I, _I,
+                                    ctypes.c_float, _I, _I, _P, _P, _P, _P, _P]),
+    "cllm_hip_moe_matmul_ws_bytes": (_SZ, [_U, _I, _I]),
+    "cllm_hip_moe_matmul_dev": (_I, [_U, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _P, _SZ, _P]),
+    "cllm_hip_moe_swiglu_dev": (_I, [_U, _I, _I, _I, _P, _P, _P, _P, _P, _I, _I, _P, _P, _P, _P, _SZ, _P]),
+    "cllm_hip_moe_down_ws_bytes": (_SZ, [_U, _I, _I, _I, _I]),
+    "cllm_hip_moe_down_dev": (_I, [_U, _I, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "cllm_hip_moe_plan": (ctypes.c_char_p, [_U, _I, _I, _I, _I, _I]),
+    "cllm_hip_lora_ws_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "cllm_hip_lora_dev": (_I, [_U, _I, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _P, _SZ, _P]),
     "cllm_hip_gguf_open": (_I, [ctypes.c_char_p, _I, ctypes.POINTER(_P)]),
     "cllm_hip_gguf_close": (_I, [_P]),
     "cllm_hip_gguf_tensor_count": (_I, [_P]),
@@ -971,3 +982,212 @@ def logprobs_dev(logits, tokens=None, top_k: int = 0) -> LogProbs:
                                      per[1].data_ptr(), tid, ttop, None if ws is None else ws.data_ptr(), nbytes,
                                      stream))
     return r
+
+
+@dataclass
+class RowGroups:
+    """Entries grouped by index: order (int32, n) lists them sorted by group, those of group g at
+    order[offsets[g]:offsets[g + 1]], those of no group from offsets[-1] on (offsets: int32, groups + 1)."""
+    offsets: object
+    order: object
+
+
+@dataclass
+class MoeRoute:
+    """A router's choice (cllm_hip_moe_route_dev): ids (int32) and weights (float32), n_rows x top_k, -1 and
+    0 for no expert, and the entries row * top_k + j grouped by expert as RowGroups has them."""
+    ids: object
+    weights: object
+    offsets: object
+    order: object
+
+
+def group_rows_dev(ids, n_groups: int) -> RowGroups:
+    """The entries of ids (int32 (n,)) grouped by id; ids outside [0, n_groups) are of no group."""
+    who, dev = "group_rows", ids.get_device()
+    torch, stream = _current(who, dev)
+    p = _addr(who, "ids", ids, torch.int32, dev)
+    if n_groups < 1:
+        raise RuntimeError(f"{who}: n_groups must be positive")
+    n = ids.numel()
+    g = RowGroups(torch.empty(n_groups + 1, dtype=torch.int32, device=ids.device),
+                  torch.empty(n, dtype=torch.int32, device=ids.device))
+    _check(load_library().cllm_hip_group_rows_dev(p, n, n_groups, g.offsets.data_ptr(), g.order.data_ptr(), stream))
+    return g
+
+
+def moe_route_dev(logits, top_k: int, bias=None, sigmoid: bool = False, normalise: bool = True,
+                  scale: float = 1.0, n_groups: int = 1, top_groups: int = 1) -> MoeRoute:
+    """A router's choice of top_k experts for the rows of logits (float32 (n_rows, n_experts), unit stride
+    along a row): softmax or sigmoid scores, chosen by logit or, with bias (float32 (n_experts,)), by
+    score + bias, from the top_groups best of n_groups groups of experts; weights are the chosen scores,
+    normalised to sum 1 or not, times scale."""
+    who, dev = "moe_route", logits.get_device()
+    torch, stream = _current(who, dev)
+    if logits.dim() != 2 or logits.dtype is not torch.float32:
+        raise RuntimeError(f"{who}: logits must be float32 n_rows x n_experts")
+    m, experts = logits.shape
+    stride, along = logits.stride()
+    if experts > 1 and along != 1:
+        raise RuntimeError(f"{who}: the logits of a row must lie side by side")
+    if m <= 1:
+        stride = experts
+    bp = None if bias is None else _addr(who, "bias", bias, torch.float32, dev, experts)
+    # one allocation: ids, order, offsets
+    k = max(top_k, 0)
+    ints = torch.empty(2 * m * k + experts + 1, dtype=torch.int32, device=logits.device)
+    weights = torch.empty((m, k), dtype=torch.float32, device=logits.device)
+    r = MoeRoute(ints[:m * k].view(m, k), weights, ints[2 * m * k:], ints[m * k:2 * m * k])
+    at = ints.data_ptr()
+    _check(load_library().cllm_hip_moe_route_dev(
+        logits.data_ptr(), stride, bp, m, experts, top_k, int(sigmoid), int(normalise), scale, n_groups,
+        top_groups, at, weights.data_ptr(), at + 8 * m * k, at + 4 * m * k, stream))
+    return r
+
+
+def _moe_args(who, x, w, t, out_dim, groups):
+    """(in_dim, rows of x, experts) of an expert product, after the checks of its tensors' sizes."""
+    if x.dim() < 2:
+        raise RuntimeError(f"{who}: activations must have two dimensions")
+    in_dim = x.shape[-1]
+    rows = x.numel() // in_dim if in_dim else 0
+    experts = groups.offsets.numel() - 1
+    if experts < 1:
+        raise RuntimeError(f"{who}: offsets must have n_experts + 1 elements")
+    per = block_size(t) if has_vec_dot(t) else 0
+    if per and in_dim % per == 0:
+        need = experts * out_dim * (in_dim // per) * type_size(t)
+        for name, m in w:
+            if m.numel() * m.element_size() != need:
+                raise RuntimeError(f"{who}: {name} has {m.numel() * m.element_size()} bytes, not {need}")
+    return in_dim, rows, experts
+
+
+def moe_matmul_dev(x, w, t: int, out_dim: int, groups: RowGroups, bias=None, per_row: int = 1, y=None):
+    """The products of entries with the matrices of their groups: entry e has row e // per_row of x
+    (float32 (n_rows, in_dim)) and w (uint8, the GGUF blocks of [n_experts][out_dim] rows of type t). Returns
+    y (n_rows * per_row, out_dim); entries of no group leave their row as it is."""
+    who, dev = "moe_matmul", x.get_device()
+    torch, stream = _current(who, dev)
+    f32, i32 = torch.float32, torch.int32
+    in_dim, rows, experts = _moe_args(who, x, (("w", w),), t, out_dim, groups)
+    n = rows * per_row
+    if y is None:
+        y = torch.empty((n, out_dim), dtype=f32, device=x.device)
+    lib = load_library()
+    nbytes = int(lib.cllm_hip_moe_matmul_ws_bytes(t, in_dim, rows))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _check(lib.cllm_hip_moe_matmul_dev(
+        t, in_dim, out_dim, experts, _addr(who, "w", w, torch.uint8, dev),
+        None if bias is None else _addr(who, "bias", bias, f32, dev, experts * out_dim),
+        _addr(who, "x", x, f32, dev), rows, per_row, _addr(who, "offsets", groups.offsets, i32, dev),
+        _addr(who, "order", groups.order, i32, dev, n), _addr(who, "y", y, f32, dev, n * out_dim), ws.data_ptr(),
+        nbytes, stream))
+    return y
+
+
+def moe_swiglu_dev(x, w_gate, w_up, t: int, n_ff: int, route: MoeRoute, bias_gate=None, bias_up=None, h=None):
+    """silu(gate) * up of every row of x (float32 (n_rows, in_dim)) and each of its chosen experts: w_gate and
+    w_up are the GGUF blocks (uint8) of [n_experts][n_ff] rows of type t. Returns h (n_rows, top_k, n_ff); what
+    has no expert is left as it is."""
+    who, dev = "moe_swiglu", x.get_device()
+    torch, stream = _current(who, dev)
+    f32, i32 = torch.float32, torch.int32
+    in_dim, rows, experts = _moe_args(who, x, (("w_gate", w_gate), ("w_up", w_up)), t, n_ff, route)
+    if route.ids.dim() != 2 or route.ids.shape[0] != rows:
+        raise RuntimeError(f"{who}: x has {rows} rows, the route {tuple(route.ids.shape)}")
+    top_k = route.ids.shape[1]
+    n = rows * top_k
+    if h is None:
+        h = torch.empty((rows, top_k, n_ff), dtype=f32, device=x.device)
+    lib = load_library()
+    nbytes = int(lib.cllm_hip_moe_matmul_ws_bytes(t, in_dim, rows))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _check(lib.cllm_hip_moe_swiglu_dev(
+        t, in_dim, n_ff, experts, _addr(who, "w_gate", w_gate, torch.uint8, dev),
+        _addr(who, "w_up", w_up, torch.uint8, dev),
+        None if bias_gate is None else _addr(who, "bias_gate", bias_gate, f32, dev, experts * n_ff),
+        None if bias_up is None else _addr(who, "bias_up", bias_up, f32, dev, experts * n_ff),
+        _addr(who, "x", x, f32, dev), rows, top_k, _addr(who, "offsets", route.offsets, i32, dev),
+        _addr(who, "order", route.order, i32, dev, n), _addr(who, "h", h, f32, dev, n * n_ff), ws.data_ptr(),
+        nbytes, stream))
+    return h
+
+
+def moe_down_dev(h, w, t: int, out_dim: int, route: MoeRoute, bias=None, base=None, y=None):
+    """The down projections of h (float32, n_rows x top_k x n_ff) with the chosen experts' matrices (GGUF blocks
+    of [n_experts][out_dim] rows of type t), summed over a row's experts with the route's weights, plus base
+    (float32 (n_rows, out_dim), the residual; may be y). Returns y (n_rows, out_dim)."""
+    who, dev = "moe_down", h.get_device()
+    torch, stream = _current(who, dev)
+    f32, i32 = torch.float32, torch.int32
+    n_ff, n, experts = _moe_args(who, h, (("w", w),), t, out_dim, route)
+    if route.ids.dim() != 2 or route.ids.numel() != n:
+        raise RuntimeError(f"{who}: h has {n} rows, the route {tuple(route.ids.shape)}")
+    rows, top_k = route.ids.shape
+    if y is None:
+        y = torch.empty((rows, out_dim), dtype=f32, device=h.device)
+    lib = load_library()
+    nbytes = int(lib.cllm_hip_moe_down_ws_bytes(t, n_ff, out_dim, rows, top_k))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
+    _check(lib.cllm_hip_moe_down_dev(
+        t, n_ff, out_dim, experts, _addr(who, "w", w, torch.uint8, dev),
+        None if bias is None else _addr(who, "bias", bias, f32, dev, experts * out_dim),
+        _addr(who, "h", h, f32, dev), rows, top_k, _addr(who, "ids", route.ids, i32, dev, n),
+        _addr(who, "weights", route.weights, f32, dev, n), _addr(who, "offsets", route.offsets, i32, dev),
+        _addr(who, "order", route.order, i32, dev, n),
+        None if base is None else _addr(who, "base", base, f32, dev, rows * out_dim),
+        _addr(who, "y", y, f32, dev, rows * out_dim), ws.data_ptr(), nbytes, stream))
+    return y
+
+
+def moe_plan(t: int, n_mats: int, in_dim: int, out_dim: int, n_experts: int, n_entries: int) -> str:
+    """The kernel and launch plan of the experts' products of n_entries entries."""
+    return load_library().cllm_hip_moe_plan(t, n_mats, in_dim, out_dim, n_experts, n_entries).decode()
+
+
+def lora_dev(x, a, b, groups: RowGroups, ranks=None, scales=None, base=None, ys=None):
+    """Low-rank adapters on the projections of x (float32 (n_rows, in_dim)), rows grouped by adapter: a[i]
+    (n_adapters, max_rank, in_dim) and b[i] (n_adapters, out_dims[i], max_rank), float16 or float32, of 1 to 4
+    projections; ranks (int32) and scales (float32) (n_adapters,). Returns the list of base[i] + scale * b[i]
+    (a[i] x) (base None: zeros), base[i] for rows of no adapter."""
+    who, dev = "lora", x.get_device()
+    torch, stream = _current(who, dev)
+    f32, i32 = torch.float32, torch.int32
+    n = len(a)
+    if n == 0 or len(b) != n or (base is not None and len(base) != n) or (ys is not None and len(ys) != n):
+        raise RuntimeError(f"{who}: a, b, base and ys must have an entry for each projection")
+    if x.dim() != 2 or a[0].dim() != 3:
+        raise RuntimeError(f"{who}: x must be n_rows x in_dim, a[i] n_adapters x max_rank x in_dim")
+    rows, in_dim = x.shape
+    adapters, max_rank = a[0].shape[:2]
+    dt = a[0].dtype
+    if dt not in (torch.float16, f32):
+        raise RuntimeError(f"{who}: adapters must be float16 or float32")
+    if groups.offsets.numel() != adapters + 1:
+        raise RuntimeError(f"{who}: offsets has {groups.offsets.numel()} elements, not {adapters + 1}")
+    outs = []
+    for i in range(n):
+        if tuple(a[i].shape) != (adapters, max_rank, in_dim) or b[i].dim() != 3 or \
+                (b[i].shape[0], b[i].shape[2]) != (adapters, max_rank):
+            raise RuntimeError(f"{who}: shapes of adapter {i} do not match: {tuple(a[i].shape)}, {tuple(b[i].shape)}")
+        outs.append(b[i].shape[1])
+    if ys is None:
+        ys = [torch.empty((rows, o), dtype=f32, device=x.device) for o in outs]
+    ptrs = ctypes.c_void_p * n
+    ap = ptrs(*[_addr(who, "a", m, dt, dev) for m in a])
+    bp = ptrs(*[_addr(who, "b", m, dt, dev) for m in b])
+    yp = ptrs(*[_addr(who, "y", y, f32, dev, rows * o) for y, o in zip(ys, outs)])
+    basep = None
+    if base is not None:
+        basep = ptrs(*[None if m is None else _addr(who, "base", m, f32, dev, rows * o) for m, o in zip(base, outs)])
+    lib = load_library()
+    nbytes = int(lib.cllm_hip_lora_ws_bytes(in_dim, n, adapters, max_rank, rows))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _check(lib.cllm_hip_lora_dev(
+        1 if dt is torch.float16 else 0, in_dim, n, ap, bp, (ctypes.c_int * n)(*outs), adapters, max_rank,
+        None if ranks is None else _addr(who, "ranks", ranks, i32, dev, adapters),
+        None if scales is None else _addr(who, "scales", scales, f32, dev, adapters),
+        _addr(who, "x", x, f32, dev), rows, _addr(who, "offsets", groups.offsets, i32, dev),
+        _addr(who, "order", groups.order, i32, dev, rows), basep, yp, ws.data_ptr(), nbytes, stream))
+    return ys

@@ -31,6 +31,7 @@
 #include "../../include/cllm_hip.h"
 #include "ggml_blocks.h"
 #include "gguf_file.h"
+#include "experts.h"
 #include "kv4.h"
 #include "launch.h"
 
@@ -1941,6 +1942,260 @@ int cllm_hip_logprobs_dev(const float* logits, int64_t row_stride, int n_rows, i
     if (rc) return rc;
     HIP_TRY(launch_logprobs(logits, row_stride, n_rows, vocab, tokens, top_k, logprobs, ranks, entropy, lse, top_ids,
                             top_logprobs, ws, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+// ---- products whose weights a row's index chooses ---------------------------------------------
+
+namespace {
+
+int check_groups(const char* who, int n_entries, int n_groups, const int32_t* offsets, const int32_t* order) {
+    if (n_entries < 0 || n_groups < 1 || n_groups > kMaxGroups)
+        return set_err(CLLM_HIP_E_ARG, "%s: 1 to %d groups, no negative count of entries", who, kMaxGroups);
+    if (n_entries > (1 << 28)) return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
+    if (n_entries == 0) return CLLM_HIP_OK;
+    if (!offsets || !order) return set_err(CLLM_HIP_E_ARG, "%s: null pointer", who);
+    if (!aligned4(offsets) || !aligned4(order)) return set_err(CLLM_HIP_E_ARG, "%s: misaligned device pointer", who);
+    return CLLM_HIP_OK;
+}
+
+// The shapes of an expert product: rows of in_dim, n_entries = rows x per_row entries.
+int check_experts(const char* who, uint32_t type, int in_dim, int out_dim, int n_experts, int n_rows, int per_row) {
+    if (!has_kernel(type)) return set_err(CLLM_HIP_E_TYPE, "%s: no kernel for this type", who);
+    if (in_dim <= 0 || in_dim % block_elems(type) != 0)
+        return set_err(CLLM_HIP_E_SHAPE, "%s: in_dim not divisible by block size", who);
+    if (out_dim < 0 || n_rows < 0) return set_err(CLLM_HIP_E_ARG, "%s: negative size", who);
+    if (n_experts < 1 || n_experts > kMaxGroups)
+        return set_err(CLLM_HIP_E_ARG, "%s: 1 to %d experts", who, kMaxGroups);
+    if (per_row < 1 || per_row > kMaxRouteTopK)
+        return set_err(CLLM_HIP_E_ARG, "%s: 1 to %d experts of a row", who, kMaxRouteTopK);
+    const int64_t entries = (int64_t)n_rows * per_row;
+    // 32-bit offsets of the activation operand, and workgroups counted in 32 bits of threads
+    const int64_t act = (int64_t)std::max((int64_t)n_rows, entries) * ((in_dim + 255) / 256) * 1024;
+    const int64_t grid = (entries / 16 + n_experts + 1) * ((out_dim + 15) / 16 + 1);
+    if (act >= (1ll << 32) || grid > UINT32_MAX / 512 || entries > (1 << 28))
+        return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
+    return CLLM_HIP_OK;
+}
+
+size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+int run_experts(const char* who, uint32_t type, int mats, int in_dim, int out_dim, int n_experts,
+                const void* const* w, const float* const* bias, const float* x, int n_rows, int per_row,
+                int n_entries, const int32_t* offsets, const int32_t* order, float* y, void* ws, hipStream_t s) {
+    (void)who;
+    ExpertArgs a{};
+    a.type = type;
+    a.mats = mats;
+    for (int i = 0; i < mats; ++i) a.w[i] = (const uint8_t*)w[i], a.bias[i] = bias[i];
+    a.k = in_dim;
+    a.n = out_dim;
+    a.x = x;
+    a.rows = n_rows;
+    a.per_row = per_row;
+    a.g = Groups{offsets, order, n_experts, n_entries};
+    a.y = y;
+    a.ws = ws;
+    HIP_TRY(launch_experts(a, s));
+    return CLLM_HIP_OK;
+}
+
+}  // namespace
+
+int cllm_hip_group_rows_dev(const int32_t* ids, int n, int n_groups, int32_t* offsets, int32_t* order, void* stream) {
+    int rc = check_groups("group_rows", n, n_groups, offsets, order);
+    if (rc) return rc;
+    if (!offsets || (n > 0 && !ids)) return set_err(CLLM_HIP_E_ARG, "group_rows: null pointer");
+    if (!aligned4(ids) || !aligned4(offsets)) return set_err(CLLM_HIP_E_ARG, "group_rows: misaligned device pointer");
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    HIP_TRY(launch_group_rows(ids, n, n_groups, offsets, order, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+int cllm_hip_moe_route_dev(const float* logits, int64_t row_stride, const float* bias, int n_rows, int n_experts,
+                           int top_k, int sigmoid, int normalise, float scale, int n_groups, int top_groups,
+                           int32_t* ids, float* weights, int32_t* offsets, int32_t* order, void* stream) {
+    if (n_rows < 0 || n_experts < 1 || n_experts > kMaxGroups || row_stride < n_experts)
+        return set_err(CLLM_HIP_E_ARG, "moe_route: 1 to %d experts, rows no closer than that", kMaxGroups);
+    if (top_k < 1 || top_k > kMaxRouteTopK || top_k > n_experts)
+        return set_err(CLLM_HIP_E_ARG, "moe_route: top_k must be 1 to %d and at most n_experts", kMaxRouteTopK);
+    if (n_groups < 1 || n_groups > kMaxRouteParts || n_experts % n_groups != 0 || top_groups < 1 || top_groups > n_groups)
+        return set_err(CLLM_HIP_E_ARG, "moe_route: 1 to %d equal groups of experts, 1 to n_groups of them kept",
+                       kMaxRouteParts);
+    if (!(scale == scale) || scale - scale != 0.0f) return set_err(CLLM_HIP_E_ARG, "moe_route: scale must be finite");
+    if ((int64_t)n_rows * top_k > (1 << 28)) return set_err(CLLM_HIP_E_ARG, "moe_route: batch too large for one launch");
+    if (!offsets || (n_rows > 0 && (!logits || !ids || !weights || !order)))
+        return set_err(CLLM_HIP_E_ARG, "moe_route: null pointer");
+    if (!aligned4(logits) || !aligned4(bias) || !aligned4(ids) || !aligned4(weights) || !aligned4(offsets) ||
+        !aligned4(order))
+        return set_err(CLLM_HIP_E_ARG, "moe_route: misaligned device pointer");
+    DeviceState* st;
+    int rc = acquire(&st);
+    if (rc) return rc;
+    RouteArgs a{logits, row_stride, bias, n_rows, n_experts, top_k, n_groups, top_groups, sigmoid != 0, normalise != 0,
+                scale, ids, weights, offsets, order};
+    HIP_TRY(launch_route(a, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+size_t cllm_hip_moe_matmul_ws_bytes(uint32_t type, int in_dim, int n_rows) {
+    if (!has_kernel(type) || in_dim <= 0 || n_rows <= 0) return 0;
+    return expert_act_bytes(type, in_dim, n_rows);
+}
+
+size_t cllm_hip_moe_down_ws_bytes(uint32_t type, int in_dim, int out_dim, int n_rows, int top_k) {
+    if (!has_kernel(type) || in_dim <= 0 || out_dim <= 0 || n_rows <= 0 || top_k <= 0) return 0;
+    const size_t entries = (size_t)n_rows * top_k;
+    return align256(expert_act_bytes(type, in_dim, (int)std::min<size_t>(entries, 1 << 28))) +
+           align256(entries * out_dim * sizeof(float));
+}
+
+namespace {
+int check_ws(const char* who, const void* ws, size_t have, size_t need) {
+    if (!aligned16(ws)) return set_err(CLLM_HIP_E_ARG, "%s: misaligned device pointer", who);
+    if (need > 0 && (!ws || have < need))
+        return set_err(CLLM_HIP_E_ARG, "%s: workspace of %zu bytes, %zu needed", who, ws ? have : (size_t)0, need);
+    return CLLM_HIP_OK;
+}
+}  // namespace
+
+int cllm_hip_moe_matmul_dev(uint32_t type, int in_dim, int out_dim, int n_experts, const void* w, const float* bias,
+                            const float* x, int n_rows, int per_row, const int32_t* offsets, const int32_t* order,
+                            float* y, void* ws, size_t ws_bytes, void* stream) {
+    int rc = check_experts("moe_matmul", type, in_dim, out_dim, n_experts, n_rows, per_row);
+    if (rc) return rc;
+    if (n_rows == 0 || out_dim == 0) return CLLM_HIP_OK;
+    if ((rc = check_groups("moe_matmul", n_rows * per_row, n_experts, offsets, order))) return rc;
+    if (!w || !x || !y) return set_err(CLLM_HIP_E_ARG, "moe_matmul: null pointer");
+    if (!aligned16(w) || !aligned16(x) || !aligned4(y) || !aligned4(bias))
+        return set_err(CLLM_HIP_E_ARG, "moe_matmul: misaligned device pointer");
+    if ((rc = check_ws("moe_matmul", ws, ws_bytes, expert_act_bytes(type, in_dim, n_rows)))) return rc;
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    return run_experts("moe_matmul", type, 1, in_dim, out_dim, n_experts, &w, &bias, x, n_rows, per_row,
+                       n_rows * per_row, offsets, order, y, ws, (hipStream_t)stream);
+}
+
+int cllm_hip_moe_swiglu_dev(uint32_t type, int in_dim, int n_ff, int n_experts, const void* w_gate, const void* w_up,
+                            const float* bias_gate, const float* bias_up, const float* x, int n_rows, int top_k,
+                            const int32_t* offsets, const int32_t* order, float* h, void* ws, size_t ws_bytes,
+                            void* stream) {
+    int rc = check_experts("moe_swiglu", type, in_dim, n_ff, n_experts, n_rows, top_k);
+    if (rc) return rc;
+    if (n_rows == 0 || n_ff == 0) return CLLM_HIP_OK;
+    if ((rc = check_groups("moe_swiglu", n_rows * top_k, n_experts, offsets, order))) return rc;
+    if (!w_gate || !w_up || !x || !h) return set_err(CLLM_HIP_E_ARG, "moe_swiglu: null pointer");
+    if (!aligned16(w_gate) || !aligned16(w_up) || !aligned16(x) || !aligned4(h) || !aligned4(bias_gate) ||
+        !aligned4(bias_up))
+        return set_err(CLLM_HIP_E_ARG, "moe_swiglu: misaligned device pointer");
+    if ((rc = check_ws("moe_swiglu", ws, ws_bytes, expert_act_bytes(type, in_dim, n_rows)))) return rc;
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    const void* w[2] = {w_gate, w_up};
+    const float* b[2] = {bias_gate, bias_up};
+    return run_experts("moe_swiglu", type, 2, in_dim, n_ff, n_experts, w, b, x, n_rows, top_k, n_rows * top_k, offsets,
+                       order, h, ws, (hipStream_t)stream);
+}
+
+int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, const void* w, const float* bias,
+                          const float* h, int n_rows, int top_k, const int32_t* ids, const float* weights,
+                          const int32_t* offsets, const int32_t* order, const float* base, float* y, void* ws,
+                          size_t ws_bytes, void* stream) {
+    int rc = check_experts("moe_down", type, n_ff, out_dim, n_experts, n_rows, top_k);
+    if (rc) return rc;
+    if (n_rows == 0 || out_dim == 0) return CLLM_HIP_OK;
+    if ((rc = check_groups("moe_down", n_rows * top_k, n_experts, offsets, order))) return rc;
+    if (!w || !h || !ids || !weights || !y) return set_err(CLLM_HIP_E_ARG, "moe_down: null pointer");
+    if (!aligned16(w) || !aligned16(h) || !aligned4(bias) || !aligned4(ids) || !aligned4(weights) || !aligned16(base) ||
+        !aligned16(y))
+        return set_err(CLLM_HIP_E_ARG, "moe_down: misaligned device pointer");
+    if (n_rows > 65535) return set_err(CLLM_HIP_E_ARG, "moe_down: batch too large for one launch");
+    if ((rc = check_ws("moe_down", ws, ws_bytes, cllm_hip_moe_down_ws_bytes(type, n_ff, out_dim, n_rows, top_k))))
+        return rc;
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    float* parts = (float*)((uint8_t*)ws + align256(expert_act_bytes(type, n_ff, n_rows * top_k)));
+    // every entry is a row of h
+    if ((rc = run_experts("moe_down", type, 1, n_ff, out_dim, n_experts, &w, &bias, h, n_rows * top_k, 1,
+                          n_rows * top_k, offsets, order, parts, ws, (hipStream_t)stream)))
+        return rc;
+    HIP_TRY(launch_expert_sum(parts, ids, weights, n_rows, top_k, n_experts, out_dim, base, y, (hipStream_t)stream));
+    return CLLM_HIP_OK;
+}
+
+const char* cllm_hip_moe_plan(uint32_t type, int n_mats, int in_dim, int out_dim, int n_experts, int n_entries) {
+    static thread_local char buf[96];
+    if (check_experts("moe_plan", type, in_dim, out_dim, n_experts, n_entries, 1) || n_mats < 1 || n_mats > 2)
+        snprintf(buf, sizeof buf, "none");
+    else
+        expert_plan_name(type, n_mats, in_dim, out_dim, n_experts, n_entries, buf, sizeof buf);
+    return buf;
+}
+
+namespace {
+int check_lora(int in_dim, int n_mats, const int* out_dims, int n_adapters, int max_rank, int n_rows) {
+    if (n_mats < 1 || n_mats > kMaxLoraMats || !out_dims)
+        return set_err(CLLM_HIP_E_ARG, "lora: 1 to %d projections", kMaxLoraMats);
+    if (in_dim <= 0 || in_dim % 4 != 0) return set_err(CLLM_HIP_E_SHAPE, "lora: in_dim must be a multiple of 4");
+    if (max_rank < 4 || max_rank > kMaxLoraRank || max_rank % 4 != 0)
+        return set_err(CLLM_HIP_E_SHAPE, "lora: max_rank must be a multiple of 4 up to %d", kMaxLoraRank);
+    if (n_adapters < 1 || n_adapters >= kMaxGroups)
+        return set_err(CLLM_HIP_E_ARG, "lora: 1 to %d adapters", kMaxGroups - 1);
+    if (n_rows < 0 || n_rows > (1 << 24)) return set_err(CLLM_HIP_E_ARG, "lora: batch too large for one launch");
+    int64_t total = 0;
+    for (int i = 0; i < n_mats; ++i) {
+        if (out_dims[i] < 0) return set_err(CLLM_HIP_E_ARG, "lora: negative out_dim");
+        total += out_dims[i];
+    }
+    if (total > (1 << 21)) return set_err(CLLM_HIP_E_ARG, "lora: outputs too wide for one launch");
+    const int64_t tiles = std::min<int64_t>(n_rows, n_rows / 16 + n_adapters + 1);
+    if (tiles * (total / 64 + n_mats) > UINT32_MAX / 256)
+        return set_err(CLLM_HIP_E_ARG, "lora: batch too large for one launch");
+    return CLLM_HIP_OK;
+}
+}  // namespace
+
+size_t cllm_hip_lora_ws_bytes(int in_dim, int n_mats, int n_adapters, int max_rank, int n_rows) {
+    if (in_dim <= 0 || n_mats < 1 || n_mats > kMaxLoraMats || n_adapters < 1 || n_adapters >= kMaxGroups ||
+        max_rank < 4 || max_rank > kMaxLoraRank || n_rows <= 0 || n_rows > (1 << 24))
+        return 0;
+    return lora_ws_bytes(n_mats, in_dim, max_rank, n_adapters, n_rows);
+}
+
+int cllm_hip_lora_dev(uint32_t type, int in_dim, int n_mats, const void* const* a, const void* const* b,
+                      const int* out_dims, int n_adapters, int max_rank, const int32_t* ranks, const float* scales,
+                      const float* x, int n_rows, const int32_t* offsets, const int32_t* order,
+                      const float* const* base, float* const* y, void* ws, size_t ws_bytes, void* stream) {
+    if (type != T_F16 && type != T_F32) return set_err(CLLM_HIP_E_TYPE, "lora: adapters must be F16 or F32");
+    int rc = check_lora(in_dim, n_mats, out_dims, n_adapters, max_rank, n_rows);
+    if (rc) return rc;
+    if (n_rows == 0) return CLLM_HIP_OK;
+    if ((rc = check_groups("lora", n_rows, n_adapters, offsets, order))) return rc;
+    if (!a || !b || !y || !x) return set_err(CLLM_HIP_E_ARG, "lora: null pointer");
+    LoraArgs l{};
+    for (int i = 0; i < n_mats; ++i) {
+        if (!a[i] || !b[i] || (!y[i] && out_dims[i] > 0)) return set_err(CLLM_HIP_E_ARG, "lora: null pointer");
+        l.a[i] = a[i], l.b[i] = b[i], l.y[i] = y[i], l.n[i] = out_dims[i];
+        l.base[i] = base ? base[i] : nullptr;
+        if (!aligned16(a[i]) || !aligned16(b[i]) || !aligned16(y[i]) || !aligned16(l.base[i]))
+            return set_err(CLLM_HIP_E_ARG, "lora: misaligned device pointer");
+    }
+    if (!aligned16(x) || !aligned4(ranks) || !aligned4(scales))
+        return set_err(CLLM_HIP_E_ARG, "lora: misaligned device pointer");
+    if ((rc = check_ws("lora", ws, ws_bytes, lora_ws_bytes(n_mats, in_dim, max_rank, n_adapters, n_rows)))) return rc;
+    DeviceState* st;
+    if ((rc = acquire(&st))) return rc;
+    l.half = type == T_F16;
+    l.k = in_dim;
+    l.mats = n_mats;
+    l.max_rank = max_rank;
+    l.ranks = ranks;
+    l.scales = scales;
+    l.x = x;
+    l.g = Groups{offsets, order, n_adapters, n_rows};
+    l.ws = (float*)ws;
+    HIP_TRY(launch_lora(l, (hipStream_t)stream));
     return CLLM_HIP_OK;
 }
 

@@ -1,0 +1,891 @@
+// k_experts.hip -- products of rows with the matrix of the row's expert, over GGUF blocks (gfx950).
+//
+// y[e] = W_x . q(x_r) of every entry e = (row r, expert x): the reference's vec_dot terms
+// (src/core/quant.cpp:549-687, 706-724) on the Q8_0 blocks of x_r (420-452), with the entries
+// grouped by expert on the device; two matrices give silu(gate) * up (src/core/engine.cpp:509-512).
+//
+// Arithmetic. A Q8_0 element is dx * c. k_expert_act writes it, times a power of two of its row, as
+// fp16 hi + lo (22 bits), the token operand of the fp16 MFMAs; the weight operand holds the blocks'
+// integers (times the 6-bit sub-scales of Q4_K / Q5_K: at most 1953, exact in fp16; Q6_K's
+// scale * (q - 32) as its fp16 rounding and the exact rest). As dx is inside the operand, nothing is
+// done per block of 32: a super-block's 256 products add up in the MFMA's fp32 accumulators and meet
+// the weight row's d once, which with the weights on the column side is one scalar of the lane.
+// Blocks of 32 (Q4_0, Q5_0, Q8_0) meet their d once a block. The K-quants' minimum term is one
+// more MFMA a super-block: the 8 minima against dx * (sum of the block's codes) in three fp16 parts.
+// The order of a super-block's elements in the operands is free, so each lane takes contiguous
+// weight bytes and the activations are written in the order that follows.
+//
+// (The weight-row GEMM applies dx per block on the VALU, one FMA per output and block, with half the
+// MFMAs; here the MFMAs are doubled and the VALU is left to unpack.)
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdio>
+
+#include "device_utils.h"
+#include "experts.h"
+#include "ggml_blocks.h"
+#include "launch.h"
+#include "mfma_common.h"
+
+namespace cllm_hip {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// ---- the activation operand -----------------------------------------------------------------
+// Row r: chunks of 256 elements, each [step 8][hi, lo][g 4][8 fp16] (16-byte fragments), 1024 bytes;
+// then (K-quants with minima) [chunk][3 parts and zeros][8 blocks] fp16, 64 bytes a chunk; then the rows'
+// exponents. Fragment (step s, g) holds elements
+//   Q4_K, Q5_K  64 g + 8 s + e                    (lane g: the 32 quant bytes of blocks 2g and 2g + 1)
+//   Q6_K        128 (g / 2) + 32 (s / 2) + 16 (g % 2) + 8 (s % 2) + e
+//   Q8_0        32 s + 8 g + e
+//   Q4_0, Q5_0  32 s + 4 g + e (e < 4), 32 s + 16 + 4 g + e - 4 (e >= 4)
+// with e = 0, 2, 1, 3 in each four where the low and high 16 bits of a dword are unpacked together.
+constexpr int kExpNaN = INT32_MIN;  // exponent of a row with an infinity or a NaN: its results are NaN
+constexpr int kTop = 13;            // rows are scaled to magnitudes below 2^(kTop + 1)
+constexpr int kMinShift = 5;        // minimum operand: 2^-5 of the scale (a block's codes add up to 4064)
+
+enum Order { kMin64, kQ6, kByte, kNibble };
+__host__ __device__ constexpr Order order_of(uint32_t t) {
+    return t == T_Q4_K || t == T_Q5_K ? kMin64 : t == T_Q6_K ? kQ6 : t == T_Q8_0 ? kByte : kNibble;
+}
+__host__ __device__ constexpr bool has_min(uint32_t t) { return t == T_Q4_K || t == T_Q5_K; }
+__host__ __device__ constexpr bool is_kq(uint32_t t) { return has_min(t) || t == T_Q6_K; }
+
+struct Act {
+    const uint8_t* frags;
+    const uint8_t* mins;
+    const int32_t* exps;
+    uint32_t row;  // bytes of a row's fragments
+    int chunks;
+};
+int chunks_of(int k) { return (k + 255) / 256; }
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+Act act_of(void* ws, uint32_t type, int k, int rows) {
+    Act a;
+    a.chunks = chunks_of(k);
+    a.row = (uint32_t)a.chunks * 1024u;
+    uint8_t* p = (uint8_t*)ws;
+    a.frags = p;
+    p += (size_t)rows * a.row;
+    a.mins = p;
+    if (has_min(type)) p += up256((size_t)rows * a.chunks * 64);
+    a.exps = (const int32_t*)p;
+    return a;
+}
+
+// One workgroup a row: the row's largest magnitude, then each quad of lanes one Q8_0 block (eight
+// elements a lane, quantize_row_q8_0 bit for bit) as scaled fp16 parts. The second read of the row
+// hits the caches. 1024 threads for few rows, where one row's latency is what counts.
+template <Order O, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_expert_act(const float* __restrict__ x, int k, uint32_t row_bytes,
+                                                        int chunks, uint8_t* __restrict__ frags,
+                                                        uint8_t* __restrict__ mins, int32_t* __restrict__ exps) {
+    __shared__ uint32_t tops[THREADS / 64];
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const f32x4* __restrict__ src = (const f32x4*)(x + (size_t)row * k);
+    uint32_t top = 0;  // the largest (bits << 1): orders magnitudes, and NaN above infinity
+    for (int i = tid; i < k / 4; i += THREADS) {
+        const f32x4 v = src[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(v[j]) << 1);
+    }
+    for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i) top = max(top, tops[i]);
+    const bool finite = top < 0xFF000000u;
+    int e = 0;
+    if (finite && top != 0) {
+        int ex;
+        (void)frexpf(__builtin_bit_cast(float, top >> 1), &ex);  // magnitude in [2^(ex - 1), 2^ex)
+        e = kTop + 1 - ex;
+    }
+    if (tid == 0) exps[row] = finite ? e : kExpNaN;
+    uint8_t* out = frags + (size_t)row * row_bytes;
+    // lanes past the row's end write zeros up to the last chunk's end (whole quads: k is a multiple of 32)
+    for (int i = tid; i < chunks * 32; i += THREADS) {
+        const int c = i >> 5, b = (i >> 2) & 7, p = i & 3;  // chunk, block, eight elements of it
+        float v[8] = {};
+        if (8 * i < k && finite) {
+            const f32x4 lo = src[2 * i], hi = src[2 * i + 1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
+        }
+        uint32_t q[2];
+        float d;
+        int s8;
+        q8_quant_quad(v, q, d, s8);
+        const float dx = ldexpf(d, e);
+        _Float16 h[8], l[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            // (rounded to fp32 first, for both parts alike: else the compiler forms hi from the product
+            // in one rounding and lo from the rounded product, and where the two hi differ lo is a step off)
+            const float t = pinned(dx * (float)(int8_t)(q[j >> 2] >> (8 * (j & 3))));
+            h[j] = (_Float16)t;
+            l[j] = (_Float16)(t - (float)h[j]);
+        }
+        uint8_t* ch = out + (size_t)c * 1024;
+        if constexpr (O == kNibble) {
+            // elements 8p .. of the block: the first (p < 2) or second four of fragments g and g + 1
+            const int g = 2 * (p & 1);
+            typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                uint8_t* at = ch + b * 128 + (g + j) * 16 + 8 * (p >> 1);
+                *(h4*)at = h4{h[4 * j], h[4 * j + 2], h[4 * j + 1], h[4 * j + 3]};
+                *(h4*)(at + 64) = h4{l[4 * j], l[4 * j + 2], l[4 * j + 1], l[4 * j + 3]};
+            }
+        } else {
+            int s, g;
+            if constexpr (O == kMin64) {
+                s = 4 * (b & 1) + p, g = b >> 1;
+            } else if constexpr (O == kQ6) {
+                s = 2 * (b & 3) + (p & 1), g = 2 * (b >> 2) + (p >> 1);
+            } else {
+                s = b, g = p;
+            }
+            uint8_t* at = ch + s * 128 + g * 16;
+            if constexpr (O == kMin64) {
+                *(wh8*)at = wh8{h[0], h[2], h[1], h[3], h[4], h[6], h[5], h[7]};
+                *(wh8*)(at + 64) = wh8{l[0], l[2], l[1], l[3], l[4], l[6], l[5], l[7]};
+            } else {
+                *(wh8*)at = wh8{h[0], h[1], h[2], h[3], h[4], h[5], h[6], h[7]};
+                *(wh8*)(at + 64) = wh8{l[0], l[1], l[2], l[3], l[4], l[5], l[6], l[7]};
+            }
+        }
+        if constexpr (O == kMin64) {
+            const int s16 = s8 + dpp_i32<DPP_QUAD_SWAP1>(s8);
+            const int sum = s16 + dpp_i32<DPP_QUAD_SWAP2>(s16);
+            float t = pinned(ldexpf(d, e - kMinShift) * (float)sum);
+            _Float16* m = (_Float16*)(mins + ((size_t)row * chunks + c) * 64) + b;
+            if (p == 0) {
+#pragma unroll
+                for (int j = 0; j < 3; ++j) {
+                    const _Float16 part = (_Float16)t;
+                    m[8 * j] = part;
+                    t -= (float)part;
+                }
+                m[24] = (_Float16)0.0f;
+            }
+        }
+    }
+}
+
+// ---- the weight operand ----------------------------------------------------------------------
+// One weight row's share of a lane group g (of 4) of a 256-element chunk: its bytes in registers,
+// then fragments of 8 fp16 integers.
+__device__ __forceinline__ wh2 as_h2(uint32_t v) { return __builtin_bit_cast(wh2, v); }
+__device__ __forceinline__ wh2 both(float v) { return wh2{(_Float16)v, (_Float16)v}; }
+__device__ __forceinline__ wh8 cat(wh2 a, wh2 b, wh2 c, wh2 d) {
+    return wh8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+template <int BYTES, class V>
+__device__ __forceinline__ V ld_any(const uint8_t* p) {  // any alignment: one load instruction
+    V v;
+    __builtin_memcpy(&v, p, BYTES);
+    return v;
+}
+
+// 6-bit scales and minima of the super-block's eight blocks, a byte each (get_scale_min_k4,
+// quant.cpp:72-80): minima as fp16
+__device__ __forceinline__ wh8 k4_minima(const u32x4& hdr) {
+    const uint32_t a = hdr.z & 0x3F3F3F3Fu;
+    const uint32_t b = ((hdr.w >> 4) & 0x0F0F0F0Fu) | ((hdr.z >> 2) & 0x30303030u);
+    const wh2 off = both(-1024.0f);
+    return cat(magic_pair(a, 0) + off, magic_pair(a, 1) + off, magic_pair(b, 0) + off, magic_pair(b, 1) + off);
+}
+// the scales of blocks 2g and 2g + 1
+__device__ __forceinline__ void k4_scales2(const u32x4& hdr, int g, float& s0, float& s1) {
+    const int sh = 16 * (g & 1);
+    const uint32_t lo = (hdr.y >> sh) & 0x3F3Fu;
+    const uint32_t hi = ((hdr.w >> sh) & 0x0F0Fu) | ((hdr.y >> (sh + 2)) & 0x3030u);
+    const uint32_t s = g < 2 ? lo : hi;
+    s0 = (float)(s & 0xFFu);
+    s1 = (float)((s >> 8) & 0xFFu);
+}
+
+template <uint32_t T>
+struct Unit;
+
+template <>
+struct Unit<T_Q4_K> {
+    static constexpr int BYTES = Q4_K_BYTES;
+    u32x4 hdr, q[2];
+    wh2 s0, c0, s1, c1;
+    __device__ __forceinline__ void load(const uint8_t* p, int g) {
+        hdr = ld_u32x4(p);
+        q[0] = ld_u32x4(p + 16 + 32 * g);
+        q[1] = ld_u32x4(p + 32 + 32 * g);
+    }
+    __device__ __forceinline__ void ready(int g) {
+        float a, b;
+        k4_scales2(hdr, g, a, b);
+        s0 = both(a), c0 = both(-1024.0f * a);
+        s1 = both(b * 0.0625f), c1 = both(-64.0f * b);
+    }
+    __device__ __forceinline__ wh8 frag(int s) const {
+        const uint32_t a = q[(s & 3) >> 1][2 * (s & 1)], b = q[(s & 3) >> 1][2 * (s & 1) + 1];
+        const uint32_t m = s < 4 ? 0x000F000Fu : 0x00F000F0u, o = 0x64006400u;
+        const wh2 k = s < 4 ? s0 : s1, c = s < 4 ? c0 : c1;
+        return cat(__builtin_elementwise_fma(as_h2((a & m) | o), k, c),
+                   __builtin_elementwise_fma(as_h2(((a >> 8) & m) | o), k, c),
+                   __builtin_elementwise_fma(as_h2((b & m) | o), k, c),
+                   __builtin_elementwise_fma(as_h2(((b >> 8) & m) | o), k, c));
+    }
+    __device__ __forceinline__ float d() const { return f16_to_f32(hdr.x & 0xFFFFu); }
+    __device__ __forceinline__ float dmin() const { return f16_to_f32(hdr.x >> 16); }
+    __device__ __forceinline__ wh8 minima() const { return k4_minima(hdr); }
+};
+
+template <>
+struct Unit<T_Q5_K> {
+    static constexpr int BYTES = Q5_K_BYTES;
+    u32x4 hdr, q[2], h[2];
+    wh2 s0, c0, s1, c1;
+    int k;  // the first block's bit of h
+    __device__ __forceinline__ void load(const uint8_t* p, int g) {
+        hdr = ld_u32x4(p);
+        h[0] = ld_u32x4(p + 16);
+        h[1] = ld_u32x4(p + 32);
+        q[0] = ld_u32x4(p + 48 + 32 * g);
+        q[1] = ld_u32x4(p + 64 + 32 * g);
+    }
+    __device__ __forceinline__ void ready(int g) {
+        float a, b;
+        k4_scales2(hdr, g, a, b);
+        s0 = both(a), c0 = both(-1024.0f * a);
+        s1 = both(b), c1 = both(-1024.0f * b);
+        k = 2 * g;
+    }
+    __device__ __forceinline__ wh8 frag(int s) const {
+        wh2 f[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t n = q[(s & 3) >> 1][2 * (s & 1) + j], b = h[(s & 3) >> 1][2 * (s & 1) + j];
+            const uint32_t v = ((s < 4 ? n : n >> 4) & 0x0F0F0F0Fu) | (((b >> (k + (s >> 2))) & 0x01010101u) << 4);
+            const wh2 m = s < 4 ? s0 : s1, c = s < 4 ? c0 : c1;
+            f[2 * j] = __builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(0x64646464u, v, 0x04020400u)), m, c);
+            f[2 * j + 1] = __builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(0x64646464u, v, 0x04030401u)), m, c);
+        }
+        return cat(f[0], f[1], f[2], f[3]);
+    }
+    __device__ __forceinline__ float d() const { return f16_to_f32(hdr.x & 0xFFFFu); }
+    __device__ __forceinline__ float dmin() const { return f16_to_f32(hdr.x >> 16); }
+    __device__ __forceinline__ wh8 minima() const { return k4_minima(hdr); }
+};
+
+template <>
+struct Unit<T_Q6_K> {
+    static constexpr int BYTES = Q6_K_BYTES;
+    u32x4 l[2], h;
+    u32x2 sc;
+    uint32_t db;
+    int u;
+    __device__ __forceinline__ void load(const uint8_t* p, int g) {
+        const int n = g >> 1;
+        u = g & 1;
+        l[0] = ld_any<16, u32x4>(p + 64 * n + 16 * u);
+        l[1] = ld_any<16, u32x4>(p + 64 * n + 32 + 16 * u);
+        h = ld_any<16, u32x4>(p + Q6_K_QH + 32 * n + 16 * u);
+        sc = ld_any<8, u32x2>(p + Q6_K_SC + 8 * n);
+        db = ld_u16(p + Q6_K_D);
+    }
+    __device__ __forceinline__ void ready(int) {}
+    // scale * (q - 32): the fp16 rounding and the rest, exact
+    __device__ __forceinline__ wh8 frag(int s, wh8& rest) const {
+        const int i = s >> 1;
+        const wh2 m = both((float)(int8_t)((sc[i >> 1] >> (16 * (i & 1) + 8 * u)) & 0xFFu));
+        const wh2 off = both(-1056.0f);
+        wh2 f[4], r[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t n = l[i & 1][2 * (s & 1) + j], b = h[2 * (s & 1) + j];
+            const uint32_t v = ((i < 2 ? n : n >> 4) & 0x0F0F0F0Fu) | (((b >> (2 * i)) & 0x03030303u) << 4);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const wh2 p = magic_pair(v, e) + off;
+                f[2 * j + e] = p * m;
+                r[2 * j + e] = __builtin_elementwise_fma(p, m, -f[2 * j + e]);
+            }
+        }
+        rest = cat(r[0], r[1], r[2], r[3]);
+        return cat(f[0], f[1], f[2], f[3]);
+    }
+    __device__ __forceinline__ float d() const { return f16_to_f32(db); }
+};
+
+// Blocks of 32: the eight elements of lane group g of one block.
+__device__ __forceinline__ wh8 nibbles8(uint32_t v, float off) {
+    const uint32_t o = 0x64006400u;
+    const wh2 one = both(1.0f), c0 = both(-1024.0f + off), k1 = both(0.0625f), c1 = both(-64.0f + off);
+    return cat(__builtin_elementwise_fma(as_h2((v & 0x000F000Fu) | o), one, c0),
+               __builtin_elementwise_fma(as_h2(((v >> 8) & 0x000F000Fu) | o), one, c0),
+               __builtin_elementwise_fma(as_h2((v & 0x00F000F0u) | o), k1, c1),
+               __builtin_elementwise_fma(as_h2(((v >> 8) & 0x00F000F0u) | o), k1, c1));
+}
+// bits 4 g .. 4 g + 3 (and 16 more) of qh to bit 4 of four bytes
+__device__ __forceinline__ uint32_t bits4(uint32_t x) {
+    return ((((x & 0xFu) * 0x00204081u) & 0x01010101u) << 4);
+}
+__device__ __forceinline__ wh8 five8(uint32_t v, uint32_t qh, int g) {
+    const uint32_t a = (v & 0x0F0F0F0Fu) | bits4(qh >> (4 * g));
+    const uint32_t b = ((v >> 4) & 0x0F0F0F0Fu) | bits4(qh >> (16 + 4 * g));
+    const wh2 c = both(-1040.0f);
+    return cat(as_h2(__builtin_amdgcn_perm(0x64646464u, a, 0x04020400u)) + c,
+               as_h2(__builtin_amdgcn_perm(0x64646464u, a, 0x04030401u)) + c,
+               as_h2(__builtin_amdgcn_perm(0x64646464u, b, 0x04020400u)) + c,
+               as_h2(__builtin_amdgcn_perm(0x64646464u, b, 0x04030401u)) + c);
+}
+
+template <>
+struct Unit<T_Q8_0> {
+    static constexpr int BYTES = Q8_0_BYTES;
+    u32x2 q;
+    uint32_t db;
+    __device__ __forceinline__ void load(const uint8_t* p, int g) {
+        q = ld_any<8, u32x2>(p + 2 + 8 * g);
+        db = ld_u16(p);
+    }
+    __device__ __forceinline__ wh8 frag(int) const { return __builtin_bit_cast(wh8, int8x8_to_h8(q.x, q.y)); }
+};
+template <>
+struct Unit<T_Q4_0> {
+    static constexpr int BYTES = Q4_0_BYTES;
+    uint32_t q, db;
+    __device__ __forceinline__ void load(const uint8_t* p, int g) {
+        q = ld_any<4, uint32_t>(p + 2 + 4 * g);
+        db = ld_u16(p);
+    }
+    __device__ __forceinline__ wh8 frag(int) const { return nibbles8(q, -8.0f); }
+};
+template <>
+struct Unit<T_Q5_0> {
+    static constexpr int BYTES = Q5_0_BYTES;
+    uint32_t q, h, db;
+    __device__ __forceinline__ void load(const uint8_t* p, int g) {
+        q = ld_any<4, uint32_t>(p + 6 + 4 * g);
+        h = ld_any<4, uint32_t>(p + 2);
+        db = ld_u16(p);
+    }
+    __device__ __forceinline__ wh8 frag(int g) const { return five8(q, h, g); }
+};
+
+struct Mul {
+    const uint8_t* w[2];
+    const float* bias[2];
+    size_t expert_bytes;
+    uint32_t row_bytes;
+    int n, nb;  // weight rows, 32-element blocks of a row
+    Act act;
+    int per_row, rows;
+    Groups g;
+    int n_blocks;
+    float* y;
+};
+
+// What a tile's entry needs: its number (-1: none), its activation row.
+__device__ __forceinline__ int entry_of(const Mul& a, const GroupTile& t, int i) {
+    const int e = i < t.count ? a.g.order[t.first + i] : -1;
+    return (uint32_t)e < (uint32_t)a.g.entries && e / a.per_row < a.rows ? e : -1;
+}
+__device__ __forceinline__ float unscaled(float v, int e) {
+    return e == kExpNaN ? __builtin_nanf("") : ldexpf(v, -e);
+}
+
+// ---- few rows to an expert ----------------------------------------------------------------------
+// A workgroup has 16 entries of an expert (its rows' 16-row MFMA side) and 16 weight rows of each of NT
+// tiles (gate and up, or 16 NT rows); its KP waves take every KP-th chunk and meet in LDS, in order.
+// Weights go from memory to registers, each byte read once by one lane; the fragments of the
+// activations come from the caches.
+template <uint32_t T, int NT, bool SWIGLU, int KP>
+__global__ __launch_bounds__(64 * KP) void k_expert_rows(Mul a) {
+    static_assert(!SWIGLU || NT == 2, "gate and up");
+    __shared__ float red[KP][NT][256];
+    __shared__ int ent[16], exps[16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int blk = blockIdx.x % a.n_blocks;
+    const GroupTile t = find_tile<16>(a.g, 0, blockIdx.x / a.n_blocks, lane);
+    if (t.count <= 0) return;
+    const int r = lane & 15, g = lane >> 4;
+    const int e = entry_of(a, t, r);
+    const int arow = e < 0 ? 0 : e / a.per_row;
+    if (threadIdx.x < 16) {
+        ent[r] = e;
+        exps[r] = a.act.exps[arow];
+    }
+    const uint8_t* ap = a.act.frags + (size_t)arow * a.act.row + 16 * g;
+    const uint8_t* wp[NT];
+    const int n0 = blk * (SWIGLU ? 16 : 16 * NT);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+        wp[i] = a.w[SWIGLU ? i : 0] + (size_t)t.group * a.expert_bytes +
+                (size_t)min(n0 + (SWIGLU ? 0 : 16 * i) + r, a.n - 1) * a.row_bytes;
+    f32x4 acc[NT];
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i] = zero;
+    for (int c = wave; c < a.act.chunks; c += KP) {
+        if constexpr (is_kq(T)) {
+            Unit<T> u[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) u[i].load(wp[i] + (size_t)c * Unit<T>::BYTES, g);
+            wh8 ah[8], al[8], am;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                ah[s] = *(const wh8*)(ap + (size_t)c * 1024 + s * 128);
+                al[s] = *(const wh8*)(ap + (size_t)c * 1024 + s * 128 + 64);
+            }
+            if constexpr (has_min(T)) am = *(const wh8*)(a.act.mins + ((size_t)arow * a.act.chunks + c) * 64 + 16 * g);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                u[i].ready(g);
+                f32x4 sum = zero;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) {
+                    if constexpr (T == T_Q6_K) {
+                        wh8 rest;
+                        const wh8 f = u[i].frag(s, rest);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], f, sum, 0, 0, 0);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], f, sum, 0, 0, 0);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], rest, sum, 0, 0, 0);
+                    } else {
+                        const wh8 f = u[i].frag(s);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], f, sum, 0, 0, 0);
+                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], f, sum, 0, 0, 0);
+                    }
+                }
+                const float d = u[i].d();
+                if constexpr (has_min(T)) {
+                    const f32x4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(am, u[i].minima(), zero, 0, 0, 0);
+                    const float dm = -(float)(1 << kMinShift) * u[i].dmin();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], fmaf(dm, m[j], acc[i][j]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], acc[i][j]);
+                }
+            }
+        } else {
+            Unit<T> u[8][NT];
+            wh8 ah[8], al[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const int b = min(8 * c + s, a.nb - 1);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) u[s][i].load(wp[i] + (size_t)b * Unit<T>::BYTES, g);
+                ah[s] = *(const wh8*)(ap + (size_t)c * 1024 + s * 128);
+                al[s] = *(const wh8*)(ap + (size_t)c * 1024 + s * 128 + 64);
+            }
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                const bool there = 8 * c + s < a.nb;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const wh8 f = u[s][i].frag(g);
+                    f32x4 sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], f, zero, 0, 0, 0);
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], f, sum, 0, 0, 0);
+                    const float d = there ? f16_to_f32(u[s][i].db) : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], acc[i][j]);
+                }
+            }
+        }
+    }
+    // lane (r, g) has tokens 4g + j of weight row r
+#pragma unroll
+    for (int i = 0; i < NT; ++i) *(f32x4*)&red[wave][i][4 * lane] = acc[i];
+    __syncthreads();
+    constexpr int OUT = SWIGLU ? 256 : 256 * NT;
+    for (int o = threadIdx.x; o < OUT; o += 64 * KP) {
+        const int i = o >> 8, tok = (o >> 4) & 15, col = o & 15;
+        const int at = 4 * (16 * (tok >> 2) + col) + (tok & 3);
+        const int en = ent[tok], row = n0 + 16 * i + col;
+        if (en < 0 || row >= a.n) continue;
+        float v = red[0][i][at], v1 = 0.0f;
+#pragma unroll
+        for (int w = 1; w < KP; ++w) v += red[w][i][at];
+        v = unscaled(v, exps[tok]);
+        const size_t b = (size_t)t.group * a.n + row;
+        if (a.bias[0]) v += a.bias[0][b];
+        if constexpr (SWIGLU) {
+            v1 = red[0][1][at];
+#pragma unroll
+            for (int w = 1; w < KP; ++w) v1 += red[w][1][at];
+            v1 = unscaled(v1, exps[tok]);
+            if (a.bias[1]) v1 += a.bias[1][b];
+            v = silu_mul(v, v1);
+        }
+        a.y[(size_t)en * a.n + row] = v;
+    }
+}
+
+// ---- many rows to an expert ----------------------------------------------------------------------
+// 32 MT entries of an expert and 256 weight rows (128 of gate and of up): four waves of 64 weight rows
+// (two 32-column MFMA tiles, gate and up of the same rows, or 64 rows) against all entries. The waves
+// share the activation fragments, which reach LDS in stages of half a chunk, two buffers, by
+// direct-to-LDS loads; each wave reads and unpacks its own weight rows, a chunk ahead, in registers.
+// LDS: [entry][32 fragments of 16 bytes], fragment f of entry i in place f ^ (i % 32), so that the 32
+// entries' reads of one fragment fall on distinct banks.
+template <int MT>
+struct Wide {
+    static constexpr int BM = 32 * MT;
+    static constexpr int FRAGS = BM * 512, MINS = BM * 64;
+    static constexpr int STAGE = FRAGS + MINS;
+    static constexpr int LDS = 2 * STAGE;
+};
+
+__device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint32_t m0) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 : : "v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
+
+template <uint32_t T, int MT, bool SWIGLU>
+__global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
+    using C = Wide<MT>;
+    constexpr int NT = 2;
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ int ent[C::BM], exps[C::BM];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int blk = blockIdx.x % a.n_blocks;
+    const GroupTile t = find_tile<C::BM>(a.g, 0, blockIdx.x / a.n_blocks, lane);
+    if (t.count <= 0) return;
+    const int r = lane & 31, h = lane >> 5;
+    for (int i = threadIdx.x; i < C::BM; i += 256) {
+        const int e = entry_of(a, t, i);
+        ent[i] = e;
+        exps[i] = a.act.exps[e < 0 ? 0 : e / a.per_row];
+    }
+    // sources of this wave's direct-to-LDS loads: BM / 2 loads of two entries a stage
+    constexpr int AL = C::BM / 8;
+    uint32_t a_off[AL];
+#pragma unroll
+    for (int j = 0; j < AL; ++j) {
+        const int i = 2 * (4 * j + wave) + h;
+        const int e = entry_of(a, t, i);
+        a_off[j] = (uint32_t)(e < 0 ? 0 : e / a.per_row) * a.act.row + 16u * (uint32_t)(r ^ (i & 31));
+    }
+    // the minima's: 16 entries a load, place q of entry i holds part q ^ (i / 2 % 4)
+    const int mi = 16 * wave + (lane >> 2);
+    uint32_t m_off = 0;
+    if (has_min(T) && mi < C::BM) {
+        const int e = entry_of(a, t, mi);
+        m_off = (uint32_t)(e < 0 ? 0 : e / a.per_row) * (uint32_t)(a.act.chunks * 64) +
+                16u * (uint32_t)((lane & 3) ^ ((mi >> 1) & 3));
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)lds;
+    auto issue = [&](int st, int buf) {
+        const uint32_t to = lds0 + (uint32_t)buf * C::STAGE;
+        const uint8_t* from = a.act.frags + (size_t)st * 512;
+#pragma unroll
+        for (int j = 0; j < AL; ++j) to_lds16(from, a_off[j], to + 1024u * (uint32_t)(4 * j + wave));
+        if (has_min(T) && (st & 1) && 16 * wave < C::BM)
+            to_lds16(a.act.mins + (size_t)(st >> 1) * 64, m_off, to + C::FRAGS + 1024u * (uint32_t)wave);
+    };
+
+    const int n0 = blk * (SWIGLU ? 128 : 256) + wave * (SWIGLU ? 32 : 64);
+    const uint8_t* wp[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+        wp[i] = a.w[SWIGLU ? i : 0] + (size_t)t.group * a.expert_bytes +
+                (size_t)min(n0 + (SWIGLU ? 0 : 32 * i) + r, a.n - 1) * a.row_bytes;
+
+    wf16 acc[NT][MT], sum[NT][MT];
+    const wf16 zero = {};
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[i][m] = sum[i][m] = zero;
+
+    const int stages = 2 * a.act.chunks;
+    Unit<T> nxt[NT][2];
+    auto load_chunk = [&](int c) {
+        if constexpr (is_kq(T)) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) nxt[i][q].load(wp[i] + (size_t)c * Unit<T>::BYTES, 2 * h + q);
+        }
+    };
+    issue(0, 0);
+    load_chunk(0);
+    Unit<T> u[NT][2];
+    auto stage = [&]<int HALF>(int st) {
+        const uint8_t* cur = lds + HALF * C::STAGE;
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's loads of the stage are in LDS
+        asm volatile("" ::: "memory");
+        __syncthreads();                     // and every wave's; the other buffer is free
+        if (st + 1 < stages) issue(st + 1, 1 - HALF);
+        if constexpr (is_kq(T)) {
+            if constexpr (HALF == 0) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) u[i][q] = nxt[i][q], u[i][q].ready(2 * h + q);
+            } else {
+                if (st + 1 < stages) load_chunk((st + 1) >> 1);
+            }
+        }
+        Unit<T> ub[4][NT][2];
+        if constexpr (!is_kq(T)) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q)
+                        ub[s][i][q].load(wp[i] + (size_t)min(4 * st + s, a.nb - 1) * Unit<T>::BYTES, 2 * h + q);
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                wh8 f[NT], rest[NT], ah[MT], al[MT];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    const uint8_t* row = cur + (32 * m + r) * 512;
+                    ah[m] = *(const wh8*)(row + 16 * ((8 * s + 2 * h + q) ^ r));
+                    al[m] = *(const wh8*)(row + 16 * ((8 * s + 4 + 2 * h + q) ^ r));
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    if constexpr (T == T_Q6_K)
+                        f[i] = u[i][q].frag(4 * HALF + s, rest[i]);
+                    else if constexpr (is_kq(T))
+                        f[i] = u[i][q].frag(4 * HALF + s);
+                    else
+                        f[i] = ub[s][i][q].frag(2 * h + q);
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const bool first = is_kq(T) ? HALF == 0 && s == 0 && q == 0 : q == 0;
+                        sum[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[m], f[i], first ? zero : sum[i][m], 0, 0, 0);
+                        sum[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[m], f[i], sum[i][m], 0, 0, 0);
+                        if constexpr (T == T_Q6_K)
+                            sum[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[m], rest[i], sum[i][m], 0, 0, 0);
+                    }
+            }
+            if constexpr (!is_kq(T)) {
+                const bool there = 4 * st + s < a.nb;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const float d = there ? f16_to_f32(ub[s][i][0].db) : 0.0f;
+#pragma unroll
+                    for (int m = 0; m < MT; ++m)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][m][e] = fmaf(d, sum[i][m][e], acc[i][m][e]);
+                }
+            }
+        }
+        if constexpr (is_kq(T)) if constexpr (HALF == 1) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const float d = u[i][0].d();
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    if constexpr (has_min(T)) {
+                        const float dm = -(float)(1 << kMinShift) * u[i][0].dmin();
+                        const wh8 mn = u[i][0].minima();
+                        const uint8_t* row = cur + C::FRAGS + (32 * m + r) * 64;
+                        wf16 f = zero;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            const wh8 x = *(const wh8*)(row + 16 * ((2 * h + q) ^ ((r >> 1) & 3)));
+                            f = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, mn, f, 0, 0, 0);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            acc[i][m][e] = fmaf(d, sum[i][m][e], fmaf(dm, f[e], acc[i][m][e]));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) acc[i][m][e] = fmaf(d, sum[i][m][e], acc[i][m][e]);
+                    }
+                }
+            }
+        }
+    };
+    for (int st = 0; st < stages; st += 2) {
+        stage.template operator()<0>(st);
+        stage.template operator()<1>(st + 1);
+    }
+
+    // lane (r, h) has entries 8 (e / 4) + 4 h + e % 4 of weight row r of each tile
+#pragma unroll
+    for (int i = 0; i < (SWIGLU ? 1 : NT); ++i) {
+        const int row = n0 + 32 * i + r;
+        if (row >= a.n) continue;
+        const size_t b = (size_t)t.group * a.n + row;
+        const float b0 = a.bias[0] ? a.bias[0][b] : 0.0f, b1 = SWIGLU && a.bias[1] ? a.bias[1][b] : 0.0f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int tok = 32 * m + 8 * (e >> 2) + 4 * h + (e & 3);
+                const int en = ent[tok];
+                if (en < 0) continue;
+                float v = unscaled(acc[i][m][e], exps[tok]) + b0;
+                if constexpr (SWIGLU) v = silu_mul(v, unscaled(acc[1][m][e], exps[tok]) + b1);
+                a.y[(size_t)en * a.n + row] = v;
+            }
+    }
+}
+
+// ---- the sum over a row's experts ----------------------------------------------------------------
+__global__ __launch_bounds__(256) void k_expert_sum(const float* __restrict__ p, const int32_t* __restrict__ ids,
+                                                    const float* __restrict__ weights, int top_k, int groups, int n,
+                                                    const float* base, float* y) {
+    const int row = blockIdx.y;
+    const int i = (blockIdx.x * 256 + threadIdx.x);
+    if (n % 4 == 0) {
+        if (4 * i >= n) return;
+        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < top_k; ++j) {
+            if ((uint32_t)ids[row * top_k + j] >= (uint32_t)groups) continue;
+            const float w = weights[row * top_k + j];
+            const f32x4 v = *(const f32x4*)(p + ((size_t)row * top_k + j) * n + 4 * i);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) s[c] = fmaf(w, v[c], s[c]);
+        }
+        const size_t at = (size_t)row * n + 4 * i;
+        if (base) s += *(const f32x4*)(base + at);
+        *(f32x4*)(y + at) = s;
+    } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int col = (blockIdx.x * 4 + c) * 256 + threadIdx.x;
+            if (col >= n) return;
+            float s = 0.0f;
+            for (int j = 0; j < top_k; ++j) {
+                if ((uint32_t)ids[row * top_k + j] >= (uint32_t)groups) continue;
+                s = fmaf(weights[row * top_k + j], p[((size_t)row * top_k + j) * n + col], s);
+            }
+            const size_t at = (size_t)row * n + col;
+            y[at] = base ? s + base[at] : s;
+        }
+    }
+}
+
+template <Order O>
+hipError_t act_launch(const ExpertArgs& a, const Act& act, hipStream_t s) {
+    if (a.rows <= 64)
+        k_expert_act<O, 1024><<<a.rows, 1024, 0, s>>>(a.x, a.k, act.row, act.chunks, (uint8_t*)act.frags,
+                                                      (uint8_t*)act.mins, (int32_t*)act.exps);
+    else
+        k_expert_act<O, 256><<<a.rows, 256, 0, s>>>(a.x, a.k, act.row, act.chunks, (uint8_t*)act.frags,
+                                                    (uint8_t*)act.mins, (int32_t*)act.exps);
+    return hipGetLastError();
+}
+
+struct Plan {
+    int wide;  // entries of a tile: 32 or 64, 0: k_expert_rows
+    int kp;
+    int n_blocks, tiles;
+};
+Plan plan_of(int mats, int k, int n, int groups, int entries) {
+    Plan p{};
+    const int per = (entries + std::min(groups, entries) - 1) / std::max(1, std::min(groups, entries));
+    p.wide = per <= 12 ? 0 : per <= 48 ? 32 : 64;
+    if (p.wide) {
+        p.n_blocks = (n + (mats == 2 ? 127 : 255)) / (mats == 2 ? 128 : 256);
+        p.tiles = p.wide == 32 ? tile_ids<32>(groups, entries) : tile_ids<64>(groups, entries);
+    } else {
+        p.kp = chunks_of(k) >= 8 ? 8 : 4;
+        p.n_blocks = (n + (mats == 2 ? 15 : 31)) / (mats == 2 ? 16 : 32);
+        p.tiles = tile_ids<16>(groups, entries);
+    }
+    return p;
+}
+
+template <uint32_t T, bool SWIGLU>
+hipError_t mul_launch(Mul& m, const Plan& p, hipStream_t s) {
+    const uint32_t grid = (uint32_t)p.n_blocks * (uint32_t)p.tiles;
+    if (p.wide == 0) {
+        if (p.kp == 8)
+            k_expert_rows<T, 2, SWIGLU, 8><<<grid, 512, 0, s>>>(m);
+        else
+            k_expert_rows<T, 2, SWIGLU, 4><<<grid, 256, 0, s>>>(m);
+    } else if (p.wide == 32) {
+        static LdsLimit limit;
+        auto* kern = k_expert_wide<T, 1, SWIGLU>;
+        if (hipError_t e = limit.raise((const void*)kern, Wide<1>::LDS)) return e;
+        kern<<<grid, 256, Wide<1>::LDS, s>>>(m);
+    } else {
+        static LdsLimit limit;
+        auto* kern = k_expert_wide<T, 2, SWIGLU>;
+        if (hipError_t e = limit.raise((const void*)kern, Wide<2>::LDS)) return e;
+        kern<<<grid, 256, Wide<2>::LDS, s>>>(m);
+    }
+    return hipGetLastError();
+}
+template <uint32_t T>
+hipError_t mul_launch2(Mul& m, int mats, const Plan& p, hipStream_t s) {
+    return mats == 2 ? mul_launch<T, true>(m, p, s) : mul_launch<T, false>(m, p, s);
+}
+
+}  // namespace
+
+size_t expert_act_bytes(uint32_t type, int k, int rows) {
+    const size_t c = (size_t)chunks_of(k);
+    return up256((size_t)rows * c * 1024 + (has_min(type) ? up256((size_t)rows * c * 64) : 0) + (size_t)rows * 4);
+}
+
+hipError_t launch_experts(const ExpertArgs& a, hipStream_t s) {
+    const Act act = act_of(a.ws, a.type, a.k, a.rows);
+    hipError_t e;
+    switch (order_of(a.type)) {
+        case kMin64: e = act_launch<kMin64>(a, act, s); break;
+        case kQ6: e = act_launch<kQ6>(a, act, s); break;
+        case kByte: e = act_launch<kByte>(a, act, s); break;
+        default: e = act_launch<kNibble>(a, act, s); break;
+    }
+    if (e != hipSuccess) return e;
+    const Plan p = plan_of(a.mats, a.k, a.n, a.g.groups, a.g.entries);
+    Mul m{};
+    m.w[0] = a.w[0], m.w[1] = a.w[1];
+    m.bias[0] = a.bias[0], m.bias[1] = a.bias[1];
+    m.row_bytes = (uint32_t)(a.k / block_elems(a.type) * (int)block_bytes(a.type));
+    m.expert_bytes = (size_t)a.n * m.row_bytes;
+    m.n = a.n;
+    m.nb = a.k / 32;
+    m.act = act;
+    m.per_row = a.per_row;
+    m.rows = a.rows;
+    m.g = a.g;
+    m.n_blocks = p.n_blocks;
+    m.y = a.y;
+    switch (a.type) {
+        case T_Q4_0: return mul_launch2<T_Q4_0>(m, a.mats, p, s);
+        case T_Q5_0: return mul_launch2<T_Q5_0>(m, a.mats, p, s);
+        case T_Q8_0: return mul_launch2<T_Q8_0>(m, a.mats, p, s);
+        case T_Q4_K: return mul_launch2<T_Q4_K>(m, a.mats, p, s);
+        case T_Q5_K: return mul_launch2<T_Q5_K>(m, a.mats, p, s);
+        case T_Q6_K: return mul_launch2<T_Q6_K>(m, a.mats, p, s);
+        default: return hipErrorInvalidValue;
+    }
+}
+
+void expert_plan_name(uint32_t type, int mats, int k, int n, int groups, int entries, char* buf, size_t cap) {
+    if (!has_kernel(type) || n <= 0 || entries <= 0) {
+        snprintf(buf, cap, "none");
+        return;
+    }
+    const Plan p = plan_of(mats, k, n, groups, entries);
+    if (p.wide)
+        snprintf(buf, cap, "k_expert_wide<%d> workgroups=%lld", p.wide, (long long)p.n_blocks * p.tiles);
+    else
+        snprintf(buf, cap, "k_expert_rows<%d> workgroups=%lld", p.kp, (long long)p.n_blocks * p.tiles);
+}
+
+hipError_t launch_expert_sum(const float* p, const int32_t* ids, const float* weights, int rows, int top_k, int groups,
+                             int n, const float* base, float* y, hipStream_t s) {
+    k_expert_sum<<<dim3((unsigned)((n + 1023) / 1024), (unsigned)rows), 256, 0, s>>>(p, ids, weights, top_k, groups, n,
+                                                                                    base, y);
+    return hipGetLastError();
+}
+
+}  // namespace cllm_hip

@@ -1,0 +1,225 @@
+// k_route.hip -- a router's choice of experts, and entries sorted by group (gfx950).
+//
+// What moves is small (a logit row is at most 4 KB); launches and dependent steps are the cost. Sorting
+// is by counting: an entry's place is the number of entries with a lower id, plus those of its own id
+// before it, so the order is stable and the same every time, without atomics or scratch.
+#include <hip/hip_runtime.h>
+
+#include "device_utils.h"
+#include "experts.h"
+
+namespace cllm_hip {
+namespace {
+
+constexpr int kSmallEntries = 512;  // up to here one workgroup routes and sorts
+constexpr int kSmallRows = 64;
+
+// ---- entries sorted by group --------------------------------------------------------------------
+// Workgroup g lists the entries of group g (the last one, the entries of none). Its 16 waves take
+// consecutive stretches of the ids: each counts its matches and the lower ids, then, behind the sums of the
+// waves before it, writes its matches.
+__global__ __launch_bounds__(1024) void k_group_rows(const int32_t* __restrict__ ids, int n, int groups,
+                                                     int32_t* __restrict__ offsets, int32_t* __restrict__ order) {
+    __shared__ int lower[16], mine[16];
+    const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int per = ((n + 1023) / 1024) * 64;  // ids to a wave, a multiple of 64
+    const int first = wave * per, last = min(n, first + per);
+    auto key = [&](int i) {
+        const int v = ids[i];
+        return (uint32_t)v < (uint32_t)groups ? v : groups;
+    };
+    int lo = 0, at = 0;
+    for (int i = first + lane; i < first + per; i += 64) {
+        const int k = i < last ? key(i) : groups + 1;
+        lo += __popcll(__ballot(k < g));
+        at += __popcll(__ballot(k == g));
+    }
+    if (lane == 0) lower[wave] = lo, mine[wave] = at;
+    __syncthreads();
+    int base = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        base += lower[w];
+        if (w < wave) before += mine[w];
+    }
+    if (threadIdx.x == 0) offsets[g] = base;
+    if (at == 0) return;
+    int to = base + before;
+    for (int i = first + lane; i < first + per; i += 64) {
+        const bool m = i < last && key(i) == g;
+        const uint64_t b = __ballot(m);
+        if (m) order[to + __popcll(b & ((1ull << lane) - 1))] = i;
+        to += __popcll(b);
+    }
+}
+
+// ---- the choice ----------------------------------------------------------------------------------
+__device__ __forceinline__ double wave_max(double v) {
+    for (int d = 32; d > 0; d >>= 1) v = fmax(v, __shfl_xor(v, d, 64));
+    return v;
+}
+__device__ __forceinline__ double wave_add(double v) {
+    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+
+// One wave chooses a row's experts. Lane l has experts V l .. V l + V - 1, so that of equal keys the lowest
+// lane's lowest slot is the lowest expert. Keys and scores are in 64 bits: scores plus a bias lie close
+// together, and the choice is then the definition's whatever the order of sums. keys: this wave's LDS for
+// 64 V doubles, used with parts only.
+template <int V>
+__device__ void choose(const RouteArgs& a, int row, int lane, double* keys) {
+    const float* z = a.logits + (size_t)row * a.stride;
+    const double none = -__builtin_inf();
+    double x[V], key[V];
+    double top = none;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int e = V * lane + j;
+        float f = e < a.experts ? z[e] : -__builtin_inff();
+        if (f != f) f = -__builtin_inff();
+        x[j] = (double)f;
+        top = fmax(top, x[j]);
+    }
+    // an expert's score: the sigmoid, or exp(x - top) (over the row's sum: below)
+    auto score = [&](double v) {
+        if (a.sigmoid) return 1.0 / (1.0 + exp(-v));
+        return v == top ? 1.0 : exp(v - top);
+    };
+    const bool all = !a.sigmoid && (a.bias || !a.normalise);  // the softmax's sum is needed
+    double sum = 1.0;
+    if (!a.sigmoid) top = wave_max(top);
+    if (all) {
+        sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += x[j] == none ? 0.0 : score(x[j]);
+        sum = wave_add(sum);
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int e = V * lane + j;
+        key[j] = x[j];
+        if (a.bias && x[j] != none) {
+            key[j] = score(x[j]) / sum + (double)a.bias[e];
+            if (key[j] != key[j]) key[j] = none;
+        }
+    }
+    if (a.parts > 1) {
+        // lane p: the score of part p; the parts that rank below top_parts keep their experts
+        const int width = a.experts / a.parts;
+#pragma unroll
+        for (int j = 0; j < V; ++j) keys[V * lane + j] = key[j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        double best = none, second = none;
+        if (lane < a.parts)
+            for (int i = 0; i < width; ++i) {
+                const int k = i + lane < width ? i + lane : (i + lane) % width;  // lanes on different banks
+                const double v = keys[lane * width + k];
+                second = fmax(second, fmin(best, v));
+                best = fmax(best, v);
+            }
+        double mine = best;
+        if (a.bias && width > 1) mine = best + second;
+        if (mine != mine) mine = none;
+        int ahead = 0;
+        for (int p = 0; p < a.parts; ++p) {
+            const double v = __shfl(mine, p, 64);
+            ahead += v > mine || (v == mine && p < lane);
+        }
+        const uint64_t keep = __ballot(lane < a.parts && ahead < a.top_parts);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int e = V * lane + j;
+            if (e >= a.experts || !((keep >> (e / width)) & 1)) key[j] = none;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+    }
+    // the k largest, one a round; lane i keeps the i-th
+    int id = -1;
+    double p = 0.0;
+    for (int i = 0; i < a.top_k; ++i) {
+        double best = key[0];
+        int slot = 0;
+#pragma unroll
+        for (int j = 1; j < V; ++j)
+            if (key[j] > best) best = key[j], slot = j;
+        const double m = wave_max(best);
+        if (m == none) break;
+        const int owner = __ffsll((unsigned long long)__ballot(best == m)) - 1;
+        const int s = __shfl(slot, owner, 64);
+        double v = none;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            v = j == s ? x[j] : v;
+            if (lane == owner && j == s) key[j] = none;
+        }
+        v = __shfl(v, owner, 64);
+        if (lane == i) id = V * owner + s, p = score(v);
+    }
+    if (a.normalise) sum = wave_add(p);
+    if (lane < a.top_k) {
+        a.ids[(size_t)row * a.top_k + lane] = id;
+        a.weights[(size_t)row * a.top_k + lane] = id < 0 || !(sum > 0.0) ? 0.0f : (float)(p / sum * (double)a.scale);
+    }
+}
+
+// SORT: one workgroup for all rows, which then sorts their entries too.
+template <int V, bool SORT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void k_route(RouteArgs a) {
+    extern __shared__ double keys[];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int row = blockIdx.x * WAVES + wave; row < a.rows; row += gridDim.x * WAVES)
+        choose<V>(a, row, lane, keys + wave * 64 * V);
+    if constexpr (SORT) {
+        __shared__ int key[kSmallEntries];
+        __threadfence_block();
+        __syncthreads();
+        const int n = a.rows * a.top_k;
+        for (int i = threadIdx.x; i < n; i += 64 * WAVES) {
+            const int v = a.ids[i];
+            key[i] = (uint32_t)v < (uint32_t)a.experts ? v : a.experts;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += 64 * WAVES) {
+            const int k = key[i];
+            int to = 0;
+            for (int j = 0; j < n; ++j) to += key[j] < k || (key[j] == k && j < i);
+            a.order[to] = i;
+        }
+        for (int e = threadIdx.x; e <= a.experts; e += 64 * WAVES) {
+            int c = 0;
+            for (int j = 0; j < n; ++j) c += key[j] < e;
+            a.offsets[e] = c;
+        }
+    }
+}
+
+template <int V>
+hipError_t route_launch(const RouteArgs& a, hipStream_t s) {
+    const bool small = a.rows <= kSmallRows && a.rows * a.top_k <= kSmallEntries;
+    const size_t per = a.parts > 1 ? 64 * V * sizeof(double) : 0;
+    if (small) {
+        if (a.rows <= 4 || V == 16)  // (of 16 experts to a lane, more waves' keys would not fit 64 KB)
+            k_route<V, true, 4><<<1, 256, 4 * per, s>>>(a);
+        else
+            k_route<V, true, 8><<<1, 512, 8 * per, s>>>(a);
+        return hipGetLastError();
+    }
+    k_route<V, false, 4><<<(a.rows + 3) / 4, 256, 4 * per, s>>>(a);
+    if (hipError_t e = hipGetLastError()) return e;
+    return launch_group_rows(a.ids, a.rows * a.top_k, a.experts, a.offsets, a.order, s);
+}
+
+}  // namespace
+
+hipError_t launch_group_rows(const int32_t* ids, int n, int groups, int32_t* offsets, int32_t* order, hipStream_t s) {
+    k_group_rows<<<groups + 1, 1024, 0, s>>>(ids, n, groups, offsets, order);
+    return hipGetLastError();
+}
+
+hipError_t launch_route(const RouteArgs& a, hipStream_t s) {
+    return a.experts <= 64 ? route_launch<1>(a, s) : a.experts <= 128 ? route_launch<2>(a, s)
+         : a.experts <= 256 ? route_launch<4>(a, s) : a.experts <= 512 ? route_launch<8>(a, s) : route_launch<16>(a, s);
+}
+
+}  // namespace cllm_hip

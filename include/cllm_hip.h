@@ -449,6 +449,92 @@ int cllm_hip_logprobs_dev(const float* logits, int64_t row_stride, int n_rows, i
                           float* entropy, float* lse, int32_t* top_ids, float* top_logprobs,
                           void* ws, size_t ws_bytes, void* stream);
 
+/* ---- products whose weights a row's index chooses (stream-ordered) -----------------------
+ * Feed-forwards of experts and low-rank adapters: rows of one batch meet different weights. No
+ * reference counterpart (its models have one feed-forward a layer, src/core/engine.cpp:508-513).
+ *
+ * Entries are grouped by index on the device: order[0..n) lists them sorted by group (ascending
+ * within a group), those of group g at order[offsets[g]] .. order[offsets[g + 1] - 1], those of no group
+ * (an index outside [0, n_groups)) from offsets[n_groups] on. At most 1024 groups. All of these calls
+ * allocate nothing and read nothing back, so they can be captured into graphs. What offsets and
+ * order hold is checked where it is used: an entry out of range is no entry.
+ *
+ * Groups n entries by ids[i] (both on the device): offsets[n_groups + 1], order[n]. */
+int cllm_hip_group_rows_dev(const int32_t* ids, int n, int n_groups, int32_t* offsets,
+                            int32_t* order, void* stream);
+
+/* A router's choice of top_k (at most 32) of n_experts (at most 1024) for n_rows rows of fp32 logits
+ * (row i at logits + i * row_stride): the top_k largest keys, equal ones by the lower expert. An
+ * expert's score is the softmax of the row's logits, or (sigmoid != 0) 1 / (1 + exp(-logit)); its key is its
+ * logit, with bias ([n_experts], may be null) its score + bias, formed in 64 bits. n_groups > 1: the
+ * experts form n_groups (at most 64) equal groups of neighbours, and only those of the top_groups best
+ * can be chosen, a group's rank being that of its largest key, with bias of the sum of its two
+ * largest (equal ones by the lower group).
+ *   ids[i][j]      the j-th choice of row i; -1 where fewer experts are left: an expert whose logit is
+ *                  NaN or -inf is never chosen (nor one whose key is)
+ *   weights[i][j]  its score, normalise != 0: over the sum of the chosen scores (0 if that is 0), times
+ *                  scale; 0 for no expert. Infinite logits share a softmax between them.
+ *   offsets, order the n_rows * top_k entries grouped by expert: entry i * top_k + j has ids[i][j]. */
+int cllm_hip_moe_route_dev(const float* logits, int64_t row_stride, const float* bias, int n_rows,
+                           int n_experts, int top_k, int sigmoid, int normalise, float scale,
+                           int n_groups, int top_groups, int32_t* ids, float* weights,
+                           int32_t* offsets, int32_t* order, void* stream);
+
+/* Products of rows with the matrices of their experts, over GGUF blocks of the six vec_dot types:
+ * w holds [n_experts][out_dim] rows of in_dim (the 3-d tensors of a GGUF file), 16-byte aligned. As in
+ * matmul_quant a row is quantized to Q8_0 (quantize_row_q8_0, bit for bit) before its products, which
+ * are those of the blocks' values, added up in fp32; a row with an infinity or a NaN gives NaN.
+ * Entry e has row e / per_row of x[n_rows][in_dim] and writes row e of y [n_rows * per_row][out_dim];
+ * entries of no expert leave their row as it is. bias ([n_experts][out_dim]) may be null.
+ * per_row is at most 32. ws: 16-byte aligned device scratch of cllm_hip_moe_matmul_ws_bytes bytes, free
+ * again when the call has run. */
+size_t cllm_hip_moe_matmul_ws_bytes(uint32_t type, int in_dim, int n_rows);
+int cllm_hip_moe_matmul_dev(uint32_t type, int in_dim, int out_dim, int n_experts, const void* w,
+                            const float* bias, const float* x, int n_rows, int per_row,
+                            const int32_t* offsets, const int32_t* order, float* y, void* ws,
+                            size_t ws_bytes, void* stream);
+
+/* The gate and up projections of the chosen experts and the product after them
+ * (src/core/engine.cpp:509-512 for each entry): h[e] = silu(gate) * up, silu(v) = v / (1 + exp(-v)), with
+ * gate and up entry e's products as above; h is [n_rows * top_k][n_ff], entry i * top_k + j in row i's
+ * j-th place. ws: cllm_hip_moe_matmul_ws_bytes(type, in_dim, n_rows) bytes. */
+int cllm_hip_moe_swiglu_dev(uint32_t type, int in_dim, int n_ff, int n_experts, const void* w_gate,
+                            const void* w_up, const float* bias_gate, const float* bias_up,
+                            const float* x, int n_rows, int top_k, const int32_t* offsets,
+                            const int32_t* order, float* h, void* ws, size_t ws_bytes, void* stream);
+
+/* The down projection and the sum over a row's experts: y[i] = (base[i] +) the sum over j of
+ * weights[i][j] * (entry's product with row i * top_k + j of h, + bias), in the order of j, the j without an
+ * expert left out. ids and weights as the router's, offsets and order of the same ids. base
+ * ([n_rows][out_dim], the residual) may be null, or y. At most 65535 rows. */
+size_t cllm_hip_moe_down_ws_bytes(uint32_t type, int n_ff, int out_dim, int n_rows, int top_k);
+int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, const void* w,
+                          const float* bias, const float* h, int n_rows, int top_k,
+                          const int32_t* ids, const float* weights, const int32_t* offsets,
+                          const int32_t* order, const float* base, float* y, void* ws,
+                          size_t ws_bytes, void* stream);
+
+/* The kernel and launch plan of the experts' products of n_entries entries (n_mats 2: gate and up);
+ * "none" for an unsupported shape. For tests and benchmarks. */
+const char* cllm_hip_moe_plan(uint32_t type, int n_mats, int in_dim, int out_dim, int n_experts,
+                              int n_entries);
+
+/* Low-rank adapters added to 1 to 4 projections of the same rows (q, k and v; gate and up):
+ * y[i][r] = base[i][r] + scales[s] * B_i,s (A_i,s x[r]) for a row r of adapter s, base[i][r] for a row of none.
+ * a[i] holds [n_adapters][max_rank][in_dim], b[i] [n_adapters][out_dims[i]][max_rank] values of type F16 or F32
+ * (lora_a and lora_b of an adapter file), n_adapters at most 1023, max_rank a multiple of 4 up to 256,
+ * in_dim a multiple of 4; a, b, out_dims, base and y are host arrays of n_mats. Adapter s has rank
+ * ranks[s] (device; null: max_rank; held to 0 .. max_rank): what stands past it is not used. scales
+ * (device) null: 1. Rows are grouped by adapter (cllm_hip_group_rows_dev, once for a batch). All sums are fp32.
+ * base (null: zeros) or its entries may be null, or the entry of y. ws: 16-byte aligned device scratch of
+ * cllm_hip_lora_ws_bytes bytes, free again when the call has run. */
+size_t cllm_hip_lora_ws_bytes(int in_dim, int n_mats, int n_adapters, int max_rank, int n_rows);
+int cllm_hip_lora_dev(uint32_t type, int in_dim, int n_mats, const void* const* a,
+                      const void* const* b, const int* out_dims, int n_adapters, int max_rank,
+                      const int32_t* ranks, const float* scales, const float* x, int n_rows,
+                      const int32_t* offsets, const int32_t* order, const float* const* base,
+                      float* const* y, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- GGUF files ------------------------------------------------------------------------ */
 
 /* A GGUF file mapped read-only, parsed like GgufLoader::load (src/core/gguf.cpp:122-275):
