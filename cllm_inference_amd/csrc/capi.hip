@@ -1971,8 +1971,10 @@ int check_experts(const char* who, uint32_t type, int in_dim, int out_dim, int n
         return set_err(CLLM_HIP_E_ARG, "%s: 1 to %d experts of a row", who, kMaxRouteTopK);
     const int64_t entries = (int64_t)n_rows * per_row;
     // 32-bit offsets of the activation operand, and workgroups counted in 32 bits of threads
-    const int64_t act = (int64_t)std::max((int64_t)n_rows, entries) * ((in_dim + 255) / 256) * 1024;
+    const int64_t act = (int64_t)std::max((int64_t)n_rows, entries) * (((in_dim + 255) / 256) * 1024 + 256);
     const int64_t grid = (entries / 16 + n_experts + 1) * ((out_dim + 15) / 16 + 1);
+    if ((int64_t)out_dim * (int64_t)row_bytes(type, in_dim) >= (1ll << 32))
+        return set_err(CLLM_HIP_E_ARG, "%s: an expert's matrix of 4 GiB and more", who);
     if (act >= (1ll << 32) || grid > UINT32_MAX / 512 || entries > (1 << 28))
         return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
     return CLLM_HIP_OK;

@@ -34,10 +34,12 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // ---- the activation operand -----------------------------------------------------------------
-// Row r: chunks of 256 elements, each [step 8][hi, lo][g 4][8 fp16] (16-byte fragments), 1024 bytes;
-// then (K-quants with minima) [chunk][3 parts and zeros][8 blocks] fp16, 64 bytes a chunk; then the rows'
-// exponents. Fragment (step s, g) holds elements
-//   Q4_K, Q5_K  64 g + 8 s + e                    (lane g: the 32 quant bytes of blocks 2g and 2g + 1)
+// Row r: chunks of 256 elements, 1024 bytes of 16-byte fragments (8 fp16: step s, lane group g, hi or lo):
+//   K-quants          [g / 2][s 8][hi, lo][g % 2], so that half a super-block is 512 bytes
+//   blocks of 32      [s 8][hi, lo][g 4]
+// and 256 bytes more; then (K-quants with minima) [row][chunk][3 parts and zeros][8 blocks] fp16, 64 bytes a
+// chunk; then the rows' exponents. Fragment (s, g) holds elements
+//   Q4_K, Q5_K  64 g + 8 s + e                    (lane group g: the 32 quant bytes of blocks 2g, 2g + 1)
 //   Q6_K        128 (g / 2) + 32 (s / 2) + 16 (g % 2) + 8 (s % 2) + e
 //   Q8_0        32 s + 8 g + e
 //   Q4_0, Q5_0  32 s + 4 g + e (e < 4), 32 s + 16 + 4 g + e - 4 (e >= 4)
@@ -61,11 +63,15 @@ struct Act {
     int chunks;
 };
 int chunks_of(int k) { return (k + 255) / 256; }
+// (An odd multiple of 256 bytes: workgroups read the same place of many rows at once, and with rows a
+// power of two apart those are in one or two of an L2's 16 channels. 2048 rows of 4096 on 8 experts of
+// 14336, gate and up: 3510 us without, @@ with it.)
+uint32_t row_of(int chunks) { return (uint32_t)chunks * 1024u + 256u; }
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 Act act_of(void* ws, uint32_t type, int k, int rows) {
     Act a;
     a.chunks = chunks_of(k);
-    a.row = (uint32_t)a.chunks * 1024u;
+    a.row = row_of(a.chunks);
     uint8_t* p = (uint8_t*)ws;
     a.frags = p;
     p += (size_t)rows * a.row;
@@ -148,13 +154,14 @@ __global__ __launch_bounds__(THREADS) void k_expert_act(const float* __restrict_
             } else {
                 s = b, g = p;
             }
-            uint8_t* at = ch + s * 128 + g * 16;
+            constexpr int LO = O == kByte ? 64 : 32;
+            uint8_t* at = ch + (O == kByte ? s * 128 + g * 16 : (g >> 1) * 512 + s * 64 + (g & 1) * 16);
             if constexpr (O == kMin64) {
                 *(wh8*)at = wh8{h[0], h[2], h[1], h[3], h[4], h[6], h[5], h[7]};
-                *(wh8*)(at + 64) = wh8{l[0], l[2], l[1], l[3], l[4], l[6], l[5], l[7]};
+                *(wh8*)(at + LO) = wh8{l[0], l[2], l[1], l[3], l[4], l[6], l[5], l[7]};
             } else {
                 *(wh8*)at = wh8{h[0], h[1], h[2], h[3], h[4], h[5], h[6], h[7]};
-                *(wh8*)(at + 64) = wh8{l[0], l[1], l[2], l[3], l[4], l[5], l[6], l[7]};
+                *(wh8*)(at + LO) = wh8{l[0], l[1], l[2], l[3], l[4], l[5], l[6], l[7]};
             }
         }
         if constexpr (O == kMin64) {
@@ -208,97 +215,85 @@ __device__ __forceinline__ void k4_scales2(const u32x4& hdr, int g, float& s0, f
     s1 = (float)((s >> 8) & 0xFFu);
 }
 
-template <uint32_t T>
-struct Unit;
-
-template <>
-struct Unit<T_Q4_K> {
-    static constexpr int BYTES = Q4_K_BYTES;
-    u32x4 hdr, q[2];
+// Lane group g of a super-block: its own bytes (Part) and, with minima, the row's header (16 bytes).
+struct Scales2 {  // of blocks 2g and 2g + 1
     wh2 s0, c0, s1, c1;
+};
+
+template <uint32_t T>
+struct Part;
+template <>
+struct Part<T_Q4_K> {
+    static constexpr int BYTES = Q4_K_BYTES;
+    u32x4 q[2];
     __device__ __forceinline__ void load(const uint8_t* p, int g) {
-        hdr = ld_u32x4(p);
-        q[0] = ld_u32x4(p + 16 + 32 * g);
-        q[1] = ld_u32x4(p + 32 + 32 * g);
+        q[0] = ld_u32x4(p + Q4_K_QS + 32 * g);
+        q[1] = ld_u32x4(p + Q4_K_QS + 32 * g + 16);
     }
-    __device__ __forceinline__ void ready(int g) {
+    static __device__ __forceinline__ Scales2 scale(const u32x4& hdr, int g) {
         float a, b;
         k4_scales2(hdr, g, a, b);
-        s0 = both(a), c0 = both(-1024.0f * a);
-        s1 = both(b * 0.0625f), c1 = both(-64.0f * b);
+        return Scales2{both(a), both(-1024.0f * a), both(b * 0.0625f), both(-64.0f * b)};
     }
-    __device__ __forceinline__ wh8 frag(int s) const {
+    __device__ __forceinline__ wh8 frag(const Scales2& c, int s, int) const {
         const uint32_t a = q[(s & 3) >> 1][2 * (s & 1)], b = q[(s & 3) >> 1][2 * (s & 1) + 1];
         const uint32_t m = s < 4 ? 0x000F000Fu : 0x00F000F0u, o = 0x64006400u;
-        const wh2 k = s < 4 ? s0 : s1, c = s < 4 ? c0 : c1;
-        return cat(__builtin_elementwise_fma(as_h2((a & m) | o), k, c),
-                   __builtin_elementwise_fma(as_h2(((a >> 8) & m) | o), k, c),
-                   __builtin_elementwise_fma(as_h2((b & m) | o), k, c),
-                   __builtin_elementwise_fma(as_h2(((b >> 8) & m) | o), k, c));
+        const wh2 k = s < 4 ? c.s0 : c.s1, z = s < 4 ? c.c0 : c.c1;
+        return cat(__builtin_elementwise_fma(as_h2((a & m) | o), k, z),
+                   __builtin_elementwise_fma(as_h2(((a >> 8) & m) | o), k, z),
+                   __builtin_elementwise_fma(as_h2((b & m) | o), k, z),
+                   __builtin_elementwise_fma(as_h2(((b >> 8) & m) | o), k, z));
     }
-    __device__ __forceinline__ float d() const { return f16_to_f32(hdr.x & 0xFFFFu); }
-    __device__ __forceinline__ float dmin() const { return f16_to_f32(hdr.x >> 16); }
-    __device__ __forceinline__ wh8 minima() const { return k4_minima(hdr); }
 };
 
 template <>
-struct Unit<T_Q5_K> {
+struct Part<T_Q5_K> {
     static constexpr int BYTES = Q5_K_BYTES;
-    u32x4 hdr, q[2], h[2];
-    wh2 s0, c0, s1, c1;
-    int k;  // the first block's bit of h
+    u32x4 q[2], h[2];
     __device__ __forceinline__ void load(const uint8_t* p, int g) {
-        hdr = ld_u32x4(p);
-        h[0] = ld_u32x4(p + 16);
-        h[1] = ld_u32x4(p + 32);
-        q[0] = ld_u32x4(p + 48 + 32 * g);
-        q[1] = ld_u32x4(p + 64 + 32 * g);
+        h[0] = ld_u32x4(p + Q5_K_QH);
+        h[1] = ld_u32x4(p + Q5_K_QH + 16);
+        q[0] = ld_u32x4(p + Q5_K_QS + 32 * g);
+        q[1] = ld_u32x4(p + Q5_K_QS + 32 * g + 16);
     }
-    __device__ __forceinline__ void ready(int g) {
+    static __device__ __forceinline__ Scales2 scale(const u32x4& hdr, int g) {
         float a, b;
         k4_scales2(hdr, g, a, b);
-        s0 = both(a), c0 = both(-1024.0f * a);
-        s1 = both(b), c1 = both(-1024.0f * b);
-        k = 2 * g;
+        return Scales2{both(a), both(-1024.0f * a), both(b), both(-1024.0f * b)};
     }
-    __device__ __forceinline__ wh8 frag(int s) const {
+    __device__ __forceinline__ wh8 frag(const Scales2& c, int s, int g) const {
+        const int hi = s >> 2;  // block 2g + hi
+        const wh2 m = hi ? c.s1 : c.s0, z = hi ? c.c1 : c.c0;
         wh2 f[4];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const uint32_t n = q[(s & 3) >> 1][2 * (s & 1) + j], b = h[(s & 3) >> 1][2 * (s & 1) + j];
-            const uint32_t v = ((s < 4 ? n : n >> 4) & 0x0F0F0F0Fu) | (((b >> (k + (s >> 2))) & 0x01010101u) << 4);
-            const wh2 m = s < 4 ? s0 : s1, c = s < 4 ? c0 : c1;
-            f[2 * j] = __builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(0x64646464u, v, 0x04020400u)), m, c);
-            f[2 * j + 1] = __builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(0x64646464u, v, 0x04030401u)), m, c);
+            const uint32_t v = ((hi ? n >> 4 : n) & 0x0F0F0F0Fu) | (((b >> (2 * g + hi)) & 0x01010101u) << 4);
+            f[2 * j] = __builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(0x64646464u, v, 0x04020400u)), m, z);
+            f[2 * j + 1] = __builtin_elementwise_fma(as_h2(__builtin_amdgcn_perm(0x64646464u, v, 0x04030401u)), m, z);
         }
         return cat(f[0], f[1], f[2], f[3]);
     }
-    __device__ __forceinline__ float d() const { return f16_to_f32(hdr.x & 0xFFFFu); }
-    __device__ __forceinline__ float dmin() const { return f16_to_f32(hdr.x >> 16); }
-    __device__ __forceinline__ wh8 minima() const { return k4_minima(hdr); }
 };
 
 template <>
-struct Unit<T_Q6_K> {
+struct Part<T_Q6_K> {
     static constexpr int BYTES = Q6_K_BYTES;
     u32x4 l[2], h;
     u32x2 sc;
     uint32_t db;
-    int u;
     __device__ __forceinline__ void load(const uint8_t* p, int g) {
-        const int n = g >> 1;
-        u = g & 1;
+        const int n = g >> 1, u = g & 1;
         l[0] = ld_any<16, u32x4>(p + 64 * n + 16 * u);
         l[1] = ld_any<16, u32x4>(p + 64 * n + 32 + 16 * u);
         h = ld_any<16, u32x4>(p + Q6_K_QH + 32 * n + 16 * u);
         sc = ld_any<8, u32x2>(p + Q6_K_SC + 8 * n);
         db = ld_u16(p + Q6_K_D);
     }
-    __device__ __forceinline__ void ready(int) {}
     // scale * (q - 32): the fp16 rounding and the rest, exact
-    __device__ __forceinline__ wh8 frag(int s, wh8& rest) const {
+    __device__ __forceinline__ wh8 frag(int s, int g, wh8& rest) const {
         const int i = s >> 1;
-        const wh2 m = both((float)(int8_t)((sc[i >> 1] >> (16 * (i & 1) + 8 * u)) & 0xFFu));
+        const wh2 m = both((float)(int8_t)(sc[i >> 1] >> (16 * (i & 1) + 8 * (g & 1))));
         const wh2 off = both(-1056.0f);
         wh2 f[4], r[4];
 #pragma unroll
@@ -341,6 +336,8 @@ __device__ __forceinline__ wh8 five8(uint32_t v, uint32_t qh, int g) {
                as_h2(__builtin_amdgcn_perm(0x64646464u, b, 0x04030401u)) + c);
 }
 
+template <uint32_t T>
+struct Unit;
 template <>
 struct Unit<T_Q8_0> {
     static constexpr int BYTES = Q8_0_BYTES;
@@ -372,6 +369,48 @@ struct Unit<T_Q5_0> {
         db = ld_u16(p);
     }
     __device__ __forceinline__ wh8 frag(int g) const { return five8(q, h, g); }
+};
+
+// Lane groups 2h and 2h + 1 of one block.
+template <uint32_t T>
+struct Pair;
+template <>
+struct Pair<T_Q8_0> {
+    u32x4 q;
+    uint32_t db;
+    __device__ __forceinline__ void load(const uint8_t* p, int h) {
+        q = ld_any<16, u32x4>(p + 2 + 16 * h);
+        db = ld_u16(p);
+    }
+    __device__ __forceinline__ wh8 frag(int i, int) const {
+        return __builtin_bit_cast(wh8, i ? int8x8_to_h8(q.z, q.w) : int8x8_to_h8(q.x, q.y));
+    }
+};
+template <>
+struct Pair<T_Q4_0> {
+    u32x2 q;
+    uint32_t db;
+    __device__ __forceinline__ void load(const uint8_t* p, int h) {
+        q = ld_any<8, u32x2>(p + 2 + 8 * h);
+        db = ld_u16(p);
+    }
+    __device__ __forceinline__ wh8 frag(int i, int) const { return nibbles8(i ? q.y : q.x, -8.0f); }
+};
+template <>
+struct Pair<T_Q5_0> {
+    u32x2 q;
+    uint32_t h5, db;
+    __device__ __forceinline__ void load(const uint8_t* p, int h) {
+        q = ld_any<8, u32x2>(p + 6 + 8 * h);
+        h5 = ld_any<4, uint32_t>(p + 2);
+        db = ld_u16(p);
+    }
+    __device__ __forceinline__ wh8 frag(int i, int h) const { return five8(i ? q.y : q.x, h5, 2 * h + i); }
+};
+
+template <uint32_t T>
+struct Bytes {
+    static constexpr uint32_t V = T == T_Q4_K ? Q4_K_BYTES : Q5_K_BYTES;
 };
 
 struct Mul {
@@ -417,7 +456,7 @@ __global__ __launch_bounds__(64 * KP) void k_expert_rows(Mul a) {
         ent[r] = e;
         exps[r] = a.act.exps[arow];
     }
-    const uint8_t* ap = a.act.frags + (size_t)arow * a.act.row + 16 * g;
+    const uint8_t* ap = a.act.frags + (size_t)arow * a.act.row + (is_kq(T) ? (g >> 1) * 512 + (g & 1) * 16 : 16 * g);
     const uint8_t* wp[NT];
     const int n0 = blk * (SWIGLU ? 16 : 16 * NT);
 #pragma unroll
@@ -430,41 +469,46 @@ __global__ __launch_bounds__(64 * KP) void k_expert_rows(Mul a) {
     for (int i = 0; i < NT; ++i) acc[i] = zero;
     for (int c = wave; c < a.act.chunks; c += KP) {
         if constexpr (is_kq(T)) {
-            Unit<T> u[NT];
+            u32x4 hdr[NT];
+            Part<T> pt[NT];
 #pragma unroll
-            for (int i = 0; i < NT; ++i) u[i].load(wp[i] + (size_t)c * Unit<T>::BYTES, g);
+            for (int i = 0; i < NT; ++i) {
+                const uint8_t* p = wp[i] + (size_t)c * Part<T>::BYTES;
+                if constexpr (has_min(T)) hdr[i] = ld_u32x4(p);
+                pt[i].load(p, g);
+            }
             wh8 ah[8], al[8], am;
 #pragma unroll
             for (int s = 0; s < 8; ++s) {
-                ah[s] = *(const wh8*)(ap + (size_t)c * 1024 + s * 128);
-                al[s] = *(const wh8*)(ap + (size_t)c * 1024 + s * 128 + 64);
+                const uint8_t* at = ap + (size_t)c * 1024 + s * 64;
+                ah[s] = *(const wh8*)at;
+                al[s] = *(const wh8*)(at + 32);
             }
             if constexpr (has_min(T)) am = *(const wh8*)(a.act.mins + ((size_t)arow * a.act.chunks + c) * 64 + 16 * g);
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                u[i].ready(g);
+                Scales2 sc;
+                if constexpr (has_min(T)) sc = Part<T>::scale(hdr[i], g);
                 f32x4 sum = zero;
 #pragma unroll
                 for (int s = 0; s < 8; ++s) {
-                    if constexpr (T == T_Q6_K) {
-                        wh8 rest;
-                        const wh8 f = u[i].frag(s, rest);
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], f, sum, 0, 0, 0);
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], f, sum, 0, 0, 0);
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], rest, sum, 0, 0, 0);
-                    } else {
-                        const wh8 f = u[i].frag(s);
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], f, sum, 0, 0, 0);
-                        sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], f, sum, 0, 0, 0);
-                    }
+                    wh8 rest, f;
+                    if constexpr (T == T_Q6_K)
+                        f = pt[i].frag(s, g, rest);
+                    else
+                        f = pt[i].frag(sc, s, g);
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], f, sum, 0, 0, 0);
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], f, sum, 0, 0, 0);
+                    if constexpr (T == T_Q6_K) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], rest, sum, 0, 0, 0);
                 }
-                const float d = u[i].d();
                 if constexpr (has_min(T)) {
-                    const f32x4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(am, u[i].minima(), zero, 0, 0, 0);
-                    const float dm = -(float)(1 << kMinShift) * u[i].dmin();
+                    const float d = f16_to_f32(hdr[i].x & 0xFFFFu);
+                    const f32x4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(am, k4_minima(hdr[i]), zero, 0, 0, 0);
+                    const float dm = -(float)(1 << kMinShift) * f16_to_f32(hdr[i].x >> 16);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], fmaf(dm, m[j], acc[i][j]));
                 } else {
+                    const float d = pt[i].d();
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], acc[i][j]);
                 }
@@ -524,18 +568,19 @@ __global__ __launch_bounds__(64 * KP) void k_expert_rows(Mul a) {
 }
 
 // ---- many rows to an expert ----------------------------------------------------------------------
-// 32 MT entries of an expert and 256 weight rows (128 of gate and of up): four waves of 64 weight rows
-// (two 32-column MFMA tiles, gate and up of the same rows, or 64 rows) against all entries. The waves
-// share the activation fragments, which reach LDS in stages of half a chunk, two buffers, by
-// direct-to-LDS loads; each wave reads and unpacks its own weight rows, a chunk ahead, in registers.
+// BM entries of an expert and 256 weight rows (128 of gate and of up): WM x 4 waves of 32 MT entries x 64 weight
+// rows (two 32-column MFMA tiles, gate and up of the same rows, or 64 rows). The waves share the activation
+// fragments, which reach LDS in stages of half a chunk, two buffers, by direct-to-LDS loads; each wave
+// loads and unpacks its weight rows' bytes a stage ahead in registers (with minima, the rows' headers in LDS).
 // LDS: [entry][32 fragments of 16 bytes], fragment f of entry i in place f ^ (i % 32), so that the 32
 // entries' reads of one fragment fall on distinct banks.
-template <int MT>
+template <int WM, int MT>
 struct Wide {
-    static constexpr int BM = 32 * MT;
-    static constexpr int FRAGS = BM * 512, MINS = BM * 64;
-    static constexpr int STAGE = FRAGS + MINS;
-    static constexpr int LDS = 2 * STAGE;
+    static constexpr int BM = 32 * MT * WM;
+    static constexpr int THREADS = 256 * WM;
+    static constexpr int FRAGS = BM * 512;                       // a stage's fragments, two buffers
+    static constexpr int MINS = 2 * FRAGS, HDRS = MINS + BM * 64;  // minima of a chunk; headers, two buffers
+    static constexpr int LDS = HDRS + 2 * 256 * 16;
 };
 
 __device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint32_t m0) {
@@ -543,175 +588,266 @@ __device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint
                  : : "v"(off), "s"(base), "s"(m0) : "memory", "m0");
 }
 
-template <uint32_t T, int MT, bool SWIGLU>
-__global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
-    using C = Wide<MT>;
+template <uint32_t T, int WM, int MT, bool SWIGLU>
+__global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
+    using C = Wide<WM, MT>;
     constexpr int NT = 2;
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int ent[C::BM], exps[C::BM];
+    __shared__ uint32_t from_a[C::BM], from_m[C::BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 2, wn = wave & 3;
     const int blk = blockIdx.x % a.n_blocks;
     const GroupTile t = find_tile<C::BM>(a.g, 0, blockIdx.x / a.n_blocks, lane);
     if (t.count <= 0) return;
     const int r = lane & 31, h = lane >> 5;
-    for (int i = threadIdx.x; i < C::BM; i += 256) {
+    for (int i = threadIdx.x; i < C::BM; i += C::THREADS) {
         const int e = entry_of(a, t, i);
+        const uint32_t row = (uint32_t)(e < 0 ? 0 : e / a.per_row);
         ent[i] = e;
-        exps[i] = a.act.exps[e < 0 ? 0 : e / a.per_row];
+        exps[i] = a.act.exps[row];
+        from_a[i] = row * a.act.row;
+        from_m[i] = row * (uint32_t)(a.act.chunks * 64);
     }
-    // sources of this wave's direct-to-LDS loads: BM / 2 loads of two entries a stage
-    constexpr int AL = C::BM / 8;
-    uint32_t a_off[AL];
+    __syncthreads();
+    const uint8_t* wbase[2];
+    uint32_t w_at[NT];  // this lane's rows
+    const int n0 = blk * (SWIGLU ? 128 : 256) + wn * (SWIGLU ? 32 : 64);
 #pragma unroll
-    for (int j = 0; j < AL; ++j) {
-        const int i = 2 * (4 * j + wave) + h;
-        const int e = entry_of(a, t, i);
-        a_off[j] = (uint32_t)(e < 0 ? 0 : e / a.per_row) * a.act.row + 16u * (uint32_t)(r ^ (i & 31));
-    }
-    // the minima's: 16 entries a load, place q of entry i holds part q ^ (i / 2 % 4)
-    const int mi = 16 * wave + (lane >> 2);
-    uint32_t m_off = 0;
-    if (has_min(T) && mi < C::BM) {
-        const int e = entry_of(a, t, mi);
-        m_off = (uint32_t)(e < 0 ? 0 : e / a.per_row) * (uint32_t)(a.act.chunks * 64) +
-                16u * (uint32_t)((lane & 3) ^ ((mi >> 1) & 3));
+    for (int i = 0; i < NT; ++i) {
+        wbase[i] = a.w[SWIGLU ? i : 0] + (size_t)t.group * a.expert_bytes;
+        w_at[i] = (uint32_t)min(n0 + (SWIGLU ? 0 : 32 * i) + r, a.n - 1) * a.row_bytes;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)lds;
+    // this wave's direct-to-LDS loads of a stage: two entries each; of the minima's 16, place q of entry i
+    // holds part q ^ (i / 2 % 4)
     auto issue = [&](int st, int buf) {
-        const uint32_t to = lds0 + (uint32_t)buf * C::STAGE;
+        const uint32_t to = lds0 + (uint32_t)buf * C::FRAGS;
         const uint8_t* from = a.act.frags + (size_t)st * 512;
 #pragma unroll
-        for (int j = 0; j < AL; ++j) to_lds16(from, a_off[j], to + 1024u * (uint32_t)(4 * j + wave));
-        if (has_min(T) && (st & 1) && 16 * wave < C::BM)
-            to_lds16(a.act.mins + (size_t)(st >> 1) * 64, m_off, to + C::FRAGS + 1024u * (uint32_t)wave);
-    };
-
-    const int n0 = blk * (SWIGLU ? 128 : 256) + wave * (SWIGLU ? 32 : 64);
-    const uint8_t* wp[NT];
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-        wp[i] = a.w[SWIGLU ? i : 0] + (size_t)t.group * a.expert_bytes +
-                (size_t)min(n0 + (SWIGLU ? 0 : 32 * i) + r, a.n - 1) * a.row_bytes;
-
-    wf16 acc[NT][MT], sum[NT][MT];
-    const wf16 zero = {};
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[i][m] = sum[i][m] = zero;
-
-    const int stages = 2 * a.act.chunks;
-    Unit<T> nxt[NT][2];
-    auto load_chunk = [&](int c) {
-        if constexpr (is_kq(T)) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int q = 0; q < 2; ++q) nxt[i][q].load(wp[i] + (size_t)c * Unit<T>::BYTES, 2 * h + q);
+        for (int j = 0; j < C::BM / (8 * WM); ++j) {
+            const int k = 4 * WM * j + wave, i = 2 * k + h;
+            to_lds16(from, from_a[i] + 16u * (uint32_t)(r ^ (i & 31)), to + 1024u * (uint32_t)k);
+        }
+        if (has_min(T) && (st & 1) && 16 * wave < C::BM) {
+            const int i = 16 * wave + (lane >> 2);
+            to_lds16(a.act.mins + (size_t)(st >> 1) * 64, from_m[i] + 16u * (uint32_t)((lane & 3) ^ ((i >> 1) & 3)),
+                     lds0 + C::MINS + 1024u * (uint32_t)wave);
+        }
+        // the headers of the next chunk: lanes 0-31 the wave's first tile's rows, 32-63 the second's
+        if (has_min(T) && !(st & 1) && wm == 0) {
+            const uint8_t* b = SWIGLU && h ? wbase[1] : wbase[0];
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                         : : "v"(b + (h ? w_at[1] : w_at[0]) + (size_t)(st >> 1) * Bytes<T>::V),
+                             "s"(lds0 + C::HDRS + 4096u * (uint32_t)((st >> 1) & 1) + 1024u * (uint32_t)wn)
+                         : "memory", "m0");
         }
     };
-    issue(0, 0);
-    load_chunk(0);
-    Unit<T> u[NT][2];
-    auto stage = [&]<int HALF>(int st) {
-        const uint8_t* cur = lds + HALF * C::STAGE;
+
+    const int stages = 2 * a.act.chunks;
+    const wf16 zero = {};
+    wf16 acc[NT][MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[i][m] = zero;
+    // fragment (s, part) of lane half h of the wave's entry 32 m + r: a_at ^ 16 (4 s + 2 part), plus 16384 m
+    // (blocks of 32: (block, part, 2 h + q) at a_at ^ 16 (8 block + 4 part + q))
+    const uint32_t a_at = (uint32_t)(wm * 32 * MT * 512 + r * 512 + 16 * (r ^ (is_kq(T) ? h : 2 * h)));
+    auto begin = [&](int st, int half) {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's loads of the stage are in LDS
         asm volatile("" ::: "memory");
         __syncthreads();                     // and every wave's; the other buffer is free
-        if (st + 1 < stages) issue(st + 1, 1 - HALF);
-        if constexpr (is_kq(T)) {
-            if constexpr (HALF == 0) {
+        if (st + 1 < stages) issue(st + 1, 1 - half);
+    };
+    issue(0, 0);
+
+    if constexpr (is_kq(T)) {
+        // A stage is 8 steps: 16 elements of K, the 8 of lane half h from lane group g = 2 HALF + h. A step's MFMAs
+        // run beside the unpacking of the next; its lo fragments are read beside the products with hi, the
+        // next step's hi beside those with lo. Weight bytes are loaded a stage ahead, like the activations.
+        constexpr int PARTS = T == T_Q6_K ? 3 : 2;
+        constexpr bool AHEAD = T == T_Q4_K;  // (registers)
+        Part<T> pt[AHEAD ? 2 : 1][NT];
+        wf16 sum[NT][MT];
+        wh8 ah[MT], al[MT], bf[2][NT], rest[2][NT];
+        Scales2 sc[NT];
+        auto load_part = [&](int st, int half) {
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+            for (int i = 0; i < NT; ++i)
+                pt[AHEAD ? half : 0][i].load(wbase[i] + (size_t)(st >> 1) * Part<T>::BYTES + w_at[i], 2 * half + h);
+        };
+        auto stage = [&]<int HALF>(int st) {
+            begin(st, HALF);
+            if (AHEAD && st + 1 < stages) load_part(st + 1, 1 - HALF);
+            const uint8_t* cur = lds + HALF * C::FRAGS;
+            const int g = 2 * HALF + h;
+            const uint8_t* hdr = lds + C::HDRS + 4096 * ((st >> 1) & 1) + 1024 * wn + 16 * r;
+            auto read_a = [&](int p, int part, wh8 (&to)[MT]) {
+                const uint8_t* from = cur + (a_at ^ (uint32_t)(16 * (4 * p + 2 * part)));
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) u[i][q] = nxt[i][q], u[i][q].ready(2 * h + q);
-            } else {
-                if (st + 1 < stages) load_chunk((st + 1) >> 1);
-            }
-        }
-        Unit<T> ub[4][NT][2];
-        if constexpr (!is_kq(T)) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s)
-#pragma unroll
-                for (int i = 0; i < NT; ++i)
-#pragma unroll
-                    for (int q = 0; q < 2; ++q)
-                        ub[s][i][q].load(wp[i] + (size_t)min(4 * st + s, a.nb - 1) * Unit<T>::BYTES, 2 * h + q);
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                wh8 f[NT], rest[NT], ah[MT], al[MT];
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const uint8_t* row = cur + (32 * m + r) * 512;
-                    ah[m] = *(const wh8*)(row + 16 * ((8 * s + 2 * h + q) ^ r));
-                    al[m] = *(const wh8*)(row + 16 * ((8 * s + 4 + 2 * h + q) ^ r));
-                }
+                for (int m = 0; m < MT; ++m) to[m] = *(const wh8*)(from + 16384 * m);
+            };
+            auto unpack = [&](int p) {
 #pragma unroll
                 for (int i = 0; i < NT; ++i) {
+                    if constexpr (has_min(T))
+                        if (p == 0) sc[i] = Part<T>::scale(*(const u32x4*)(hdr + 512 * i), g);
                     if constexpr (T == T_Q6_K)
-                        f[i] = u[i][q].frag(4 * HALF + s, rest[i]);
-                    else if constexpr (is_kq(T))
-                        f[i] = u[i][q].frag(4 * HALF + s);
+                        bf[p & 1][i] = pt[AHEAD ? HALF : 0][i].frag(p, g, rest[p & 1][i]);
                     else
-                        f[i] = ub[s][i][q].frag(2 * h + q);
+                        bf[p & 1][i] = pt[AHEAD ? HALF : 0][i].frag(sc[i], p, g);
+                }
+            };
+            float dq[NT];
+            read_a(0, 0, ah);
+            unpack(0);
+#pragma unroll
+            for (int p = 0; p < 8; ++p) {
+                __builtin_amdgcn_sched_barrier(0);
+                read_a(p, 1, al);
+                if (p < 7) unpack(p + 1);
+                if (!AHEAD && p == 7) {
+                    if constexpr (T == T_Q6_K) {
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) dq[i] = pt[0][i].d();
+                    }
+                    if (st + 1 < stages) load_part(st + 1, 1 - HALF);
                 }
 #pragma unroll
-                for (int i = 0; i < NT; ++i)
+                for (int part = 0; part < PARTS; ++part) {
+#pragma unroll
+                    for (int i = 0; i < NT; ++i)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m)
+                            sum[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                                part == PARTS - 1 ? al[m] : ah[m], PARTS == 3 && part == 1 ? rest[p & 1][i] : bf[p & 1][i],
+                                HALF == 0 && p == 0 && part == 0 ? zero : sum[i][m], 0, 0, 0);
+                    if (part == PARTS - 2 && p < 7) read_a(p + 1, 0, ah);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x100, MT, 0);  // lo of this step
+#pragma unroll
+                for (int g = 0; g < PARTS * NT * MT; ++g) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // an MFMA
+                    __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);  // unpacking beside it
+                    if (g == (PARTS - 1) * NT * MT - 1) __builtin_amdgcn_sched_group_barrier(0x100, MT, 0);  // the next hi
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (HALF == 1) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    float d, dm = 0.0f;
+                    wh8 mn;
+                    if constexpr (has_min(T)) {
+                        const u32x4 v = *(const u32x4*)(hdr + 512 * i);
+                        d = f16_to_f32(v.x & 0xFFFFu);
+                        dm = -(float)(1 << kMinShift) * f16_to_f32(v.x >> 16);
+                        mn = k4_minima(v);
+                    } else {
+                        d = dq[i];
+                    }
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
-                        const bool first = is_kq(T) ? HALF == 0 && s == 0 && q == 0 : q == 0;
-                        sum[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[m], f[i], first ? zero : sum[i][m], 0, 0, 0);
-                        sum[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(al[m], f[i], sum[i][m], 0, 0, 0);
-                        if constexpr (T == T_Q6_K)
-                            sum[i][m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah[m], rest[i], sum[i][m], 0, 0, 0);
-                    }
-            }
-            if constexpr (!is_kq(T)) {
-                const bool there = 4 * st + s < a.nb;
+                        if constexpr (has_min(T)) {
+                            const uint8_t* row = lds + C::MINS + (32 * MT * wm + 32 * m + r) * 64;
+                            wf16 f = zero;
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const float d = there ? f16_to_f32(ub[s][i][0].db) : 0.0f;
+                            for (int q = 0; q < 2; ++q) {
+                                const wh8 x = *(const wh8*)(row + 16 * ((2 * h + q) ^ ((r >> 1) & 3)));
+                                f = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, mn, f, 0, 0, 0);
+                            }
 #pragma unroll
-                    for (int m = 0; m < MT; ++m)
+                            for (int e = 0; e < 16; ++e)
+                                acc[i][m][e] = fmaf(d, sum[i][m][e], fmaf(dm, f[e], acc[i][m][e]));
+                        } else {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[i][m][e] = fmaf(d, sum[i][m][e], acc[i][m][e]);
-                }
-            }
-        }
-        if constexpr (is_kq(T)) if constexpr (HALF == 1) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const float d = u[i][0].d();
-#pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    if constexpr (has_min(T)) {
-                        const float dm = -(float)(1 << kMinShift) * u[i][0].dmin();
-                        const wh8 mn = u[i][0].minima();
-                        const uint8_t* row = cur + C::FRAGS + (32 * m + r) * 64;
-                        wf16 f = zero;
-#pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            const wh8 x = *(const wh8*)(row + 16 * ((2 * h + q) ^ ((r >> 1) & 3)));
-                            f = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, mn, f, 0, 0, 0);
+                            for (int e = 0; e < 16; ++e) acc[i][m][e] = fmaf(d, sum[i][m][e], acc[i][m][e]);
                         }
-#pragma unroll
-                        for (int e = 0; e < 16; ++e)
-                            acc[i][m][e] = fmaf(d, sum[i][m][e], fmaf(dm, f[e], acc[i][m][e]));
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) acc[i][m][e] = fmaf(d, sum[i][m][e], acc[i][m][e]);
+                        asm volatile("" : "+v"(acc[i][m]));  // not sunk to where the sums are read next
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
+        };
+        load_part(0, 0);
+        for (int st = 0; st < stages; st += 2) {
+            stage.template operator()<0>(st);
+            stage.template operator()<1>(st + 1);
         }
-    };
-    for (int st = 0; st < stages; st += 2) {
-        stage.template operator()<0>(st);
-        stage.template operator()<1>(st + 1);
+    } else {
+        // A stage is 4 blocks. Items (block, entry tile, weight tile): an item's four MFMAs run beside the
+        // multiplication with d of the item before it. Everything is read or unpacked into the registers
+        // that the items no longer need: a block's fragments an item or two ahead, a stage's weight
+        // bytes a stage ahead.
+        constexpr int N = NT * MT;
+        Pair<T> u[4][NT];
+        auto load_block = [&](int st, int s) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) u[s][i].load(wbase[i] + (size_t)min(4 * st + s, a.nb - 1) * Unit<T>::BYTES + w_at[i], h);
+        };
+#pragma unroll
+        for (int s = 0; s < 4; ++s) load_block(0, s);
+        auto stage = [&]<int HALF>(int st) {
+            begin(st, HALF);
+            const uint8_t* cur = lds + HALF * C::FRAGS;
+            wh8 af[2][2][2], bf[NT][2];  // [entry tile, or block parity][q][part]
+            float d[2][NT];
+            wf16 f[2];
+            auto read = [&](int s, int m) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+                        af[MT == 2 ? m : s & 1][q][part] =
+                            *(const wh8*)(cur + (a_at ^ (uint32_t)(16 * (8 * s + 4 * part + q))) + 16384 * m);
+            };
+            auto unpack = [&](int s, int i) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q) bf[i][q] = u[s][i].frag(q, h);
+                d[s & 1][i] = 4 * st + s < a.nb ? f16_to_f32(u[s][i].db) : 0.0f;
+            };
+            auto fold = [&](int it) {
+                const int s = it / N, m = it % N / NT, i = it % NT;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][m][e] = fmaf(d[s & 1][i], f[it & 1][e], acc[i][m][e]);
+                asm volatile("" : "+v"(acc[i][m]));  // not sunk to where the sums are read next
+            };
+            read(0, 0);
+            unpack(0, 0);
+#pragma unroll
+            for (int it = 0; it < 4 * N; ++it) {
+                const int s = it / N, m = it % N / NT, i = it % NT;
+                __builtin_amdgcn_sched_barrier(0);
+                if (it % N == 0) {
+                    if (MT == 2) read(s, 1);
+                    unpack(s, 1);
+                    if (MT == 1 && s < 3) read(s + 1, 0);
+                }
+                if (it % N == 1 && st + 1 < stages) load_block(st + 1, s);
+                if (MT == 2 && it % N == 2 && s < 3) read(s + 1, 0);
+                if (it % N == N - 1 && s < 3) unpack(s + 1, 0);
+                wf16 z = zero;
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+                        z = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[MT == 2 ? m : s & 1][q][part], bf[i][q], z, 0, 0, 0);
+                f[it & 1] = z;
+                if (it > 0) fold(it - 1);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x002, 8, 0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            fold(4 * N - 1);
+        };
+        for (int st = 0; st < stages; st += 2) {
+            stage.template operator()<0>(st);
+            stage.template operator()<1>(st + 1);
+        }
     }
 
     // lane (r, h) has entries 8 (e / 4) + 4 h + e % 4 of weight row r of each tile
@@ -725,7 +861,7 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int tok = 32 * m + 8 * (e >> 2) + 4 * h + (e & 3);
+                const int tok = 32 * MT * wm + 32 * m + 8 * (e >> 2) + 4 * h + (e & 3);
                 const int en = ent[tok];
                 if (en < 0) continue;
                 float v = unscaled(acc[i][m][e], exps[tok]) + b0;
@@ -782,17 +918,18 @@ hipError_t act_launch(const ExpertArgs& a, const Act& act, hipStream_t s) {
 }
 
 struct Plan {
-    int wide;  // entries of a tile: 32 or 64, 0: k_expert_rows
+    int wide;  // entries of a tile: 32, 64 or 128; 0: k_expert_rows
     int kp;
     int n_blocks, tiles;
 };
 Plan plan_of(int mats, int k, int n, int groups, int entries) {
     Plan p{};
-    const int per = (entries + std::min(groups, entries) - 1) / std::max(1, std::min(groups, entries));
+    const int live = std::max(1, std::min(groups, entries)), per = (entries + live - 1) / live;
     p.wide = per <= 12 ? 0 : per <= 48 ? 32 : 64;
     if (p.wide) {
         p.n_blocks = (n + (mats == 2 ? 127 : 255)) / (mats == 2 ? 128 : 256);
-        p.tiles = p.wide == 32 ? tile_ids<32>(groups, entries) : tile_ids<64>(groups, entries);
+        p.tiles = p.wide == 32 ? tile_ids<32>(groups, entries)
+                : p.wide == 64 ? tile_ids<64>(groups, entries) : tile_ids<128>(groups, entries);
     } else {
         p.kp = chunks_of(k) >= 8 ? 8 : 4;
         p.n_blocks = (n + (mats == 2 ? 15 : 31)) / (mats == 2 ? 16 : 32);
@@ -801,25 +938,24 @@ Plan plan_of(int mats, int k, int n, int groups, int entries) {
     return p;
 }
 
+template <uint32_t T, int WM, int MT, bool SWIGLU>
+hipError_t wide_launch(Mul& m, uint32_t grid, hipStream_t s) {
+    static LdsLimit limit;
+    auto* kern = k_expert_wide<T, WM, MT, SWIGLU>;
+    if (hipError_t e = limit.raise((const void*)kern, Wide<WM, MT>::LDS)) return e;
+    kern<<<grid, 256 * WM, Wide<WM, MT>::LDS, s>>>(m);
+    return hipGetLastError();
+}
+
 template <uint32_t T, bool SWIGLU>
 hipError_t mul_launch(Mul& m, const Plan& p, hipStream_t s) {
     const uint32_t grid = (uint32_t)p.n_blocks * (uint32_t)p.tiles;
-    if (p.wide == 0) {
-        if (p.kp == 8)
-            k_expert_rows<T, 2, SWIGLU, 8><<<grid, 512, 0, s>>>(m);
-        else
-            k_expert_rows<T, 2, SWIGLU, 4><<<grid, 256, 0, s>>>(m);
-    } else if (p.wide == 32) {
-        static LdsLimit limit;
-        auto* kern = k_expert_wide<T, 1, SWIGLU>;
-        if (hipError_t e = limit.raise((const void*)kern, Wide<1>::LDS)) return e;
-        kern<<<grid, 256, Wide<1>::LDS, s>>>(m);
-    } else {
-        static LdsLimit limit;
-        auto* kern = k_expert_wide<T, 2, SWIGLU>;
-        if (hipError_t e = limit.raise((const void*)kern, Wide<2>::LDS)) return e;
-        kern<<<grid, 256, Wide<2>::LDS, s>>>(m);
-    }
+    if (p.wide == 32) return wide_launch<T, 1, 1, SWIGLU>(m, grid, s);
+    if (p.wide == 64) return wide_launch<T, 1, 2, SWIGLU>(m, grid, s);
+    if (p.kp == 8)
+        k_expert_rows<T, 2, SWIGLU, 8><<<grid, 512, 0, s>>>(m);
+    else
+        k_expert_rows<T, 2, SWIGLU, 4><<<grid, 256, 0, s>>>(m);
     return hipGetLastError();
 }
 template <uint32_t T>
@@ -831,7 +967,7 @@ hipError_t mul_launch2(Mul& m, int mats, const Plan& p, hipStream_t s) {
 
 size_t expert_act_bytes(uint32_t type, int k, int rows) {
     const size_t c = (size_t)chunks_of(k);
-    return up256((size_t)rows * c * 1024 + (has_min(type) ? up256((size_t)rows * c * 64) : 0) + (size_t)rows * 4);
+    return up256((size_t)rows * row_of((int)c) + (has_min(type) ? up256((size_t)rows * c * 64) : 0) + (size_t)rows * 4);
 }
 
 hipError_t launch_experts(const ExpertArgs& a, hipStream_t s) {
