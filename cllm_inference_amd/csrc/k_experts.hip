@@ -343,31 +343,18 @@ struct Unit<T_Q8_0> {
     static constexpr int BYTES = Q8_0_BYTES;
     u32x2 q;
     uint32_t db;
-    __device__ __forceinline__ void load(const uint8_t* p, int g) {
-        q = ld_any<8, u32x2>(p + 2 + 8 * g);
-        db = ld_u16(p);
-    }
     __device__ __forceinline__ wh8 frag(int) const { return __builtin_bit_cast(wh8, int8x8_to_h8(q.x, q.y)); }
 };
 template <>
 struct Unit<T_Q4_0> {
     static constexpr int BYTES = Q4_0_BYTES;
     uint32_t q, db;
-    __device__ __forceinline__ void load(const uint8_t* p, int g) {
-        q = ld_any<4, uint32_t>(p + 2 + 4 * g);
-        db = ld_u16(p);
-    }
     __device__ __forceinline__ wh8 frag(int) const { return nibbles8(q, -8.0f); }
 };
 template <>
 struct Unit<T_Q5_0> {
     static constexpr int BYTES = Q5_0_BYTES;
     uint32_t q, h, db;
-    __device__ __forceinline__ void load(const uint8_t* p, int g) {
-        q = ld_any<4, uint32_t>(p + 6 + 4 * g);
-        h = ld_any<4, uint32_t>(p + 2);
-        db = ld_u16(p);
-    }
     __device__ __forceinline__ wh8 frag(int g) const { return five8(q, h, g); }
 };
 
@@ -435,136 +422,274 @@ __device__ __forceinline__ float unscaled(float v, int e) {
     return e == kExpNaN ? __builtin_nanf("") : ldexpf(v, -e);
 }
 
+// One weight row's share of lane group g of a chunk: 64 elements (16-row tiles).
+template <uint32_t T>
+struct WeightChunk {
+    Part<T> p;
+    u32x4 hdr;
+    __device__ __forceinline__ void load(const uint8_t* row, int c, int, int g) {
+        const uint8_t* at = row + (size_t)c * Part<T>::BYTES;
+        if constexpr (has_min(T)) hdr = ld_u32x4(at);
+        p.load(at, g);
+    }
+};
+// Blocks of 32: lane group g loads blocks g and 4 + g whole, and the groups then exchange quarters (a 4 x 4
+// transposition between lane groups and registers): a third of the loads of each group's own quarters.
+__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
+    const auto v = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = v[0], b = v[1];
+}
+__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
+    const auto v = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = v[0], b = v[1];
+}
+// m[j] of lane group b becomes m[b] of lane group j
+__device__ __forceinline__ void transpose4(uint32_t (&m)[4]) {
+    swap32(m[0], m[2]);
+    swap32(m[1], m[3]);
+    swap16(m[0], m[1]);
+    swap16(m[2], m[3]);
+}
+template <uint32_t T>
+    requires(!is_kq(T))
+struct WeightChunk<T> {
+    static constexpr int QW = T == T_Q8_0 ? 2 : 1;  // dwords of a quarter
+    static constexpr int QS = T == T_Q5_0 ? 6 : 2;  // the quants' place in a block
+    u32x4 q[2][QW];
+    uint32_t db[2], qh[2];
+    __device__ __forceinline__ void load(const uint8_t* row, int c, int nb, int g) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint8_t* at = row + (size_t)min(8 * c + 4 * k + g, nb - 1) * Unit<T>::BYTES;
+#pragma unroll
+            for (int j = 0; j < QW; ++j) q[k][j] = ld_any<16, u32x4>(at + QS + 16 * j);
+            db[k] = ld_u16(at);
+            if constexpr (T == T_Q5_0) qh[k] = ld_any<4, uint32_t>(at + 2);
+        }
+    }
+    // blocks 4 k .. 4 k + 3, this lane group's eight elements of each
+    __device__ __forceinline__ void units(int k, Unit<T> (&u)[4]) const {
+        uint32_t m[4];
+        if constexpr (T == T_Q8_0) {
+            // quarter j is dwords 2j and 2j + 1
+            uint32_t lo[4] = {q[k][0].x, q[k][0].z, q[k][1].x, q[k][1].z};
+            uint32_t hi[4] = {q[k][0].y, q[k][0].w, q[k][1].y, q[k][1].w};
+            transpose4(lo);
+            transpose4(hi);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j].q = u32x2{lo[j], hi[j]};
+        } else {
+            uint32_t v[4] = {q[k][0].x, q[k][0].y, q[k][0].z, q[k][0].w};
+            transpose4(v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j].q = v[j];
+        }
+        if constexpr (T == T_Q5_0) {
+            uint32_t v[4] = {qh[k], qh[k], qh[k], qh[k]};
+            transpose4(v);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j].h = v[j];
+        }
+        m[0] = m[1] = m[2] = m[3] = db[k];
+        transpose4(m);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j].db = m[j];
+    }
+};
+// acc += a chunk of 16 entries x the NT tiles' rows; frag(s, part): the activations' fragments
+template <uint32_t T, int NT, class Frag>
+__device__ __forceinline__ void chunk_product(const WeightChunk<T> (&w)[NT], int c, int nb, int g, Frag frag, wh8 am,
+                                              f32x4 (&acc)[NT]) {
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (is_kq(T)) {
+        f32x4 sum[NT];
+        Scales2 sc[NT];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            sum[i] = zero;
+            if constexpr (has_min(T)) sc[i] = Part<T>::scale(w[i].hdr, g);
+        }
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const wh8 ah = frag(s, 0), al = frag(s, 1);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                wh8 rest, f;
+                if constexpr (T == T_Q6_K)
+                    f = w[i].p.frag(s, g, rest);
+                else
+                    f = w[i].p.frag(sc[i], s, g);
+                sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, f, sum[i], 0, 0, 0);
+                sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, f, sum[i], 0, 0, 0);
+                if constexpr (T == T_Q6_K) sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, rest, sum[i], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            if constexpr (has_min(T)) {
+                const float d = f16_to_f32(w[i].hdr.x & 0xFFFFu);
+                const f32x4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(am, k4_minima(w[i].hdr), zero, 0, 0, 0);
+                const float dm = -(float)(1 << kMinShift) * f16_to_f32(w[i].hdr.x >> 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[i][j], fmaf(dm, m[j], acc[i][j]));
+            } else {
+                const float d = w[i].p.d();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[i][j], acc[i][j]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            Unit<T> u[NT][4];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) w[i].units(k, u[i]);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int s = 4 * k + b;
+                const wh8 ah = frag(s, 0), al = frag(s, 1);
+                const bool there = 8 * c + s < nb;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const wh8 f = u[i][b].frag(g);
+                    f32x4 sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, f, zero, 0, 0, 0);
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, f, sum, 0, 0, 0);
+                    const float d = there ? f16_to_f32(u[i][b].db) : 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], acc[i][j]);
+                }
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint32_t m0) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+                 : : "v"(off), "s"(base), "s"(m0) : "memory", "m0");
+}
+
 // ---- few rows to an expert ----------------------------------------------------------------------
-// A workgroup has 16 entries of an expert (its rows' 16-row MFMA side) and 16 weight rows of each of NT
-// tiles (gate and up, or 16 NT rows); its KP waves take every KP-th chunk and meet in LDS, in order.
-// Weights go from memory to registers, each byte read once by one lane; the fragments of the
-// activations come from the caches.
-template <uint32_t T, int NT, bool SWIGLU, int KP>
-__global__ __launch_bounds__(64 * KP) void k_expert_rows(Mul a) {
-    static_assert(!SWIGLU || NT == 2, "gate and up");
-    __shared__ float red[KP][NT][256];
-    __shared__ int ent[16], exps[16];
+// ROWS entries of an expert (16, or 4 of single tokens) and the weight rows of NS waves, two 16-row tiles each
+// (gate and up of the same rows, or 32 rows); KP groups of NS waves take every KP-th chunk and meet in LDS, in
+// order. A wave's weight bytes go to registers a chunk ahead; a group's activation fragments go to LDS a chunk
+// ahead, by direct-to-LDS loads (one an entry). LDS: [entry][64 fragments of 16 bytes], fragment f of entry
+// i in place f ^ (i % 8), so that eight entries' reads of one fragment fall on distinct banks.
+// What counts is how many bytes are on their way: the weights come from HBM, some 2 us away when all CUs read,
+// so a CU needs 40 KB and more in flight. Many rows of 16 entries: NS = 4, KP = 1; single tokens: NS = 1 and K
+// split over the workgroup, as their few tiles alone would not fill the chip.
+template <uint32_t T, int KP, int NS, int ROWS, bool SWIGLU>
+__global__ __launch_bounds__(64 * KP * NS, KP == 16 || KP == 8 ? 4 : 3) void k_expert_few(Mul a) {
+    constexpr int NT = 2, LOADS = ROWS / NS, MIN = has_min(T) ? 64 * ROWS : 0, BUF = 1024 * ROWS + MIN;
+    extern __shared__ __align__(16) uint8_t lds[];  // [KP][2][BUF]
+    __shared__ int ent[ROWS], exps[ROWS];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kp = wave / NS, ns = wave % NS;
     const int blk = blockIdx.x % a.n_blocks;
-    const GroupTile t = find_tile<16>(a.g, 0, blockIdx.x / a.n_blocks, lane);
+    const GroupTile t = find_tile<ROWS>(a.g, 0, blockIdx.x / a.n_blocks, lane);
     if (t.count <= 0) return;
     const int r = lane & 15, g = lane >> 4;
-    const int e = entry_of(a, t, r);
-    const int arow = e < 0 ? 0 : e / a.per_row;
-    if (threadIdx.x < 16) {
-        ent[r] = e;
-        exps[r] = a.act.exps[arow];
-    }
-    const uint8_t* ap = a.act.frags + (size_t)arow * a.act.row + (is_kq(T) ? (g >> 1) * 512 + (g & 1) * 16 : 16 * g);
+    const int n0 = (blk * NS + ns) * (SWIGLU ? 16 : 32);
     const uint8_t* wp[NT];
-    const int n0 = blk * (SWIGLU ? 16 : 16 * NT);
 #pragma unroll
     for (int i = 0; i < NT; ++i)
         wp[i] = a.w[SWIGLU ? i : 0] + (size_t)t.group * a.expert_bytes +
                 (size_t)min(n0 + (SWIGLU ? 0 : 16 * i) + r, a.n - 1) * a.row_bytes;
+    const int chunks = a.act.chunks;
+    WeightChunk<T> wt[2][NT];
+    if (kp < chunks) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) wt[0][i].load(wp[i], kp, a.nb, g);  // on their way while the entries are looked up
+    }
+    const int er = r & (ROWS - 1);
+    const int e = entry_of(a, t, er);
+    const int arow = e < 0 ? 0 : e / a.per_row;
+    if (threadIdx.x < ROWS) {
+        ent[er] = e;
+        exps[er] = a.act.exps[arow];
+    }
+    // this wave's loads: entries ns, ns + NS, .. (the rows of those lanes)
+    const uint8_t* from[LOADS];
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+        from[j] = a.act.frags + (size_t)(uint32_t)__builtin_amdgcn_readlane(arow, ns + NS * j) * a.act.row;
+    const uint32_t m_off = (uint32_t)__shfl(arow, (lane >> 2) & (ROWS - 1), 64) * (uint32_t)(chunks * 64) +
+                           16u * (uint32_t)((lane & 3) ^ ((lane >> 3) & 3));
+    uint8_t* mine = lds + kp * 2 * BUF;
+    const uint32_t m0 = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)mine;
+    auto issue = [&](int c, int buf) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) {
+            const int i = ns + NS * j;
+            if (i < t.count)
+                to_lds16(from[j] + (size_t)c * 1024, 16u * (uint32_t)(lane ^ (i & 7)),
+                         m0 + (uint32_t)(BUF * buf + 1024 * i));
+        }
+        if (has_min(T) && ns == NS - 1 && lane < 4 * ROWS)
+            to_lds16(a.act.mins + (size_t)c * 64, m_off, m0 + (uint32_t)(BUF * buf + 1024 * ROWS));
+    };
+    // fragment (s, part) of this lane's entry and group: a_at ^ a constant
+    const uint32_t a_at = (uint32_t)er * 1024u + 16u * (uint32_t)((is_kq(T) ? (g >> 1) * 32 + (g & 1) : g) ^ (er & 7));
     f32x4 acc[NT];
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int i = 0; i < NT; ++i) acc[i] = zero;
-    for (int c = wave; c < a.act.chunks; c += KP) {
-        if constexpr (is_kq(T)) {
-            u32x4 hdr[NT];
-            Part<T> pt[NT];
+    for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (kp < chunks) issue(kp, 0);
+    auto chunk = [&]<int PAR>(int c) {
+        __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's loads are in LDS, and every wave's of the group
+        asm volatile("" ::: "memory");
+        if constexpr (NS > 1) __syncthreads();
+        if (c + KP < chunks) {
+            issue(c + KP, 1 - PAR);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const uint8_t* p = wp[i] + (size_t)c * Part<T>::BYTES;
-                if constexpr (has_min(T)) hdr[i] = ld_u32x4(p);
-                pt[i].load(p, g);
-            }
-            wh8 ah[8], al[8], am;
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const uint8_t* at = ap + (size_t)c * 1024 + s * 64;
-                ah[s] = *(const wh8*)at;
-                al[s] = *(const wh8*)(at + 32);
-            }
-            if constexpr (has_min(T)) am = *(const wh8*)(a.act.mins + ((size_t)arow * a.act.chunks + c) * 64 + 16 * g);
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                Scales2 sc;
-                if constexpr (has_min(T)) sc = Part<T>::scale(hdr[i], g);
-                f32x4 sum = zero;
-#pragma unroll
-                for (int s = 0; s < 8; ++s) {
-                    wh8 rest, f;
-                    if constexpr (T == T_Q6_K)
-                        f = pt[i].frag(s, g, rest);
-                    else
-                        f = pt[i].frag(sc, s, g);
-                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], f, sum, 0, 0, 0);
-                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], f, sum, 0, 0, 0);
-                    if constexpr (T == T_Q6_K) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], rest, sum, 0, 0, 0);
-                }
-                if constexpr (has_min(T)) {
-                    const float d = f16_to_f32(hdr[i].x & 0xFFFFu);
-                    const f32x4 m = __builtin_amdgcn_mfma_f32_16x16x32_f16(am, k4_minima(hdr[i]), zero, 0, 0, 0);
-                    const float dm = -(float)(1 << kMinShift) * f16_to_f32(hdr[i].x >> 16);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], fmaf(dm, m[j], acc[i][j]));
-                } else {
-                    const float d = pt[i].d();
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], acc[i][j]);
-                }
-            }
-        } else {
-            Unit<T> u[8][NT];
-            wh8 ah[8], al[8];
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const int b = min(8 * c + s, a.nb - 1);
-#pragma unroll
-                for (int i = 0; i < NT; ++i) u[s][i].load(wp[i] + (size_t)b * Unit<T>::BYTES, g);
-                ah[s] = *(const wh8*)(ap + (size_t)c * 1024 + s * 128);
-                al[s] = *(const wh8*)(ap + (size_t)c * 1024 + s * 128 + 64);
-            }
-#pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                const bool there = 8 * c + s < a.nb;
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    const wh8 f = u[s][i].frag(g);
-                    f32x4 sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah[s], f, zero, 0, 0, 0);
-                    sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(al[s], f, sum, 0, 0, 0);
-                    const float d = there ? f16_to_f32(u[s][i].db) : 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(d, sum[j], acc[i][j]);
-                }
-            }
+            for (int i = 0; i < NT; ++i) wt[1 - PAR][i].load(wp[i], c + KP, a.nb, g);
         }
+        if (c >= chunks) return;
+        const uint8_t* cur = mine + PAR * BUF;
+        auto frag = [&](int s, int part) {
+            return *(const wh8*)(cur + (a_at ^ (uint32_t)(is_kq(T) ? 64 * s + 32 * part : 128 * s + 64 * part)));
+        };
+        wh8 am;
+        if constexpr (has_min(T)) am = *(const wh8*)(cur + 1024 * ROWS + er * 64 + 16 * (g ^ ((er >> 1) & 3)));
+        chunk_product<T, NT>(wt[PAR], c, a.nb, g, frag, am, acc);
+    };
+    for (int c = kp; c - kp < chunks; c += 2 * KP) {
+        chunk.template operator()<0>(c);
+        if (c - kp + KP < chunks) chunk.template operator()<1>(c + KP);
     }
-    // lane (r, g) has tokens 4g + j of weight row r
+    // lane (r, g) has entries 4g + j of weight row r of each tile
+    if constexpr (KP > 1) {
+        float* red = (float*)lds;  // [wave][NT][256]
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NT; ++i) *(f32x4*)&red[wave][i][4 * lane] = acc[i];
-    __syncthreads();
-    constexpr int OUT = SWIGLU ? 256 : 256 * NT;
-    for (int o = threadIdx.x; o < OUT; o += 64 * KP) {
-        const int i = o >> 8, tok = (o >> 4) & 15, col = o & 15;
-        const int at = 4 * (16 * (tok >> 2) + col) + (tok & 3);
-        const int en = ent[tok], row = n0 + 16 * i + col;
-        if (en < 0 || row >= a.n) continue;
-        float v = red[0][i][at], v1 = 0.0f;
+        for (int i = 0; i < NT; ++i) *(f32x4*)(red + (wave * NT + i) * 256 + 4 * lane) = acc[i];
+        __syncthreads();
+        if (kp != 0) return;
 #pragma unroll
-        for (int w = 1; w < KP; ++w) v += red[w][i][at];
-        v = unscaled(v, exps[tok]);
+        for (int k = 1; k < KP; ++k)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[i] += *(const f32x4*)(red + ((k * NS + ns) * NT + i) * 256 + 4 * lane);
+    } else {
+        __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < (SWIGLU ? 1 : NT); ++i) {
+        const int row = n0 + 16 * i + r;
+        if (row >= a.n) continue;
         const size_t b = (size_t)t.group * a.n + row;
-        if (a.bias[0]) v += a.bias[0][b];
-        if constexpr (SWIGLU) {
-            v1 = red[0][1][at];
+        const float b0 = a.bias[0] ? a.bias[0][b] : 0.0f, b1 = SWIGLU && a.bias[1] ? a.bias[1][b] : 0.0f;
 #pragma unroll
-            for (int w = 1; w < KP; ++w) v1 += red[w][1][at];
-            v1 = unscaled(v1, exps[tok]);
-            if (a.bias[1]) v1 += a.bias[1][b];
-            v = silu_mul(v, v1);
+        for (int j = 0; j < 4; ++j) {
+            const int tok = 4 * g + j, en = tok < ROWS ? ent[tok & (ROWS - 1)] : -1;
+            if (en < 0) continue;
+            float v = unscaled(acc[i][j], exps[tok & (ROWS - 1)]) + b0;
+            if constexpr (SWIGLU) v = silu_mul(v, unscaled(acc[1][j], exps[tok & (ROWS - 1)]) + b1);
+            a.y[(size_t)en * a.n + row] = v;
         }
-        a.y[(size_t)en * a.n + row] = v;
     }
+}
+template <uint32_t T, int KP, int NS, int ROWS>
+constexpr int few_lds() {
+    const int buf = KP * 2 * (1024 * ROWS + (has_min(T) ? 64 * ROWS : 0)), red = KP > 1 ? KP * NS * 2048 : 0;
+    return buf > red ? buf : red;
 }
 
 // ---- many rows to an expert ----------------------------------------------------------------------
@@ -582,11 +707,6 @@ struct Wide {
     static constexpr int MINS = 2 * FRAGS, HDRS = MINS + BM * 64;  // minima of a chunk; headers, two buffers
     static constexpr int LDS = HDRS + 2 * 256 * 16;
 };
-
-__device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint32_t m0) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 : : "v"(off), "s"(base), "s"(m0) : "memory", "m0");
-}
 
 template <uint32_t T, int WM, int MT, bool SWIGLU>
 __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
@@ -918,24 +1038,36 @@ hipError_t act_launch(const ExpertArgs& a, const Act& act, hipStream_t s) {
 }
 
 struct Plan {
-    int wide;  // entries of a tile: 32, 64 or 128; 0: k_expert_rows
-    int kp;
+    int rows;  // entries of a tile: 4 or 16 (k_expert_few), 32 or 64 (k_expert_wide)
+    int kp;    // K parts of k_expert_few's workgroups
     int n_blocks, tiles;
 };
 Plan plan_of(int mats, int k, int n, int groups, int entries) {
     Plan p{};
     const int live = std::max(1, std::min(groups, entries)), per = (entries + live - 1) / live;
-    p.wide = per <= 12 ? 0 : per <= 48 ? 32 : 64;
-    if (p.wide) {
-        p.n_blocks = (n + (mats == 2 ? 127 : 255)) / (mats == 2 ? 128 : 256);
-        p.tiles = p.wide == 32 ? tile_ids<32>(groups, entries)
-                : p.wide == 64 ? tile_ids<64>(groups, entries) : tile_ids<128>(groups, entries);
-    } else {
-        p.kp = chunks_of(k) >= 8 ? 8 : 4;
-        p.n_blocks = (n + (mats == 2 ? 15 : 31)) / (mats == 2 ? 16 : 32);
-        p.tiles = tile_ids<16>(groups, entries);
+    p.rows = per <= 2 ? 4 : per <= 16 ? 16 : per <= 32 ? 32 : 64;
+    p.kp = 1;
+    const int block = (p.rows == 4 ? 32 : p.rows == 16 ? 128 : 256) / mats;
+    p.n_blocks = (n + block - 1) / block;
+    p.tiles = p.rows == 4 ? tile_ids<4>(groups, entries) : p.rows == 16 ? tile_ids<16>(groups, entries)
+            : p.rows == 32 ? tile_ids<32>(groups, entries) : tile_ids<64>(groups, entries);
+    if (p.rows == 4) {
+        const long waves = (long)std::min(p.tiles, entries) * p.n_blocks;
+        p.kp = chunks_of(k) >= 12 && waves * 8 < 4096 ? 16 : chunks_of(k) >= 6 && waves * 4 < 8192 ? 8 : 4;
     }
     return p;
+}
+
+template <uint32_t T, int KP, int NS, int ROWS, bool SWIGLU>
+hipError_t few_launch(Mul& m, uint32_t grid, hipStream_t s) {
+    constexpr int LDS = few_lds<T, KP, NS, ROWS>();
+    auto* kern = k_expert_few<T, KP, NS, ROWS, SWIGLU>;
+    if constexpr (LDS > 60 * 1024) {
+        static LdsLimit limit;
+        if (hipError_t e = limit.raise((const void*)kern, LDS)) return e;
+    }
+    kern<<<grid, 64 * KP * NS, LDS, s>>>(m);
+    return hipGetLastError();
 }
 
 template <uint32_t T, int WM, int MT, bool SWIGLU>
@@ -950,13 +1082,12 @@ hipError_t wide_launch(Mul& m, uint32_t grid, hipStream_t s) {
 template <uint32_t T, bool SWIGLU>
 hipError_t mul_launch(Mul& m, const Plan& p, hipStream_t s) {
     const uint32_t grid = (uint32_t)p.n_blocks * (uint32_t)p.tiles;
-    if (p.wide == 32) return wide_launch<T, 1, 1, SWIGLU>(m, grid, s);
-    if (p.wide == 64) return wide_launch<T, 1, 2, SWIGLU>(m, grid, s);
-    if (p.kp == 8)
-        k_expert_rows<T, 2, SWIGLU, 8><<<grid, 512, 0, s>>>(m);
-    else
-        k_expert_rows<T, 2, SWIGLU, 4><<<grid, 256, 0, s>>>(m);
-    return hipGetLastError();
+    if (p.rows == 64) return wide_launch<T, 1, 2, SWIGLU>(m, grid, s);
+    if (p.rows == 32) return wide_launch<T, 1, 1, SWIGLU>(m, grid, s);
+    if (p.rows == 16) return few_launch<T, 1, 4, 16, SWIGLU>(m, grid, s);
+    if (p.kp == 16) return few_launch<T, 16, 1, 4, SWIGLU>(m, grid, s);
+    if (p.kp == 8) return few_launch<T, 8, 1, 4, SWIGLU>(m, grid, s);
+    return few_launch<T, 4, 1, 4, SWIGLU>(m, grid, s);
 }
 template <uint32_t T>
 hipError_t mul_launch2(Mul& m, int mats, const Plan& p, hipStream_t s) {
@@ -1011,10 +1142,10 @@ void expert_plan_name(uint32_t type, int mats, int k, int n, int groups, int ent
         return;
     }
     const Plan p = plan_of(mats, k, n, groups, entries);
-    if (p.wide)
-        snprintf(buf, cap, "k_expert_wide<%d> workgroups=%lld", p.wide, (long long)p.n_blocks * p.tiles);
+    if (p.rows <= 16)
+        snprintf(buf, cap, "k_expert_few<%d,%d> workgroups=%lld", p.kp, p.rows, (long long)p.n_blocks * p.tiles);
     else
-        snprintf(buf, cap, "k_expert_rows<%d> workgroups=%lld", p.kp, (long long)p.n_blocks * p.tiles);
+        snprintf(buf, cap, "k_expert_wide<%d> workgroups=%lld", p.rows, (long long)p.n_blocks * p.tiles);
 }
 
 hipError_t launch_expert_sum(const float* p, const int32_t* ids, const float* weights, int rows, int top_k, int groups,
