@@ -512,16 +512,22 @@ __device__ __forceinline__ void chunk_product(const WeightChunk<T> (&w)[NT], int
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
             const wh8 ah = frag(s, 0), al = frag(s, 1);
+            wh8 f[NT], rest[NT];
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
-                wh8 rest, f;
                 if constexpr (T == T_Q6_K)
-                    f = w[i].p.frag(s, g, rest);
+                    f[i] = w[i].p.frag(s, g, rest[i]);
                 else
-                    f = w[i].p.frag(sc[i], s, g);
-                sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, f, sum[i], 0, 0, 0);
-                sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, f, sum[i], 0, 0, 0);
-                if constexpr (T == T_Q6_K) sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, rest, sum[i], 0, 0, 0);
+                    f[i] = w[i].p.frag(sc[i], s, g);
+            }
+            // (a product waits for the one before it in its accumulator: the tiles in turn)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, f[i], sum[i], 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, f[i], sum[i], 0, 0, 0);
+            if constexpr (T == T_Q6_K) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, rest[i], sum[i], 0, 0, 0);
             }
         }
 #pragma unroll
@@ -576,9 +582,10 @@ __device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint
 // i in place f ^ (i % 8), so that eight entries' reads of one fragment fall on distinct banks.
 // What counts is how many bytes are on their way: the weights come from HBM, some 2 us away when all CUs read,
 // so a CU needs 40 KB and more in flight. Many rows of 16 entries: NS = 4, KP = 1; single tokens: NS = 1 and K
-// split over the workgroup, as their few tiles alone would not fill the chip.
+// split over the workgroup, as their few tiles alone would not fill the chip; long rows: both, as
+// neighbouring chunks read at the same time are longer runs of memory.
 template <uint32_t T, int KP, int NS, int ROWS, bool SWIGLU>
-__global__ __launch_bounds__(64 * KP * NS, KP == 16 || KP == 8 ? 4 : 3) void k_expert_few(Mul a) {
+__global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_few(Mul a) {
     constexpr int NT = 2, LOADS = ROWS / NS, MIN = has_min(T) ? 64 * ROWS : 0, BUF = 1024 * ROWS + MIN;
     extern __shared__ __align__(16) uint8_t lds[];  // [KP][2][BUF]
     __shared__ int ent[ROWS], exps[ROWS];
@@ -1038,22 +1045,26 @@ hipError_t act_launch(const ExpertArgs& a, const Act& act, hipStream_t s) {
 }
 
 struct Plan {
-    int rows;  // entries of a tile: 4 or 16 (k_expert_few), 32 or 64 (k_expert_wide)
-    int kp;    // K parts of k_expert_few's workgroups
+    int rows;  // entries of a tile: 4, 8 or 16 (k_expert_few), 32 or 64 (k_expert_wide)
+    int kp;    // K parts of k_expert_few's workgroups (tiles of 8: 4)
     int n_blocks, tiles;
 };
 Plan plan_of(int mats, int k, int n, int groups, int entries) {
     Plan p{};
     const int live = std::max(1, std::min(groups, entries)), per = (entries + live - 1) / live;
-    p.rows = per <= 2 ? 4 : per <= 16 ? 16 : per <= 32 ? 32 : 64;
-    p.kp = 1;
-    const int block = (p.rows == 4 ? 32 : p.rows == 16 ? 128 : 256) / mats;
+    // 8: rows of 8192 elements and more (24 rows over 8 experts, down Q6_K 14336: 183 us, 250 on tiles of 16;
+    // gate and up Q4_K of 4096: 181 and 153)
+    p.rows = per <= 2 ? 4 : per <= 8 && chunks_of(k) >= 32 ? 8 : per <= 16 ? 16 : per <= 32 ? 32 : 64;
+    p.kp = p.rows == 8 ? 4 : 1;
+    const int block = (p.rows == 4 ? 32 : p.rows == 8 ? 64 : p.rows == 16 ? 128 : 256) / mats;
     p.n_blocks = (n + block - 1) / block;
-    p.tiles = p.rows == 4 ? tile_ids<4>(groups, entries) : p.rows == 16 ? tile_ids<16>(groups, entries)
+    p.tiles = p.rows == 4 ? tile_ids<4>(groups, entries) : p.rows == 8 ? tile_ids<8>(groups, entries) : p.rows == 16 ? tile_ids<16>(groups, entries)
             : p.rows == 32 ? tile_ids<32>(groups, entries) : tile_ids<64>(groups, entries);
     if (p.rows == 4) {
+        // K in 8 parts where 4 would leave a CU fewer than 16 waves and have long ways each (one row of down
+        // projections of 14336: @@)
         const long waves = (long)std::min(p.tiles, entries) * p.n_blocks;
-        p.kp = chunks_of(k) >= 12 && waves * 8 < 4096 ? 16 : chunks_of(k) >= 6 && waves * 4 < 8192 ? 8 : 4;
+        p.kp = chunks_of(k) >= 32 && waves * 4 < 4096 ? 8 : 4;
     }
     return p;
 }
@@ -1084,8 +1095,8 @@ hipError_t mul_launch(Mul& m, const Plan& p, hipStream_t s) {
     const uint32_t grid = (uint32_t)p.n_blocks * (uint32_t)p.tiles;
     if (p.rows == 64) return wide_launch<T, 1, 2, SWIGLU>(m, grid, s);
     if (p.rows == 32) return wide_launch<T, 1, 1, SWIGLU>(m, grid, s);
+    if (p.rows == 8) return few_launch<T, 4, 2, 8, SWIGLU>(m, grid, s);
     if (p.rows == 16) return few_launch<T, 1, 4, 16, SWIGLU>(m, grid, s);
-    if (p.kp == 16) return few_launch<T, 16, 1, 4, SWIGLU>(m, grid, s);
     if (p.kp == 8) return few_launch<T, 8, 1, 4, SWIGLU>(m, grid, s);
     return few_launch<T, 4, 1, 4, SWIGLU>(m, grid, s);
 }
