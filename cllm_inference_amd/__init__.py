@@ -1037,7 +1037,8 @@ def moe_route_dev(logits, top_k: int, bias=None, sigmoid: bool = False, normalis
     k = max(top_k, 0)
     ints = torch.empty(2 * m * k + experts + 1, dtype=torch.int32, device=logits.device)
     weights = torch.empty((m, k), dtype=torch.float32, device=logits.device)
-    r = MoeRoute(ints[:m * k].view(m, k), weights, ints[2 * m * k:], ints[m * k:2 * m * k])
+    ids, order, offsets = ints.split((m * k, m * k, experts + 1))
+    r = MoeRoute(ids.view(m, k), weights, offsets, order)
     at = ints.data_ptr()
     _check(load_library().cllm_hip_moe_route_dev(
         logits.data_ptr(), stride, bp, m, experts, top_k, int(sigmoid), int(normalise), scale, n_groups,

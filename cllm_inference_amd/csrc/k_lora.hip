@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device_utils.h"
 #include "experts.h"
@@ -18,12 +19,14 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h16x4 __attribute__((ext_vector_type(4)));
 
+constexpr int kMaxParts = 8;  // of K
+
 struct Down {
     const void* a[kMaxLoraMats];
     const int32_t* ranks;
     const float* x;
     Groups g;
-    int k, max_rank, parts, k_part;  // k_part: elements of a part, a multiple of 64
+    int k, max_rank, parts, k_part;  // k_part: elements of a part, a multiple of 256
     int rank_blocks;                 // of 16 RT ranks
     float* t;                        // [mat][part][entry][max_rank]
 };
@@ -42,21 +45,31 @@ struct Up {
 __device__ __forceinline__ int rank_of(const int32_t* ranks, int max_rank, int group) {
     return ranks ? min(max(ranks[group], 0), max_rank) : max_rank;
 }
-template <bool HALF>
-__device__ __forceinline__ f32x4 load4(const void* p, size_t at) {
-    if constexpr (HALF) {
-        const h16x4 v = *(const h16x4*)((const _Float16*)p + at);
-        return f32x4{(float)v.x, (float)v.y, (float)v.z, (float)v.w};
-    } else {
-        return *(const f32x4*)((const float*)p + at);
-    }
-}
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 
-// Tile of 16 rows of an adapter x RT tiles of 16 ranks x a part of K. Lane (r, q) loads elements 4q .. 4q + 3
-// of every 16 of K, of row r and of rank r, which four MFMAs take one by one; the four waves take every fourth
-// 64 elements and meet in LDS.
-template <bool HALF, int RT>
+// VL neighbouring elements of a lane: 16 bytes (8 of binary16, 4 of fp32), or 8 where rows of binary16 are no
+// multiple of 16 bytes (or 16 ranks at most).
+template <bool HALF, int VL>
+struct Piece {
+    static_assert(VL == 4 || HALF, "fp32: 4");
+    std::conditional_t<!HALF, f32x4, std::conditional_t<VL == 8, h16x8, h16x4>> v;
+    __device__ __forceinline__ void load(const void* p, size_t at) {
+        using V = decltype(v);
+        if constexpr (HALF)
+            v = *(const V*)((const _Float16*)p + at);
+        else
+            v = *(const V*)((const float*)p + at);
+    }
+    __device__ __forceinline__ void zero() { v = decltype(v){}; }
+    __device__ __forceinline__ float at(int i) const { return (float)v[i]; }
+};
+
+// Tile of 16 rows of an adapter x RT tiles of 16 ranks x a part of K. Lane (r, q) loads VL elements from 4 VL b + q VL
+// on, of row r and of rank r, which VL MFMAs take one by one; the four waves take every fourth 64 elements, each
+// loaded while the 64 before are multiplied, and meet in LDS.
+template <bool HALF, int VL, int RT>
 __global__ __launch_bounds__(256) void k_lora_down(Down a) {
+    constexpr int NB = 16 / VL;  // pieces of 64 elements
     __shared__ float red[4][RT][256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const GroupTile t = find_tile<16>(a.g, 0, blockIdx.x, lane);
@@ -66,34 +79,55 @@ __global__ __launch_bounds__(256) void k_lora_down(Down a) {
     const int rank = rank_of(a.ranks, a.max_rank, t.group);
     if (r0 >= rank) return;  // (the second launch takes ranks past it for zero)
     const int r = lane & 15, q = lane >> 4;
+    const int k0 = part * a.k_part, k1 = min(a.k, k0 + a.k_part);
+    const size_t arow = (size_t)t.group * a.max_rank;
+    Piece<HALF, VL> av[2][NB][RT];
+    f32x4 xv[2][NB][VL / 4];
+    auto load_a = [&](int k, int buf) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < RT; ++i) {
+                const int at = k + VL * (4 * b + q), row = r0 + 16 * i + r;
+                if (at < k1 && row < rank)
+                    av[buf][b][i].load(a.a[mat], (arow + row) * a.k + at);
+                else
+                    av[buf][b][i].zero();
+            }
+    };
+    load_a(k0 + 64 * wave, 0);  // on its way while the rows are looked up
     int e = r < t.count ? a.g.order[t.first + r] : -1;
     if ((uint32_t)e >= (uint32_t)a.g.entries) e = -1;
     const float* xp = a.x + (size_t)max(e, 0) * a.k;
-    const size_t arow = (size_t)t.group * a.max_rank;
-    const int k0 = part * a.k_part, k1 = min(a.k, k0 + a.k_part);
+    auto load_x = [&](int k, int buf) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int h = 0; h < VL / 4; ++h) {
+                const int at = k + VL * (4 * b + q) + 4 * h;
+                xv[buf][b][h] = at < k1 && e >= 0 ? *(const f32x4*)(xp + at) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+    };
+    load_x(k0 + 64 * wave, 0);
     f32x4 acc[RT];
 #pragma unroll
     for (int i = 0; i < RT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int k = k0 + 64 * wave; k < k1; k += 256) {
-        f32x4 xv[4], av[4][RT];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int at = k + 16 * b + 4 * q;
-            const bool in = at < k1;
-            xv[b] = in && e >= 0 ? *(const f32x4*)(xp + at) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-                const int row = r0 + 16 * i + r;
-                av[b][i] = in && row < rank ? load4<HALF>(a.a[mat], (arow + row) * a.k + at) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            }
+    auto step = [&]<int BUF>(int k) {
+        if (k + 256 < k1) {
+            load_a(k + 256, 1 - BUF);
+            load_x(k + 256, 1 - BUF);
         }
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < VL; ++j)
 #pragma unroll
                 for (int i = 0; i < RT; ++i)
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[b][j], av[b][i][j], acc[i], 0, 0, 0);
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(xv[BUF][b][j / 4][j % 4], av[BUF][b][i].at(j), acc[i], 0, 0, 0);
+    };
+    for (int k = k0 + 64 * wave; k < k1; k += 512) {
+        step.template operator()<0>(k);
+        if (k + 256 < k1) step.template operator()<1>(k + 256);
     }
 #pragma unroll
     for (int i = 0; i < RT; ++i) *(f32x4*)&red[wave][i][4 * lane] = acc[i];
@@ -109,11 +143,13 @@ __global__ __launch_bounds__(256) void k_lora_down(Down a) {
         if (r0 + 16 * i + col < rank) out[16 * i] = ((red[0][i][at] + red[1][i][at]) + red[2][i][at]) + red[3][i][at];
 }
 
-// Tile of 16 rows of an adapter (or of none) x the columns of a workgroup's four waves. The rows' rank sums
-// stand in LDS; lane (r, q) loads B's elements 4q .. 4q + 3 of every 16 ranks of output column r, and ends with
-// four neighbouring columns of one row.
-template <bool HALF>
+// Tile of 16 rows of an adapter (or of none) x the columns of a workgroup's four waves, 16 TILES each. The rows'
+// rank sums stand in LDS; lane (r, q) loads VL of B's elements of every 4 VL ranks of output column r, and ends
+// with four neighbouring columns of one row. A wave's elements of B (of the first 4 VL NCH ranks) and of the
+// shared projection are on their way before the rank sums are read.
+template <bool HALF, int VL, int NCH, int TILES>
 __global__ __launch_bounds__(256) void k_lora_up(Up a) {
+    constexpr int CH = 4 * VL;  // ranks of a chunk
     __shared__ float ts[16][kMaxLoraRank + 4];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const GroupTile t = find_tile<16>(a.g, 1, blockIdx.x, lane);
@@ -126,49 +162,94 @@ __global__ __launch_bounds__(256) void k_lora_up(Up a) {
     const bool none = t.group == a.g.groups;
     if (none && base == y) return;
     const int rank = none ? 0 : rank_of(a.ranks, a.max_rank, t.group);
-    const int chunks = (rank + 15) / 16;
-    const float scale = none ? 0.0f : a.scales ? a.scales[t.group] : 1.0f;
+    const int chunks = (rank + CH - 1) / CH;
     const int r = lane & 15, q = lane >> 4, n = a.n[mat];
-    for (int i = threadIdx.x; i < 16 * 16 * chunks; i += 256) {
-        const int tok = i / (16 * chunks), c = i - tok * 16 * chunks;
+    const int n0 = (blk * 4 + wave) * 16 * TILES;
+    const size_t brow = (size_t)t.group * n;
+    Piece<HALF, VL> w[TILES][NCH];
+    auto load_b = [&](int c0) {
+#pragma unroll
+        for (int j = 0; j < TILES; ++j)
+#pragma unroll
+            for (int c = 0; c < NCH; ++c) {
+                const int at = CH * (c0 + c) + VL * q;
+                if (at < rank)
+                    w[j][c].load(a.b[mat], (brow + min(n0 + 16 * j + r, n - 1)) * a.max_rank + at);
+                else
+                    w[j][c].zero();
+            }
+    };
+    load_b(0);
+    int e = r < t.count ? a.g.order[t.first + r] : -1;
+    if ((uint32_t)e >= (uint32_t)a.g.entries) e = -1;
+    const bool vec = n % 4 == 0;
+    f32x4 s[TILES];
+    const size_t out = (size_t)max(e, 0) * n + n0 + 4 * q;
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) {
+        s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const int col = n0 + 16 * j + 4 * q;
+        if (base && e >= 0) {
+            if (vec) {
+                if (col < n) s[j] = *(const f32x4*)(base + out + 16 * j);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (col + i < n) s[j][i] = base[out + 16 * j + i];
+            }
+        }
+    }
+    const float scale = none ? 0.0f : a.scales ? a.scales[t.group] : 1.0f;
+    for (int i = threadIdx.x; i < 16 * CH * chunks; i += 256) {
+        const int tok = i / (CH * chunks), c = i - tok * CH * chunks;
         const int en = tok < t.count ? a.g.order[t.first + tok] : -1;
         float v = 0.0f;
         if (c < rank && (uint32_t)en < (uint32_t)a.g.entries) {
             const float* src = a.t + ((size_t)mat * a.parts * a.g.entries + en) * a.max_rank + c;
-            for (int p = 0; p < a.parts; ++p) v += src[(size_t)p * a.g.entries * a.max_rank];
+            const size_t step = (size_t)a.g.entries * a.max_rank;
+            float u[kMaxParts];
+#pragma unroll
+            for (int p = 0; p < kMaxParts; ++p) u[p] = p < a.parts ? src[p * step] : 0.0f;
+#pragma unroll
+            for (int p = 0; p < kMaxParts; ++p) v += u[p];
         }
         ts[tok][c] = v * scale;
     }
     __syncthreads();
-    int e = r < t.count ? a.g.order[t.first + r] : -1;
-    if ((uint32_t)e >= (uint32_t)a.g.entries) e = -1;
-    const size_t brow = (size_t)t.group * n;
-    for (int j = 0; j < a.tiles; ++j) {
-        const int n0 = (blk * 4 + wave) * 16 * a.tiles + 16 * j;
-        if (n0 >= n) break;
-        f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int row = min(n0 + r, n - 1);
-        for (int c = 0; c < chunks; ++c) {
-            const int at = 16 * c + 4 * q;
-            f32x4 w = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (at < rank) {
-                w = load4<HALF>(a.b[mat], (brow + row) * a.max_rank + at);
+    // the adapter's part apart from the projection's, which may be far larger, and then one addition
+    f32x4 d[TILES];
 #pragma unroll
-                for (int i = 1; i < 4; ++i) w[i] = at + i < rank ? w[i] : 0.0f;
+    for (int j = 0; j < TILES; ++j) d[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c0 = 0; c0 < chunks; c0 += NCH) {
+        if (c0 > 0) load_b(c0);
+#pragma unroll
+        for (int c = 0; c < NCH; ++c) {
+            if (c0 + c >= chunks) break;
+            const int at = CH * (c0 + c) + VL * q;
+            float v[VL];
+#pragma unroll
+            for (int i = 0; i < VL; i += 4) {
+                const f32x4 x = *(const f32x4*)&ts[r][at + i];
+                v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
             }
-            const f32x4 v = *(const f32x4*)&ts[r][at];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i], v[i], s, 0, 0, 0);
+            for (int i = 0; i < VL; ++i)
+#pragma unroll
+                for (int j = 0; j < TILES; ++j)  // (ranks past the adapter's: whatever stands there)
+                    d[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(at + i < rank ? w[j][c].at(i) : 0.0f, v[i], d[j], 0, 0, 0);
         }
-        if (e < 0) continue;
-        const int col = n0 + 4 * q;
-        const size_t at = (size_t)e * n + col;
-        if (n % 4 == 0) {
-            if (col < n) *(f32x4*)(y + at) = base ? *(const f32x4*)(base + at) + s : s;
+    }
+    if (e < 0) return;
+#pragma unroll
+    for (int j = 0; j < TILES; ++j) {
+        const int col = n0 + 16 * j + 4 * q;
+        s[j] += d[j];
+        if (vec) {
+            if (col < n) *(f32x4*)(y + out + 16 * j) = s[j];
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                if (col + i < n) y[at + i] = base ? base[at + i] + s[i] : s[i];
+                if (col + i < n) y[out + 16 * j + i] = s[j][i];
         }
     }
 }
@@ -176,17 +257,34 @@ __global__ __launch_bounds__(256) void k_lora_up(Up a) {
 struct LoraPlan {
     int parts, k_part;
 };
+// K in parts of 512 and more, as many as make 1024 workgroups (at most 8).
 LoraPlan lora_plan(int mats, int k, int groups, int rows) {
     const int wgs = std::max(1, std::min(tile_ids<16>(groups, rows), rows)) * mats;
-    int parts = std::max(1, std::min((512 + wgs - 1) / wgs, (k + 511) / 512));
-    parts = std::min(parts, 8);
+    int parts = std::max(1, std::min((1024 + wgs - 1) / wgs, (k + 511) / 512));
+    parts = std::min(parts, kMaxParts);
     LoraPlan p;
-    p.k_part = ((k + parts - 1) / parts + 63) / 64 * 64;
+    p.k_part = ((k + parts - 1) / parts + 255) / 256 * 256;
     p.parts = (k + p.k_part - 1) / p.k_part;
     return p;
 }
 
-template <bool HALF>
+template <bool HALF, int VL>
+hipError_t down_launch(Down& d, dim3 grid, int rt, hipStream_t s) {
+    if (rt == 1)
+        k_lora_down<HALF, VL, 1><<<grid, 256, 0, s>>>(d);
+    else
+        k_lora_down<HALF, VL, 2><<<grid, 256, 0, s>>>(d);
+    return hipGetLastError();
+}
+template <bool HALF, int VL, int NCH>
+hipError_t up_launch(Up& u, dim3 grid, int tiles, hipStream_t s) {
+    if (tiles == 1)
+        k_lora_up<HALF, VL, NCH, 1><<<grid, 256, 0, s>>>(u);
+    else
+        k_lora_up<HALF, VL, NCH, 4><<<grid, 256, 0, s>>>(u);
+    return hipGetLastError();
+}
+
 hipError_t lora_launch(const LoraArgs& a, hipStream_t s) {
     const LoraPlan p = lora_plan(a.mats, a.k, a.g.groups, a.g.entries);
     Down d{};
@@ -207,18 +305,18 @@ hipError_t lora_launch(const LoraArgs& a, hipStream_t s) {
     const int rt = a.max_rank <= 16 ? 1 : 2;
     d.rank_blocks = (a.max_rank + 16 * rt - 1) / (16 * rt);
     const dim3 grid(tiles, (unsigned)p.parts, (unsigned)(a.mats * d.rank_blocks));
-    if (rt == 1)
-        k_lora_down<HALF, 1><<<grid, 256, 0, s>>>(d);
-    else
-        k_lora_down<HALF, 2><<<grid, 256, 0, s>>>(d);
-    if (hipError_t e = hipGetLastError()) return e;
+    hipError_t e = !a.half ? down_launch<false, 4>(d, grid, rt, s)
+                 : a.k % 8 == 0 ? down_launch<true, 8>(d, grid, rt, s) : down_launch<true, 4>(d, grid, rt, s);
+    if (e != hipSuccess) return e;
     const unsigned up_tiles = (unsigned)tile_ids<16>(a.g.groups + 1, a.g.entries);
     u.tiles = up_tiles >= 16 ? 4 : 1;
     int blocks = 0;
     for (int i = 0; i < a.mats; ++i) u.block_end[i] = blocks += (a.n[i] + 64 * u.tiles - 1) / (64 * u.tiles);
     if (blocks == 0) return hipSuccess;
-    k_lora_up<HALF><<<dim3(up_tiles, (unsigned)blocks), 256, 0, s>>>(u);
-    return hipGetLastError();
+    const dim3 up(up_tiles, (unsigned)blocks);
+    if (!a.half) return up_launch<false, 4, 2>(u, up, u.tiles, s);
+    if (a.max_rank > 16 && a.max_rank % 8 == 0) return up_launch<true, 8, 2>(u, up, u.tiles, s);
+    return up_launch<true, 4, 1>(u, up, u.tiles, s);
 }
 
 }  // namespace
@@ -227,8 +325,6 @@ size_t lora_ws_bytes(int mats, int k, int max_rank, int groups, int rows) {
     return (size_t)mats * lora_plan(mats, k, groups, rows).parts * rows * max_rank * sizeof(float);
 }
 
-hipError_t launch_lora(const LoraArgs& a, hipStream_t s) {
-    return a.half ? lora_launch<true>(a, s) : lora_launch<false>(a, s);
-}
+hipError_t launch_lora(const LoraArgs& a, hipStream_t s) { return lora_launch(a, s); }
 
 }  // namespace cllm_hip

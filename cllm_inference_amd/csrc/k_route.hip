@@ -22,17 +22,43 @@ __global__ __launch_bounds__(1024) void k_group_rows(const int32_t* __restrict__
                                                      int32_t* __restrict__ offsets, int32_t* __restrict__ order) {
     __shared__ int lower[16], mine[16];
     const int g = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int per = ((n + 1023) / 1024) * 64;  // ids to a wave, a multiple of 64
-    const int first = wave * per, last = min(n, first + per);
-    auto key = [&](int i) {
-        const int v = ids[i];
-        return (uint32_t)v < (uint32_t)groups ? v : groups;
+    // 1024 ids to a step of a wave: four loads of four neighbouring ids a lane, all on their way at once
+    const int per = ((n + 16 * 1024 - 1) / (16 * 1024)) * 1024;
+    const int first = min(wave * per, n), last = min(n, first + per);
+    const bool vec = ((uintptr_t)ids & 15u) == 0;
+    auto step = [&](int i, int (&k)[16]) {
+        if (vec && i + 1024 <= last) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int4 v = *(const int4*)(ids + i + 256 * j + 4 * lane);
+                k[4 * j] = v.x, k[4 * j + 1] = v.y, k[4 * j + 2] = v.z, k[4 * j + 3] = v.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int at = i + 256 * (j >> 2) + 4 * lane + (j & 3);
+                k[j] = at < last ? ids[at] : -2;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const int at = i + 256 * (j >> 2) + 4 * lane + (j & 3);
+            k[j] = at >= last ? groups + 1 : (uint32_t)k[j] < (uint32_t)groups ? k[j] : groups;
+        }
     };
     int lo = 0, at = 0;
-    for (int i = first + lane; i < first + per; i += 64) {
-        const int k = i < last ? key(i) : groups + 1;
-        lo += __popcll(__ballot(k < g));
-        at += __popcll(__ballot(k == g));
+    for (int i = first; i < last; i += 1024) {
+        int k[16];
+        step(i, k);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            lo += k[j] < g;
+            at += k[j] == g;
+        }
+    }
+    for (int d = 32; d > 0; d >>= 1) {
+        lo += __shfl_xor(lo, d, 64);
+        at += __shfl_xor(at, d, 64);
     }
     if (lane == 0) lower[wave] = lo, mine[wave] = at;
     __syncthreads();
@@ -45,18 +71,52 @@ __global__ __launch_bounds__(1024) void k_group_rows(const int32_t* __restrict__
     if (threadIdx.x == 0) offsets[g] = base;
     if (at == 0) return;
     int to = base + before;
-    for (int i = first + lane; i < first + per; i += 64) {
-        const bool m = i < last && key(i) == g;
-        const uint64_t b = __ballot(m);
-        if (m) order[to + __popcll(b & ((1ull << lane) - 1))] = i;
-        to += __popcll(b);
+    const uint64_t below = (1ull << lane) - 1;
+    for (int i = first; i < last; i += 1024) {
+        int k[16];
+        step(i, k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // neighbouring ids are one lane's: those of the lanes below, then its own before this one
+            int ahead = 0, all = 0;
+            uint64_t b[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                b[c] = __ballot(k[4 * j + c] == g);
+                ahead += __popcll(b[c] & below);
+                all += __popcll(b[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (k[4 * j + c] == g) order[to + ahead++] = i + 256 * j + 4 * lane + c;
+            to += all;
+        }
     }
 }
 
 // ---- the choice ----------------------------------------------------------------------------------
+// The largest of the lanes' values, in every lane (moves between lanes by DPP: no LDS latency).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)u, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)(u >> 32), (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
+__device__ __forceinline__ double lane_f64(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)lo | ((uint64_t)hi << 32));
+}
 __device__ __forceinline__ double wave_max(double v) {
-    for (int d = 32; d > 0; d >>= 1) v = fmax(v, __shfl_xor(v, d, 64));
-    return v;
+    v = fmax(v, dpp_f64<DPP_QUAD_SWAP1, 0xF>(v));
+    v = fmax(v, dpp_f64<DPP_QUAD_SWAP2, 0xF>(v));
+    v = fmax(v, dpp_f64<DPP_ROW_HALF_MIRROR, 0xF>(v));
+    v = fmax(v, dpp_f64<DPP_ROW_MIRROR, 0xF>(v));
+    v = fmax(v, dpp_f64<0x142, 0xA>(v));  // a row's last lane to the next row
+    v = fmax(v, dpp_f64<0x143, 0xC>(v));  // lane 31 to the upper half
+    return lane_f64(v, 63);
 }
 __device__ __forceinline__ double wave_add(double v) {
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
@@ -105,28 +165,37 @@ __device__ void choose(const RouteArgs& a, int row, int lane, double* keys) {
         }
     }
     if (a.parts > 1) {
-        // lane p: the score of part p; the parts that rank below top_parts keep their experts
-        const int width = a.experts / a.parts;
+            const int width = a.experts / a.parts;
 #pragma unroll
         for (int j = 0; j < V; ++j) keys[V * lane + j] = key[j];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
+        // `share` neighbouring lanes to a part, every share-th key each, then their two largest joined
+        int share = 64;
+        while (share * a.parts > 64) share >>= 1;
+        const int part = lane / share;
         double best = none, second = none;
-        if (lane < a.parts)
-            for (int i = 0; i < width; ++i) {
-                const int k = i + lane < width ? i + lane : (i + lane) % width;  // lanes on different banks
-                const double v = keys[lane * width + k];
+        if (part < a.parts)
+            for (int i = lane & (share - 1); i < width; i += share) {
+                const double v = keys[part * width + i];
                 second = fmax(second, fmin(best, v));
                 best = fmax(best, v);
             }
+        for (int d = 1; d < share; d <<= 1) {
+            const double b = __shfl_xor(best, d, 64), s = __shfl_xor(second, d, 64);
+            second = fmax(fmin(best, b), fmax(second, s));
+            best = fmax(best, b);
+        }
         double mine = best;
         if (a.bias && width > 1) mine = best + second;
         if (mine != mine) mine = none;
         int ahead = 0;
         for (int p = 0; p < a.parts; ++p) {
-            const double v = __shfl(mine, p, 64);
-            ahead += v > mine || (v == mine && p < lane);
+            const double v = lane_f64(mine, p * share);
+            ahead += v > mine || (v == mine && p < part);
         }
-        const uint64_t keep = __ballot(lane < a.parts && ahead < a.top_parts);
+        const uint64_t kept = __ballot(part < a.parts && ahead < a.top_parts);
+        uint64_t keep = 0;  // bit p: part p
+        for (int p = 0; p < a.parts; ++p) keep |= ((kept >> (p * share)) & 1) << p;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int e = V * lane + j;
@@ -136,7 +205,7 @@ __device__ void choose(const RouteArgs& a, int row, int lane, double* keys) {
     }
     // the k largest, one a round; lane i keeps the i-th
     int id = -1;
-    double p = 0.0;
+    double p = 0.0, mine_x = none;
     for (int i = 0; i < a.top_k; ++i) {
         double best = key[0];
         int slot = 0;
@@ -146,16 +215,17 @@ __device__ void choose(const RouteArgs& a, int row, int lane, double* keys) {
         const double m = wave_max(best);
         if (m == none) break;
         const int owner = __ffsll((unsigned long long)__ballot(best == m)) - 1;
-        const int s = __shfl(slot, owner, 64);
+        const int s = __builtin_amdgcn_readlane(slot, owner);
         double v = none;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             v = j == s ? x[j] : v;
             if (lane == owner && j == s) key[j] = none;
         }
-        v = __shfl(v, owner, 64);
-        if (lane == i) id = V * owner + s, p = score(v);
+        v = lane_f64(v, owner);
+        if (lane == i) id = V * owner + s, mine_x = v;
     }
+    if (id >= 0) p = score(mine_x);
     if (a.normalise) sum = wave_add(p);
     if (lane < a.top_k) {
         a.ids[(size_t)row * a.top_k + lane] = id;
