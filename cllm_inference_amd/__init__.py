@@ -1158,37 +1158,44 @@ def lora_dev(x, a, b, groups: RowGroups, ranks=None, scales=None, base=None, ys=
     n = len(a)
     if n == 0 or len(b) != n or (base is not None and len(base) != n) or (ys is not None and len(ys) != n):
         raise RuntimeError(f"{who}: a, b, base and ys must have an entry for each projection")
-    if x.dim() != 2 or a[0].dim() != 3:
+    first = a[0]
+    if x.dim() != 2 or first.dim() != 3:
         raise RuntimeError(f"{who}: x must be n_rows x in_dim, a[i] n_adapters x max_rank x in_dim")
     rows, in_dim = x.shape
-    adapters, max_rank = a[0].shape[:2]
-    dt = a[0].dtype
-    if dt not in (torch.float16, f32):
+    shape, dt = first.shape, first.dtype
+    adapters, max_rank, k = shape
+    half = dt is torch.float16
+    if not half and dt is not f32:
         raise RuntimeError(f"{who}: adapters must be float16 or float32")
-    if groups.offsets.numel() != adapters + 1:
-        raise RuntimeError(f"{who}: offsets has {groups.offsets.numel()} elements, not {adapters + 1}")
-    outs = []
+    if k != in_dim:
+        raise RuntimeError(f"{who}: x has rows of {in_dim}, a of {k}")
+    ptrs, ints = ctypes.c_void_p * n, ctypes.c_int * n
+    outs, ap, bp, yp = ints(), ptrs(), ptrs(), ptrs()
+    basep = None if base is None else ptrs()
+    new = [] if ys is None else ys
     for i in range(n):
-        if tuple(a[i].shape) != (adapters, max_rank, in_dim) or b[i].dim() != 3 or \
-                (b[i].shape[0], b[i].shape[2]) != (adapters, max_rank):
-            raise RuntimeError(f"{who}: shapes of adapter {i} do not match: {tuple(a[i].shape)}, {tuple(b[i].shape)}")
-        outs.append(b[i].shape[1])
-    if ys is None:
-        ys = [torch.empty((rows, o), dtype=f32, device=x.device) for o in outs]
-    ptrs = ctypes.c_void_p * n
-    ap = ptrs(*[_addr(who, "a", m, dt, dev) for m in a])
-    bp = ptrs(*[_addr(who, "b", m, dt, dev) for m in b])
-    yp = ptrs(*[_addr(who, "y", y, f32, dev, rows * o) for y, o in zip(ys, outs)])
-    basep = None
-    if base is not None:
-        basep = ptrs(*[None if m is None else _addr(who, "base", m, f32, dev, rows * o) for m, o in zip(base, outs)])
+        m, w = a[i], b[i]
+        if m.shape != shape or w.dim() != 3 or w.shape[0] != adapters or w.shape[2] != max_rank:
+            raise RuntimeError(f"{who}: shapes of adapter {i} do not match: {tuple(m.shape)}, {tuple(w.shape)}")
+        ap[i] = _addr(who, "a", m, dt, dev)
+        bp[i] = _addr(who, "b", w, dt, dev)
+        outs[i] = out = w.shape[1]
+        if ys is None:
+            y = torch.empty((rows, out), dtype=f32, device=x.device)
+            new.append(y)
+            yp[i] = y.data_ptr()
+        else:
+            yp[i] = _addr(who, "y", ys[i], f32, dev, rows * out)
+        if basep is not None and base[i] is not None:
+            basep[i] = _addr(who, "base", base[i], f32, dev, rows * out)
+    ys = new
     lib = load_library()
-    nbytes = int(lib.cllm_hip_lora_ws_bytes(in_dim, n, adapters, max_rank, rows))
+    nbytes = lib.cllm_hip_lora_ws_bytes(in_dim, n, adapters, max_rank, rows)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _check(lib.cllm_hip_lora_dev(
-        1 if dt is torch.float16 else 0, in_dim, n, ap, bp, (ctypes.c_int * n)(*outs), adapters, max_rank,
+        1 if half else 0, in_dim, n, ap, bp, outs, adapters, max_rank,
         None if ranks is None else _addr(who, "ranks", ranks, i32, dev, adapters),
         None if scales is None else _addr(who, "scales", scales, f32, dev, adapters),
-        _addr(who, "x", x, f32, dev), rows, _addr(who, "offsets", groups.offsets, i32, dev),
+        _addr(who, "x", x, f32, dev), rows, _addr(who, "offsets", groups.offsets, i32, dev, adapters + 1),
         _addr(who, "order", groups.order, i32, dev, rows), basep, yp, ws.data_ptr(), nbytes, stream))
     return ys

@@ -39,7 +39,7 @@ struct Up {
     const float* scales;
     const float* t;
     Groups g;
-    int mats, max_rank, parts, tiles;  // tiles: 16-column tiles of a wave
+    int mats, max_rank, parts, steps;  // steps: column blocks of a workgroup
 };
 
 __device__ __forceinline__ int rank_of(const int32_t* ranks, int max_rank, int group) {
@@ -143,10 +143,11 @@ __global__ __launch_bounds__(256) void k_lora_down(Down a) {
         if (r0 + 16 * i + col < rank) out[16 * i] = ((red[0][i][at] + red[1][i][at]) + red[2][i][at]) + red[3][i][at];
 }
 
-// Tile of 16 rows of an adapter (or of none) x the columns of a workgroup's four waves, 16 TILES each. The rows'
-// rank sums stand in LDS; lane (r, q) loads VL of B's elements of every 4 VL ranks of output column r, and ends
-// with four neighbouring columns of one row. A wave's elements of B (of the first 4 VL NCH ranks) and of the
-// shared projection are on their way before the rank sums are read.
+// Tile of 16 rows of an adapter (or of none) x the columns of a workgroup: `steps` blocks of four waves' 16 TILES
+// each. The rows' rank sums stand in LDS; lane (r, q) loads VL of B's elements of every 4 VL ranks of output column
+// r, and ends with four neighbouring columns of one row. A block's elements of B (of the first 4 VL NCH ranks)
+// and of the shared projection are on their way while the block before is multiplied, the first ones while the
+// rank sums are read.
 template <bool HALF, int VL, int NCH, int TILES>
 __global__ __launch_bounds__(256) void k_lora_up(Up a) {
     constexpr int CH = 4 * VL;  // ranks of a chunk
@@ -156,7 +157,7 @@ __global__ __launch_bounds__(256) void k_lora_up(Up a) {
     if (t.count <= 0) return;
     int mat = 0;
     while (mat + 1 < a.mats && (int)blockIdx.y >= a.block_end[mat]) ++mat;
-    const int blk = (int)blockIdx.y - (mat ? a.block_end[mat - 1] : 0);
+    const int blk = ((int)blockIdx.y - (mat ? a.block_end[mat - 1] : 0)) * a.steps;
     const float* base = a.base[mat];
     float* y = a.y[mat];
     const bool none = t.group == a.g.groups;
@@ -164,93 +165,104 @@ __global__ __launch_bounds__(256) void k_lora_up(Up a) {
     const int rank = none ? 0 : rank_of(a.ranks, a.max_rank, t.group);
     const int chunks = (rank + CH - 1) / CH;
     const int r = lane & 15, q = lane >> 4, n = a.n[mat];
-    const int n0 = (blk * 4 + wave) * 16 * TILES;
-    const size_t brow = (size_t)t.group * n;
-    Piece<HALF, VL> w[TILES][NCH];
-    auto load_b = [&](int c0) {
+    const size_t brow = none ? 0 : (size_t)t.group * n;
+    const int cols = 64 * TILES, first = blk * cols + wave * 16 * TILES;
+    const int steps = min(a.steps, (n - blk * cols + cols - 1) / cols);
+    Piece<HALF, VL> w[2][TILES][NCH];
+    auto load_b = [&](int n0, int c0, int buf) {
+        if (rank == 0) return;
 #pragma unroll
         for (int j = 0; j < TILES; ++j)
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
-                const int at = CH * (c0 + c) + VL * q;
-                if (at < rank)
-                    w[j][c].load(a.b[mat], (brow + min(n0 + 16 * j + r, n - 1)) * a.max_rank + at);
-                else
-                    w[j][c].zero();
+                // (ranks past the adapter's are dropped where they are used)
+                const int at = min(CH * (c0 + c) + VL * q, a.max_rank - VL);
+                w[buf][j][c].load(a.b[mat], (brow + min(n0 + 16 * j + r, n - 1)) * a.max_rank + at);
             }
     };
-    load_b(0);
+    load_b(first, 0, 0);
     int e = r < t.count ? a.g.order[t.first + r] : -1;
     if ((uint32_t)e >= (uint32_t)a.g.entries) e = -1;
     const bool vec = n % 4 == 0;
-    f32x4 s[TILES];
-    const size_t out = (size_t)max(e, 0) * n + n0 + 4 * q;
+    f32x4 s[2][TILES];
+    const size_t out = (size_t)max(e, 0) * n + 4 * q;
+    // (lanes past the rows or columns read what others read: no branches between the loads)
+    const int e0 = __builtin_amdgcn_readfirstlane(max(e, 0));
+    const float* from = base ? base + (size_t)(e < 0 ? e0 : e) * n : nullptr;
+    auto load_base = [&](int n0, int buf) {
+        if (!from || !vec) return;
 #pragma unroll
-    for (int j = 0; j < TILES; ++j) {
-        s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const int col = n0 + 16 * j + 4 * q;
-        if (base && e >= 0) {
-            if (vec) {
-                if (col < n) s[j] = *(const f32x4*)(base + out + 16 * j);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (col + i < n) s[j][i] = base[out + 16 * j + i];
-            }
-        }
-    }
+        for (int j = 0; j < TILES; ++j) s[buf][j] = *(const f32x4*)(from + min(n0 + 16 * j + 4 * q, n - 4));
+    };
+    load_base(first, 0);
     const float scale = none ? 0.0f : a.scales ? a.scales[t.group] : 1.0f;
-    for (int i = threadIdx.x; i < 16 * CH * chunks; i += 256) {
-        const int tok = i / (CH * chunks), c = i - tok * CH * chunks;
-        const int en = tok < t.count ? a.g.order[t.first + tok] : -1;
-        float v = 0.0f;
-        if (c < rank && (uint32_t)en < (uint32_t)a.g.entries) {
-            const float* src = a.t + ((size_t)mat * a.parts * a.g.entries + en) * a.max_rank + c;
+    // four neighbouring ranks of a row to a thread, every part's on its way at once
+    const int tok = threadIdx.x >> 4, en0 = tok < t.count ? a.g.order[t.first + tok] : -1;
+    const bool row = (uint32_t)en0 < (uint32_t)a.g.entries;
+    for (int c = 4 * (threadIdx.x & 15); c < CH * chunks; c += 64) {
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (row && c < rank) {
+            const float* src = a.t + ((size_t)mat * a.parts * a.g.entries + en0) * a.max_rank + c;
             const size_t step = (size_t)a.g.entries * a.max_rank;
-            float u[kMaxParts];
+            f32x4 u[kMaxParts];
 #pragma unroll
-            for (int p = 0; p < kMaxParts; ++p) u[p] = p < a.parts ? src[p * step] : 0.0f;
+            for (int p = 0; p < kMaxParts; ++p)
+                u[p] = p < a.parts ? *(const f32x4*)(src + p * step) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int p = 0; p < kMaxParts; ++p) v += u[p];
+#pragma unroll
+            for (int k = 1; k < 4; ++k) v[k] = c + k < rank ? v[k] : 0.0f;  // (ranks past the adapter's are not written)
         }
-        ts[tok][c] = v * scale;
+        *(f32x4*)&ts[tok][c] = v * scale;
     }
     __syncthreads();
-    // the adapter's part apart from the projection's, which may be far larger, and then one addition
-    f32x4 d[TILES];
+    auto step = [&]<int BUF>(int i) {
+        const int n0 = first + i * cols;
+        if (i + 1 < steps) {
+            load_b(n0 + cols, 0, 1 - BUF);
+            load_base(n0 + cols, 1 - BUF);
+        }
+        // the adapter's part apart from the projection's, which may be far larger, and then one addition
+        f32x4 d[TILES];
 #pragma unroll
-    for (int j = 0; j < TILES; ++j) d[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = 0; c0 < chunks; c0 += NCH) {
-        if (c0 > 0) load_b(c0);
+        for (int j = 0; j < TILES; ++j) d[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c0 = 0; c0 < chunks; c0 += NCH) {
+            if (c0 > 0) load_b(n0, c0, BUF);
 #pragma unroll
-        for (int c = 0; c < NCH; ++c) {
-            if (c0 + c >= chunks) break;
-            const int at = CH * (c0 + c) + VL * q;
-            float v[VL];
+            for (int c = 0; c < NCH; ++c) {
+                if (c0 + c >= chunks) break;
+                const int at = CH * (c0 + c) + VL * q;
+                float v[VL];
 #pragma unroll
-            for (int i = 0; i < VL; i += 4) {
-                const f32x4 x = *(const f32x4*)&ts[r][at + i];
-                v[i] = x.x, v[i + 1] = x.y, v[i + 2] = x.z, v[i + 3] = x.w;
+                for (int k = 0; k < VL; k += 4) {
+                    const f32x4 x = *(const f32x4*)&ts[r][at + k];
+                    v[k] = x.x, v[k + 1] = x.y, v[k + 2] = x.z, v[k + 3] = x.w;
+                }
+#pragma unroll
+                for (int k = 0; k < VL; ++k)
+#pragma unroll
+                    for (int j = 0; j < TILES; ++j)  // (ranks past the adapter's: whatever stands there)
+                        d[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(at + k < rank ? w[BUF][j][c].at(k) : 0.0f, v[k], d[j], 0, 0, 0);
             }
-#pragma unroll
-            for (int i = 0; i < VL; ++i)
-#pragma unroll
-                for (int j = 0; j < TILES; ++j)  // (ranks past the adapter's: whatever stands there)
-                    d[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(at + i < rank ? w[j][c].at(i) : 0.0f, v[i], d[j], 0, 0, 0);
         }
-    }
-    if (e < 0) return;
+        if (e < 0) return;
 #pragma unroll
-    for (int j = 0; j < TILES; ++j) {
-        const int col = n0 + 16 * j + 4 * q;
-        s[j] += d[j];
-        if (vec) {
-            if (col < n) *(f32x4*)(y + out + 16 * j) = s[j];
-        } else {
+        for (int j = 0; j < TILES; ++j) {
+            const int col = n0 + 16 * j + 4 * q;
+            if (vec) {
+                if (col < n) *(f32x4*)(y + out + n0 + 16 * j) = base ? s[BUF][j] + d[j] : d[j];
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (col + i < n) y[out + 16 * j + i] = s[j][i];
+                for (int k = 0; k < 4; ++k) {
+                    const size_t at = out + n0 + 16 * j + k;
+                    if (col + k < n) y[at] = base ? base[at] + d[j][k] : d[j][k];
+                }
+            }
         }
+    };
+    for (int i = 0; i < steps; i += 2) {
+        step.template operator()<0>(i);
+        if (i + 1 < steps) step.template operator()<1>(i + 1);
     }
 }
 
@@ -281,7 +293,7 @@ hipError_t up_launch(Up& u, dim3 grid, int tiles, hipStream_t s) {
     if (tiles == 1)
         k_lora_up<HALF, VL, NCH, 1><<<grid, 256, 0, s>>>(u);
     else
-        k_lora_up<HALF, VL, NCH, 4><<<grid, 256, 0, s>>>(u);
+        k_lora_up<HALF, VL, NCH, 2><<<grid, 256, 0, s>>>(u);
     return hipGetLastError();
 }
 
@@ -309,14 +321,19 @@ hipError_t lora_launch(const LoraArgs& a, hipStream_t s) {
                  : a.k % 8 == 0 ? down_launch<true, 8>(d, grid, rt, s) : down_launch<true, 4>(d, grid, rt, s);
     if (e != hipSuccess) return e;
     const unsigned up_tiles = (unsigned)tile_ids<16>(a.g.groups + 1, a.g.entries);
-    u.tiles = up_tiles >= 16 ? 4 : 1;
+    // few tiles: small blocks, one a workgroup; else as many as leave 1024 workgroups, at most 8
+    const int wide = up_tiles >= 16 ? 2 : 1;
     int blocks = 0;
-    for (int i = 0; i < a.mats; ++i) u.block_end[i] = blocks += (a.n[i] + 64 * u.tiles - 1) / (64 * u.tiles);
+    for (int i = 0; i < a.mats; ++i) blocks += (a.n[i] + 64 * wide - 1) / (64 * wide);
+    u.steps = (int)std::max<int64_t>(1, std::min<int64_t>(8, (int64_t)blocks * up_tiles / 1024));
+    blocks = 0;
+    for (int i = 0; i < a.mats; ++i)
+        u.block_end[i] = blocks += (a.n[i] + 64 * wide * u.steps - 1) / (64 * wide * u.steps);
     if (blocks == 0) return hipSuccess;
     const dim3 up(up_tiles, (unsigned)blocks);
-    if (!a.half) return up_launch<false, 4, 2>(u, up, u.tiles, s);
-    if (a.max_rank > 16 && a.max_rank % 8 == 0) return up_launch<true, 8, 2>(u, up, u.tiles, s);
-    return up_launch<true, 4, 1>(u, up, u.tiles, s);
+    if (!a.half) return up_launch<false, 4, 2>(u, up, wide, s);
+    if (a.max_rank > 16 && a.max_rank % 8 == 0) return up_launch<true, 8, 2>(u, up, wide, s);
+    return up_launch<true, 4, 1>(u, up, wide, s);
 }
 
 }  // namespace
