@@ -358,41 +358,55 @@ struct Unit<T_Q5_0> {
     __device__ __forceinline__ wh8 frag(int g) const { return five8(q, h, g); }
 };
 
-// Lane groups 2h and 2h + 1 of one block.
+// Two neighbouring blocks of a row of 32-row tiles: lane half h loads block h whole, then the halves exchange
+// so that each has its 16 elements (lane groups 2h and 2h + 1) of both.
+__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
+    const auto v = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = v[0], b = v[1];
+}
+__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
+    const auto v = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = v[0], b = v[1];
+}
 template <uint32_t T>
-struct Pair;
-template <>
-struct Pair<T_Q8_0> {
-    u32x4 q;
-    uint32_t db;
-    __device__ __forceinline__ void load(const uint8_t* p, int h) {
-        q = ld_any<16, u32x4>(p + 2 + 16 * h);
-        db = ld_u16(p);
+struct BlockPair {
+    static constexpr int BYTES = T == T_Q8_0 ? Q8_0_BYTES : T == T_Q4_0 ? Q4_0_BYTES : Q5_0_BYTES;
+    static constexpr int HALF = T == T_Q8_0 ? 4 : 2;  // dwords of half a block's quants
+    static constexpr int QS = T == T_Q5_0 ? 6 : 2;
+    uint32_t q[2][HALF], d[2], h5[2];  // loaded: this half's block's two halves; after exchange(): of both blocks
+    __device__ __forceinline__ void load(const uint8_t* at) {
+#pragma unroll
+        for (int k = 0; k < HALF / 2; ++k) {
+            const u32x4 v = ld_any<16, u32x4>(at + QS + 16 * k);
+            uint32_t* to = HALF == 4 ? q[k] : q[0];
+            to[0] = v.x, to[1] = v.y;
+            if constexpr (HALF == 4)
+                to[2] = v.z, to[3] = v.w;
+            else
+                q[1][0] = v.z, q[1][1] = v.w;
+        }
+        d[0] = ld_u16(at);
+        if constexpr (T == T_Q5_0) h5[0] = ld_any<4, uint32_t>(at + 2);
     }
-    __device__ __forceinline__ wh8 frag(int i, int) const {
-        return __builtin_bit_cast(wh8, i ? int8x8_to_h8(q.z, q.w) : int8x8_to_h8(q.x, q.y));
+    __device__ __forceinline__ void exchange() {
+#pragma unroll
+        for (int k = 0; k < HALF; ++k) swap32(q[0][k], q[1][k]);
+        d[1] = d[0];
+        swap32(d[0], d[1]);
+        if constexpr (T == T_Q5_0) {
+            h5[1] = h5[0];
+            swap32(h5[0], h5[1]);
+        }
     }
-};
-template <>
-struct Pair<T_Q4_0> {
-    u32x2 q;
-    uint32_t db;
-    __device__ __forceinline__ void load(const uint8_t* p, int h) {
-        q = ld_any<8, u32x2>(p + 2 + 8 * h);
-        db = ld_u16(p);
+    // lane group 2h + i of block b
+    __device__ __forceinline__ wh8 frag(int b, int i, int h) const {
+        if constexpr (T == T_Q8_0)
+            return __builtin_bit_cast(wh8, int8x8_to_h8(q[b][2 * i], q[b][2 * i + 1]));
+        else if constexpr (T == T_Q4_0)
+            return nibbles8(q[b][i], -8.0f);
+        else
+            return five8(q[b][i], h5[b], 2 * h + i);
     }
-    __device__ __forceinline__ wh8 frag(int i, int) const { return nibbles8(i ? q.y : q.x, -8.0f); }
-};
-template <>
-struct Pair<T_Q5_0> {
-    u32x2 q;
-    uint32_t h5, db;
-    __device__ __forceinline__ void load(const uint8_t* p, int h) {
-        q = ld_any<8, u32x2>(p + 6 + 8 * h);
-        h5 = ld_any<4, uint32_t>(p + 2);
-        db = ld_u16(p);
-    }
-    __device__ __forceinline__ wh8 frag(int i, int h) const { return five8(i ? q.y : q.x, h5, 2 * h + i); }
 };
 
 template <uint32_t T>
@@ -435,14 +449,6 @@ struct WeightChunk {
 };
 // Blocks of 32: lane group g loads blocks g and 4 + g whole, and the groups then exchange quarters (a 4 x 4
 // transposition between lane groups and registers): a third of the loads of each group's own quarters.
-__device__ __forceinline__ void swap32(uint32_t& a, uint32_t& b) {
-    const auto v = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-    a = v[0], b = v[1];
-}
-__device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
-    const auto v = __builtin_amdgcn_permlane16_swap(a, b, false, false);
-    a = v[0], b = v[1];
-}
 // m[j] of lane group b becomes m[b] of lane group j
 __device__ __forceinline__ void transpose4(uint32_t (&m)[4]) {
     swap32(m[0], m[2]);
@@ -908,13 +914,14 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
         // that the items no longer need: a block's fragments an item or two ahead, a stage's weight
         // bytes a stage ahead.
         constexpr int N = NT * MT;
-        Pair<T> u[4][NT];
-        auto load_block = [&](int st, int s) {
+        BlockPair<T> u[2][NT];
+        auto load_pair = [&](int st, int k) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) u[s][i].load(wbase[i] + (size_t)min(4 * st + s, a.nb - 1) * Unit<T>::BYTES + w_at[i], h);
+            for (int i = 0; i < NT; ++i)
+                u[k][i].load(wbase[i] + (size_t)min(4 * st + 2 * k + h, a.nb - 1) * BlockPair<T>::BYTES + w_at[i]);
         };
-#pragma unroll
-        for (int s = 0; s < 4; ++s) load_block(0, s);
+        load_pair(0, 0);
+        load_pair(0, 1);
         auto stage = [&]<int HALF>(int st) {
             begin(st, HALF);
             const uint8_t* cur = lds + HALF * C::FRAGS;
@@ -930,9 +937,10 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
                             *(const wh8*)(cur + (a_at ^ (uint32_t)(16 * (8 * s + 4 * part + q))) + 16384 * m);
             };
             auto unpack = [&](int s, int i) {
+                if ((s & 1) == 0) u[s >> 1][i].exchange();
 #pragma unroll
-                for (int q = 0; q < 2; ++q) bf[i][q] = u[s][i].frag(q, h);
-                d[s & 1][i] = 4 * st + s < a.nb ? f16_to_f32(u[s][i].db) : 0.0f;
+                for (int q = 0; q < 2; ++q) bf[i][q] = u[s >> 1][i].frag(s & 1, q, h);
+                d[s & 1][i] = 4 * st + s < a.nb ? f16_to_f32(u[s >> 1][i].d[s & 1]) : 0.0f;
             };
             auto fold = [&](int it) {
                 const int s = it / N, m = it % N / NT, i = it % NT;
@@ -951,7 +959,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
                     unpack(s, 1);
                     if (MT == 1 && s < 3) read(s + 1, 0);
                 }
-                if (it % N == 1 && st + 1 < stages) load_block(st + 1, s);
+                if (it % N == 1 && (s & 1) && st + 1 < stages) load_pair(st + 1, s >> 1);
                 if (MT == 2 && it % N == 2 && s < 3) read(s + 1, 0);
                 if (it % N == N - 1 && s < 3) unpack(s + 1, 0);
                 wf16 z = zero;
