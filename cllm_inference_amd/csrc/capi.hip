@@ -1960,7 +1960,8 @@ int check_groups(const char* who, int n_entries, int n_groups, const int32_t* of
 }
 
 // The shapes of an expert product: rows of in_dim, n_entries = rows x per_row entries.
-int check_experts(const char* who, uint32_t type, int in_dim, int out_dim, int n_experts, int n_rows, int per_row) {
+int check_experts(const char* who, uint32_t type, int mats, int in_dim, int out_dim, int n_experts, int n_rows,
+                  int per_row) {
     if (!has_kernel(type)) return set_err(CLLM_HIP_E_TYPE, "%s: no kernel for this type", who);
     if (in_dim <= 0 || in_dim % block_elems(type) != 0)
         return set_err(CLLM_HIP_E_SHAPE, "%s: in_dim not divisible by block size", who);
@@ -1971,21 +1972,20 @@ int check_experts(const char* who, uint32_t type, int in_dim, int out_dim, int n
         return set_err(CLLM_HIP_E_ARG, "%s: 1 to %d experts of a row", who, kMaxRouteTopK);
     const int64_t entries = (int64_t)n_rows * per_row;
     // 32-bit offsets of the activation operand, and workgroups counted in 32 bits of threads
-    const int64_t act = (int64_t)std::max((int64_t)n_rows, entries) * (((in_dim + 255) / 256) * 1024 + 256);
-    const int64_t grid = (entries / 16 + n_experts + 1) * ((out_dim + 15) / 16 + 1);
+    const int64_t act = (int64_t)std::max((int64_t)n_rows, entries) * ((in_dim + 255) / 256) * 1024;
     if ((int64_t)out_dim * (int64_t)row_bytes(type, in_dim) >= (1ll << 32))
         return set_err(CLLM_HIP_E_ARG, "%s: an expert's matrix of 4 GiB and more", who);
-    if (act >= (1ll << 32) || grid > UINT32_MAX / 512 || entries > (1 << 28))
+    if (act >= (1ll << 32) || entries > (1 << 28) ||
+        expert_workgroups(type, mats, in_dim, out_dim, n_experts, (int)entries) > UINT32_MAX / 512)
         return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
     return CLLM_HIP_OK;
 }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-int run_experts(const char* who, uint32_t type, int mats, int in_dim, int out_dim, int n_experts,
+int run_experts(uint32_t type, int mats, int in_dim, int out_dim, int n_experts,
                 const void* const* w, const float* const* bias, const float* x, int n_rows, int per_row,
                 int n_entries, const int32_t* offsets, const int32_t* order, float* y, void* ws, hipStream_t s) {
-    (void)who;
     ExpertArgs a{};
     a.type = type;
     a.mats = mats;
@@ -2065,7 +2065,7 @@ int check_ws(const char* who, const void* ws, size_t have, size_t need) {
 int cllm_hip_moe_matmul_dev(uint32_t type, int in_dim, int out_dim, int n_experts, const void* w, const float* bias,
                             const float* x, int n_rows, int per_row, const int32_t* offsets, const int32_t* order,
                             float* y, void* ws, size_t ws_bytes, void* stream) {
-    int rc = check_experts("moe_matmul", type, in_dim, out_dim, n_experts, n_rows, per_row);
+    int rc = check_experts("moe_matmul", type, 1, in_dim, out_dim, n_experts, n_rows, per_row);
     if (rc) return rc;
     if (n_rows == 0 || out_dim == 0) return CLLM_HIP_OK;
     if ((rc = check_groups("moe_matmul", n_rows * per_row, n_experts, offsets, order))) return rc;
@@ -2075,7 +2075,7 @@ int cllm_hip_moe_matmul_dev(uint32_t type, int in_dim, int out_dim, int n_expert
     if ((rc = check_ws("moe_matmul", ws, ws_bytes, expert_act_bytes(type, in_dim, n_rows)))) return rc;
     DeviceState* st;
     if ((rc = acquire(&st))) return rc;
-    return run_experts("moe_matmul", type, 1, in_dim, out_dim, n_experts, &w, &bias, x, n_rows, per_row,
+    return run_experts(type, 1, in_dim, out_dim, n_experts, &w, &bias, x, n_rows, per_row,
                        n_rows * per_row, offsets, order, y, ws, (hipStream_t)stream);
 }
 
@@ -2083,7 +2083,7 @@ int cllm_hip_moe_swiglu_dev(uint32_t type, int in_dim, int n_ff, int n_experts, 
                             const float* bias_gate, const float* bias_up, const float* x, int n_rows, int top_k,
                             const int32_t* offsets, const int32_t* order, float* h, void* ws, size_t ws_bytes,
                             void* stream) {
-    int rc = check_experts("moe_swiglu", type, in_dim, n_ff, n_experts, n_rows, top_k);
+    int rc = check_experts("moe_swiglu", type, 2, in_dim, n_ff, n_experts, n_rows, top_k);
     if (rc) return rc;
     if (n_rows == 0 || n_ff == 0) return CLLM_HIP_OK;
     if ((rc = check_groups("moe_swiglu", n_rows * top_k, n_experts, offsets, order))) return rc;
@@ -2096,7 +2096,7 @@ int cllm_hip_moe_swiglu_dev(uint32_t type, int in_dim, int n_ff, int n_experts, 
     if ((rc = acquire(&st))) return rc;
     const void* w[2] = {w_gate, w_up};
     const float* b[2] = {bias_gate, bias_up};
-    return run_experts("moe_swiglu", type, 2, in_dim, n_ff, n_experts, w, b, x, n_rows, top_k, n_rows * top_k, offsets,
+    return run_experts(type, 2, in_dim, n_ff, n_experts, w, b, x, n_rows, top_k, n_rows * top_k, offsets,
                        order, h, ws, (hipStream_t)stream);
 }
 
@@ -2104,7 +2104,7 @@ int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, c
                           const float* h, int n_rows, int top_k, const int32_t* ids, const float* weights,
                           const int32_t* offsets, const int32_t* order, const float* base, float* y, void* ws,
                           size_t ws_bytes, void* stream) {
-    int rc = check_experts("moe_down", type, n_ff, out_dim, n_experts, n_rows, top_k);
+    int rc = check_experts("moe_down", type, 1, n_ff, out_dim, n_experts, n_rows, top_k);
     if (rc) return rc;
     if (n_rows == 0 || out_dim == 0) return CLLM_HIP_OK;
     if ((rc = check_groups("moe_down", n_rows * top_k, n_experts, offsets, order))) return rc;
@@ -2119,7 +2119,7 @@ int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, c
     if ((rc = acquire(&st))) return rc;
     float* parts = (float*)((uint8_t*)ws + align256(expert_act_bytes(type, n_ff, n_rows * top_k)));
     // every entry is a row of h
-    if ((rc = run_experts("moe_down", type, 1, n_ff, out_dim, n_experts, &w, &bias, h, n_rows * top_k, 1,
+    if ((rc = run_experts(type, 1, n_ff, out_dim, n_experts, &w, &bias, h, n_rows * top_k, 1,
                           n_rows * top_k, offsets, order, parts, ws, (hipStream_t)stream)))
         return rc;
     HIP_TRY(launch_expert_sum(parts, ids, weights, n_rows, top_k, n_experts, out_dim, base, y, (hipStream_t)stream));
@@ -2128,7 +2128,7 @@ int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, c
 
 const char* cllm_hip_moe_plan(uint32_t type, int n_mats, int in_dim, int out_dim, int n_experts, int n_entries) {
     static thread_local char buf[96];
-    if (check_experts("moe_plan", type, in_dim, out_dim, n_experts, n_entries, 1) || n_mats < 1 || n_mats > 2)
+    if (n_mats < 1 || n_mats > 2 || check_experts("moe_plan", type, n_mats, in_dim, out_dim, n_experts, n_entries, 1))
         snprintf(buf, sizeof buf, "none");
     else
         expert_plan_name(type, n_mats, in_dim, out_dim, n_experts, n_entries, buf, sizeof buf);
@@ -2152,7 +2152,7 @@ int check_lora(int in_dim, int n_mats, const int* out_dims, int n_adapters, int 
     }
     if (total > (1 << 21)) return set_err(CLLM_HIP_E_ARG, "lora: outputs too wide for one launch");
     const int64_t tiles = std::min<int64_t>(n_rows, n_rows / 16 + n_adapters + 1);
-    if (tiles * (total / 64 + n_mats) > UINT32_MAX / 256)
+    if (std::max(tiles * (total / 64 + n_mats), tiles * n_mats * ((max_rank + 15) / 16)) > UINT32_MAX / 256)
         return set_err(CLLM_HIP_E_ARG, "lora: batch too large for one launch");
     return CLLM_HIP_OK;
 }

@@ -37,7 +37,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // Row r: chunks of 256 elements, 1024 bytes of 16-byte fragments (8 fp16: step s, lane group g, hi or lo):
 //   K-quants          [g / 2][s 8][hi, lo][g % 2], so that half a super-block is 512 bytes
 //   blocks of 32      [s 8][hi, lo][g 4]
-// and 256 bytes more; then (K-quants with minima) [row][chunk][3 parts and zeros][8 blocks] fp16, 64 bytes a
+// then (K-quants with minima) [row][chunk][3 parts and zeros][8 blocks] fp16, 64 bytes a
 // chunk; then the rows' exponents. Fragment (s, g) holds elements
 //   Q4_K, Q5_K  64 g + 8 s + e                    (lane group g: the 32 quant bytes of blocks 2g, 2g + 1)
 //   Q6_K        128 (g / 2) + 32 (s / 2) + 16 (g % 2) + 8 (s % 2) + e
@@ -63,15 +63,11 @@ struct Act {
     int chunks;
 };
 int chunks_of(int k) { return (k + 255) / 256; }
-// (An odd multiple of 256 bytes: workgroups read the same place of many rows at once, and with rows a
-// power of two apart those are in one or two of an L2's 16 channels. 2048 rows of 4096 on 8 experts of
-// 14336, gate and up: 3510 us without, @@ with it.)
-uint32_t row_of(int chunks) { return (uint32_t)chunks * 1024u + 256u; }
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 Act act_of(void* ws, uint32_t type, int k, int rows) {
     Act a;
     a.chunks = chunks_of(k);
-    a.row = row_of(a.chunks);
+    a.row = (uint32_t)a.chunks * 1024u;
     uint8_t* p = (uint8_t*)ws;
     a.frags = p;
     p += (size_t)rows * a.row;
@@ -575,9 +571,12 @@ __device__ __forceinline__ void chunk_product(const WeightChunk<T> (&w)[NT], int
     }
 }
 
+// 64 x 16 bytes straight to LDS at m0 (the same in every lane), lane i's from base + off (the lanes' own) to m0 + 16 i.
+// In assembly, as the compiler, which would wait for them before any LDS read, is not to see these loads; nor
+// does it see that the load needs a wait state behind the write of M0.
 __device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint32_t m0) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-                 : : "v"(off), "s"(base), "s"(m0) : "memory", "m0");
+                 : : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane((int)m0)) : "memory", "m0");
 }
 
 // ---- few rows to an expert ----------------------------------------------------------------------
@@ -706,35 +705,32 @@ constexpr int few_lds() {
 }
 
 // ---- many rows to an expert ----------------------------------------------------------------------
-// BM entries of an expert and 256 weight rows (128 of gate and of up): WM x 4 waves of 32 MT entries x 64 weight
-// rows (two 32-column MFMA tiles, gate and up of the same rows, or 64 rows). The waves share the activation
+// 32 MT entries of an expert and 256 weight rows (128 of gate and of up): four waves of 64 weight rows (two 32-column MFMA tiles, gate and up of the same rows, or 64 rows). The waves share the activation
 // fragments, which reach LDS in stages of half a chunk, two buffers, by direct-to-LDS loads; each wave
 // loads and unpacks its weight rows' bytes a stage ahead in registers (with minima, the rows' headers in LDS).
 // LDS: [entry][32 fragments of 16 bytes], fragment f of entry i in place f ^ (i % 32), so that the 32
 // entries' reads of one fragment fall on distinct banks.
-template <int WM, int MT>
+template <int MT>
 struct Wide {
-    static constexpr int BM = 32 * MT * WM;
-    static constexpr int THREADS = 256 * WM;
+    static constexpr int BM = 32 * MT;
     static constexpr int FRAGS = BM * 512;                       // a stage's fragments, two buffers
     static constexpr int MINS = 2 * FRAGS, HDRS = MINS + BM * 64;  // minima of a chunk; headers, two buffers
     static constexpr int LDS = HDRS + 2 * 256 * 16;
 };
 
-template <uint32_t T, int WM, int MT, bool SWIGLU>
-__global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
-    using C = Wide<WM, MT>;
+template <uint32_t T, int MT, bool SWIGLU>
+__global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
+    using C = Wide<MT>;
     constexpr int NT = 2;
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ int ent[C::BM], exps[C::BM];
     __shared__ uint32_t from_a[C::BM], from_m[C::BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave >> 2, wn = wave & 3;
     const int blk = blockIdx.x % a.n_blocks;
     const GroupTile t = find_tile<C::BM>(a.g, 0, blockIdx.x / a.n_blocks, lane);
     if (t.count <= 0) return;
     const int r = lane & 31, h = lane >> 5;
-    for (int i = threadIdx.x; i < C::BM; i += C::THREADS) {
+    for (int i = threadIdx.x; i < C::BM; i += 256) {
         const int e = entry_of(a, t, i);
         const uint32_t row = (uint32_t)(e < 0 ? 0 : e / a.per_row);
         ent[i] = e;
@@ -745,7 +741,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
     __syncthreads();
     const uint8_t* wbase[2];
     uint32_t w_at[NT];  // this lane's rows
-    const int n0 = blk * (SWIGLU ? 128 : 256) + wn * (SWIGLU ? 32 : 64);
+    const int n0 = blk * (SWIGLU ? 128 : 256) + wave * (SWIGLU ? 32 : 64);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
         wbase[i] = a.w[SWIGLU ? i : 0] + (size_t)t.group * a.expert_bytes;
@@ -758,8 +754,8 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
         const uint32_t to = lds0 + (uint32_t)buf * C::FRAGS;
         const uint8_t* from = a.act.frags + (size_t)st * 512;
 #pragma unroll
-        for (int j = 0; j < C::BM / (8 * WM); ++j) {
-            const int k = 4 * WM * j + wave, i = 2 * k + h;
+        for (int j = 0; j < C::BM / 8; ++j) {
+            const int k = 4 * j + wave, i = 2 * k + h;
             to_lds16(from, from_a[i] + 16u * (uint32_t)(r ^ (i & 31)), to + 1024u * (uint32_t)k);
         }
         if (has_min(T) && (st & 1) && 16 * wave < C::BM) {
@@ -768,11 +764,12 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
                      lds0 + C::MINS + 1024u * (uint32_t)wave);
         }
         // the headers of the next chunk: lanes 0-31 the wave's first tile's rows, 32-63 the second's
-        if (has_min(T) && !(st & 1) && wm == 0) {
+        if (has_min(T) && !(st & 1)) {
             const uint8_t* b = SWIGLU && h ? wbase[1] : wbase[0];
             asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                          : : "v"(b + (h ? w_at[1] : w_at[0]) + (size_t)(st >> 1) * Bytes<T>::V),
-                             "s"(lds0 + C::HDRS + 4096u * (uint32_t)((st >> 1) & 1) + 1024u * (uint32_t)wn)
+                             "s"(__builtin_amdgcn_readfirstlane(
+                                 (int)(lds0 + C::HDRS + 4096u * (uint32_t)((st >> 1) & 1) + 1024u * (uint32_t)wave)))
                          : "memory", "m0");
         }
     };
@@ -786,7 +783,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
         for (int m = 0; m < MT; ++m) acc[i][m] = zero;
     // fragment (s, part) of lane half h of the wave's entry 32 m + r: a_at ^ 16 (4 s + 2 part), plus 16384 m
     // (blocks of 32: (block, part, 2 h + q) at a_at ^ 16 (8 block + 4 part + q))
-    const uint32_t a_at = (uint32_t)(wm * 32 * MT * 512 + r * 512 + 16 * (r ^ (is_kq(T) ? h : 2 * h)));
+    const uint32_t a_at = (uint32_t)(r * 512 + 16 * (r ^ (is_kq(T) ? h : 2 * h)));
     auto begin = [&](int st, int half) {
         __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's loads of the stage are in LDS
         asm volatile("" ::: "memory");
@@ -815,7 +812,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
             if (AHEAD && st + 1 < stages) load_part(st + 1, 1 - HALF);
             const uint8_t* cur = lds + HALF * C::FRAGS;
             const int g = 2 * HALF + h;
-            const uint8_t* hdr = lds + C::HDRS + 4096 * ((st >> 1) & 1) + 1024 * wn + 16 * r;
+            const uint8_t* hdr = lds + C::HDRS + 4096 * ((st >> 1) & 1) + 1024 * wave + 16 * r;
             auto read_a = [&](int p, int part, wh8 (&to)[MT]) {
                 const uint8_t* from = cur + (a_at ^ (uint32_t)(16 * (4 * p + 2 * part)));
 #pragma unroll
@@ -883,7 +880,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
                         if constexpr (has_min(T)) {
-                            const uint8_t* row = lds + C::MINS + (32 * MT * wm + 32 * m + r) * 64;
+                            const uint8_t* row = lds + C::MINS + (32 * m + r) * 64;
                             wf16 f = zero;
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
@@ -996,7 +993,7 @@ __global__ __launch_bounds__(256 * WM, 2) void k_expert_wide(Mul a) {
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                const int tok = 32 * MT * wm + 32 * m + 8 * (e >> 2) + 4 * h + (e & 3);
+                const int tok = 32 * m + 8 * (e >> 2) + 4 * h + (e & 3);
                 const int en = ent[tok];
                 if (en < 0) continue;
                 float v = unscaled(acc[i][m][e], exps[tok]) + b0;
@@ -1057,22 +1054,28 @@ struct Plan {
     int kp;    // K parts of k_expert_few's workgroups (tiles of 8: 4)
     int n_blocks, tiles;
 };
-Plan plan_of(int mats, int k, int n, int groups, int entries) {
+Plan plan_of(uint32_t type, int mats, int k, int n, int groups, int entries) {
     Plan p{};
     const int live = std::max(1, std::min(groups, entries)), per = (entries + live - 1) / live;
-    // 8: rows of 8192 elements and more (24 rows over 8 experts, down Q6_K 14336: 183 us, 250 on tiles of 16;
-    // gate and up Q4_K of 4096: 181 and 153)
-    p.rows = per <= 2 ? 4 : per <= 8 && chunks_of(k) >= 32 ? 8 : per <= 16 ? 16 : per <= 32 ? 32 : 64;
+    // By the mean number of entries of an expert (MI355X, us, tile of fewer | of more entries):
+    //  4 | 16  16 entries over 8 experts, gate and up Q4_K 4096 x 14336: 117 | 132; rows of 2048, 256 over 128: 66 | 59
+    //  8       rows of 8192 and more: 24 over 8, down Q4_K 14336: 78, on tiles of 16 114; 80 Q6_K: 236, 257
+    // 16 | 32  128 over 8, gate and up Q4_K 4096: 209 | 188; 2048 over 128, rows of 2048: 103 | 112
+    // 32 | 64  Q4_K, whose bytes stay ahead in either tile's registers: 512 over 8: 452 | 439, 1024: 684 | 701, 2048:
+    //          1241 | 1197; the others: 512, down Q6_K: 545 | 439, Q8_0: 962 | 642
+    const int chunks = chunks_of(k);
+    p.rows = per <= (chunks >= 12 ? 2 : 1) ? 4 : per <= 12 && chunks >= 32 ? 8 : per <= (chunks >= 32 ? 24 : 16) ? 16
+           : per <= (type == T_Q4_K ? 192 : 32) ? 32 : 64;
     p.kp = p.rows == 8 ? 4 : 1;
     const int block = (p.rows == 4 ? 32 : p.rows == 8 ? 64 : p.rows == 16 ? 128 : 256) / mats;
     p.n_blocks = (n + block - 1) / block;
     p.tiles = p.rows == 4 ? tile_ids<4>(groups, entries) : p.rows == 8 ? tile_ids<8>(groups, entries) : p.rows == 16 ? tile_ids<16>(groups, entries)
             : p.rows == 32 ? tile_ids<32>(groups, entries) : tile_ids<64>(groups, entries);
     if (p.rows == 4) {
-        // K in 8 parts where 4 would leave a CU fewer than 16 waves and have long ways each (one row of down
-        // projections of 14336: @@)
+        // K in 8 parts where 4 would leave a CU fewer than 16 waves and have long ways each (3 rows over 8 experts,
+        // down Q4_0 14336: 73 us, 80 in 4 parts; one row, gate and up Q4_K 4096: 43 and 38)
         const long waves = (long)std::min(p.tiles, entries) * p.n_blocks;
-        p.kp = chunks_of(k) >= 32 && waves * 4 < 4096 ? 8 : 4;
+        p.kp = chunks >= 32 && waves * 4 < 4096 ? 8 : 4;
     }
     return p;
 }
@@ -1089,20 +1092,20 @@ hipError_t few_launch(Mul& m, uint32_t grid, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <uint32_t T, int WM, int MT, bool SWIGLU>
+template <uint32_t T, int MT, bool SWIGLU>
 hipError_t wide_launch(Mul& m, uint32_t grid, hipStream_t s) {
     static LdsLimit limit;
-    auto* kern = k_expert_wide<T, WM, MT, SWIGLU>;
-    if (hipError_t e = limit.raise((const void*)kern, Wide<WM, MT>::LDS)) return e;
-    kern<<<grid, 256 * WM, Wide<WM, MT>::LDS, s>>>(m);
+    auto* kern = k_expert_wide<T, MT, SWIGLU>;
+    if (hipError_t e = limit.raise((const void*)kern, Wide<MT>::LDS)) return e;
+    kern<<<grid, 256, Wide<MT>::LDS, s>>>(m);
     return hipGetLastError();
 }
 
 template <uint32_t T, bool SWIGLU>
 hipError_t mul_launch(Mul& m, const Plan& p, hipStream_t s) {
     const uint32_t grid = (uint32_t)p.n_blocks * (uint32_t)p.tiles;
-    if (p.rows == 64) return wide_launch<T, 1, 2, SWIGLU>(m, grid, s);
-    if (p.rows == 32) return wide_launch<T, 1, 1, SWIGLU>(m, grid, s);
+    if (p.rows == 64) return wide_launch<T, 2, SWIGLU>(m, grid, s);
+    if (p.rows == 32) return wide_launch<T, 1, SWIGLU>(m, grid, s);
     if (p.rows == 8) return few_launch<T, 4, 2, 8, SWIGLU>(m, grid, s);
     if (p.rows == 16) return few_launch<T, 1, 4, 16, SWIGLU>(m, grid, s);
     if (p.kp == 8) return few_launch<T, 8, 1, 4, SWIGLU>(m, grid, s);
@@ -1117,7 +1120,7 @@ hipError_t mul_launch2(Mul& m, int mats, const Plan& p, hipStream_t s) {
 
 size_t expert_act_bytes(uint32_t type, int k, int rows) {
     const size_t c = (size_t)chunks_of(k);
-    return up256((size_t)rows * row_of((int)c) + (has_min(type) ? up256((size_t)rows * c * 64) : 0) + (size_t)rows * 4);
+    return up256((size_t)rows * c * 1024 + (has_min(type) ? up256((size_t)rows * c * 64) : 0) + (size_t)rows * 4);
 }
 
 hipError_t launch_experts(const ExpertArgs& a, hipStream_t s) {
@@ -1130,7 +1133,7 @@ hipError_t launch_experts(const ExpertArgs& a, hipStream_t s) {
         default: e = act_launch<kNibble>(a, act, s); break;
     }
     if (e != hipSuccess) return e;
-    const Plan p = plan_of(a.mats, a.k, a.n, a.g.groups, a.g.entries);
+    const Plan p = plan_of(a.type, a.mats, a.k, a.n, a.g.groups, a.g.entries);
     Mul m{};
     m.w[0] = a.w[0], m.w[1] = a.w[1];
     m.bias[0] = a.bias[0], m.bias[1] = a.bias[1];
@@ -1160,11 +1163,16 @@ void expert_plan_name(uint32_t type, int mats, int k, int n, int groups, int ent
         snprintf(buf, cap, "none");
         return;
     }
-    const Plan p = plan_of(mats, k, n, groups, entries);
+    const Plan p = plan_of(type, mats, k, n, groups, entries);
     if (p.rows <= 16)
         snprintf(buf, cap, "k_expert_few<%d,%d> workgroups=%lld", p.kp, p.rows, (long long)p.n_blocks * p.tiles);
     else
         snprintf(buf, cap, "k_expert_wide<%d> workgroups=%lld", p.rows, (long long)p.n_blocks * p.tiles);
+}
+
+int64_t expert_workgroups(uint32_t type, int mats, int k, int n, int groups, int entries) {
+    const Plan p = plan_of(type, mats, k, n, groups, entries);
+    return (int64_t)p.n_blocks * p.tiles;
 }
 
 hipError_t launch_expert_sum(const float* p, const int32_t* ids, const float* weights, int rows, int top_k, int groups,

@@ -175,7 +175,7 @@ def _entry_products(orc, x, per_row, ids, values, mags, k):
 # rows x per_row entries over the experts: single tokens, a few rows to an expert, tens (32-entry tiles),
 # hundreds (64-entry tiles, more than one to an expert); weight rows no multiple of any tile; odd lengths
 SHAPES = [(1, 4, 1, 256, 16), (1, 8, 2, 512, 100), (2, 2, 2, 2048, 33), (5, 16, 3, 768, 257), (33, 8, 2, 256, 130),
-          (24, 2, 2, 512, 290), (150, 3, 1, 768, 300), (90, 2, 2, 256, 70)]
+          (24, 2, 2, 512, 290), (150, 3, 1, 768, 300), (90, 2, 2, 256, 70), (13, 2, 1, 8192, 40), (3, 4, 1, 8448, 65)]
 
 
 @pytest.mark.parametrize("qt", TYPES, ids=lambda t: S.TYPE_NAMES[t])
