@@ -705,11 +705,18 @@ constexpr int few_lds() {
 }
 
 // ---- many rows to an expert ----------------------------------------------------------------------
-// 32 MT entries of an expert and 256 weight rows (128 of gate and of up): four waves of 64 weight rows (two 32-column MFMA tiles, gate and up of the same rows, or 64 rows). The waves share the activation
+// 32 MT entries of an expert and 256 weight rows (128 of gate and of up): four waves of 64 weight rows (two
+// 32-column MFMA tiles, gate and up of the same rows, or 64 rows). The waves share the activation
 // fragments, which reach LDS in stages of half a chunk, two buffers, by direct-to-LDS loads; each wave
 // loads and unpacks its weight rows' bytes a stage ahead in registers (with minima, the rows' headers in LDS).
 // LDS: [entry][32 fragments of 16 bytes], fragment f of entry i in place f ^ (i % 32), so that the 32
 // entries' reads of one fragment fall on distinct banks.
+// Measured (MI355X): 2048 rows, two of 8 experts each, gate and up Q4_K of 4096 x 14336: 2.00 ms, 962 GFLOP,
+// 481 TFLOP/s, and as many again for lo: 74% of what the library's fp16 product reaches. With nothing
+// loaded in the loop 1.44 ms: the activations' way to LDS (7.3 GB, from L2) is the rest; the weights' is
+// hidden. A register spilled into that loop costs much: 2.57 ms with 10. 128 entries to eight waves,
+// which halves the weights' unpacking: slower (3.32 | 2.42 ms), as eight waves in step at
+// each stage leave the matrix cores idle. Down Q6_K 14336 x 4096, three products: 1.72 ms, 839 TFLOP/s.
 template <int MT>
 struct Wide {
     static constexpr int BM = 32 * MT;
@@ -753,10 +760,12 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
     auto issue = [&](int st, int buf) {
         const uint32_t to = lds0 + (uint32_t)buf * C::FRAGS;
         const uint8_t* from = a.act.frags + (size_t)st * 512;
+        uint32_t swz = 16u * (uint32_t)(r ^ (2 * wave + h));  // 16 (r ^ (i % 32)), but for bits 3 and 4 of i
+        asm volatile("" : "+v"(swz));                         // (not a register for each j)
 #pragma unroll
         for (int j = 0; j < C::BM / 8; ++j) {
             const int k = 4 * j + wave, i = 2 * k + h;
-            to_lds16(from, from_a[i] + 16u * (uint32_t)(r ^ (i & 31)), to + 1024u * (uint32_t)k);
+            to_lds16(from, from_a[i] + (swz ^ (128u * (uint32_t)(j & 3))), to + 1024u * (uint32_t)k);
         }
         if (has_min(T) && (st & 1) && 16 * wave < C::BM) {
             const int i = 16 * wave + (lane >> 2);
@@ -765,12 +774,14 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
         }
         // the headers of the next chunk: lanes 0-31 the wave's first tile's rows, 32-63 the second's
         if (has_min(T) && !(st & 1)) {
-            const uint8_t* b = SWIGLU && h ? wbase[1] : wbase[0];
-            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
-                         : : "v"(b + (h ? w_at[1] : w_at[0]) + (size_t)(st >> 1) * Bytes<T>::V),
-                             "s"(__builtin_amdgcn_readfirstlane(
-                                 (int)(lds0 + C::HDRS + 4096u * (uint32_t)((st >> 1) & 1) + 1024u * (uint32_t)wave)))
-                         : "memory", "m0");
+            const uint32_t to_h = lds0 + C::HDRS + 4096u * (uint32_t)((st >> 1) & 1) + 1024u * (uint32_t)wave;
+            const size_t chunk = (size_t)(st >> 1) * Bytes<T>::V;
+            if (!SWIGLU)
+                to_lds16(wbase[0] + chunk, h ? w_at[1] : w_at[0], to_h);
+            else if (h == 0)
+                to_lds16(wbase[0] + chunk, w_at[0], to_h);
+            else
+                to_lds16(wbase[1] + chunk, w_at[1], to_h);
         }
     };
 
@@ -805,7 +816,10 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
         auto load_part = [&](int st, int half) {
 #pragma unroll
             for (int i = 0; i < NT; ++i)
-                pt[AHEAD ? half : 0][i].load(wbase[i] + (size_t)(st >> 1) * Part<T>::BYTES + w_at[i], 2 * half + h);
+                if constexpr (T == T_Q4_K)
+                    pt[half][i].load(wbase[i] + (size_t)(st >> 1) * Part<T>::BYTES + 64 * half + (w_at[i] + 32u * (uint32_t)h), 0);
+                else
+                    pt[0][i].load(wbase[i] + (size_t)(st >> 1) * Part<T>::BYTES + w_at[i], 2 * half + h);
         };
         auto stage = [&]<int HALF>(int st) {
             begin(st, HALF);
@@ -813,8 +827,10 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
             const uint8_t* cur = lds + HALF * C::FRAGS;
             const int g = 2 * HALF + h;
             const uint8_t* hdr = lds + C::HDRS + 4096 * ((st >> 1) & 1) + 1024 * wave + 16 * r;
+            uint32_t a_now = a_at;
+            if constexpr (has_min(T)) asm volatile("" : "+v"(a_now));  // (not a register for each fragment's place)
             auto read_a = [&](int p, int part, wh8 (&to)[MT]) {
-                const uint8_t* from = cur + (a_at ^ (uint32_t)(16 * (4 * p + 2 * part)));
+                const uint8_t* from = cur + (a_now ^ (uint32_t)(16 * (4 * p + 2 * part)));
 #pragma unroll
                 for (int m = 0; m < MT; ++m) to[m] = *(const wh8*)(from + 16384 * m);
             };
