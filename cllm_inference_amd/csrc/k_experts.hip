@@ -5,7 +5,7 @@
 // grouped by expert on the device; two matrices give silu(gate) * up (src/core/engine.cpp:509-512).
 //
 // Arithmetic. A Q8_0 element is dx * c. k_expert_act writes it, times a power of two of its row, as
-// fp16 hi + lo (22 bits), the token operand of the fp16 MFMAs; the weight operand holds the blocks'
+// fp16 hi + lo (22 bits; the Q8_0 product has 24 + 8), the token operand of the fp16 MFMAs; the weight operand holds the blocks'
 // integers (times the 6-bit sub-scales of Q4_K / Q5_K: at most 1953, exact in fp16; Q6_K's
 // scale * (q - 32) as its fp16 rounding and the exact rest). As dx is inside the operand, nothing is
 // done per block of 32: a super-block's 256 products add up in the MFMA's fp32 accumulators and meet
@@ -79,7 +79,9 @@ Act act_of(void* ws, uint32_t type, int k, int rows) {
 
 // One workgroup a row: the row's largest magnitude, then each quad of lanes one Q8_0 block (eight
 // elements a lane, quantize_row_q8_0 bit for bit) as scaled fp16 parts. The second read of the row
-// hits the caches. 1024 threads for few rows, where one row's latency is what counts.
+// hits the caches. 1024 threads for few rows, where one row's latency is what counts. A row is read once and
+// 4 bytes an element written: the copy rate bounds it (4096 rows of 14336: 470 MB, 116 us, 4.0 TB/s); a
+// single row of 14336 takes 5.7 us, of which 3 are two dependent passes over 56 KB by one CU.
 template <Order O, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_expert_act(const float* __restrict__ x, int k, uint32_t row_bytes,
                                                         int chunks, uint8_t* __restrict__ frags,
@@ -589,6 +591,10 @@ __device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint
 // so a CU needs 40 KB and more in flight. Many rows of 16 entries: NS = 4, KP = 1; single tokens: NS = 1 and K
 // split over the workgroup, as their few tiles alone would not fill the chip; long rows: both, as
 // neighbouring chunks read at the same time are longer runs of memory.
+// Measured (MI355X): one row, two of 8 experts: gate and up Q4_K 4096 x 14336 132 MB, with k_expert_act 38 us
+// (3.5 TB/s); down Q6_K 14336 x 4096 96 MB, 33 us. 61 rows, eight of 128 experts, 2048 x 768 Q4_K: 226 MB, 66 us with
+// k_expert_act (3.4 TB/s); with no weight loads in its loop still 47, of which the unpacking is 24, the MFMAs 9,
+// the rest starts, the entries' look-up and barriers: its 768 columns leave each workgroup 8 chunks to work on.
 template <uint32_t T, int KP, int NS, int ROWS, bool SWIGLU>
 __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_few(Mul a) {
     constexpr int NT = 2, LOADS = ROWS / NS, MIN = has_min(T) ? 64 * ROWS : 0, BUF = 1024 * ROWS + MIN;
@@ -1070,18 +1076,18 @@ struct Plan {
     int kp;    // K parts of k_expert_few's workgroups (tiles of 8: 4)
     int n_blocks, tiles;
 };
-Plan plan_of(uint32_t type, int mats, int k, int n, int groups, int entries) {
+Plan plan_of(int mats, int k, int n, int groups, int entries) {
     Plan p{};
     const int live = std::max(1, std::min(groups, entries)), per = (entries + live - 1) / live;
     // By the mean number of entries of an expert (MI355X, us, tile of fewer | of more entries):
     //  4 | 16  16 entries over 8 experts, gate and up Q4_K 4096 x 14336: 117 | 132; rows of 2048, 256 over 128: 66 | 59
     //  8       rows of 8192 and more: 24 over 8, down Q4_K 14336: 78, on tiles of 16 114; 80 Q6_K: 236, 257
     // 16 | 32  128 over 8, gate and up Q4_K 4096: 209 | 188; 2048 over 128, rows of 2048: 103 | 112
-    // 32 | 64  Q4_K, whose bytes stay ahead in either tile's registers: 512 over 8: 452 | 439, 1024: 684 | 701, 2048:
-    //          1241 | 1197; the others: 512, down Q6_K: 545 | 439, Q8_0: 962 | 642
+    // 32 | 64  gate and up Q4_K 4096: 260 over 8: 296 | 279, 400: 336 | 343, 512: 410 | 387, 1024: 678 | 617; Q5_K, 400:
+    //          467 | 427; down Q6_K 14336, 400: 546 | 441
     const int chunks = chunks_of(k);
     p.rows = per <= (chunks >= 12 ? 2 : 1) ? 4 : per <= 12 && chunks >= 32 ? 8 : per <= (chunks >= 32 ? 24 : 16) ? 16
-           : per <= (type == T_Q4_K ? 192 : 32) ? 32 : 64;
+           : per <= 32 ? 32 : 64;
     p.kp = p.rows == 8 ? 4 : 1;
     const int block = (p.rows == 4 ? 32 : p.rows == 8 ? 64 : p.rows == 16 ? 128 : 256) / mats;
     p.n_blocks = (n + block - 1) / block;
@@ -1149,7 +1155,7 @@ hipError_t launch_experts(const ExpertArgs& a, hipStream_t s) {
         default: e = act_launch<kNibble>(a, act, s); break;
     }
     if (e != hipSuccess) return e;
-    const Plan p = plan_of(a.type, a.mats, a.k, a.n, a.g.groups, a.g.entries);
+    const Plan p = plan_of(a.mats, a.k, a.n, a.g.groups, a.g.entries);
     Mul m{};
     m.w[0] = a.w[0], m.w[1] = a.w[1];
     m.bias[0] = a.bias[0], m.bias[1] = a.bias[1];
@@ -1179,15 +1185,15 @@ void expert_plan_name(uint32_t type, int mats, int k, int n, int groups, int ent
         snprintf(buf, cap, "none");
         return;
     }
-    const Plan p = plan_of(type, mats, k, n, groups, entries);
+    const Plan p = plan_of(mats, k, n, groups, entries);
     if (p.rows <= 16)
         snprintf(buf, cap, "k_expert_few<%d,%d> workgroups=%lld", p.kp, p.rows, (long long)p.n_blocks * p.tiles);
     else
         snprintf(buf, cap, "k_expert_wide<%d> workgroups=%lld", p.rows, (long long)p.n_blocks * p.tiles);
 }
 
-int64_t expert_workgroups(uint32_t type, int mats, int k, int n, int groups, int entries) {
-    const Plan p = plan_of(type, mats, k, n, groups, entries);
+int64_t expert_workgroups(int mats, int k, int n, int groups, int entries) {
+    const Plan p = plan_of(mats, k, n, groups, entries);
     return (int64_t)p.n_blocks * p.tiles;
 }
 

@@ -17,7 +17,8 @@ constexpr int kSmallRows = 64;
 // ---- entries sorted by group --------------------------------------------------------------------
 // Workgroup g lists the entries of group g (the last one, the entries of none). Its 16 waves take
 // consecutive stretches of the ids: each counts its matches and the lower ids, then, behind the sums of the
-// waves before it, writes its matches.
+// waves before it, writes its matches. Every workgroup reads all ids: 32792 ids (131 KB) and 257 workgroups,
+// 34 MB from L2, 10 us (one load at a time: 22 us); two dependent passes, not the bytes, bound it.
 __global__ __launch_bounds__(1024) void k_group_rows(const int32_t* __restrict__ ids, int n, int groups,
                                                      int32_t* __restrict__ offsets, int32_t* __restrict__ order) {
     __shared__ int lower[16], mine[16];
