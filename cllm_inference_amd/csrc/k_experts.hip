@@ -1026,6 +1026,7 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
 }
 
 // ---- the sum over a row's experts ----------------------------------------------------------------
+// Bound by its bytes: 2048 rows x 2 of 4096 and the sums 100 MB, 17 us (5.9 TB/s, partly from caches); one row 4.7 us.
 __global__ __launch_bounds__(256) void k_expert_sum(const float* __restrict__ p, const int32_t* __restrict__ ids,
                                                     const float* __restrict__ weights, int top_k, int groups, int n,
                                                     const float* base, float* y) {
