@@ -238,6 +238,26 @@ def test_moe_swiglu(gpu, orc, qt, rows, experts, top_k, k, n):
 
 
 @pytest.mark.parametrize("qt", TYPES, ids=lambda t: S.TYPE_NAMES[t])
+@pytest.mark.parametrize("rows,tile", [(1, "<8,4>"), (7, "<4,8>")])
+def test_swiglu_of_long_rows_with_an_expert_chosen_twice(gpu, orc, qt, rows, tile):
+    rng = np.random.default_rng(qt + rows)
+    experts, k, n = 2, 8448, 37
+    assert tile in gpu.moe_plan(qt, 2, k, n, experts, rows * 2)
+    wg, wu = S.make_weight(qt, experts * n, k, 31), S.make_weight(qt, experts * n, k, 32)
+    x = S.make_activation(rows, k, 33)
+    ids = rng.integers(0, experts, (rows, 2)).astype(np.int32)
+    ids[0] = 1  # the same expert in both places
+    h = gpu.moe_swiglu_dev(_cu(x), _cu(wg), _cu(wu), qt, n, _groups(gpu, ids, experts)).cpu().numpy().reshape(-1, n)
+    assert np.array_equal(h[0], h[1])
+    g, eg = _entry_products(orc, x, 2, ids, *M.expert_values(wg, qt, experts, n, k), k)
+    u, eu = _entry_products(orc, x, 2, ids, *M.expert_values(wu, qt, experts, n, k), k)
+    want = M.silu(g) * u
+    # as above
+    bound = 1.1 * eg * (np.abs(u) + eu) + np.abs(M.silu(g)) * eu + np.abs(want) * 2.0 ** -21 + 2.0 ** -126
+    assert (np.abs(h - want) <= bound).all(), float((np.abs(h - want) / bound).max())
+
+
+@pytest.mark.parametrize("qt", TYPES, ids=lambda t: S.TYPE_NAMES[t])
 @pytest.mark.parametrize("rows,experts,top_k,k,n", [(1, 8, 2, 512, 64), (9, 16, 4, 256, 99), (70, 4, 2, 768, 130)])
 @pytest.mark.parametrize("kind", ["spread", "dropped"])
 def test_moe_down(gpu, orc, qt, rows, experts, top_k, k, n, kind):
