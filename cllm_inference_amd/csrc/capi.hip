@@ -1976,7 +1976,7 @@ int check_experts(const char* who, uint32_t type, int mats, int in_dim, int out_
     if ((int64_t)out_dim * (int64_t)row_bytes(type, in_dim) >= (1ll << 32))
         return set_err(CLLM_HIP_E_ARG, "%s: an expert's matrix of 4 GiB and more", who);
     if (act >= (1ll << 32) || entries > (1 << 28) ||
-        expert_workgroups(mats, in_dim, out_dim, n_experts, (int)entries) > UINT32_MAX / 512)
+        expert_workgroups(type, mats, in_dim, out_dim, n_experts, (int)entries) > UINT32_MAX / 512)
         return set_err(CLLM_HIP_E_ARG, "%s: batch too large for one launch", who);
     return CLLM_HIP_OK;
 }

@@ -58,7 +58,7 @@ struct ExpertArgs {
 size_t expert_act_bytes(uint32_t type, int k, int rows);
 hipError_t launch_experts(const ExpertArgs& a, hipStream_t stream);
 // Workgroups (of at most 512 threads) of that launch.
-int64_t expert_workgroups(int mats, int k, int n, int groups, int entries);
+int64_t expert_workgroups(uint32_t type, int mats, int k, int n, int groups, int entries);
 void expert_plan_name(uint32_t type, int mats, int k, int n, int groups, int entries, char* buf, size_t cap);
 // y[r] = (base[r] +) sum over j of weights[r][j] * p[r top_k + j], the j with an id in range
 hipError_t launch_expert_sum(const float* p, const int32_t* ids, const float* weights, int rows, int top_k,

@@ -814,7 +814,7 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
         // run beside the unpacking of the next; its lo fragments are read beside the products with hi, the
         // next step's hi beside those with lo. Weight bytes are loaded a stage ahead, like the activations.
         constexpr int PARTS = T == T_Q6_K ? 3 : 2;
-        constexpr bool AHEAD = T == T_Q4_K;  // (registers)
+        constexpr bool AHEAD = T == T_Q4_K || MT == 1;  // (registers; 32 entries, down Q6_K 14336, 120 rows: 378 | 308 us)
         Part<T> pt[AHEAD ? 2 : 1][NT];
         wf16 sum[NT][MT];
         wh8 ah[MT], al[MT], bf[2][NT], rest[2][NT];
@@ -825,7 +825,7 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
                 if constexpr (T == T_Q4_K)
                     pt[half][i].load(wbase[i] + (size_t)(st >> 1) * Part<T>::BYTES + 64 * half + (w_at[i] + 32u * (uint32_t)h), 0);
                 else
-                    pt[0][i].load(wbase[i] + (size_t)(st >> 1) * Part<T>::BYTES + w_at[i], 2 * half + h);
+                    pt[AHEAD ? half : 0][i].load(wbase[i] + (size_t)(st >> 1) * Part<T>::BYTES + w_at[i], 2 * half + h);
         };
         auto stage = [&]<int HALF>(int st) {
             begin(st, HALF);
@@ -834,7 +834,7 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
             const int g = 2 * HALF + h;
             const uint8_t* hdr = lds + C::HDRS + 4096 * ((st >> 1) & 1) + 1024 * wave + 16 * r;
             uint32_t a_now = a_at;
-            if constexpr (has_min(T)) asm volatile("" : "+v"(a_now));  // (not a register for each fragment's place)
+            if constexpr (has_min(T) || MT == 1) asm volatile("" : "+v"(a_now));  // (not a register for each fragment's place)
             auto read_a = [&](int p, int part, wh8 (&to)[MT]) {
                 const uint8_t* from = cur + (a_now ^ (uint32_t)(16 * (4 * p + 2 * part)));
 #pragma unroll
@@ -897,7 +897,7 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
                         dm = -(float)(1 << kMinShift) * f16_to_f32(v.x >> 16);
                         mn = k4_minima(v);
                     } else {
-                        d = dq[i];
+                        d = AHEAD ? pt[AHEAD ? 1 : 0][i].d() : dq[i];
                     }
 #pragma unroll
                     for (int m = 0; m < MT; ++m) {
@@ -1077,18 +1077,21 @@ struct Plan {
     int kp;    // K parts of k_expert_few's workgroups (tiles of 8: 4)
     int n_blocks, tiles;
 };
-Plan plan_of(int mats, int k, int n, int groups, int entries) {
+Plan plan_of(uint32_t type, int mats, int k, int n, int groups, int entries) {
     Plan p{};
     const int live = std::max(1, std::min(groups, entries)), per = (entries + live - 1) / live;
     // By the mean number of entries of an expert (MI355X, us, tile of fewer | of more entries):
     //  4 | 16  16 entries over 8 experts, gate and up Q4_K 4096 x 14336: 117 | 132; rows of 2048, 256 over 128: 66 | 59
     //  8       rows of 8192 and more: 24 over 8, down Q4_K 14336: 78, on tiles of 16 114; 80 Q6_K: 236, 257
     // 16 | 32  128 over 8, gate and up Q4_K 4096: 209 | 188; 2048 over 128, rows of 2048: 103 | 112
+    //          down 14336: 180 over 8: Q4_K 186 | 205, Q6_K 347 | 306, 120 Q6_K 256 | 305
     // 32 | 64  gate and up Q4_K 4096: 260 over 8: 296 | 279, 400: 336 | 343, 512: 410 | 387, 1024: 678 | 617; Q5_K, 400:
-    //          467 | 427; down Q6_K 14336, 400: 546 | 441
+    //          443 | 422, 280: 369 | 362; Q8_0 1408 x 1376, 2036 over 60: 160 | 144;
+    //          Q6_K, whose bytes stay ahead in a tile of 32 only: down 14336, 280: 308 | 440, 400: 478 | 441; 4800 over 128
+    //          experts of 2048 x 768: 225 | 239
     const int chunks = chunks_of(k);
-    p.rows = per <= (chunks >= 12 ? 2 : 1) ? 4 : per <= 12 && chunks >= 32 ? 8 : per <= (chunks >= 32 ? 24 : 16) ? 16
-           : per <= 32 ? 32 : 64;
+    p.rows = per <= (chunks >= 12 ? 2 : 1) ? 4 : per <= 12 && chunks >= 32 ? 8 : per <= (chunks >= 32 && type != T_Q6_K ? 24 : 16) ? 16
+           : per <= (type == T_Q6_K ? 40 : 32) ? 32 : 64;
     p.kp = p.rows == 8 ? 4 : 1;
     const int block = (p.rows == 4 ? 32 : p.rows == 8 ? 64 : p.rows == 16 ? 128 : 256) / mats;
     p.n_blocks = (n + block - 1) / block;
@@ -1156,7 +1159,7 @@ hipError_t launch_experts(const ExpertArgs& a, hipStream_t s) {
         default: e = act_launch<kNibble>(a, act, s); break;
     }
     if (e != hipSuccess) return e;
-    const Plan p = plan_of(a.mats, a.k, a.n, a.g.groups, a.g.entries);
+    const Plan p = plan_of(a.type, a.mats, a.k, a.n, a.g.groups, a.g.entries);
     Mul m{};
     m.w[0] = a.w[0], m.w[1] = a.w[1];
     m.bias[0] = a.bias[0], m.bias[1] = a.bias[1];
@@ -1186,15 +1189,15 @@ void expert_plan_name(uint32_t type, int mats, int k, int n, int groups, int ent
         snprintf(buf, cap, "none");
         return;
     }
-    const Plan p = plan_of(mats, k, n, groups, entries);
+    const Plan p = plan_of(type, mats, k, n, groups, entries);
     if (p.rows <= 16)
         snprintf(buf, cap, "k_expert_few<%d,%d> workgroups=%lld", p.kp, p.rows, (long long)p.n_blocks * p.tiles);
     else
         snprintf(buf, cap, "k_expert_wide<%d> workgroups=%lld", p.rows, (long long)p.n_blocks * p.tiles);
 }
 
-int64_t expert_workgroups(int mats, int k, int n, int groups, int entries) {
-    const Plan p = plan_of(mats, k, n, groups, entries);
+int64_t expert_workgroups(uint32_t type, int mats, int k, int n, int groups, int entries) {
+    const Plan p = plan_of(type, mats, k, n, groups, entries);
     return (int64_t)p.n_blocks * p.tiles;
 }
 
