@@ -592,7 +592,7 @@ __device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint
 // split over the workgroup, as their few tiles alone would not fill the chip; long rows: both, as
 // neighbouring chunks read at the same time are longer runs of memory.
 // Measured (MI355X): one row, two of 8 experts: gate and up Q4_K 4096 x 14336 132 MB, with k_expert_act 38 us
-// (3.5 TB/s); down Q6_K 14336 x 4096 96 MB, 33 us. 61 rows, eight of 128 experts, 2048 x 768 Q4_K: 226 MB, 66 us with
+// (3.5 TB/s); down Q6_K 14336 x 4096 96 MB, 31 us. 61 rows, eight of 128 experts, 2048 x 768 Q4_K: 226 MB, 66 us with
 // k_expert_act (3.4 TB/s); with no weight loads in its loop still 47, of which the unpacking is 24, the MFMAs 9,
 // the rest starts, the entries' look-up and barriers: its 768 columns leave each workgroup 8 chunks to work on.
 template <uint32_t T, int KP, int NS, int ROWS, bool SWIGLU>
@@ -722,7 +722,7 @@ constexpr int few_lds() {
 // loaded in the loop 1.44 ms: the activations' way to LDS (7.3 GB, from L2) is the rest; the weights' is
 // hidden. A register spilled into that loop costs much: 2.57 ms with 10. 128 entries to eight waves,
 // which halves the weights' unpacking: slower (3.32 | 2.42 ms), as eight waves in step at
-// each stage leave the matrix cores idle. Down Q6_K 14336 x 4096, three products: 1.72 ms, 839 TFLOP/s.
+// each stage leave the matrix cores idle. Down Q6_K 14336 x 4096, three products: 1.69 ms, 853 TFLOP/s.
 template <int MT>
 struct Wide {
     static constexpr int BM = 32 * MT;
