@@ -7,13 +7,19 @@
 // Arithmetic. A Q8_0 element is dx * c. k_expert_act writes it, times a power of two of its row, as
 // fp16 hi + lo (22 bits; the Q8_0 product has 24 + 8), the token operand of the fp16 MFMAs; the weight operand holds the blocks'
 // integers (times the 6-bit sub-scales of Q4_K / Q5_K: at most 1953, exact in fp16; Q6_K's
-// scale * (q - 32) as its fp16 rounding and the exact rest). As dx is inside the operand, nothing is
-// done per block of 32: a super-block's 256 products add up in the MFMA's fp32 accumulators and meet
+// scale * (q - 32) as its fp16 rounding and the exact rest, whose product with lo, 2^-22 of the whole, is left
+// out). As dx is inside the operand, nothing is done per block of 32: a super-block's 256 products add up in the MFMA's fp32 accumulators and meet
 // the weight row's d once, which with the weights on the column side is one scalar of the lane.
 // Blocks of 32 (Q4_0, Q5_0, Q8_0) meet their d once a block. The K-quants' minimum term is one
 // more MFMA a super-block: the 8 minima against dx * (sum of the block's codes) in three fp16 parts.
 // The order of a super-block's elements in the operands is free, so each lane takes contiguous
 // weight bytes and the activations are written in the order that follows.
+//
+// One power of two for a row holds to those 22 bits only blocks whose loudness (largest element) is within a
+// range of 2^kSpread: below it lo is a subnormal and then nothing. A row that spreads further has its range where most of
+// its blocks are; the others, often one or two that are far louder, are zeros in the operand and stand beside
+// it as their exact codes and dx. far_sums forms their products, a block at a time, for all entries of a tile that
+// have any. So no value that fp32 holds is lost, and a tile pays for the blocks apart that it has.
 //
 // (The weight-row GEMM applies dx per block on the VALU, one FMA per output and block, with half the
 // MFMAs; here the MFMAs are doubled and the VALU is left to unpack.)
@@ -38,15 +44,22 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 //   K-quants          [g / 2][s 8][hi, lo][g % 2], so that half a super-block is 512 bytes
 //   blocks of 32      [s 8][hi, lo][g 4]
 // then (K-quants with minima) [row][chunk][3 parts and zeros][8 blocks] fp16, 64 bytes a
-// chunk; then the rows' exponents. Fragment (s, g) holds elements
+// chunk; then the rows' exponents; then, written for rows with blocks apart only, [row] a bit a block (whether it is
+// apart), dx and the sum of the codes of each block (fp32), its 32 codes as fp16 in their own order (zeros of
+// blocks that are not apart). Fragment (s, g) holds elements
 //   Q4_K, Q5_K  64 g + 8 s + e                    (lane group g: the 32 quant bytes of blocks 2g, 2g + 1)
 //   Q6_K        128 (g / 2) + 32 (s / 2) + 16 (g % 2) + 8 (s % 2) + e
 //   Q8_0        32 s + 8 g + e
 //   Q4_0, Q5_0  32 s + 4 g + e (e < 4), 32 s + 16 + 4 g + e - 4 (e >= 4)
 // with e = 0, 2, 1, 3 in each four where the low and high 16 bits of a dword are unpacked together.
 constexpr int kExpNaN = INT32_MIN;  // exponent of a row with an infinity or a NaN: its results are NaN
-constexpr int kTop = 13;            // rows are scaled to magnitudes below 2^(kTop + 1)
+constexpr int kExpFar = 1 << 20;    // added to the exponent of a row that has blocks apart
+constexpr int kTop = 14;            // rows are scaled to magnitudes below 2^(kTop + 1) (-128 codes of subnormals: 4 / 3 of it)
 constexpr int kMinShift = 5;        // minimum operand: 2^-5 of the scale (a block's codes add up to 4064)
+// A block within 2^kSpread of the loudest has an element of 2^5 and more, so a dx of 2^-2 and more, and hi + lo of any of
+// its values c dx is within 2^-23 of it (lo's least step is 2^-24, half of it 2^-23 of 2^-2).
+constexpr int kSpread = kTop - 5;
+constexpr int kLoudness = 288;  // exponents of fp32 values, from -149 on
 
 enum Order { kMin64, kQ6, kByte, kNibble };
 __host__ __device__ constexpr Order order_of(uint32_t t) {
@@ -59,8 +72,13 @@ struct Act {
     const uint8_t* frags;
     const uint8_t* mins;
     const int32_t* exps;
+    const uint8_t* far;
     uint32_t row;  // bytes of a row's fragments
     int chunks;
+    // of a row's blocks apart: the places of dx and of the codes, and all bytes
+    __host__ __device__ uint32_t far_scales() const { return ((uint32_t)chunks + 15u) & ~15u; }
+    __host__ __device__ uint32_t far_codes() const { return far_scales() + (uint32_t)chunks * 64u; }
+    __host__ __device__ size_t far_row() const { return (size_t)far_codes() + (size_t)chunks * 512u; }
 };
 int chunks_of(int k) { return (k + 255) / 256; }
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
@@ -74,54 +92,113 @@ Act act_of(void* ws, uint32_t type, int k, int rows) {
     a.mins = p;
     if (has_min(type)) p += up256((size_t)rows * a.chunks * 64);
     a.exps = (const int32_t*)p;
+    p += up256((size_t)rows * 4);
+    a.far = p;
     return a;
 }
 
-// One workgroup a row: the row's largest magnitude, then each quad of lanes one Q8_0 block (eight
-// elements a lane, quantize_row_q8_0 bit for bit) as scaled fp16 parts. The second read of the row
-// hits the caches. 1024 threads for few rows, where one row's latency is what counts. A row is read once and
-// 4 bytes an element written: the copy rate bounds it (4096 rows of 14336: 470 MB, 116 us, 4.0 TB/s); a
-// single row of 14336 takes 5.7 us, of which 3 are two dependent passes over 56 KB by one CU.
+// One workgroup a row: how loud its blocks are, then each quad of lanes one Q8_0 block (eight
+// elements a lane, quantize_row_q8_0 bit for bit) as scaled fp16 parts. What a thread reads first it keeps, the rest
+// is read again from the caches. 1024 threads for few rows, where one row's latency is what counts. A row is
+// read once and 4 bytes an element written: the copy rate bounds it (4096 rows of 14336: 470 MB, 116 us, 4.0
+// TB/s); a single row of 14336 takes 5.7 us, of which 3 are two dependent passes over 56 KB by one CU. A row with
+// blocks apart takes two more passes, and writes 2.3 bytes an element more.
 template <Order O, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_expert_act(const float* __restrict__ x, int k, uint32_t row_bytes,
-                                                        int chunks, uint8_t* __restrict__ frags,
-                                                        uint8_t* __restrict__ mins, int32_t* __restrict__ exps) {
-    __shared__ uint32_t tops[THREADS / 64];
-    const int row = blockIdx.x, tid = threadIdx.x;
+__global__ __launch_bounds__(THREADS) void k_expert_act(const float* __restrict__ x, int k, Act act) {
+    __shared__ uint32_t tops[THREADS / 64], lows[THREADS / 64], best;
+    __shared__ int loud[kLoudness];
+    const int row = blockIdx.x, tid = threadIdx.x, chunks = act.chunks;
     const f32x4* __restrict__ src = (const f32x4*)(x + (size_t)row * k);
-    uint32_t top = 0;  // the largest (bits << 1): orders magnitudes, and NaN above infinity
-    for (int i = tid; i < k / 4; i += THREADS) {
-        const f32x4 v = src[i];
+    uint8_t* mins = (uint8_t*)act.mins;
+    int32_t* exps = (int32_t*)act.exps;
+    // the largest of a block, (bits << 1), in a quad of lanes that has its eight elements each: orders magnitudes, and NaN
+    // above infinity. (A quad has a block or none: k is a multiple of 32.)
+    auto block_top = [&](const f32x4& v, const f32x4& w) {
+        uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(v[j]) << 1);
+        for (int j = 0; j < 4; ++j) m = max(m, max(__float_as_uint(v[j]) << 1, __float_as_uint(w[j]) << 1));
+        m = max(m, (uint32_t)dpp_i32<DPP_QUAD_SWAP1>((int)m));
+        return max(m, (uint32_t)dpp_i32<DPP_QUAD_SWAP2>((int)m));
+    };
+    auto loudness = [&](uint32_t m) {
+        int ex;
+        (void)frexpf(__builtin_bit_cast(float, m >> 1), &ex);  // magnitude in [2^(ex - 1), 2^ex)
+        return ex;
+    };
+    uint32_t top = 0, low = UINT32_MAX;  // the loudest block, the quietest (less 1) but for blocks of zeros
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 lo0 = zero, hi0 = zero;  // the first eight of this thread, read once
+    if (8 * tid < k) lo0 = src[2 * tid], hi0 = src[2 * tid + 1];
+    for (int i = tid; i < k / 8; i += THREADS) {
+        const uint32_t m = i == tid ? block_top(lo0, hi0) : block_top(src[2 * i], src[2 * i + 1]);
+        top = max(top, m);
+        low = min(low, m - 1);
     }
-    for (int d = 32; d > 0; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
-    if ((tid & 63) == 0) tops[tid >> 6] = top;
+    for (int d = 32; d >= 4; d >>= 1) {
+        top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+        low = min(low, (uint32_t)__shfl_xor((int)low, d, 64));
+    }
+    if ((tid & 63) == 0) tops[tid >> 6] = top, lows[tid >> 6] = low;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < THREADS / 64; ++i) top = max(top, tops[i]);
+    for (int i = 0; i < THREADS / 64; ++i) top = max(top, tops[i]), low = min(low, lows[i]);
     const bool finite = top < 0xFF000000u;
-    int e = 0;
+    bool far = false;
+    int ex = kTop + 1;  // the range's top: blocks of loudness ex - kSpread to ex
     if (finite && top != 0) {
-        int ex;
-        (void)frexpf(__builtin_bit_cast(float, top >> 1), &ex);  // magnitude in [2^(ex - 1), 2^ex)
-        e = kTop + 1 - ex;
+        ex = loudness(top);
+        far = ex - loudness(low + 1) > kSpread;
     }
-    if (tid == 0) exps[row] = finite ? e : kExpNaN;
-    uint8_t* out = frags + (size_t)row * row_bytes;
+    if (far) {  // the range with the most blocks; of equal ones the loudest
+        for (int i = tid; i < kLoudness; i += THREADS) loud[i] = 0;
+        if (tid == 0) best = 0;
+        __syncthreads();
+        for (int i = tid; i < k / 8; i += THREADS) {
+            const uint32_t m = block_top(src[2 * i], src[2 * i + 1]);
+            if ((i & 3) == 0 && m != 0) atomicAdd(&loud[loudness(m) + 149], 1);
+        }
+        __syncthreads();
+        for (int i = tid; i < kLoudness; i += THREADS) {
+            int n = 0;
+            for (int j = max(0, i - kSpread); j <= i; ++j) n += loud[j];
+            atomicMax(&best, ((uint32_t)min(n, 65535) << 16) | (uint32_t)i);
+        }
+        __syncthreads();
+        ex = (int)(best & 0xFFFFu) - 149;
+    }
+    const int e = kTop + 1 - ex;
+    if (tid == 0) exps[row] = !finite ? kExpNaN : far ? e + kExpFar : e;
+    uint8_t* out = (uint8_t*)act.frags + (size_t)row * act.row;
+    uint8_t* apart = (uint8_t*)act.far + (size_t)row * act.far_row();
     // lanes past the row's end write zeros up to the last chunk's end (whole quads: k is a multiple of 32)
     for (int i = tid; i < chunks * 32; i += THREADS) {
         const int c = i >> 5, b = (i >> 2) & 7, p = i & 3;  // chunk, block, eight elements of it
-        float v[8] = {};
-        if (8 * i < k && finite) {
-            const f32x4 lo = src[2 * i], hi = src[2 * i + 1];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = lo[j], v[4 + j] = hi[j];
-        }
+        f32x4 lo = lo0, hi = hi0;
+        if (i != tid && 8 * i < k) lo = src[2 * i], hi = src[2 * i + 1];
+        if (!finite || 8 * i >= k) lo = hi = zero;
+        const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
         uint32_t q[2];
         float d;
         int s8;
         q8_quant_quad(v, q, d, s8);
+        if (far) {
+            const uint32_t m = block_top(lo, hi);
+            const int l = loudness(m);
+            const bool out_of = m != 0 && (l > ex || l < ex - kSpread);
+            const int s16 = s8 + dpp_i32<DPP_QUAD_SWAP1>(s8);
+            const int sum = s16 + dpp_i32<DPP_QUAD_SWAP2>(s16);
+            const wu4 none = {0, 0, 0, 0};
+            *(wu4*)(apart + act.far_codes() + (size_t)(i >> 2) * 64 + 16 * p) = out_of ? int8x8_to_h8(q[0], q[1]) : none;
+            if (p == 0) *(float2*)(apart + act.far_scales() + (size_t)(i >> 2) * 8) = out_of ? make_float2(d, (float)sum) : make_float2(0.0f, 0.0f);
+            const uint32_t bits = (uint32_t)(__ballot(out_of) >> (tid & 32));  // four alike a block
+            if ((i & 31) == 0) {
+                uint32_t byte = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) byte |= ((bits >> (4 * j)) & 1u) << j;
+                apart[c] = (uint8_t)byte;
+            }
+            if (out_of) d = 0.0f;
+        }
         const float dx = ldexpf(d, e);
         _Float16 h[8], l[8];
 #pragma unroll
@@ -433,6 +510,8 @@ __device__ __forceinline__ int entry_of(const Mul& a, const GroupTile& t, int i)
 __device__ __forceinline__ float unscaled(float v, int e) {
     return e == kExpNaN ? __builtin_nanf("") : ldexpf(v, -e);
 }
+// (of a row with blocks apart: done where those were added)
+__device__ __forceinline__ float result(float v, int e) { return e >= kExpFar / 2 ? v : unscaled(v, e); }
 
 // One weight row's share of lane group g of a chunk: 64 elements (16-row tiles).
 template <uint32_t T>
@@ -573,6 +652,159 @@ __device__ __forceinline__ void chunk_product(const WeightChunk<T> (&w)[NT], int
     }
 }
 
+// ---- blocks apart -------------------------------------------------------------------------------
+// Lane group g's eight elements (8 g on) of one block of 32 of a weight row: integers as fp16 (Q6_K: scale * (q - 32) as
+// in the operand above), the block's scale and, of types with minima, its minimum.
+template <uint32_t T>
+struct CodeBlock {
+    wh8 f, rest;
+    float d, m;
+    __device__ __forceinline__ void load(const uint8_t* row, int b, int g) {
+        uint32_t v[2];
+        float off = 0.0f;
+        if constexpr (is_kq(T)) {
+            const uint8_t* at = row + (size_t)(b >> 3) * (T == T_Q6_K ? Q6_K_BYTES : T == T_Q4_K ? Q4_K_BYTES : Q5_K_BYTES);
+            b &= 7;
+            if constexpr (T == T_Q6_K) {
+                const int n = b >> 2, i = b & 3;
+                const u32x2 l = ld_any<8, u32x2>(at + 64 * n + 32 * (i & 1) + 8 * g);
+                const u32x2 h = ld_any<8, u32x2>(at + Q6_K_QH + 32 * n + 8 * g);
+                const wh2 sc = both((float)(int8_t)at[Q6_K_SC + 8 * n + 2 * i + (g >> 1)]);
+                d = f16_to_f32(ld_u16(at + Q6_K_D));
+                wh2 p[4], r[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t u = ((l[k >> 1] >> (4 * (i >> 1))) & 0x0F0F0F0Fu) | (((h[k >> 1] >> (2 * i)) & 0x03030303u) << 4);
+                    const wh2 q = magic_pair(u, k & 1) + both(-1056.0f);
+                    p[k] = q * sc;
+                    r[k] = __builtin_elementwise_fma(q, sc, -p[k]);
+                }
+                f = cat(p[0], p[1], p[2], p[3]);
+                rest = cat(r[0], r[1], r[2], r[3]);
+                return;
+            } else {
+                const u32x4 hdr = ld_u32x4(at);
+                int sc, mn;
+                k4_scale_min(hdr.y, hdr.z, hdr.w, b, sc, mn);
+                d = f16_to_f32(hdr.x & 0xFFFFu) * (float)sc;
+                m = f16_to_f32(hdr.x >> 16) * (float)mn;
+                const u32x2 q = ld_any<8, u32x2>(at + (T == T_Q4_K ? Q4_K_QS : Q5_K_QS) + 32 * (b >> 1) + 8 * g);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) v[k] = (q[k] >> (4 * (b & 1))) & 0x0F0F0F0Fu;
+                if constexpr (T == T_Q5_K) {
+                    const u32x2 h = ld_any<8, u32x2>(at + Q5_K_QH + 8 * g);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) v[k] |= ((h[k] >> b) & 0x01010101u) << 4;
+                }
+            }
+        } else {
+            const uint8_t* at = row + (size_t)b * Unit<T>::BYTES;
+            d = f16_to_f32(ld_u16(at));
+            if constexpr (T == T_Q8_0) {
+                const u32x2 q = ld_any<8, u32x2>(at + 2 + 8 * g);
+                f = __builtin_bit_cast(wh8, int8x8_to_h8(q.x, q.y));
+                return;
+            } else {
+                // elements from 16 on are the high nibbles
+                const u32x2 q = ld_any<8, u32x2>(at + (T == T_Q5_0 ? 6 : 2) + 8 * (g & 1));
+#pragma unroll
+                for (int k = 0; k < 2; ++k) v[k] = (q[k] >> (4 * (g >> 1))) & 0x0F0F0F0Fu;
+                off = T == T_Q5_0 ? -16.0f : -8.0f;
+                if constexpr (T == T_Q5_0) {
+                    const uint32_t h = ld_any<4, uint32_t>(at + 2) >> (8 * g);
+                    v[0] |= bits4(h);
+                    v[1] |= bits4(h >> 4);
+                }
+            }
+        }
+        const wh2 c = both(-1024.0f + off);
+        f = cat(magic_pair(v[0], 0) + c, magic_pair(v[0], 1) + c, magic_pair(v[1], 0) + c, magic_pair(v[1], 1) + c);
+    }
+};
+
+// The lane, found anew: what is done for few tiles holds no register over the loop of all.
+__device__ __forceinline__ int lane_again() {
+    uint32_t zero;
+    asm volatile("s_mov_b32 %0, 0" : "=s"(zero));
+    return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+}
+
+// The sums of the blocks apart of a tile's entries, of M entries and two tiles of M weight rows from n0 on (gate and up of the
+// same rows, or 2 M rows), as a matrix instruction leaves them (M 16: lane (r, g) has entries 4g + j of row r; 32:
+// 8 (j / 4) + 4h + j % 4). The products of a block's codes are whole numbers below 2^24, exact in fp32, and meet
+// d and dx once; its minimum meets the sum of the codes. e: the entry of lane r, far: whether its row has blocks
+// apart, rows: the tile's entries (lanes past them have them again). Looking the blocks up takes about 1 us,
+// then every block that any entry has apart a little less (loads, one after another).
+// Measured (MI355X), no row | every 64th row | all rows with one block apart, us: one row, gate and up Q4_K 4096 x 14336
+// 36 | 43 | 43, down Q6_K 39 | 45 | 45; 61 rows over 128 experts, 2048 x 768 Q4_K 59 | 61 | 69; 2048 rows over 8, gate
+// and up Q4_K 2040 | 2063 | 2207, down Q6_K 1871 | 1885 | 1970. (Whole rows as codes, which needs no range to be
+// found: 36 | 148 | 142, 2007 | 5312 | 20269.)
+template <uint32_t T, int M, bool SWIGLU, class V>
+__device__ __forceinline__ void far_sums(const Mul& a, int group, int n0, int e, bool far, int rows, int lane, V (&sum)[2]) {
+    constexpr int N = M == 16 ? 4 : 16, NT = 2;  // values of a lane
+    const int r = lane & (M - 1), g = lane / M;
+    const int row = far ? e / a.per_row : 0;
+    const size_t bytes = a.act.far_row();
+    const uint8_t* own = a.act.far + (size_t)row * bytes;
+    const uint32_t set = (uint32_t)(__ballot(far) & ((1ull << rows) - 1));
+    const uint8_t* wp[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+        wp[i] = a.w[SWIGLU ? i : 0] + (size_t)group * a.expert_bytes + (size_t)min(n0 + (SWIGLU ? 0 : M * i) + r, a.n - 1) * a.row_bytes;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) sum[i] = V{};
+    for (int w0 = 0; 4 * w0 < a.act.chunks; w0 += 64) {
+        uint32_t word = 0;  // 32 blocks a lane: those that any entry has apart
+        for (uint32_t left = set; left; left &= left - 1) {
+            const int of = __builtin_amdgcn_readlane(row, __ffs(left) - 1);
+            if (4 * (w0 + lane) < a.act.chunks) word |= *(const uint32_t*)(a.act.far + (size_t)of * bytes + 4 * (w0 + lane));
+        }
+        for (uint64_t some = __ballot(word != 0); some; some &= some - 1) {
+            const int l = __ffsll((unsigned long long)some) - 1;
+            for (uint32_t left = (uint32_t)__builtin_amdgcn_readlane((int)word, l); left; left &= left - 1) {
+                const int b = 32 * (w0 + l) + __ffs(left) - 1;
+                if (b >= a.nb) break;  // (bits past the last chunk)
+                float2 s = make_float2(0.0f, 0.0f);
+                if (far) s = *(const float2*)(own + a.act.far_scales() + 8 * (size_t)b);
+                V part[NT];
+                float d[NT], m[NT];
+#pragma unroll
+                for (int q = 0; q < M / 16; ++q) {
+                    const int gq = M == 16 ? g : 2 * q + g;
+                    wh8 x = {};
+                    if (far) x = *(const wh8*)(own + a.act.far_codes() + 64 * (size_t)b + 16 * gq);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        CodeBlock<T> w;
+                        w.load(wp[i], b, gq);
+                        if (q == 0) part[i] = V{};
+                        if constexpr (M == 16) {
+                            part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w.f, part[i], 0, 0, 0);
+                            if constexpr (T == T_Q6_K) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w.rest, part[i], 0, 0, 0);
+                        } else {
+                            part[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w.f, part[i], 0, 0, 0);
+                            if constexpr (T == T_Q6_K) part[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w.rest, part[i], 0, 0, 0);
+                        }
+                        d[i] = w.d;
+                        if constexpr (has_min(T)) m[i] = w.m;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    const int at = M == 16 ? 4 * g + j : 8 * (j >> 2) + 4 * g + (j & 3);
+                    const float dx = __shfl(s.x, at, 64), codes = __shfl(s.y, at, 64);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) {
+                        // (the weights' factors first: they overflow only where the term does)
+                        sum[i][j] = fmaf(d[i] * part[i][j], dx, sum[i][j]);
+                        if constexpr (has_min(T)) sum[i][j] = fmaf(-(m[i] * codes), dx, sum[i][j]);
+                    }
+                }
+            }
+        }
+    }
+}
+
 // 64 x 16 bytes straight to LDS at m0 (the same in every lane), lane i's from base + off (the lanes' own) to m0 + 16 i.
 // In assembly, as the compiler, which would wait for them before any LDS read, is not to see these loads; nor
 // does it see that the load needs a wait state behind the write of M0.
@@ -600,6 +832,8 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
     constexpr int NT = 2, LOADS = ROWS / NS, MIN = has_min(T) ? 64 * ROWS : 0, BUF = 1024 * ROWS + MIN;
     extern __shared__ __align__(16) uint8_t lds[];  // [KP][2][BUF]
     __shared__ int ent[ROWS], exps[ROWS];
+    // the sums of blocks apart, each lane's own: kept here over the loop, which has no registers for them
+    __shared__ f32x4 apart[NS][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kp = wave / NS, ns = wave % NS;
     const int blk = blockIdx.x % a.n_blocks;
@@ -607,6 +841,10 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
     if (t.count <= 0) return;
     const int r = lane & 15, g = lane >> 4;
     const int n0 = (blk * NS + ns) * (SWIGLU ? 16 : 32);
+    if (kp == 0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) apart[ns][i][lane] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
     const uint8_t* wp[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -621,9 +859,23 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
     const int er = r & (ROWS - 1);
     const int e = entry_of(a, t, er);
     const int arow = e < 0 ? 0 : e / a.per_row;
+    const int ex = a.act.exps[arow];
+    const bool far = e >= 0 && ex >= kExpFar / 2;
     if (threadIdx.x < ROWS) {
         ent[er] = e;
-        exps[er] = a.act.exps[arow];
+        exps[er] = far ? ex - kExpFar : ex;
+    }
+    if (__builtin_expect(__ballot(far) != 0, 0)) {
+        if (kp == 0) {
+            f32x4 sum[NT];
+            far_sums<T, 16, SWIGLU>(a, t.group, n0, e, far, ROWS, lane, sum);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) apart[ns][i][lane] = sum[i];
+        }
+        if (kp < chunks) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) wt[0][i].load(wp[i], kp, a.nb, g);  // (once more: not held over it)
+        }
     }
     // this wave's loads: entries ns, ns + NS, .. (the rows of those lanes)
     const uint8_t* from[LOADS];
@@ -665,7 +917,7 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
         auto frag = [&](int s, int part) {
             return *(const wh8*)(cur + (a_at ^ (uint32_t)(is_kq(T) ? 64 * s + 32 * part : 128 * s + 64 * part)));
         };
-        wh8 am;
+        wh8 am = {};
         if constexpr (has_min(T)) am = *(const wh8*)(cur + 1024 * ROWS + er * 64 + 16 * (g ^ ((er >> 1) & 3)));
         chunk_product<T, NT>(wt[PAR], c, a.nb, g, frag, am, acc);
     };
@@ -698,8 +950,8 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
         for (int j = 0; j < 4; ++j) {
             const int tok = 4 * g + j, en = tok < ROWS ? ent[tok & (ROWS - 1)] : -1;
             if (en < 0) continue;
-            float v = unscaled(acc[i][j], exps[tok & (ROWS - 1)]) + b0;
-            if constexpr (SWIGLU) v = silu_mul(v, unscaled(acc[1][j], exps[tok & (ROWS - 1)]) + b1);
+            float v = unscaled(acc[i][j], exps[tok & (ROWS - 1)]) + apart[ns][i][lane][j] + b0;
+            if constexpr (SWIGLU) v = silu_mul(v, unscaled(acc[1][j], exps[tok & (ROWS - 1)]) + apart[ns][1][lane][j] + b1);
             a.y[(size_t)en * a.n + row] = v;
         }
     }
@@ -747,7 +999,7 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
         const int e = entry_of(a, t, i);
         const uint32_t row = (uint32_t)(e < 0 ? 0 : e / a.per_row);
         ent[i] = e;
-        exps[i] = a.act.exps[row];
+        exps[i] = e < 0 ? 0 : a.act.exps[row];
         from_a[i] = row * a.act.row;
         from_m[i] = row * (uint32_t)(a.act.chunks * 64);
     }
@@ -1004,6 +1256,21 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
         }
     }
 
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        const int again = lane_again(), x = exps[32 * m + (again & 31)];
+        if (__builtin_expect(__ballot(x >= kExpFar / 2) != 0, 0)) {
+            wf16 sum[NT];
+            far_sums<T, 32, SWIGLU>(a, t.group, n0, ent[32 * m + (again & 31)], x >= kExpFar / 2, 32, again, sum);
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int of = exps[32 * m + 8 * (e >> 2) + 4 * (again >> 5) + (e & 3)];
+                    if (of >= kExpFar / 2) acc[i][m][e] = unscaled(acc[i][m][e], of - kExpFar) + sum[i][e];
+                }
+        }
+    }
     // lane (r, h) has entries 8 (e / 4) + 4 h + e % 4 of weight row r of each tile
 #pragma unroll
     for (int i = 0; i < (SWIGLU ? 1 : NT); ++i) {
@@ -1018,8 +1285,8 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
                 const int tok = 32 * m + 8 * (e >> 2) + 4 * h + (e & 3);
                 const int en = ent[tok];
                 if (en < 0) continue;
-                float v = unscaled(acc[i][m][e], exps[tok]) + b0;
-                if constexpr (SWIGLU) v = silu_mul(v, unscaled(acc[1][m][e], exps[tok]) + b1);
+                float v = result(acc[i][m][e], exps[tok]) + b0;
+                if constexpr (SWIGLU) v = silu_mul(v, result(acc[1][m][e], exps[tok]) + b1);
                 a.y[(size_t)en * a.n + row] = v;
             }
     }
@@ -1064,11 +1331,9 @@ __global__ __launch_bounds__(256) void k_expert_sum(const float* __restrict__ p,
 template <Order O>
 hipError_t act_launch(const ExpertArgs& a, const Act& act, hipStream_t s) {
     if (a.rows <= 64)
-        k_expert_act<O, 1024><<<a.rows, 1024, 0, s>>>(a.x, a.k, act.row, act.chunks, (uint8_t*)act.frags,
-                                                      (uint8_t*)act.mins, (int32_t*)act.exps);
+        k_expert_act<O, 1024><<<a.rows, 1024, 0, s>>>(a.x, a.k, act);
     else
-        k_expert_act<O, 256><<<a.rows, 256, 0, s>>>(a.x, a.k, act.row, act.chunks, (uint8_t*)act.frags,
-                                                    (uint8_t*)act.mins, (int32_t*)act.exps);
+        k_expert_act<O, 256><<<a.rows, 256, 0, s>>>(a.x, a.k, act);
     return hipGetLastError();
 }
 
@@ -1145,8 +1410,8 @@ hipError_t mul_launch2(Mul& m, int mats, const Plan& p, hipStream_t s) {
 }  // namespace
 
 size_t expert_act_bytes(uint32_t type, int k, int rows) {
-    const size_t c = (size_t)chunks_of(k);
-    return up256((size_t)rows * c * 1024 + (has_min(type) ? up256((size_t)rows * c * 64) : 0) + (size_t)rows * 4);
+    const Act a = act_of(nullptr, type, k, rows);
+    return up256((size_t)(uintptr_t)a.far + (size_t)rows * a.far_row());
 }
 
 hipError_t launch_experts(const ExpertArgs& a, hipStream_t s) {

@@ -483,7 +483,8 @@ int cllm_hip_moe_route_dev(const float* logits, int64_t row_stride, const float*
 /* Products of rows with the matrices of their experts, over GGUF blocks of the six vec_dot types:
  * w holds [n_experts][out_dim] rows of in_dim (the 3-d tensors of a GGUF file), 16-byte aligned. As in
  * matmul_quant a row is quantized to Q8_0 (quantize_row_q8_0, bit for bit) before its products, which
- * are those of the blocks' values, added up in fp32; a row with an infinity or a NaN gives NaN.
+ * are those of the blocks' values, each within 2^-23 (products with Q6_K weights: 2^-21) of itself however far apart the
+ * blocks of a row are, added up in fp32; a row with an infinity or a NaN gives NaN.
  * Entry e has row e / per_row of x[n_rows][in_dim] and writes row e of y [n_rows * per_row][out_dim];
  * entries of no expert leave their row as it is. bias ([n_experts][out_dim]) may be null.
  * per_row is at most 32. ws: 16-byte aligned device scratch of cllm_hip_moe_matmul_ws_bytes bytes, free
