@@ -1959,9 +1959,10 @@ int check_groups(const char* who, int n_entries, int n_groups, const int32_t* of
     return CLLM_HIP_OK;
 }
 
-// The shapes of an expert product: rows of in_dim, n_entries = rows x per_row entries.
+// The shapes of an expert product: rows of in_dim, n_entries = rows x per_row entries; x_rows: the rows that are
+// quantized (every entry's own on the way down, where h has one for each).
 int check_experts(const char* who, uint32_t type, int mats, int in_dim, int out_dim, int n_experts, int n_rows,
-                  int per_row) {
+                  int per_row, int64_t x_rows) {
     if (!has_kernel(type)) return set_err(CLLM_HIP_E_TYPE, "%s: no kernel for this type", who);
     if (in_dim <= 0 || in_dim % block_elems(type) != 0)
         return set_err(CLLM_HIP_E_SHAPE, "%s: in_dim not divisible by block size", who);
@@ -1972,7 +1973,7 @@ int check_experts(const char* who, uint32_t type, int mats, int in_dim, int out_
         return set_err(CLLM_HIP_E_ARG, "%s: 1 to %d experts of a row", who, kMaxRouteTopK);
     const int64_t entries = (int64_t)n_rows * per_row;
     // 32-bit offsets of the activation operand, and workgroups counted in 32 bits of threads
-    const int64_t act = (int64_t)std::max((int64_t)n_rows, entries) * ((in_dim + 255) / 256) * 1024;
+    const int64_t act = x_rows * ((in_dim + 255) / 256) * 1024;
     if ((int64_t)out_dim * (int64_t)row_bytes(type, in_dim) >= (1ll << 32))
         return set_err(CLLM_HIP_E_ARG, "%s: an expert's matrix of 4 GiB and more", who);
     if (act >= (1ll << 32) || entries > (1 << 28) ||
@@ -2065,7 +2066,7 @@ int check_ws(const char* who, const void* ws, size_t have, size_t need) {
 int cllm_hip_moe_matmul_dev(uint32_t type, int in_dim, int out_dim, int n_experts, const void* w, const float* bias,
                             const float* x, int n_rows, int per_row, const int32_t* offsets, const int32_t* order,
                             float* y, void* ws, size_t ws_bytes, void* stream) {
-    int rc = check_experts("moe_matmul", type, 1, in_dim, out_dim, n_experts, n_rows, per_row);
+    int rc = check_experts("moe_matmul", type, 1, in_dim, out_dim, n_experts, n_rows, per_row, n_rows);
     if (rc) return rc;
     if (n_rows == 0 || out_dim == 0) return CLLM_HIP_OK;
     if ((rc = check_groups("moe_matmul", n_rows * per_row, n_experts, offsets, order))) return rc;
@@ -2083,7 +2084,7 @@ int cllm_hip_moe_swiglu_dev(uint32_t type, int in_dim, int n_ff, int n_experts, 
                             const float* bias_gate, const float* bias_up, const float* x, int n_rows, int top_k,
                             const int32_t* offsets, const int32_t* order, float* h, void* ws, size_t ws_bytes,
                             void* stream) {
-    int rc = check_experts("moe_swiglu", type, 2, in_dim, n_ff, n_experts, n_rows, top_k);
+    int rc = check_experts("moe_swiglu", type, 2, in_dim, n_ff, n_experts, n_rows, top_k, n_rows);
     if (rc) return rc;
     if (n_rows == 0 || n_ff == 0) return CLLM_HIP_OK;
     if ((rc = check_groups("moe_swiglu", n_rows * top_k, n_experts, offsets, order))) return rc;
@@ -2104,7 +2105,7 @@ int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, c
                           const float* h, int n_rows, int top_k, const int32_t* ids, const float* weights,
                           const int32_t* offsets, const int32_t* order, const float* base, float* y, void* ws,
                           size_t ws_bytes, void* stream) {
-    int rc = check_experts("moe_down", type, 1, n_ff, out_dim, n_experts, n_rows, top_k);
+    int rc = check_experts("moe_down", type, 1, n_ff, out_dim, n_experts, n_rows, top_k, (int64_t)n_rows * top_k);
     if (rc) return rc;
     if (n_rows == 0 || out_dim == 0) return CLLM_HIP_OK;
     if ((rc = check_groups("moe_down", n_rows * top_k, n_experts, offsets, order))) return rc;
@@ -2128,7 +2129,7 @@ int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, c
 
 const char* cllm_hip_moe_plan(uint32_t type, int n_mats, int in_dim, int out_dim, int n_experts, int n_entries) {
     static thread_local char buf[96];
-    if (n_mats < 1 || n_mats > 2 || check_experts("moe_plan", type, n_mats, in_dim, out_dim, n_experts, n_entries, 1))
+    if (n_mats < 1 || n_mats > 2 || check_experts("moe_plan", type, n_mats, in_dim, out_dim, n_experts, n_entries, 1, 0))
         snprintf(buf, sizeof buf, "none");
     else
         expert_plan_name(type, n_mats, in_dim, out_dim, n_experts, n_entries, buf, sizeof buf);

@@ -487,7 +487,8 @@ int cllm_hip_moe_route_dev(const float* logits, int64_t row_stride, const float*
  * blocks of a row are, added up in fp32; a row with an infinity or a NaN gives NaN.
  * Entry e has row e / per_row of x[n_rows][in_dim] and writes row e of y [n_rows * per_row][out_dim];
  * entries of no expert leave their row as it is. bias ([n_experts][out_dim]) may be null.
- * per_row is at most 32. ws: 16-byte aligned device scratch of cllm_hip_moe_matmul_ws_bytes bytes, free
+ * per_row is at most 32. One call takes what 32-bit offsets reach: 1024 bytes for every 256 elements (or part of them) of
+ * the quantized rows and the matrix of an expert each stay under 4 GiB, entries at most 2^28. ws: 16-byte aligned device scratch of cllm_hip_moe_matmul_ws_bytes bytes, free
  * again when the call has run. */
 size_t cllm_hip_moe_matmul_ws_bytes(uint32_t type, int in_dim, int n_rows);
 int cllm_hip_moe_matmul_dev(uint32_t type, int in_dim, int out_dim, int n_experts, const void* w,
@@ -506,8 +507,8 @@ int cllm_hip_moe_swiglu_dev(uint32_t type, int in_dim, int n_ff, int n_experts, 
 
 /* The down projection and the sum over a row's experts: y[i] = (base[i] +) the sum over j of
  * weights[i][j] * (entry's product with row i * top_k + j of h, + bias), in the order of j, the j without an
- * expert left out. ids and weights as the router's, offsets and order of the same ids. base
- * ([n_rows][out_dim], the residual) may be null, or y. At most 65535 rows. */
+ * expert left out (the quantized rows are the n_rows * top_k of h). ids and weights as the router's, offsets and
+ * order of the same ids. base ([n_rows][out_dim], the residual) may be null, or y. At most 65535 rows. */
 size_t cllm_hip_moe_down_ws_bytes(uint32_t type, int n_ff, int out_dim, int n_rows, int top_k);
 int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, const void* w,
                           const float* bias, const float* h, int n_rows, int top_k,
@@ -515,8 +516,8 @@ int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, c
                           const int32_t* order, const float* base, float* y, void* ws,
                           size_t ws_bytes, void* stream);
 
-/* The kernel and launch plan of the experts' products of n_entries entries (n_mats 2: gate and up);
- * "none" for an unsupported shape. For tests and benchmarks. */
+/* The kernel and launch plan of the experts' products of n_entries entries (n_mats 2: gate and up), whatever rows
+ * they have; "none" for an unsupported shape. For tests and benchmarks. */
 const char* cllm_hip_moe_plan(uint32_t type, int n_mats, int in_dim, int out_dim, int n_experts,
                               int n_entries);
 
