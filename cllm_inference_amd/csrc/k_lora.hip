@@ -343,8 +343,12 @@ hipError_t lora_launch(const LoraArgs& a, hipStream_t s) {
 
 }  // namespace
 
+// Room for the sums of every batch up to `rows`. The parts of K fall in steps as the rows grow, so what a batch writes,
+// parts x rows, goes up and down: bounded here by what grows with the rows. A single row's parts are the most of all;
+// and as parts < 1024 / workgroups + 1 and a workgroup has 16 rows at most, parts x rows < 16384 / mats + rows.
 size_t lora_ws_bytes(int mats, int k, int max_rank, int groups, int rows) {
-    return (size_t)mats * lora_plan(mats, k, groups, rows).parts * rows * max_rank * sizeof(float);
+    const size_t most = (size_t)lora_plan(mats, k, groups, 1).parts * rows, split = (size_t)(16384 + mats - 1) / mats + rows;
+    return (size_t)mats * std::min(most, split) * max_rank * sizeof(float);
 }
 
 hipError_t launch_lora(const LoraArgs& a, hipStream_t s) { return lora_launch(a, s); }

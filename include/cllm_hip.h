@@ -487,9 +487,10 @@ int cllm_hip_moe_route_dev(const float* logits, int64_t row_stride, const float*
  * blocks of a row are, added up in fp32; a row with an infinity or a NaN gives NaN.
  * Entry e has row e / per_row of x[n_rows][in_dim] and writes row e of y [n_rows * per_row][out_dim];
  * entries of no expert leave their row as it is. bias ([n_experts][out_dim]) may be null.
- * per_row is at most 32. One call takes what 32-bit offsets reach: 1024 bytes for every 256 elements (or part of them) of
- * the quantized rows and the matrix of an expert each stay under 4 GiB, entries at most 2^28. ws: 16-byte aligned device scratch of cllm_hip_moe_matmul_ws_bytes bytes, free
- * again when the call has run. */
+ * per_row is at most 32. One call takes what 32-bit offsets reach: 1024 bytes for every 256 elements (or
+ * part of them) of the quantized rows and the matrix of an expert each stay under 4 GiB, entries at most 2^28.
+ * ws: 16-byte aligned device scratch of cllm_hip_moe_matmul_ws_bytes bytes (enough for every smaller batch
+ * too, as moe_down's), free again when the call has run. */
 size_t cllm_hip_moe_matmul_ws_bytes(uint32_t type, int in_dim, int n_rows);
 int cllm_hip_moe_matmul_dev(uint32_t type, int in_dim, int out_dim, int n_experts, const void* w,
                             const float* bias, const float* x, int n_rows, int per_row,
@@ -529,7 +530,8 @@ const char* cllm_hip_moe_plan(uint32_t type, int n_mats, int in_dim, int out_dim
  * ranks[s] (device; null: max_rank; held to 0 .. max_rank): what stands past it is not used. scales
  * (device) null: 1. Rows are grouped by adapter (cllm_hip_group_rows_dev, once for a batch). All sums are fp32.
  * base (null: zeros) or its entries may be null, or the entry of y. ws: 16-byte aligned device scratch of
- * cllm_hip_lora_ws_bytes bytes, free again when the call has run. */
+ * cllm_hip_lora_ws_bytes bytes, free again when the call has run; the size for n_rows is enough for every smaller
+ * batch too. */
 size_t cllm_hip_lora_ws_bytes(int in_dim, int n_mats, int n_adapters, int max_rank, int n_rows);
 int cllm_hip_lora_dev(uint32_t type, int in_dim, int n_mats, const void* const* a,
                       const void* const* b, const int* out_dims, int n_adapters, int max_rank,

@@ -48,3 +48,25 @@ def test_plans_of_many_entries():
     assert "k_expert_wide" in C.moe_plan(Q4_K, 2, 7168, 2048, 256, 160000)
     assert "k_expert_wide" in C.moe_plan(Q4_K, 1, 7168, 2048, 256, 1 << 22)
     assert C.moe_plan(Q4_K, 2, 7168, 2048, 256, (1 << 28) + 1) == "none"
+
+
+@pytest.mark.parametrize("k,mats,adapters,rank", [(4096, 3, 4, 16), (4096, 1, 5, 32), (4096, 2, 32, 64), (896, 4, 1023, 8),
+                                                  (14336, 4, 1, 256), (512, 1, 1, 4), (1000, 2, 7, 12)])
+def test_an_adapter_workspace_serves_every_smaller_batch(k, mats, adapters, rank):
+    size = C.load_library().cllm_hip_lora_ws_bytes
+    sizes = [size(k, mats, adapters, rank, n) for n in range(1, 17001)]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+    assert sizes[0] >= mats * rank * 4
+    # a row's sums, once for each projection at least
+    assert all(s >= mats * rank * 4 * n for n, s in enumerate(sizes, 1))
+    assert size(k, mats, adapters, rank, 1 << 24) >= sizes[-1]
+
+
+def test_expert_workspaces_serve_every_smaller_batch():
+    lib = C.load_library()
+    for t, k in ((Q8_0, 96), (Q4_K, 768)):
+        m = [lib.cllm_hip_moe_matmul_ws_bytes(t, k, n) for n in range(1, 300)]
+        assert m == sorted(m)
+        for per in (1, 5):
+            d = [lib.cllm_hip_moe_down_ws_bytes(t, k, 33, n, per) for n in range(1, 300)]
+            assert d == sorted(d)

@@ -29,3 +29,36 @@ def test_more_entries_than_their_own_rows_would_allow(gpu, orc):
     got = y[torch.from_numpy(at).cuda()].cpu().numpy()
     for e in range(experts):
         assert (np.abs(got[:, e] - xr @ values[e].T) <= M.product_bound(mags[e], xr, k)).all()
+
+
+@pytest.mark.parametrize("adapters,mats,rank,k", [(4, 3, 16, 4096), (5, 1, 32, 4096), (3, 2, 12, 1000)])
+def test_one_adapter_workspace_for_batches_of_all_sizes(gpu, adapters, mats, rank, k):
+    """The workspace of the largest batch takes the smaller ones, and no batch writes behind its own size."""
+    import ctypes
+
+    import torch
+    lib = gpu.load_library()
+    rng = np.random.default_rng(adapters)
+    most, out = 5500, 24
+    x = _cu(rng.standard_normal((most, k)).astype(np.float32))
+    a = [_cu((rng.standard_normal((adapters, rank, k)) / np.sqrt(k)).astype(np.float16)) for _ in range(mats)]
+    b = [_cu(rng.standard_normal((adapters, out, rank)).astype(np.float16)) for _ in range(mats)]
+    ids = _cu(rng.integers(0, adapters, most).astype(np.int32))
+    size = lambda n: lib.cllm_hip_lora_ws_bytes(k, mats, adapters, rank, n)  # noqa: E731
+    whole = torch.empty(size(most) + 4096, dtype=torch.uint8, device="cuda")
+    ptrs = ctypes.c_void_p * mats
+    for n in (1, 15, 333, 720, 1040, 2048, 2272, 3199, 3200, 4097, 5000, 5407, 5408, 5500):
+        g = gpu.group_rows_dev(ids[:n], adapters)
+        want = gpu.lora_dev(x[:n], a, b, g)
+        ys = [torch.empty((n, out), device="cuda") for _ in range(mats)]
+        whole.fill_(0x5A)
+        # (once with the room of the largest batch, once with no more than its own)
+        for room in (size(most), size(n)):
+            rc = lib.cllm_hip_lora_dev(1, k, mats, ptrs(*[t.data_ptr() for t in a]), ptrs(*[t.data_ptr() for t in b]),
+                                       (ctypes.c_int * mats)(*[out] * mats), adapters, rank, None, None, x.data_ptr(), n,
+                                       g.offsets.data_ptr(), g.order.data_ptr(), None,
+                                       ptrs(*[t.data_ptr() for t in ys]), whole.data_ptr(), room,
+                                       torch.cuda.current_stream().cuda_stream)
+            assert rc == 0, (n, lib.cllm_hip_last_error())
+            assert all(torch.equal(y, w) for y, w in zip(ys, want)), n
+        assert (whole[size(n):] == 0x5A).all(), n
