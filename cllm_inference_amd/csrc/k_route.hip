@@ -5,6 +5,8 @@
 // before it, so the order is stable and the same every time, without atomics or scratch.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "device_utils.h"
 #include "experts.h"
 
@@ -278,7 +280,8 @@ hipError_t route_launch(const RouteArgs& a, hipStream_t s) {
             k_route<V, true, 8><<<1, 512, 8 * per, s>>>(a);
         return hipGetLastError();
     }
-    k_route<V, false, 4><<<(a.rows + 3) / 4, 256, 4 * per, s>>>(a);
+    // (a grid's threads are counted in 32 bits: more than 2^26 rows take turns)
+    k_route<V, false, 4><<<std::min((a.rows + 3) / 4, 1 << 22), 256, 4 * per, s>>>(a);
     if (hipError_t e = hipGetLastError()) return e;
     return launch_group_rows(a.ids, a.rows * a.top_k, a.experts, a.offsets, a.order, s);
 }

@@ -62,3 +62,20 @@ def test_one_adapter_workspace_for_batches_of_all_sizes(gpu, adapters, mats, ran
             assert rc == 0, (n, lib.cllm_hip_last_error())
             assert all(torch.equal(y, w) for y, w in zip(ys, want)), n
         assert (whole[size(n):] == 0x5A).all(), n
+
+
+def test_more_rows_than_a_grid_has_threads_for(gpu):
+    """2^26 + 5 rows of two experts: a wave each would be 2^32 threads and more."""
+    import torch
+    rows = (1 << 26) + 5
+    z = torch.zeros((rows, 2), device="cuda")
+    z[1::2, 1] = 1.0
+    z[-1] = torch.tensor([3.0, -3.0])
+    print("route", rows, flush=True)
+    r = gpu.moe_route_dev(z, 1, normalise=True)
+    ids = r.ids.view(-1)
+    want = (z[:, 1] > z[:, 0]).to(torch.int32)
+    assert torch.equal(ids, want) and bool((r.weights == 1).all())
+    assert r.offsets.tolist() == [0, int((want == 0).sum()), rows]
+    order = torch.cat([torch.nonzero(want == 0).view(-1), torch.nonzero(want == 1).view(-1)]).to(torch.int32)
+    assert torch.equal(r.order, order)
