@@ -904,7 +904,9 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
     for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     if (kp < chunks) issue(kp, 0);
     auto chunk = [&]<int PAR>(int c) {
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // this wave's loads are in LDS, and every wave's of the group
+        // this wave's loads are in LDS, and its reads of the other buffer done, which is loaded next (of a group of
+        // waves the barrier says both for all)
+        __builtin_amdgcn_s_waitcnt(NS > 1 ? 0x0F70 : 0x0070);
         asm volatile("" ::: "memory");
         if constexpr (NS > 1) __syncthreads();
         if (c + KP < chunks) {
