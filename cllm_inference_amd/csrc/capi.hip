@@ -1982,8 +1982,6 @@ int check_experts(const char* who, uint32_t type, int mats, int in_dim, int out_
     return CLLM_HIP_OK;
 }
 
-size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
-
 int run_experts(uint32_t type, int mats, int in_dim, int out_dim, int n_experts,
                 const void* const* w, const float* const* bias, const float* x, int n_rows, int per_row,
                 int n_entries, const int32_t* offsets, const int32_t* order, float* y, void* ws, hipStream_t s) {
@@ -2050,8 +2048,8 @@ size_t cllm_hip_moe_matmul_ws_bytes(uint32_t type, int in_dim, int n_rows) {
 size_t cllm_hip_moe_down_ws_bytes(uint32_t type, int in_dim, int out_dim, int n_rows, int top_k) {
     if (!has_kernel(type) || in_dim <= 0 || out_dim <= 0 || n_rows <= 0 || top_k <= 0) return 0;
     const size_t entries = (size_t)n_rows * top_k;
-    return align256(expert_act_bytes(type, in_dim, (int)std::min<size_t>(entries, 1 << 28))) +
-           align256(entries * out_dim * sizeof(float));
+    return up256(expert_act_bytes(type, in_dim, (int)std::min<size_t>(entries, 1 << 28))) +
+           up256(entries * out_dim * sizeof(float));
 }
 
 namespace {
@@ -2118,7 +2116,7 @@ int cllm_hip_moe_down_dev(uint32_t type, int n_ff, int out_dim, int n_experts, c
         return rc;
     DeviceState* st;
     if ((rc = acquire(&st))) return rc;
-    float* parts = (float*)((uint8_t*)ws + align256(expert_act_bytes(type, n_ff, n_rows * top_k)));
+    float* parts = (float*)((uint8_t*)ws + up256(expert_act_bytes(type, n_ff, n_rows * top_k)));
     // every entry is a row of h
     if ((rc = run_experts(type, 1, n_ff, out_dim, n_experts, &w, &bias, h, n_rows * top_k, 1,
                           n_rows * top_k, offsets, order, parts, ws, (hipStream_t)stream)))

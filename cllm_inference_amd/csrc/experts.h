@@ -16,6 +16,9 @@ constexpr int kMaxRouteParts = 64;
 constexpr int kMaxLoraMats = 4;
 constexpr int kMaxLoraRank = 256;
 
+// Parts of a workspace start at multiples of 256 bytes.
+inline size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
 // Entries grouped by index: order lists them sorted by group, those of group g at
 // order[offsets[g]] .. order[offsets[g + 1] - 1], those of no group from offsets[groups] on.
 struct Groups {

@@ -81,7 +81,6 @@ struct Act {
     __host__ __device__ size_t far_row() const { return (size_t)far_codes() + (size_t)chunks * 512u; }
 };
 int chunks_of(int k) { return (k + 255) / 256; }
-size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 Act act_of(void* ws, uint32_t type, int k, int rows) {
     Act a;
     a.chunks = chunks_of(k);

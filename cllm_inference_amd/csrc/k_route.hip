@@ -168,7 +168,7 @@ __device__ void choose(const RouteArgs& a, int row, int lane, double* keys) {
         }
     }
     if (a.parts > 1) {
-            const int width = a.experts / a.parts;
+        const int width = a.experts / a.parts;
 #pragma unroll
         for (int j = 0; j < V; ++j) keys[V * lane + j] = key[j];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
