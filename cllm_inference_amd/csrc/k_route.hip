@@ -13,8 +13,7 @@
 namespace cllm_hip {
 namespace {
 
-constexpr int kSmallEntries = 512;  // up to here one workgroup routes and sorts
-constexpr int kSmallRows = 64;
+constexpr int kSmallEntries = 64;  // up to here one workgroup can route and sort
 
 // ---- entries sorted by group --------------------------------------------------------------------
 // Workgroup g lists the entries of group g (the last one, the entries of none). Its 16 waves take
@@ -271,7 +270,13 @@ __global__ __launch_bounds__(64 * WAVES) void k_route(RouteArgs a) {
 
 template <int V>
 hipError_t route_launch(const RouteArgs& a, hipStream_t s) {
-    const bool small = a.rows <= kSmallRows && a.rows * a.top_k <= kSmallEntries;
+    // One workgroup for all rows, or a wave a row over the chip and a launch that sorts. The second launch costs 3 to 4 us; a
+    // second turn of the waves, and comparing every entry with every other, soon as much. MI355X, us, one | two
+    // launches: 8 rows top 8 of 64 experts 7.0 | 8.1, of 256 8.4 | 9.1, of 512 11.9 | 11.2; 16 rows 11.9 | 8.2, 14.6 | 9.3; 64
+    // rows 41 | 8.8, 53 | 9.8. 1024 experts (four waves) 4 rows 13.0 | 16.9, 5 19.6 | 16.7; top 32 of 64 2 rows 10.2 | 11.6,
+    // 4 12.5 | 11.7. Two turns for few entries of few experts: 16 rows top 2 of 8 6.0 | 7.3, top 4 of 32 7.9 | 7.7.
+    const int entries = a.rows * a.top_k;
+    const bool small = (a.rows <= (V == 16 ? 4 : 8) && entries <= kSmallEntries) || (V == 1 && a.rows <= 16 && entries <= 32);
     const size_t per = a.parts > 1 ? 64 * V * sizeof(double) : 0;
     if (small) {
         if (a.rows <= 4 || V == 16)  // (of 16 experts to a lane, more waves' keys would not fit 64 KB)

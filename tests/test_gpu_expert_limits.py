@@ -79,3 +79,19 @@ def test_more_rows_than_a_grid_has_threads_for(gpu):
     assert r.offsets.tolist() == [0, int((want == 0).sum()), rows]
     order = torch.cat([torch.nonzero(want == 0).view(-1), torch.nonzero(want == 1).view(-1)]).to(torch.int32)
     assert torch.equal(r.order, order)
+
+
+@pytest.mark.parametrize("experts,top_k", [(8, 1), (8, 2), (32, 4), (64, 8), (256, 8), (256, 32), (512, 8), (1024, 8)])
+@pytest.mark.parametrize("bias", [False, True])
+def test_a_row_is_routed_alike_in_batches_of_any_size(gpu, experts, top_k, bias):
+    """One launch or two, with a wave's rows in turn or apart: a row's choice is the same, and so is the order."""
+    import torch
+    gen = torch.Generator("cuda").manual_seed(experts + top_k)
+    z = torch.randn((65, experts), device="cuda", generator=gen)
+    b = torch.randn(experts, device="cuda", generator=gen) * 0.1 if bias else None
+    whole = gpu.moe_route_dev(z, top_k, bias=b, sigmoid=bias)
+    for m in (1, 2, 3, 4, 5, 7, 8, 9, 10, 15, 16, 17, 31, 32, 33, 64):
+        r = gpu.moe_route_dev(z[:m], top_k, bias=b, sigmoid=bias)
+        assert torch.equal(r.ids, whole.ids[:m]) and torch.equal(r.weights, whole.weights[:m]), m
+        offsets, order = M.grouped(r.ids.cpu().numpy().reshape(-1), experts)
+        assert np.array_equal(r.offsets.cpu().numpy(), offsets) and np.array_equal(r.order.cpu().numpy(), order), m
