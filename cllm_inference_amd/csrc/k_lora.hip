@@ -274,7 +274,8 @@ __global__ __launch_bounds__(256) void k_lora_up(Up a) {
 struct LoraPlan {
     int parts, k_part;
 };
-// K in parts of 512 and more, as many as make 1024 workgroups (at most 8).
+// K in parts of 512 and more, as many as make 1024 workgroups (at most 8). 512 | 1024 | 2048 workgroups, MI355X, us: 256
+// rows of 16 adapters on q, k and v 18.8 | 17.0 | 17.2, 2045 rows of rank 32 43.7 | 42.1 | 42.2; elsewhere no difference.
 LoraPlan lora_plan(int mats, int k, int groups, int rows) {
     const int wgs = std::max(1, std::min(tile_ids<16>(groups, rows), rows)) * mats;
     int parts = std::max(1, std::min((1024 + wgs - 1) / wgs, (k + 511) / 512));
@@ -326,10 +327,17 @@ hipError_t lora_launch(const LoraArgs& a, hipStream_t s) {
                  : a.k % 8 == 0 ? down_launch<true, 8>(d, grid, rt, s) : down_launch<true, 4>(d, grid, rt, s);
     if (e != hipSuccess) return e;
     const unsigned up_tiles = (unsigned)tile_ids<16>(a.g.groups + 1, a.g.entries);
-    // few tiles: small blocks, one a workgroup; else as many as leave 1024 workgroups, at most 8
-    const int wide = up_tiles >= 16 ? 2 : 1;
+    // A wave's columns, 16 or 32 (rank sums read once for both). Few workgroups are better off with 16, as are many of short
+    // ranks, whose loads of B then hide; long ranks are bound by the products. MI355X, us, 16 | 32, both launches: 16 rows,
+    // 13 tiles 9.3 | 9.4; 300 rows of fp32 rank 32 x 4096 15.7 | 14.5; 128 rows 12.5 | 12.1; 512 rows 22.0 | 23.6, 1000 rows 28.9 |
+    // 31.3, 2045 rows 42.2 | 47.2; 64 rows of 32 adapters of rank 64 x 28672 43.7 | 50.5; rank 256, 2045 rows 156 | 142
+    int64_t pairs = 0;
+    for (int i = 0; i < a.mats; ++i) pairs += (a.n[i] + 127) / 128;
+    const int wide = up_tiles >= 16 && (a.max_rank > 64 || pairs * up_tiles < 1024) ? 2 : 1;
     int blocks = 0;
     for (int i = 0; i < a.mats; ++i) blocks += (a.n[i] + 64 * wide - 1) / (64 * wide);
+    // column blocks of a workgroup: as many as leave 1024 workgroups, at most 8 (512 | 1024 | 2048 workgroups: 1000 rows
+    // of rank 32 x 4096 25.7 | 23.8 | 25.1, 64 adapters of rank 16 in 64 rows 12.8 | 12.1 | 13.9, 2045 rows 42.2 | 42.1 | 44.2)
     u.steps = (int)std::max<int64_t>(1, std::min<int64_t>(8, (int64_t)blocks * up_tiles / 1024));
     blocks = 0;
     for (int i = 0; i < a.mats; ++i)

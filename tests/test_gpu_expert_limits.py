@@ -95,3 +95,19 @@ def test_a_row_is_routed_alike_in_batches_of_any_size(gpu, experts, top_k, bias)
         assert torch.equal(r.ids, whole.ids[:m]) and torch.equal(r.weights, whole.weights[:m]), m
         offsets, order = M.grouped(r.ids.cpu().numpy().reshape(-1), experts)
         assert np.array_equal(r.offsets.cpu().numpy(), offsets) and np.array_equal(r.order.cpu().numpy(), order), m
+
+
+# many tiles of narrow columns, several column blocks to a workgroup; the same of long ranks, which take wide ones; columns
+# that end inside a block, rows that end inside a tile
+@pytest.mark.parametrize("rows,adapters,rank,outs", [(70, 32, 64, [14336, 130]), (1500, 3, 20, [4100]), (1003, 5, 8, [2050, 515]),
+                                                     (300, 9, 132, [8200]), (1200, 2, 256, [1028])])
+@pytest.mark.parametrize("dt", [np.float16, np.float32])
+def test_wide_outputs_of_many_rows(gpu, rows, adapters, rank, outs, dt):
+    import test_gpu_lora as L
+    c = L._case(rows, adapters, rank, 96, outs, dt, rows)
+    print("lora", rows, adapters, rank, outs, dt.__name__, flush=True)
+    for i, y in enumerate(L._run(gpu, c)):
+        want, tol = L._want(c, i)
+        assert (np.abs(y.cpu().numpy() - want) <= tol).all()
+        out = (c["ids"] < 0) | (c["ids"] >= adapters)
+        assert np.array_equal(y.cpu().numpy()[out], c["base"][i][out])
