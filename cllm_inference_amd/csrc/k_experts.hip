@@ -54,7 +54,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // with e = 0, 2, 1, 3 in each four where the low and high 16 bits of a dword are unpacked together.
 constexpr int kExpNaN = INT32_MIN;  // exponent of a row with an infinity or a NaN: its results are NaN
 constexpr int kExpFar = 1 << 20;    // added to the exponent of a row that has blocks apart
-constexpr int kTop = 14;            // rows are scaled to magnitudes below 2^(kTop + 1) (-128 codes of subnormals: 4 / 3 of it)
+constexpr int kTop = 14;            // rows are scaled to magnitudes below 2^(kTop + 1) (-128 codes of subnormals: 1.01 of it)
 constexpr int kMinShift = 5;        // minimum operand: 2^-5 of the scale (a block's codes add up to 4064)
 // A block within 2^kSpread of the loudest has an element of 2^5 and more, so a dx of 2^-2 and more, and hi + lo of any of
 // its values c dx is within 2^-23 of it (lo's least step is 2^-24, half of it 2^-23 of 2^-2).
@@ -99,9 +99,8 @@ Act act_of(void* ws, uint32_t type, int k, int rows) {
 // One workgroup a row: how loud its blocks are, then each quad of lanes one Q8_0 block (eight
 // elements a lane, quantize_row_q8_0 bit for bit) as scaled fp16 parts. What a thread reads first it keeps, the rest
 // is read again from the caches. 1024 threads for few rows, where one row's latency is what counts. A row is
-// read once and 4 bytes an element written: the copy rate bounds it (4096 rows of 14336: 470 MB, 116 us, 4.0
-// TB/s); a single row of 14336 takes 5.7 us, of which 3 are two dependent passes over 56 KB by one CU. A row with
-// blocks apart takes two more passes, and writes 2.3 bytes an element more.
+// read once and 4 bytes an element written: the copy rate bounds it (4096 rows of 14336: 470 MB, 104 us, 4.5
+// TB/s); a single row of 14336 takes 5.0 us: two dependent passes over 56 KB by one CU. A row with blocks apart takes two more passes, and writes 2.3 bytes an element more.
 template <Order O, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_expert_act(const float* __restrict__ x, int k, Act act) {
     __shared__ uint32_t tops[THREADS / 64], lows[THREADS / 64], best;
@@ -822,10 +821,11 @@ __device__ __forceinline__ void to_lds16(const uint8_t* base, uint32_t off, uint
 // so a CU needs 40 KB and more in flight. Many rows of 16 entries: NS = 4, KP = 1; single tokens: NS = 1 and K
 // split over the workgroup, as their few tiles alone would not fill the chip; long rows: both, as
 // neighbouring chunks read at the same time are longer runs of memory.
-// Measured (MI355X): one row, two of 8 experts: gate and up Q4_K 4096 x 14336 132 MB, with k_expert_act 38 us
-// (3.5 TB/s); down Q6_K 14336 x 4096 96 MB, 31 us. 61 rows, eight of 128 experts, 2048 x 768 Q4_K: 226 MB, 66 us with
-// k_expert_act (3.4 TB/s); with no weight loads in its loop still 47, of which the unpacking is 24, the MFMAs 9,
-// the rest starts, the entries' look-up and barriers: its 768 columns leave each workgroup 8 chunks to work on.
+// Measured (MI355X; a kernel alone is the profiler's median, which carries up to 2 us of its own): one row, two of 8 experts,
+// gate and up Q4_K 4096 x 14336: 132 MB, a pass with k_expert_act 37 us (3.5 TB/s), this kernel 38, at least 34; down
+// Q6_K 14336 x 4096: 96 MB, 32 (3.0 TB/s), at least 30. 61 rows, eight of 128 experts, 2048 x 768 Q4_K: 226 MB, 68 (3.3 TB/s);
+// with no weight loads in its loop still 47, of which the unpacking is 24, the MFMAs 9, the rest starts,
+// the entries' look-up and barriers: its 768 columns leave each workgroup 8 chunks to work on.
 template <uint32_t T, int KP, int NS, int ROWS, bool SWIGLU>
 __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_few(Mul a) {
     constexpr int NT = 2, LOADS = ROWS / NS, MIN = has_min(T) ? 64 * ROWS : 0, BUF = 1024 * ROWS + MIN;
@@ -970,12 +970,12 @@ constexpr int few_lds() {
 // loads and unpacks its weight rows' bytes a stage ahead in registers (with minima, the rows' headers in LDS).
 // LDS: [entry][32 fragments of 16 bytes], fragment f of entry i in place f ^ (i % 32), so that the 32
 // entries' reads of one fragment fall on distinct banks.
-// Measured (MI355X): 2048 rows, two of 8 experts each, gate and up Q4_K of 4096 x 14336: 2.00 ms, 962 GFLOP,
-// 481 TFLOP/s, and as many again for lo: 74% of what the library's fp16 product reaches. With nothing
+// Measured (MI355X): 2048 rows, two of 8 experts each, gate and up Q4_K of 4096 x 14336: 1.95 ms, 962 GFLOP,
+// 493 TFLOP/s, and as many again for lo: 76% of what the library's fp16 product reaches. With nothing
 // loaded in the loop 1.44 ms: the activations' way to LDS (7.3 GB, from L2) is the rest; the weights' is
 // hidden. A register spilled into that loop costs much: 2.57 ms with 10. 128 entries to eight waves,
 // which halves the weights' unpacking: slower (3.32 | 2.42 ms), as eight waves in step at
-// each stage leave the matrix cores idle. Down Q6_K 14336 x 4096, three products: 1.69 ms, 853 TFLOP/s.
+// each stage leave the matrix cores idle. Down Q6_K 14336 x 4096, three products: 1.70 ms, 849 TFLOP/s.
 template <int MT>
 struct Wide {
     static constexpr int BM = 32 * MT;

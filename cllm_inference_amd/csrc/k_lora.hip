@@ -1,9 +1,9 @@
 // k_lora.hip -- low-rank adapters of the requests of a batch beside shared projections (gfx950).
 //
 // y_i[r] = base_i[r] + s_a B_i,a (A_i,a x_r) for row r with adapter a, rows grouped by adapter. Reads of A
-// and B (few rows to an adapter) or of x, base and y (prompts) bound it; products are on fp32 MFMA, so that
-// fp32 rows meet binary16 or fp32 adapters without a rounding, and 16 x 16 tiles lose nothing that the
-// reads would not hide. Two launches: the ranks' sums, split over K where the rows alone do not fill the
+// and B (few rows to an adapter) or of x, base and y (prompts) are what it cannot do without; products are on fp32 MFMA,
+// so that fp32 rows meet binary16 or fp32 adapters without a rounding. Tiles are 16 rows of one adapter: with two rows to an
+// adapter seven eighths of the products are for nothing, 8 to 10 us of the second launch for 64 rows. Two launches: the ranks' sums, split over K where the rows alone do not fill the
 // chip (the second launch adds the parts, in order), then the outputs with the shared projection added.
 #include <hip/hip_runtime.h>
 
@@ -67,9 +67,9 @@ struct Piece {
 // Tile of 16 rows of an adapter x RT tiles of 16 ranks x a part of K. Lane (r, q) loads VL elements from 4 VL b + q VL
 // on, of row r and of rank r, which VL MFMAs take one by one; the four waves take every fourth 64 elements, each
 // loaded while the 64 before are multiplied, and meet in LDS.
-// Measured (MI355X): 64 rows of 32 adapters, two matrices of rank 64, K 4096: 25 MB of binary16 at most, 13.7 us; one
+// Measured (MI355X): 64 rows of 32 adapters (27 named), two matrices of rank 64, K 4096: 21 MB of binary16, 13.9 us; one
 // row 4.8; 2045 rows of 5 adapters, rank 32, fp32: 34 MB of x,
-// 19 us. Starts and the waves' meeting bound it, not the bytes.
+// 19 us (1.8 TB/s). Neither is near its bytes; what a workgroup's start and the waves' meeting take was not measured apart.
 template <bool HALF, int VL, int RT>
 __global__ __launch_bounds__(256) void k_lora_down(Down a) {
     constexpr int NB = 16 / VL;  // pieces of 64 elements
@@ -151,8 +151,9 @@ __global__ __launch_bounds__(256) void k_lora_down(Down a) {
 // r, and ends with four neighbouring columns of one row. A block's elements of B (of the first 4 VL NCH ranks)
 // and of the shared projection are on their way while the block before is multiplied, the first ones while the
 // rank sums are read.
-// Measured (MI355X): 64 rows of 32 adapters, rank 64, 2 x 14336 columns: 117 MB of B, 41.6 us (2.8 TB/s; the fp32 MFMAs
-// 8 to 10 of it); 2045 rows, rank 32, 4096 columns: 67 MB of base and y, 28 us.
+// Measured (MI355X): 64 rows of 32 adapters (27 named), 2 x 14336 columns: B of all 64 ranks, which is read whatever an
+// adapter's rank, 99 MB (of the ranks that count 74), 35 us (2.8 TB/s; the fp32 MFMAs 8 to 10 of it); 2045 rows, rank 32,
+// 4096 columns: 67 MB of base and y, 24 us (2.8 TB/s).
 template <bool HALF, int VL, int NCH, int TILES>
 __global__ __launch_bounds__(256) void k_lora_up(Up a) {
     constexpr int CH = 4 * VL;  // ranks of a chunk

@@ -222,3 +222,23 @@ def test_a_captured_call_takes_rows_of_any_spread(gpu, orc):
         eager = run()
         torch.cuda.synchronize()
         assert torch.equal(y, eager)
+
+
+@pytest.mark.parametrize("rows", [2, 70])
+def test_rows_of_subnormals(gpu, orc, rows):
+    """Rows whose blocks' largest elements are subnormals (scales round up to twice their value there, codes to -128),
+    alone and beside a loud block; weights that bring the products back to normal numbers."""
+    k, n, experts = 512, 40, 1
+    w = S.make_weight(S.Q8_0, n, k, 9).reshape(n, -1, 34).copy()
+    w[:, :, :2] = np.full(2, 30000, np.float16).view(np.uint8)[:2]
+    rng = np.random.default_rng(rows)
+    tops = rng.choice([1, 63, 64, 65, 100, 127, 128, 190, 191, 255, 4000, 70000, 1 << 22, 1 << 25], (rows, k // 32, 1))
+    x = (rng.integers(-tops, tops + 1, (rows, k // 32, 32)) * 2.0 ** -149).astype(np.float32)
+    x[:, :, 3:4] = (tops * 2.0 ** -149).astype(np.float32)
+    x[1::2, 4] *= np.float32(2.0 ** 90)
+    x[0] = np.where(np.arange(k // 32)[:, None] == 2, x[0], 0)
+    x = x.reshape(rows, k)
+    y = gpu.moe_matmul_dev(_cu(x), _cu(w.reshape(-1)), S.Q8_0, n, _route(gpu, np.zeros((rows, 1), np.int32), experts))
+    want, bound = _products(orc, w, S.Q8_0, x, np.zeros((rows, 1), np.int32), 1, experts, n, k)
+    # (a result among the subnormals is rounded to a step of 2^-149)
+    assert (np.abs(y.cpu().numpy() - want) <= bound + 2.0 ** -149).all()
