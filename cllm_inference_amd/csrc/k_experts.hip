@@ -830,6 +830,8 @@ template <uint32_t T, int KP, int NS, int ROWS, bool SWIGLU>
 __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_few(Mul a) {
     constexpr int NT = 2, LOADS = ROWS / NS, MIN = has_min(T) ? 64 * ROWS : 0, BUF = 1024 * ROWS + MIN;
     extern __shared__ __align__(16) uint8_t lds[];  // [KP][2][BUF]
+    // (HELD: in registers, which Q4_0 and Q5_0 have: with 128 bytes more of LDS a CU holds three workgroups, not four)
+    constexpr bool HELD = ROWS == 16 && (T == T_Q4_0 || T == T_Q5_0);
     __shared__ int ent[ROWS], exps[ROWS];
     // the sums of blocks apart, each lane's own: kept here over the loop, which has no registers for them
     __shared__ f32x4 apart[NS][NT][64];
@@ -860,9 +862,10 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
     const int arow = e < 0 ? 0 : e / a.per_row;
     const int ex = a.act.exps[arow];
     const bool far = e >= 0 && ex >= kExpFar / 2;
-    if (threadIdx.x < ROWS) {
+    const int own = far ? ex - kExpFar : ex;
+    if (!HELD && threadIdx.x < ROWS) {
         ent[er] = e;
-        exps[er] = far ? ex - kExpFar : ex;
+        exps[er] = own;
     }
     if (__builtin_expect(__ballot(far) != 0, 0)) {
         if (kp == 0) {
@@ -941,6 +944,11 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
     } else {
         __syncthreads();
     }
+    int en4[4], ex4[4];
+    if constexpr (HELD) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) en4[j] = __shfl(e, 4 * g + j, 64), ex4[j] = __shfl(own, 4 * g + j, 64);
+    }
 #pragma unroll
     for (int i = 0; i < (SWIGLU ? 1 : NT); ++i) {
         const int row = n0 + 16 * i + r;
@@ -949,10 +957,11 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
         const float b0 = a.bias[0] ? a.bias[0][b] : 0.0f, b1 = SWIGLU && a.bias[1] ? a.bias[1][b] : 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int tok = 4 * g + j, en = tok < ROWS ? ent[tok & (ROWS - 1)] : -1;
+            const int tok = 4 * g + j, en = HELD ? en4[j] : tok < ROWS ? ent[tok & (ROWS - 1)] : -1;
             if (en < 0) continue;
-            float v = unscaled(acc[i][j], exps[tok & (ROWS - 1)]) + apart[ns][i][lane][j] + b0;
-            if constexpr (SWIGLU) v = silu_mul(v, unscaled(acc[1][j], exps[tok & (ROWS - 1)]) + apart[ns][1][lane][j] + b1);
+            const int x = HELD ? ex4[j] : exps[tok & (ROWS - 1)];
+            float v = unscaled(acc[i][j], x) + apart[ns][i][lane][j] + b0;
+            if constexpr (SWIGLU) v = silu_mul(v, unscaled(acc[1][j], x) + apart[ns][1][lane][j] + b1);
             a.y[(size_t)en * a.n + row] = v;
         }
     }
