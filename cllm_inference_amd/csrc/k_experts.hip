@@ -651,72 +651,75 @@ __device__ __forceinline__ void chunk_product(const WeightChunk<T> (&w)[NT], int
 }
 
 // ---- blocks apart -------------------------------------------------------------------------------
-// Lane group g's eight elements (8 g on) of one block of 32 of a weight row: integers as fp16 (Q6_K: scale * (q - 32) as
-// in the operand above), the block's scale and, of types with minima, its minimum.
+// Lane group g's eight elements (8 g on) of one block of 32 of a weight row: the bytes, then integers as fp16 (Q6_K:
+// scale * (q - 32) as in the operand above), the block's scale and, of types with minima, its minimum.
 template <uint32_t T>
 struct CodeBlock {
-    wh8 f, rest;
-    float d, m;
+    u32x4 hdr;  // Q4_K, Q5_K: d, dmin and the 6-bit scales; else d and, of Q6_K, the block's scale, of Q5_0 the high bits
+    u32x2 q, h;
     __device__ __forceinline__ void load(const uint8_t* row, int b, int g) {
-        uint32_t v[2];
-        float off = 0.0f;
         if constexpr (is_kq(T)) {
             const uint8_t* at = row + (size_t)(b >> 3) * (T == T_Q6_K ? Q6_K_BYTES : T == T_Q4_K ? Q4_K_BYTES : Q5_K_BYTES);
             b &= 7;
             if constexpr (T == T_Q6_K) {
                 const int n = b >> 2, i = b & 3;
-                const u32x2 l = ld_any<8, u32x2>(at + 64 * n + 32 * (i & 1) + 8 * g);
-                const u32x2 h = ld_any<8, u32x2>(at + Q6_K_QH + 32 * n + 8 * g);
-                const wh2 sc = both((float)(int8_t)at[Q6_K_SC + 8 * n + 2 * i + (g >> 1)]);
-                d = f16_to_f32(ld_u16(at + Q6_K_D));
-                wh2 p[4], r[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t u = ((l[k >> 1] >> (4 * (i >> 1))) & 0x0F0F0F0Fu) | (((h[k >> 1] >> (2 * i)) & 0x03030303u) << 4);
-                    const wh2 q = magic_pair(u, k & 1) + both(-1056.0f);
-                    p[k] = q * sc;
-                    r[k] = __builtin_elementwise_fma(q, sc, -p[k]);
-                }
-                f = cat(p[0], p[1], p[2], p[3]);
-                rest = cat(r[0], r[1], r[2], r[3]);
-                return;
+                q = ld_any<8, u32x2>(at + 64 * n + 32 * (i & 1) + 8 * g);
+                h = ld_any<8, u32x2>(at + Q6_K_QH + 32 * n + 8 * g);
+                hdr.x = ld_u16(at + Q6_K_D);
+                hdr.y = at[Q6_K_SC + 8 * n + 2 * i + (g >> 1)];
             } else {
-                const u32x4 hdr = ld_u32x4(at);
-                int sc, mn;
-                k4_scale_min(hdr.y, hdr.z, hdr.w, b, sc, mn);
-                d = f16_to_f32(hdr.x & 0xFFFFu) * (float)sc;
-                m = f16_to_f32(hdr.x >> 16) * (float)mn;
-                const u32x2 q = ld_any<8, u32x2>(at + (T == T_Q4_K ? Q4_K_QS : Q5_K_QS) + 32 * (b >> 1) + 8 * g);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) v[k] = (q[k] >> (4 * (b & 1))) & 0x0F0F0F0Fu;
-                if constexpr (T == T_Q5_K) {
-                    const u32x2 h = ld_any<8, u32x2>(at + Q5_K_QH + 8 * g);
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) v[k] |= ((h[k] >> b) & 0x01010101u) << 4;
-                }
+                hdr = ld_u32x4(at);
+                q = ld_any<8, u32x2>(at + (T == T_Q4_K ? Q4_K_QS : Q5_K_QS) + 32 * (b >> 1) + 8 * g);
+                if constexpr (T == T_Q5_K) h = ld_any<8, u32x2>(at + Q5_K_QH + 8 * g);
             }
         } else {
             const uint8_t* at = row + (size_t)b * Unit<T>::BYTES;
-            d = f16_to_f32(ld_u16(at));
-            if constexpr (T == T_Q8_0) {
-                const u32x2 q = ld_any<8, u32x2>(at + 2 + 8 * g);
-                f = __builtin_bit_cast(wh8, int8x8_to_h8(q.x, q.y));
-                return;
-            } else {
-                // elements from 16 on are the high nibbles
-                const u32x2 q = ld_any<8, u32x2>(at + (T == T_Q5_0 ? 6 : 2) + 8 * (g & 1));
+            hdr.x = ld_u16(at);
+            // (elements from 16 on are the high nibbles)
+            q = ld_any<8, u32x2>(at + (T == T_Q5_0 ? 6 : 2) + 8 * (T == T_Q8_0 ? g : g & 1));
+            if constexpr (T == T_Q5_0) hdr.y = ld_any<4, uint32_t>(at + 2);
+        }
+    }
+    __device__ __forceinline__ wh8 unpack(int b, int g, wh8& rest, float& d, float& m) const {
+        uint32_t v[2];
+        float off = 0.0f;
+        d = f16_to_f32(hdr.x & 0xFFFFu);
+        if constexpr (T == T_Q8_0) {
+            return __builtin_bit_cast(wh8, int8x8_to_h8(q.x, q.y));
+        } else if constexpr (T == T_Q6_K) {
+            const int i = b & 3;
+            const wh2 sc = both((float)(int8_t)hdr.y);
+            wh2 p[4], r[4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) v[k] = (q[k] >> (4 * (g >> 1))) & 0x0F0F0F0Fu;
-                off = T == T_Q5_0 ? -16.0f : -8.0f;
-                if constexpr (T == T_Q5_0) {
-                    const uint32_t h = ld_any<4, uint32_t>(at + 2) >> (8 * g);
-                    v[0] |= bits4(h);
-                    v[1] |= bits4(h >> 4);
-                }
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t u = ((q[k >> 1] >> (4 * (i >> 1))) & 0x0F0F0F0Fu) | (((h[k >> 1] >> (2 * i)) & 0x03030303u) << 4);
+                const wh2 c = magic_pair(u, k & 1) + both(-1056.0f);
+                p[k] = c * sc;
+                r[k] = __builtin_elementwise_fma(c, sc, -p[k]);
+            }
+            rest = cat(r[0], r[1], r[2], r[3]);
+            return cat(p[0], p[1], p[2], p[3]);
+        } else if constexpr (is_kq(T)) {
+            int sc, mn;
+            k4_scale_min(hdr.y, hdr.z, hdr.w, b & 7, sc, mn);
+            d *= (float)sc;
+            m = f16_to_f32(hdr.x >> 16) * (float)mn;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                v[k] = (q[k] >> (4 * (b & 1))) & 0x0F0F0F0Fu;
+                if constexpr (T == T_Q5_K) v[k] |= ((h[k] >> (b & 7)) & 0x01010101u) << 4;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) v[k] = (q[k] >> (4 * (g >> 1))) & 0x0F0F0F0Fu;
+            off = T == T_Q5_0 ? -16.0f : -8.0f;
+            if constexpr (T == T_Q5_0) {
+                v[0] |= bits4(hdr.y >> (8 * g));
+                v[1] |= bits4(hdr.y >> (8 * g + 4));
             }
         }
         const wh2 c = both(-1024.0f + off);
-        f = cat(magic_pair(v[0], 0) + c, magic_pair(v[0], 1) + c, magic_pair(v[1], 0) + c, magic_pair(v[1], 1) + c);
+        return cat(magic_pair(v[0], 0) + c, magic_pair(v[0], 1) + c, magic_pair(v[1], 0) + c, magic_pair(v[1], 1) + c);
     }
 };
 
@@ -731,14 +734,16 @@ __device__ __forceinline__ int lane_again() {
 // same rows, or 2 M rows), as a matrix instruction leaves them (M 16: lane (r, g) has entries 4g + j of row r; 32:
 // 8 (j / 4) + 4h + j % 4). The products of a block's codes are whole numbers below 2^24, exact in fp32, and meet
 // d and dx once; its minimum meets the sum of the codes. e: the entry of lane r, far: whether its row has blocks
-// apart, rows: the tile's entries (lanes past them have them again). Looking the blocks up takes about 1 us,
-// then every block that any entry has apart a little less (loads, one after another).
+// apart, rows: the tile's entries (lanes past them have them again). The blocks that any entry has apart are taken
+// one after another; of KP waves each takes every KP-th. AHEAD: the next one's loads are on their way, where registers allow.
 // Measured (MI355X), no row | every 64th row | all rows with one block apart, us: one row, gate and up Q4_K 4096 x 14336
-// 36 | 43 | 43, down Q6_K 39 | 45 | 45; 61 rows over 128 experts, 2048 x 768 Q4_K 59 | 61 | 69; 2048 rows over 8, gate
-// and up Q4_K 2040 | 2063 | 2207, down Q6_K 1871 | 1885 | 1970. (Whole rows as codes, which needs no range to be
-// found: 36 | 148 | 142, 2007 | 5312 | 20269.)
-template <uint32_t T, int M, bool SWIGLU, class V>
-__device__ __forceinline__ void far_sums(const Mul& a, int group, int n0, int e, bool far, int rows, int lane, V (&sum)[2]) {
+// 36 | 45 | 45, down Q6_K 39 | 47 | 47; 61 rows over 128 experts, 2048 x 768 Q4_K 59 | 61 | 68; 2048 rows over 8, gate
+// and up Q4_K 1944 | 1978 | 2019, down Q6_K 1796 | 1815 | 1800. (Whole rows as codes, which needs no range to be
+// found: 36 | 148 | 142, 2007 | 5312 | 20269.) Each of 2048 rows with 4 apart in places of its own, so that a tile has most:
+// 6.3 and 3.6 ms (without AHEAD 7.8 and 4.3); a block then takes some 1.2 us, most of it the lanes' arithmetic.
+template <uint32_t T, int M, int KP, bool AHEAD, bool SWIGLU, class V>
+__device__ __forceinline__ void far_sums(const Mul& a, int group, int n0, int e, bool far, int rows, int kp, int lane,
+                                         V (&sum)[2]) {
     constexpr int N = M == 16 ? 4 : 16, NT = 2;  // values of a lane
     const int r = lane & (M - 1), g = lane / M;
     const int row = far ? e / a.per_row : 0;
@@ -751,55 +756,101 @@ __device__ __forceinline__ void far_sums(const Mul& a, int group, int n0, int e,
         wp[i] = a.w[SWIGLU ? i : 0] + (size_t)group * a.expert_bytes + (size_t)min(n0 + (SWIGLU ? 0 : M * i) + r, a.n - 1) * a.row_bytes;
 #pragma unroll
     for (int i = 0; i < NT; ++i) sum[i] = V{};
-    for (int w0 = 0; 4 * w0 < a.act.chunks; w0 += 64) {
-        uint32_t word = 0;  // 32 blocks a lane: those that any entry has apart
-        for (uint32_t left = set; left; left &= left - 1) {
-            const int of = __builtin_amdgcn_readlane(row, __ffs(left) - 1);
-            if (4 * (w0 + lane) < a.act.chunks) word |= *(const uint32_t*)(a.act.far + (size_t)of * bytes + 4 * (w0 + lane));
+    // the blocks that any entry has apart, in order: 32 to a lane's word
+    int w0 = -64, l = 0;
+    uint32_t word = 0, left = 0;
+    uint64_t some = 0;
+    auto any = [&]() {
+        while (left == 0) {
+            if (some != 0) {
+                l = __ffsll((unsigned long long)some) - 1;
+                some &= some - 1;
+                left = (uint32_t)__builtin_amdgcn_readlane((int)word, l);
+                continue;
+            }
+            w0 += 64;
+            if (4 * w0 >= a.act.chunks) return -1;
+            word = 0;
+            const uint32_t at = 4u * (uint32_t)min(w0 + lane, (a.act.chunks - 1) >> 2);
+            for (int i = 0; i < rows; i += 4) {  // (four rows' words on their way at once; those of no entry are dropped)
+                uint32_t v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    v[k] = *(const uint32_t*)(a.act.far + (size_t)__builtin_amdgcn_readlane(row, i + k) * bytes + at);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) word |= (set >> (i + k)) & 1 ? v[k] : 0u;
+            }
+            if (4 * (w0 + lane) >= a.act.chunks) word = 0;
+            some = __ballot(word != 0);
         }
-        for (uint64_t some = __ballot(word != 0); some; some &= some - 1) {
-            const int l = __ffsll((unsigned long long)some) - 1;
-            for (uint32_t left = (uint32_t)__builtin_amdgcn_readlane((int)word, l); left; left &= left - 1) {
-                const int b = 32 * (w0 + l) + __ffs(left) - 1;
-                if (b >= a.nb) break;  // (bits past the last chunk)
-                float2 s = make_float2(0.0f, 0.0f);
-                if (far) s = *(const float2*)(own + a.act.far_scales() + 8 * (size_t)b);
-                V part[NT];
-                float d[NT], m[NT];
+        const int b = 32 * (w0 + l) + __ffs(left) - 1;
+        left &= left - 1;
+        return b < a.nb ? b : -1;  // (bits past the last chunk: nothing follows)
+    };
+    int count = 0;
+    auto next = [&]() {
+        int b = any();
+        while (KP > 1 && b >= 0 && count++ % KP != kp) b = any();
+        return b;
+    };
+    struct Loads {
+        CodeBlock<T> w[M / 16][NT];
+        wh8 x[M / 16];
+        float2 s;
+    };
+    auto load = [&](int b, Loads& to) {
+        to.s = make_float2(0.0f, 0.0f);
+        if (far) to.s = *(const float2*)(own + a.act.far_scales() + 8 * (size_t)b);
 #pragma unroll
-                for (int q = 0; q < M / 16; ++q) {
-                    const int gq = M == 16 ? g : 2 * q + g;
-                    wh8 x = {};
-                    if (far) x = *(const wh8*)(own + a.act.far_codes() + 64 * (size_t)b + 16 * gq);
+        for (int q = 0; q < M / 16; ++q) {
+            const int gq = M == 16 ? g : 2 * q + g;
+            to.x[q] = wh8{};
+            if (far) to.x[q] = *(const wh8*)(own + a.act.far_codes() + 64 * (size_t)b + 16 * gq);
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        CodeBlock<T> w;
-                        w.load(wp[i], b, gq);
-                        if (q == 0) part[i] = V{};
-                        if constexpr (M == 16) {
-                            part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w.f, part[i], 0, 0, 0);
-                            if constexpr (T == T_Q6_K) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x, w.rest, part[i], 0, 0, 0);
-                        } else {
-                            part[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w.f, part[i], 0, 0, 0);
-                            if constexpr (T == T_Q6_K) part[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, w.rest, part[i], 0, 0, 0);
-                        }
-                        d[i] = w.d;
-                        if constexpr (has_min(T)) m[i] = w.m;
-                    }
-                }
+            for (int i = 0; i < NT; ++i) to.w[q][i].load(wp[i], b, gq);
+        }
+    };
+    Loads cur;
+    int b = next();
+    if (AHEAD && b >= 0) load(b, cur);
+    while (b >= 0) {
+        if (!AHEAD) load(b, cur);
+        const int after = next();
+        Loads ahead;
+        if (AHEAD) {
+            ahead = cur;
+            if (after >= 0) load(after, ahead);
+        }
+        V part[NT];
+        float d[NT], m[NT];
 #pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const int at = M == 16 ? 4 * g + j : 8 * (j >> 2) + 4 * g + (j & 3);
-                    const float dx = __shfl(s.x, at, 64), codes = __shfl(s.y, at, 64);
+        for (int q = 0; q < M / 16; ++q)
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) {
-                        // (the weights' factors first: they overflow only where the term does)
-                        sum[i][j] = fmaf(d[i] * part[i][j], dx, sum[i][j]);
-                        if constexpr (has_min(T)) sum[i][j] = fmaf(-(m[i] * codes), dx, sum[i][j]);
-                    }
+            for (int i = 0; i < NT; ++i) {
+                wh8 rest;
+                const wh8 f = cur.w[q][i].unpack(b, M == 16 ? g : 2 * q + g, rest, d[i], m[i]);
+                if (q == 0) part[i] = V{};
+                if constexpr (M == 16) {
+                    part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(cur.x[q], f, part[i], 0, 0, 0);
+                    if constexpr (T == T_Q6_K) part[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(cur.x[q], rest, part[i], 0, 0, 0);
+                } else {
+                    part[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(cur.x[q], f, part[i], 0, 0, 0);
+                    if constexpr (T == T_Q6_K) part[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(cur.x[q], rest, part[i], 0, 0, 0);
                 }
             }
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const int at = M == 16 ? 4 * g + j : 8 * (j >> 2) + 4 * g + (j & 3);
+            const float dx = __shfl(cur.s.x, at, 64), codes = __shfl(cur.s.y, at, 64);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                // (the weights' factors first: they overflow only where the term does)
+                sum[i][j] = fmaf(d[i] * part[i][j], dx, sum[i][j]);
+                if constexpr (has_min(T)) sum[i][j] = fmaf(-(m[i] * codes), dx, sum[i][j]);
+            }
         }
+        if (AHEAD) cur = ahead;
+        b = after;
     }
 }
 
@@ -868,12 +919,23 @@ __global__ __launch_bounds__(64 * KP * NS, KP * NS == 8 ? 4 : 3) void k_expert_f
         exps[er] = own;
     }
     if (__builtin_expect(__ballot(far) != 0, 0)) {
-        if (kp == 0) {
-            f32x4 sum[NT];
-            far_sums<T, 16, SWIGLU>(a, t.group, n0, e, far, ROWS, lane, sum);
+        f32x4 sum[NT];
+        far_sums<T, 16, KP, false, SWIGLU>(a, t.group, n0, e, far, ROWS, kp, lane, sum);
+        f32x4* parts = (f32x4*)lds;  // [wave][NT][64]
+        if constexpr (KP > 1) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) apart[ns][i][lane] = sum[i];
+            for (int i = 0; i < NT; ++i) parts[(wave * NT + i) * 64 + lane] = sum[i];
+            __syncthreads();
         }
+        if (kp == 0) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int k = 1; k < KP; ++k) sum[i] += parts[((k * NS + ns) * NT + i) * 64 + lane];
+                apart[ns][i][lane] = sum[i];
+            }
+        }
+        if constexpr (KP > 1) __syncthreads();
         if (kp < chunks) {
 #pragma unroll
             for (int i = 0; i < NT; ++i) wt[0][i].load(wp[i], kp, a.nb, g);  // (once more: not held over it)
@@ -1271,7 +1333,7 @@ __global__ __launch_bounds__(256, 2) void k_expert_wide(Mul a) {
         const int again = lane_again(), x = exps[32 * m + (again & 31)];
         if (__builtin_expect(__ballot(x >= kExpFar / 2) != 0, 0)) {
             wf16 sum[NT];
-            far_sums<T, 32, SWIGLU>(a, t.group, n0, ent[32 * m + (again & 31)], x >= kExpFar / 2, 32, again, sum);
+            far_sums<T, 32, 1, MT == 2, SWIGLU>(a, t.group, n0, ent[32 * m + (again & 31)], x >= kExpFar / 2, 32, 0, again, sum);
 #pragma unroll
             for (int i = 0; i < NT; ++i)
 #pragma unroll
